@@ -58,6 +58,18 @@ extern "C" {
 #define NHIP_ACT_NONE 0
 #define NHIP_ACT_RELU 1
 #define NHIP_ACT_SIGMOID 4
+/* x * sigmoid(x), ncnn's Swish layer (group norm only; no activation_type of
+ * ncnn's has this value). */
+#define NHIP_ACT_SILU 64
+
+/* Element types.  The graph's blobs are F32, I8 or I32 (Input blobs read by
+ * Dequantize / Requantize / Embed); the token operators below take F32, F16
+ * and BF16. */
+#define NHIP_DTYPE_F32 0
+#define NHIP_DTYPE_I8 1
+#define NHIP_DTYPE_I32 2
+#define NHIP_DTYPE_F16 3
+#define NHIP_DTYPE_BF16 4
 
 /* ---------------------------------------------------------------------------
  * Device, memory, stream.  The reference has no device (everything runs in
@@ -328,6 +340,152 @@ int nhip_dequantize_i32_f32(const int32_t* input, float* output, int32_t n,
                             int32_t c, int64_t plane, const float* scale,
                             int32_t scale_count, const float* bias,
                             int32_t bias_count, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Token operators: what follows the trunk when a decoder reads its features.
+ * No counterpart in the reference (its importer has none of these layers).
+ * All pointers are device pointers unless said otherwise; `dtype` is
+ * NHIP_DTYPE_F32, F16 or BF16 and holds for every tensor of a call but the
+ * integer ones.  Sums, softmax statistics and angles are held in fp32 or
+ * more, results rounded once.  Strides count elements; channels and head
+ * channels are always contiguous.  Tensors may have any alignment that their
+ * type needs; 16-byte aligned rows take the wide loads.  The calls allocate
+ * nothing, so they may be recorded into a HIP graph.
+ * ------------------------------------------------------------------------- */
+
+/* Group norm with an activation, channels last:
+ *   y = act((x - mean) / sqrt(var + eps) * gamma[c] + beta[c])
+ * with mean and (biased) variance over the pixels and channels of one group
+ * of one image (ncnn's GroupNorm).  gamma, beta: host fp32 [channels], both
+ * or neither NULL (NULL: 1 and 0).  channels a multiple of groups and at most
+ * 4096; eps >= 0; activation NONE, RELU or SILU. */
+typedef struct nhip_norm_plan* nhip_norm_t;
+#define NHIP_LAYOUT_TOKENS 0 /* [n][pixels][channels] */
+#define NHIP_LAYOUT_BLOBS 1  /* [n][channels][pixels], the layers' blobs */
+int nhip_group_norm_create(int32_t channels, int32_t groups, const float* gamma,
+                           const float* beta, float eps, int32_t activation,
+                           nhip_norm_t* plan);
+int nhip_group_norm_workspace_size(nhip_norm_t plan, int32_t dtype,
+                                   int32_t layout, int32_t n, int64_t pixels,
+                                   uint64_t* bytes);
+/* input: `layout` with image_stride elements between images and row_stride
+ * between pixels (TOKENS) or channels (BLOBS); output: [n][pixels][channels]
+ * contiguous, in either layout.  It may be the input where the input is such
+ * a tensor too (contiguous TOKENS); otherwise they do not overlap. */
+int nhip_group_norm_forward(nhip_norm_t plan, const void* input, int32_t dtype,
+                            int32_t layout, int32_t n, int64_t pixels,
+                            int64_t image_stride, int64_t row_stride,
+                            void* output, void* workspace,
+                            uint64_t workspace_bytes, void* stream);
+int nhip_norm_destroy(nhip_norm_t plan);
+
+/* Rotary positions with 1 to 4 axes (time, height, width, ...).  A head's
+ * first 2 * sum(sections) channels are rotated in pairs; sections[a] pairs in
+ * a row belong to axis a.  Pair i turns by positions[token][axis(i)] *
+ * inv_freq[i] radians: (x1, x2) -> (x1 cos - x2 sin, x1 sin + x2 cos).  The
+ * pair is (i, i + pairs) or, with `neighbours`, (2i, 2i + 1); the head's other
+ * channels are copied.  inv_freq: host fp32 [pairs], finite.  The turn is
+ * formed in 64-bit fixed point, so that every int32 position, negative ones
+ * too, has an exact angle. */
+typedef struct nhip_rotary_plan* nhip_rotary_t;
+int nhip_rotary_create(int32_t head_dim, int32_t axes, const int32_t* sections,
+                       const float* inv_freq, int32_t neighbours,
+                       nhip_rotary_t* plan);
+/* x, y: [batch][tokens][heads][head_dim] with strides (batch, token, head); y
+ * may be x with the same strides, otherwise they do not overlap.  positions:
+ * int32 [batch][tokens][axes], batches positions_stride elements apart (0:
+ * one for all).  inverse != 0 turns back. */
+int nhip_rotary_forward(nhip_rotary_t plan, const void* x, int32_t dtype,
+                        int32_t batch, int32_t tokens, int32_t heads,
+                        const int64_t* x_strides, const int32_t* positions,
+                        int64_t positions_stride, int32_t inverse, void* y,
+                        const int64_t* y_strides, void* stream);
+int nhip_rotary_destroy(nhip_rotary_t plan);
+
+/* Attention: for every query row
+ *   out = sum_j p_j value_j,  p = softmax_j(scale * query . key_j)
+ * over the keys that the row may see; a row that may see none is 0.  Query
+ * head h reads the key and value head h / (heads / kv_heads).
+ * head_dim 1 to 256. */
+typedef struct nhip_attention_desc {
+  int32_t dtype;
+  int32_t batch;
+  int32_t queries; /* query rows of a sequence */
+  int32_t keys;    /* key rows of a sequence; of a cache: the longest there is */
+  int32_t heads;
+  int32_t kv_heads; /* divides heads */
+  int32_t head_dim;
+  float scale;
+} nhip_attention_desc;
+
+/* Cross attention to an encoder's states.  query [batch][queries][heads][d],
+ * key and value [batch][keys][kv_heads][d], each with strides (batch, token,
+ * head) of its own; out [batch][queries][heads][d] contiguous.  A row sees
+ * the keys before key_lengths[b] (int32 [batch], clamped to 0..keys; NULL: all)
+ * whose key_mask is not 0 (bytes [batch][keys], batches mask_stride elements
+ * apart, 0: one for all; NULL: all).  What stands in other keys' and values'
+ * places is not used, whatever it is. */
+int nhip_cross_attention_workspace_size(const nhip_attention_desc* desc,
+                                        uint64_t* bytes);
+int nhip_cross_attention_forward(
+    const nhip_attention_desc* desc, const void* query,
+    const int64_t* query_strides, const void* key, const int64_t* key_strides,
+    const void* value, const int64_t* value_strides, const int32_t* key_lengths,
+    const uint8_t* key_mask, int64_t mask_stride, void* out, void* workspace,
+    uint64_t workspace_bytes, void* stream);
+
+/* A cache of keys and values in 8 bits.  A page holds block_tokens tokens of
+ * one sequence: codes k, v int8 [pages][kv_heads][block_tokens][head_dim] and
+ * a scale for each page and head, k_scale, v_scale fp32 [pages][kv_heads]; a
+ * code q stands for q * scale.  block_tokens: 16, 32, 64, 128 or 256;
+ * head_dim a multiple of 8, at most 256; codes 16-byte aligned.  Which pages a sequence has
+ * stands in its row of a block table: int32 [batch][table_pages], token t in
+ * page table[b][t / block_tokens].  Tokens of a page number outside
+ * 0..pages-1, or past the table, are not written, read as 0 and not seen. */
+typedef struct nhip_kv8_cache {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t pages;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t block_tokens;
+} nhip_kv8_cache;
+
+/* Tokens starts[b] .. starts[b] + counts[b] - 1 of sequence b (int32; a
+ * negative start adds nothing; counts NULL: `tokens`, otherwise clamped to
+ * 0..tokens) from key and value [batch][tokens][kv_heads][head_dim] with
+ * strides (batch, token, head).  A page's scale is the largest finite |x| of
+ * its new tokens times fp32(1/127) (at least 2^-126 unless all are 0), and not
+ * less than what it was where the page already held tokens before starts[b];
+ * when it grows, those are requantised.  Codes: x / scale to the nearest,
+ * halves away from zero, clamped to +-127 (infinities too), NaN to 0.  Sequences that
+ * share a page must not append to it in one call. */
+int nhip_kv8_append(const nhip_kv8_cache* cache, int32_t dtype, const void* key,
+                    const int64_t* key_strides, const void* value,
+                    const int64_t* value_strides, int32_t batch, int32_t tokens,
+                    const int32_t* block_table, int64_t table_pages,
+                    const int32_t* starts, const int32_t* counts, void* stream);
+/* The values of tokens starts[b] .. starts[b] + tokens - 1, to key and value
+ * [batch][tokens][kv_heads][head_dim] contiguous. */
+int nhip_kv8_read(const nhip_kv8_cache* cache, int32_t dtype, int32_t batch,
+                  int32_t tokens, const int32_t* block_table,
+                  int64_t table_pages, const int32_t* starts, void* key,
+                  void* value, void* stream);
+/* Attention over the cache: as the cross attention with the first lengths[b]
+ * cached tokens of sequence b as keys and values (int32 [batch], clamped to
+ * 0..desc->keys).  causal != 0: the queries are the last tokens of their
+ * sequence, row i sees the first lengths[b] - queries + 1 + i tokens. */
+int nhip_kv8_attention_workspace_size(const nhip_attention_desc* desc,
+                                      const nhip_kv8_cache* cache,
+                                      uint64_t* bytes);
+int nhip_kv8_attention_forward(
+    const nhip_attention_desc* desc, const nhip_kv8_cache* cache,
+    const void* query, const int64_t* query_strides,
+    const int32_t* block_table, int64_t table_pages, const int32_t* lengths,
+    int32_t causal, void* out, void* workspace, uint64_t workspace_bytes,
+    void* stream);
 
 #ifdef __cplusplus
 }

@@ -37,10 +37,6 @@
 extern "C" {
 #endif
 
-#define NHIP_DTYPE_F32 0
-#define NHIP_DTYPE_I8 1
-#define NHIP_DTYPE_I32 2 /* Input blobs read by Dequantize / Requantize / Embed */
-
 typedef struct nhip_graph* nhip_graph_t;
 
 /* Parse and lower a model held in memory.  input_shapes: NULL, or

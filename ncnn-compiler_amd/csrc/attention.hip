@@ -1,0 +1,154 @@
+// Attention entry points: checks, the choice of the split over the keys, and
+// dispatch by element type (kernels: attention.h).
+#include <algorithm>
+#include <cmath>
+
+#include "attention.h"
+
+namespace nhip {
+namespace {
+
+// Checks the sizes and fills them in; the number of parts of the keys.
+int attn_args(const nhip_attention_desc* d, AttnArgs* a) {
+  if (!d) return fail(NHIP_STATUS_NULL_POINTER, "attention: null descriptor");
+  if (!elem_size(d->dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "attention: dtype has to be F32, F16 or BF16");
+  if (d->batch < 0 || d->queries < 0 || d->keys < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative extent");
+  if (d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads)
+    return fail(NHIP_STATUS_INVALID_SHAPE, "attention: kv_heads has to divide heads");
+  if (d->head_dim <= 0 || d->head_dim > 256) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: head_dim has to be 1 to 256");
+  if (!std::isfinite(d->scale)) return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: scale has to be finite");
+  a->batch = d->batch;
+  a->queries = d->queries;
+  a->keys = d->keys;
+  a->heads = d->heads;
+  a->kv_heads = d->kv_heads;
+  a->group = d->heads / d->kv_heads;
+  a->d = d->head_dim;
+  a->scale_log2 = d->scale * 1.4426950408889634f;
+  // 2^30 leaves room for the last tile's keys and rows past the end
+  const int64_t most = int64_t(1) << 30;
+  if (d->keys > most || (int64_t)d->queries * a->group > most)
+    return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: at most 2^30 keys, and rows of a key/value head");
+  a->rows = d->queries * a->group;
+  a->row_tiles = (int)ceil_div(std::max(a->rows, 1), attn::kRowTile);
+  // few rows: the keys are split until there are two workgroups for every CU,
+  // each part with at least 128 keys
+  const int64_t heads = (int64_t)d->batch * d->kv_heads;
+  if (heads > 0x7fffffff / a->row_tiles) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: too many rows");
+  const int64_t wgs = std::max<int64_t>(1, heads * a->row_tiles);
+  const int64_t want = std::max<int64_t>(1, 2 * cu_count() / wgs);
+  a->splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(d->keys, 128), 64}));
+  return ok();
+}
+
+uint64_t attn_workspace(const AttnArgs& a) {
+  if (a.splits == 1) return 0;
+  return (uint64_t)a.batch * a.kv_heads * a.rows * a.splits * (a.d * sizeof(float) + sizeof(float2));
+}
+
+int attn_forward(AttnArgs& a, const nhip_attention_desc* d, int src, const void* query, const int64_t* qs, void* out,
+                 void* workspace, uint64_t workspace_bytes, void* stream) {
+  const int es = elem_size(d->dtype);
+  if (!aligned_to(query, es) || !aligned_to(out, es))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: a tensor is not aligned to its type");
+  a.q = query;
+  a.o = out;
+  for (int i = 0; i < 3; ++i) {
+    if (qs[i] < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative stride");
+    a.qs[i] = qs[i];
+  }
+  const uint64_t need = attn_workspace(a);
+  if (need) {
+    if (!workspace) return fail(NHIP_STATUS_NULL_POINTER, "attention: null workspace");
+    if (workspace_bytes < need || !aligned_to(workspace, 16))
+      return fail(NHIP_STATUS_OUTPUT_CAPACITY_INSUFFICIENT, "attention: workspace too small or not 16-byte aligned");
+    a.part_ml = (float2*)workspace;
+    a.part_o = (float*)(a.part_ml + (uint64_t)a.batch * a.kv_heads * a.rows * a.splits);
+  }
+  switch (d->dtype) {
+    case NHIP_DTYPE_F32: return attn_run_f32(a, src, as_stream(stream));
+    case NHIP_DTYPE_F16: return attn_run_f16(a, src, as_stream(stream));
+    default: return attn_run_bf16(a, src, as_stream(stream));
+  }
+}
+
+// 16-byte aligned rows, near enough for a tile's to be reached with 31 bits.
+bool vec_rows(const void* p, const int64_t* strides, int es) {
+  const int v = 16 / es;
+  return aligned_to(p, 16) && strides[0] % v == 0 && strides[1] % v == 0 && strides[2] % v == 0 &&
+         strides[1] <= (int64_t(1) << 24) / es;
+}
+
+}  // namespace
+}  // namespace nhip
+
+using namespace nhip;
+
+extern "C" {
+
+int nhip_cross_attention_workspace_size(const nhip_attention_desc* desc, uint64_t* bytes) {
+  if (!bytes) return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
+  AttnArgs a{};
+  NHIP_TRY(attn_args(desc, &a));
+  *bytes = attn_workspace(a);
+  return ok();
+}
+
+int nhip_cross_attention_forward(const nhip_attention_desc* desc, const void* query, const int64_t* query_strides,
+                                 const void* key, const int64_t* key_strides, const void* value,
+                                 const int64_t* value_strides, const int32_t* key_lengths, const uint8_t* key_mask,
+                                 int64_t mask_stride, void* out, void* workspace, uint64_t workspace_bytes,
+                                 void* stream) {
+  AttnArgs a{};
+  NHIP_TRY(attn_args(desc, &a));
+  if (desc->batch == 0 || desc->queries == 0) return ok();
+  if (!query || !query_strides || !out || !key_strides || !value_strides || (desc->keys && (!key || !value)))
+    return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
+  const int es = elem_size(desc->dtype);
+  if (!aligned_to(key, es) || !aligned_to(value, es) || !aligned_to(key_lengths, 4))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: a tensor is not aligned to its type");
+  a.k = key;
+  a.v = value;
+  for (int i = 0; i < 3; ++i) {
+    if (key_strides[i] < 0 || value_strides[i] < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative stride");
+    a.ks[i] = key_strides[i];
+    a.vs[i] = value_strides[i];
+  }
+  a.lengths = key_lengths;
+  a.mask = key_mask;
+  if (mask_stride < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative stride");
+  a.mask_stride = mask_stride;
+  const bool vec = desc->head_dim % (16 / es) == 0 && vec_rows(query, query_strides, es) &&
+                   vec_rows(key, key_strides, es) && vec_rows(value, value_strides, es);
+  return attn_forward(a, desc, vec ? kSrcVec : kSrcAny, query, query_strides, out, workspace, workspace_bytes, stream);
+}
+
+int nhip_kv8_attention_workspace_size(const nhip_attention_desc* desc, const nhip_kv8_cache* cache, uint64_t* bytes) {
+  if (!bytes || !cache) return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
+  AttnArgs a{};
+  NHIP_TRY(attn_args(desc, &a));
+  *bytes = attn_workspace(a);
+  return ok();
+}
+
+int nhip_kv8_attention_forward(const nhip_attention_desc* desc, const nhip_kv8_cache* cache, const void* query,
+                               const int64_t* query_strides, const int32_t* block_table, int64_t table_pages,
+                               const int32_t* lengths, int32_t causal, void* out, void* workspace,
+                               uint64_t workspace_bytes, void* stream) {
+  AttnArgs a{};
+  NHIP_TRY(attn_args(desc, &a));
+  NHIP_TRY(kv8_args(cache, block_table, table_pages, &a.cache));
+  if (cache->kv_heads != desc->kv_heads || cache->head_dim != desc->head_dim)
+    return fail(NHIP_STATUS_INVALID_SHAPE, "attention: the cache has other heads");
+  if (desc->batch == 0 || desc->queries == 0) return ok();
+  if (!query || !query_strides || !out || !lengths) return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
+  if (!aligned_to(lengths, 4)) return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: a tensor is not aligned to its type");
+  a.lengths = lengths;
+  a.causal = causal != 0;
+  const int v = 16 / elem_size(desc->dtype);
+  if (!aligned_to(query, 16) || query_strides[0] % v || query_strides[1] % v || query_strides[2] % v)
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: query rows over the cache have to be 16-byte aligned");
+  return attn_forward(a, desc, kSrcInt8, query, query_strides, out, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

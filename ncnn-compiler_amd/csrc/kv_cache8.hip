@@ -1,0 +1,235 @@
+// The 8-bit cache of keys and values: tokens quantised into pages with a
+// scale for each page and head, and read back as values.  (The attention over
+// it: attention.h.)
+//
+// Compiled with -ffp-contract=off: a code is the rounding of one separately
+// rounded product, so that it can be restated bit for bit.
+#include <algorithm>
+
+#include "elem.h"
+#include "kv_cache8.h"
+
+namespace nhip {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct AppendArgs {
+  Kv8 c;
+  const void* x[2];      // keys, values
+  int64_t xs[2][3];      // batch, token, head
+  const int32_t* starts;
+  const int32_t* counts;
+  int32_t tokens, touch;  // pages that a sequence may touch
+};
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+
+// One workgroup: one page of one sequence, one head, keys or values.  The new
+// tokens are read twice (the second time from the cache that the first filled):
+// for their largest magnitude and to be quantised.
+template <class T, int V>
+__global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
+  __shared__ float red[kThreads / 64];
+  const int which = blockIdx.x & 1;
+  const uint32_t rest = blockIdx.x >> 1;
+  const int h = rest % a.c.kv_heads;
+  const uint32_t rest2 = rest / a.c.kv_heads;
+  const int j = rest2 % a.touch, b = rest2 / a.touch;
+  const int start = a.starts[b];
+  const int count = a.counts ? min(a.counts[b], a.tokens) : a.tokens;
+  if (start < 0 || count <= 0) return;
+  const int bt = 1 << a.c.shift;
+  const int64_t page = (int64_t)(start >> a.c.shift) + j;
+  const int64_t t0 = max((int64_t)start, page << a.c.shift);
+  const int64_t t1 = min((int64_t)start + count, (page + 1) << a.c.shift);
+  if (t0 >= t1) return;
+  const int64_t id = kv8_page(a.c, b, page);
+  if (id < 0) return;
+  const int d = a.c.head_dim;
+  int8_t* code = (which ? a.c.v : a.c.k) + ((id * a.c.kv_heads + h) << a.c.shift) * d;
+  float* scale = (which ? a.c.v_scale : a.c.k_scale) + id * a.c.kv_heads + h;
+  const T* x = (const T*)a.x[which] + b * a.xs[which][0] + (t0 - start) * a.xs[which][1] + h * a.xs[which][2];
+  const int64_t xt = a.xs[which][1];
+  const int vecs = d / V, fresh = (int)(t1 - t0) * vecs;
+  const int had = (int)(t0 - (page << a.c.shift));  // tokens that the page holds
+
+  float most = 0.f;
+  for (int i = threadIdx.x; i < fresh; i += kThreads) {
+    float t[V];
+    Vec<T, V>::load(x + i / vecs * xt + i % vecs * V, t);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float m = fabsf(t[e]);
+      most = m <= 3.402823466e38f ? fmaxf(most, m) : most;  // NaN and infinities do not count
+    }
+  }
+  most = wave_max(most);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float was = had ? *scale : 0.f;
+  const float want = most > 0.f ? fmaxf(most * (1.0f / 127.0f), kScaleLeast) : 0.f;
+  const float now = fmaxf(want, was);
+  const float inv = now > 0.f ? 1.0f / now : 0.f;
+  __syncthreads();  // everybody has read the scale
+  if (threadIdx.x == 0) *scale = now;
+  if (now != was) {
+    const float ratio = was * inv;
+    for (int i = threadIdx.x; i < had * d; i += kThreads) code[i] = quantize_i8((float)code[i], ratio);
+  }
+  int8_t* to = code + had * d;
+  for (int i = threadIdx.x; i < fresh; i += kThreads) {
+    float t[V];
+    Vec<T, V>::load(x + i / vecs * xt + i % vecs * V, t);
+    int q[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) q[e] = quantize_q(t[e], inv);
+    if constexpr (V >= 4) {
+#pragma unroll
+      for (int e = 0; e < V; e += 4)
+        reinterpret_cast<uint32_t*>(to + i * V)[e / 4] = pack_i8x4(q[e], q[e + 1], q[e + 2], q[e + 3]);
+    } else {
+      to[i] = (int8_t)q[0];
+    }
+  }
+}
+
+struct ReadArgs {
+  Kv8 c;
+  void* out[2];
+  const int32_t* starts;
+  int64_t items;  // of keys: batch * tokens * kv_heads * head_dim / 8
+  int32_t tokens;
+};
+
+template <class T>
+__global__ __launch_bounds__(kThreads) void kv8_read_kernel(ReadArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int which = blockIdx.y;
+  if (i >= a.items) return;
+  const int vecs = a.c.head_dim / 8;
+  const int c = (int)(i % vecs) * 8;
+  const int64_t r = i / vecs;
+  const int h = (int)(r % a.c.kv_heads);
+  const int64_t bt = r / a.c.kv_heads;
+  const int b = (int)(bt / a.tokens);
+  const int64_t t = (int64_t)a.starts[b] + bt % a.tokens;
+  const int64_t id = t < 0 ? -1 : kv8_page(a.c, b, t >> a.c.shift);
+  float v[8] = {};
+  if (id >= 0) {
+    const int64_t at = (((id * a.c.kv_heads + h) << a.c.shift) + (t & ((1 << a.c.shift) - 1))) * a.c.head_dim + c;
+    const int2 q = *reinterpret_cast<const int2*>((which ? a.c.v : a.c.k) + at);
+    const float s = (which ? a.c.v_scale : a.c.k_scale)[id * a.c.kv_heads + h];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3))) * s;
+  }
+  T* out = (T*)a.out[which] + i * 8;
+#pragma unroll
+  for (int e = 0; e < 8; e += kVec<T>) Vec<T, kVec<T>>::store(out + e, reinterpret_cast<float(&)[kVec<T>]>(v[e]));
+}
+
+template <class T>
+int append_run(const AppendArgs& a, uint32_t wgs, bool vec, hipStream_t s) {
+  if (vec)
+    NHIP_LAUNCH("kv8_append", (kv8_append_kernel<T, kVec<T>>), dim3(wgs), dim3(kThreads), 0, s, a);
+  else
+    NHIP_LAUNCH("kv8_append", (kv8_append_kernel<T, 1>), dim3(wgs), dim3(kThreads), 0, s, a);
+  return check_launch("kv8_append");
+}
+
+template <class T>
+int read_run(const ReadArgs& a, hipStream_t s) {
+  NHIP_LAUNCH("kv8_read", kv8_read_kernel<T>, dim3((uint32_t)ceil_div(a.items, kThreads), 2), dim3(kThreads), 0, s, a);
+  return check_launch("kv8_read");
+}
+
+}  // namespace
+
+int kv8_args(const nhip_kv8_cache* cache, const int32_t* table, int64_t table_pages, Kv8* c) {
+  if (!cache) return fail(NHIP_STATUS_NULL_POINTER, "kv8: null cache");
+  if (cache->kv_heads <= 0 || cache->pages < 0 || table_pages < 0)
+    return fail(NHIP_STATUS_INVALID_SHAPE, "kv8: extents have to be positive");
+  if (cache->head_dim <= 0 || cache->head_dim > 256 || cache->head_dim % 8)
+    return fail(NHIP_STATUS_INVALID_SHAPE, "kv8: head_dim has to be a multiple of 8, 256 at most");
+  int shift = 4;
+  while (shift < 8 && (1 << shift) != cache->block_tokens) ++shift;
+  if ((1 << shift) != cache->block_tokens)
+    return fail(NHIP_STATUS_INVALID_SHAPE, "kv8: block_tokens has to be 16, 32, 64, 128 or 256");
+  if (!cache->k || !cache->v || !cache->k_scale || !cache->v_scale || (!table && table_pages))
+    return fail(NHIP_STATUS_NULL_POINTER, "kv8: null pointer");
+  if (!aligned_to(cache->k, 16) || !aligned_to(cache->v, 16) || !aligned_to(cache->k_scale, 4) ||
+      !aligned_to(cache->v_scale, 4) || !aligned_to(table, 4))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "kv8: a tensor is not aligned");
+  *c = Kv8{cache->k, cache->v, cache->k_scale, cache->v_scale, table, cache->pages, table_pages,
+           cache->kv_heads, cache->head_dim, shift};
+  return ok();
+}
+
+}  // namespace nhip
+
+using namespace nhip;
+
+extern "C" {
+
+int nhip_kv8_append(const nhip_kv8_cache* cache, int32_t dtype, const void* key, const int64_t* key_strides,
+                    const void* value, const int64_t* value_strides, int32_t batch, int32_t tokens,
+                    const int32_t* block_table, int64_t table_pages, const int32_t* starts, const int32_t* counts,
+                    void* stream) {
+  AppendArgs a{};
+  NHIP_TRY(kv8_args(cache, block_table, table_pages, &a.c));
+  const int es = elem_size(dtype);
+  if (!es) return fail(NHIP_STATUS_UNSUPPORTED, "kv8: dtype has to be F32, F16 or BF16");
+  if (batch < 0 || tokens < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "kv8: negative extent");
+  if (batch == 0 || tokens == 0) return ok();
+  if (!key || !value || !key_strides || !value_strides || !starts)
+    return fail(NHIP_STATUS_NULL_POINTER, "kv8: null pointer");
+  if (!aligned_to(key, es) || !aligned_to(value, es))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "kv8: a tensor is not aligned to its type");
+  a.x[0] = key;
+  a.x[1] = value;
+  const int v = 16 / es;
+  bool vec = aligned_to(key, 16) && aligned_to(value, 16);  // head_dim is a multiple of 8
+  for (int i = 0; i < 3; ++i) {
+    a.xs[0][i] = key_strides[i];
+    a.xs[1][i] = value_strides[i];
+    if (a.xs[0][i] < 0 || a.xs[1][i] < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "kv8: negative stride");
+    vec = vec && a.xs[0][i] % v == 0 && a.xs[1][i] % v == 0;
+  }
+  a.starts = starts;
+  a.counts = counts;
+  a.tokens = tokens;
+  const int bt = 1 << a.c.shift;
+  a.touch = (int)(((int64_t)tokens + bt - 2) / bt + 1);
+  const int64_t wgs = (int64_t)batch * a.touch;
+  if (wgs > 0x7fffffff / 2 / a.c.kv_heads) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "kv8: too many pages in one call");
+  return NHIP_FOR_ELEM(dtype, T, append_run<T>(a, (uint32_t)(wgs * a.c.kv_heads * 2), vec, as_stream(stream)));
+}
+
+int nhip_kv8_read(const nhip_kv8_cache* cache, int32_t dtype, int32_t batch, int32_t tokens,
+                  const int32_t* block_table, int64_t table_pages, const int32_t* starts, void* key, void* value,
+                  void* stream) {
+  ReadArgs a{};
+  NHIP_TRY(kv8_args(cache, block_table, table_pages, &a.c));
+  if (!elem_size(dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "kv8: dtype has to be F32, F16 or BF16");
+  if (batch < 0 || tokens < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "kv8: negative extent");
+  if (batch == 0 || tokens == 0) return ok();
+  if (!key || !value || !starts) return fail(NHIP_STATUS_NULL_POINTER, "kv8: null pointer");
+  if (!aligned_to(key, 16) || !aligned_to(value, 16))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "kv8: the values read have to be 16-byte aligned");
+  a.out[0] = key;
+  a.out[1] = value;
+  a.starts = starts;
+  a.tokens = tokens;
+  const int64_t rows = (int64_t)batch * tokens;
+  if (rows > (int64_t(0x7fffffff) * kThreads) / a.c.kv_heads / a.c.head_dim)
+    return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "kv8: too many tokens in one call");
+  a.items = rows * a.c.kv_heads * (a.c.head_dim / 8);
+  return NHIP_FOR_ELEM(dtype, T, read_run<T>(a, as_stream(stream)));
+}
+
+}  // extern "C"

@@ -14,6 +14,7 @@ reference's single-image [C,H,W] blobs.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -29,6 +30,7 @@ STATUS_NAMES = {
 
 ALGO_AUTO, ALGO_IMPLICIT_GEMM, ALGO_WINOGRAD = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_SIGMOID = 0, 1, 4
+ACT_SILU = 64  # group norm only
 
 # Every symbol include/nhip.h declares (checked by the CPU test suite).
 EXPORTS = (
@@ -49,6 +51,10 @@ EXPORTS = (
     "nhip_global_avgpool_innerproduct_f32_forward", "nhip_relu_f32", "nhip_relu_i8",
     "nhip_add_f32", "nhip_global_avgpool_f32", "nhip_quantize_f32_i8",
     "nhip_requantize_i32_i8", "nhip_dequantize_i32_f32",
+    "nhip_group_norm_create", "nhip_group_norm_workspace_size", "nhip_group_norm_forward", "nhip_norm_destroy",
+    "nhip_rotary_create", "nhip_rotary_forward", "nhip_rotary_destroy",
+    "nhip_cross_attention_workspace_size", "nhip_cross_attention_forward",
+    "nhip_kv8_append", "nhip_kv8_read", "nhip_kv8_attention_workspace_size", "nhip_kv8_attention_forward",
 )
 
 # Every symbol include/nhip_graph.h declares.
@@ -57,7 +63,8 @@ GRAPH_EXPORTS = (
     "nhip_graph_io_info", "nhip_graph_infer_shapes", "nhip_graph_run",
     "nhip_graph_run_host", "nhip_graph_destroy",
 )
-DTYPE_F32, DTYPE_I8, DTYPE_I32 = 0, 1, 2
+DTYPE_F32, DTYPE_I8, DTYPE_I32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2, 3, 4
+LAYOUT_TOKENS, LAYOUT_BLOBS = 0, 1
 _NP_DTYPE = {DTYPE_F32: np.float32, DTYPE_I8: np.int8, DTYPE_I32: np.int32}
 
 
@@ -75,8 +82,19 @@ class ConvDesc(ctypes.Structure):
         "activation_type", "group", "algorithm")]
 
 
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "dtype", "batch", "queries", "keys", "heads", "kv_heads", "head_dim")] + [("scale", ctypes.c_float)]
+
+
+class Kv8Desc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        ("pages", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("kv_heads", "head_dim", "block_tokens")]
+
+
 _lib = None
 _P = ctypes.c_void_p
+_Strides = ctypes.c_int64 * 3
 
 
 def load():
@@ -139,6 +157,22 @@ def load():
         "nhip_requantize_i32_i8": [_P, _P, i32, i32, i64, _P, i32, _P, i32, _P, i32, i32, _P],
         "nhip_dequantize_i32_f32": [_P, _P, i32, i32, i64, _P, i32, _P, i32, _P],
     }
+    A, K8, S, U = (ctypes.POINTER(x) for x in (AttentionDesc, Kv8Desc, i64, u64))
+    sig.update({
+        "nhip_group_norm_create": [i32, i32, _P, _P, f32, i32, ctypes.POINTER(_P)],
+        "nhip_group_norm_workspace_size": [_P, i32, i32, i32, i64, U],
+        "nhip_group_norm_forward": [_P, _P, i32, i32, i32, i64, i64, i64, _P, _P, u64, _P],
+        "nhip_norm_destroy": [_P],
+        "nhip_rotary_create": [i32, i32, _P, _P, i32, ctypes.POINTER(_P)],
+        "nhip_rotary_forward": [_P, _P, i32, i32, i32, i32, S, _P, i64, i32, _P, S, _P],
+        "nhip_rotary_destroy": [_P],
+        "nhip_cross_attention_workspace_size": [A, U],
+        "nhip_cross_attention_forward": [A, _P, S, _P, S, _P, S, _P, _P, i64, _P, _P, u64, _P],
+        "nhip_kv8_append": [K8, i32, _P, S, _P, S, i32, i32, _P, i64, _P, _P, _P],
+        "nhip_kv8_read": [K8, i32, i32, i32, _P, i64, _P, _P, _P, _P],
+        "nhip_kv8_attention_workspace_size": [A, K8, U],
+        "nhip_kv8_attention_forward": [A, K8, _P, S, _P, i64, _P, i32, _P, _P, u64, _P],
+    })
     i64p, i32p, vpp = ctypes.POINTER(i64), ctypes.POINTER(i32), ctypes.POINTER(_P)
     sig.update({
         "nhip_graph_load": [ctypes.c_char_p, u64, _P, u64, i64p, i32, vpp],
@@ -630,6 +664,277 @@ def dequantize(x, scale, bias=None, stream=None):
     check(load().nhip_dequantize_i32_f32(_ptr(x), _ptr(out), n, c, plane, _ptr(s), s.numel(), _ptr(b),
                                          0 if b is None else b.numel(), _stream(stream)))
     return out
+
+
+# ------------------------------------------------------------ token operators
+_ELEM = {}
+
+
+def _elem(t, *like):
+    """The element type code of a device tensor whose channels are contiguous;
+    `like`: tensors that have to have its type and device."""
+    torch = _torch()
+    if not _ELEM:
+        _ELEM.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16})
+    for x in (t, *like):
+        if not isinstance(x, torch.Tensor) or not x.is_cuda:
+            raise TypeError("nhip expects a CUDA (HIP) device tensor")
+        if x.dtype != t.dtype or x.device != t.device:
+            raise TypeError(f"expected {t.dtype} on {t.device}, got {x.dtype} on {x.device}")
+        if x.shape[-1] > 1 and x.stride(-1) != 1:
+            raise ValueError("channels have to be contiguous")
+    if t.device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"{t.device} is not the current device")
+    if t.dtype not in _ELEM:
+        raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}")
+    return _ELEM[t.dtype]
+
+
+def _ints(t, device, shape, what):
+    """Pointer of a contiguous int32 device tensor of that shape."""
+    if t.dtype != _torch().int32 or t.device != device or not t.is_contiguous() or tuple(t.shape) != shape:
+        raise ValueError(f"{what} has to be a contiguous int32 tensor of shape {shape} on {device}")
+    return t.data_ptr()
+
+
+def _output(out, like, shape, stream, dtype=None):
+    """`out`, checked, or a new tensor that `stream` may write."""
+    torch = _torch()
+    dtype = dtype or like.dtype
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=like.device)
+        if stream is not None:
+            out.record_stream(stream)
+    elif out.dtype != dtype or out.device != like.device or not out.is_contiguous() or tuple(out.shape) != tuple(shape):
+        raise ValueError(f"out has to be a contiguous {dtype} tensor of shape {tuple(shape)} on {like.device}")
+    return out
+
+
+def _scratch(workspace, nbytes, device, stream):
+    """(tensor, pointer, bytes) of the caller's workspace or a new one, which
+    stays allocated until `stream` is done with it."""
+    if workspace is None:
+        if not nbytes:
+            return None, None, 0
+        workspace = _torch().empty(nbytes, dtype=_torch().uint8, device=device)
+        if stream is not None:
+            workspace.record_stream(stream)
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+@functools.lru_cache(4096)
+def _strides(strides):
+    return _Strides(*strides)
+
+
+class GroupNorm(_Plan):
+    """Group norm with an activation (ACT_NONE, ACT_RELU, ACT_SILU), channels
+    last.  gamma, beta: [channels] or both None."""
+    _destroy = "nhip_norm_destroy"
+
+    def __init__(self, groups, channels, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, blobs=False):
+        super().__init__()
+        self.channels, self.layout = channels, LAYOUT_BLOBS if blobs else LAYOUT_TOKENS
+        self._g, self._b = (None if v is None else np.ascontiguousarray(v, dtype=np.float32) for v in (gamma, beta))
+        for v in (self._g, self._b):
+            if v is not None and v.shape != (channels,):
+                raise ValueError(f"gamma and beta have to have {channels} elements")
+        check(load().nhip_group_norm_create(channels, groups, _np_ptr(self._g), _np_ptr(self._b), eps, act,
+                                            ctypes.byref(self.handle)))
+        self._sizes = {}
+
+    def workspace_size(self, dtype_code, n, pixels) -> int:
+        key = (dtype_code, n, pixels)
+        if key not in self._sizes:
+            b = ctypes.c_uint64()
+            check(load().nhip_group_norm_workspace_size(self.handle, dtype_code, self.layout, n, pixels, ctypes.byref(b)))
+            if len(self._sizes) > 4096:
+                self._sizes.clear()
+            self._sizes[key] = b.value
+        return self._sizes[key]
+
+    def forward(self, x, out=None, workspace=None, stream=None):
+        """x [n, pixels, channels] (any image and pixel strides) or
+        [n, h, w, channels] -> the same shape; with blobs=True x
+        [n, channels, h, w] or [n, channels, pixels] -> [n, pixels, channels]."""
+        if self.layout == LAYOUT_BLOBS:
+            v = x if x.dim() == 3 else x.view(x.shape[0], x.shape[1], -1)
+            n, c, pixels = v.shape
+            shape = (n, pixels, c)
+        else:
+            v = x if x.dim() == 3 else x.view(x.shape[0], -1, x.shape[3])
+            n, pixels, c = v.shape
+            shape = x.shape
+        code = _elem(v)
+        if c != self.channels:
+            raise ValueError(f"x has {c} channels, expected {self.channels}")
+        out = _output(out, x, shape, stream)
+        ws, ptr, nbytes = _scratch(workspace, self.workspace_size(code, n, pixels), x.device, stream)
+        check(load().nhip_group_norm_forward(self.handle, v.data_ptr(), code, self.layout, n, pixels, v.stride(0),
+                                             max(v.stride(1), v.shape[2]) if v.shape[1] == 1 else v.stride(1),
+                                             out.data_ptr(), ptr, nbytes, _stream(stream)))
+        return out
+
+
+class Rotary(_Plan):
+    """Rotary positions over the axes that `sections` counts pairs for.
+    inv_freq: [sum(sections)]; default theta^(-i / sections[a]) for pair i of
+    axis a.  neighbours: pairs (2i, 2i + 1) instead of (i, i + pairs)."""
+    _destroy = "nhip_rotary_destroy"
+
+    def __init__(self, head_dim, sections, inv_freq=None, theta=10000.0, neighbours=False):
+        super().__init__()
+        self.head_dim, self.axes = head_dim, len(sections)
+        if inv_freq is None:
+            inv_freq = [float(theta) ** (-i / s) for s in sections for i in range(s)]
+        sec = np.ascontiguousarray(sections, dtype=np.int32)
+        freq = np.ascontiguousarray(inv_freq, dtype=np.float32)
+        if freq.shape != (int(sec.sum()),):
+            raise ValueError(f"inv_freq has shape {freq.shape}, expected ({int(sec.sum())},)")
+        check(load().nhip_rotary_create(head_dim, self.axes, _np_ptr(sec), _np_ptr(freq), 1 if neighbours else 0,
+                                        ctypes.byref(self.handle)))
+
+    def forward(self, x, positions, inverse=False, out=None, stream=None):
+        """x [batch, tokens, heads, head_dim] (any strides of the first
+        three), positions int32 [batch or 1, tokens, axes]; out may be x."""
+        b, n, h, d = x.shape
+        if d != self.head_dim:
+            raise ValueError(f"x has {d} channels to a head, expected {self.head_dim}")
+        code = _elem(x)
+        per = positions.shape[0]
+        if per not in (1, b):
+            raise ValueError("positions have to have the batch's size or 1")
+        pos = _ints(positions, x.device, (per, n, self.axes), "positions")
+        if out is None:
+            out = _output(None, x, x.shape, stream)
+        elif out.shape != x.shape:
+            raise ValueError(f"out has to have shape {tuple(x.shape)}")
+        else:
+            _elem(x, out)
+        check(load().nhip_rotary_forward(self.handle, x.data_ptr(), code, b, n, h, _strides(x.stride()[:3]), pos,
+                                         n * self.axes if per > 1 else 0, 1 if inverse else 0, out.data_ptr(),
+                                         _strides(out.stride()[:3]), _stream(stream)))
+        return out
+
+
+@functools.lru_cache(4096)
+def _attention(code, b, lq, lk, h, hkv, d, scale):
+    """(descriptor, workspace bytes)."""
+    desc = AttentionDesc(code, b, lq, lk, h, hkv, d, float(d) ** -0.5 if scale is None else float(scale))
+    n = ctypes.c_uint64()
+    check(load().nhip_cross_attention_workspace_size(ctypes.byref(desc), ctypes.byref(n)))
+    return desc, n.value
+
+
+def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, out=None, workspace=None, stream=None):
+    """softmax(scale * q k^T) v: q [batch, queries, heads, d], k and v
+    [batch, keys, kv_heads, d] (any strides of the first three).  key_lengths:
+    int32 [batch]; key_mask: bool [batch, keys] or [keys], True where a key
+    counts.  A row that sees no key is 0.  scale: default d ** -0.5."""
+    torch = _torch()
+    b, lq, h, d = q.shape
+    lk, hkv = k.shape[1], k.shape[2]
+    code = _elem(q, k, v)
+    if tuple(k.shape) != (b, lk, hkv, d) or v.shape != k.shape:
+        raise ValueError(f"k and v have shapes {tuple(k.shape)} and {tuple(v.shape)}: expected [{b}, keys, kv_heads, {d}]")
+    desc, need = _attention(code, b, lq, lk, h, hkv, d, scale)
+    lengths = None if key_lengths is None else _ints(key_lengths, q.device, (b,), "key_lengths")
+    mask, mask_stride = None, 0
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or key_mask.device != q.device or tuple(key_mask.shape) not in ((b, lk), (lk,)):
+            raise ValueError(f"key_mask has to be a bool tensor of shape {(b, lk)} or {(lk,)} on {q.device}")
+        if lk > 1 and key_mask.stride(-1) != 1:
+            raise ValueError("key_mask's keys have to be contiguous")
+        mask, mask_stride = key_mask.data_ptr(), key_mask.stride(0) if key_mask.dim() == 2 else 0
+    out = _output(out, q, q.shape, stream)
+    ws, ptr, nbytes = _scratch(workspace, need, q.device, stream)
+    check(load().nhip_cross_attention_forward(desc, q.data_ptr(), _strides(q.stride()[:3]), k.data_ptr(),
+                                              _strides(k.stride()[:3]), v.data_ptr(), _strides(v.stride()[:3]),
+                                              lengths, mask, mask_stride, out.data_ptr(), ptr, nbytes, _stream(stream)))
+    return out
+
+
+class KvCache8:
+    """Keys and values in 8 bits, in pages of block_tokens tokens with a scale
+    for each page and head (include/nhip.h: nhip_kv8_cache).  Which pages a
+    sequence has is the caller's: block tables are int32 [batch, pages of a
+    sequence]."""
+
+    def __init__(self, pages, kv_heads, head_dim, block_tokens=64, device="cuda"):
+        torch = _torch()
+        shape = (pages, kv_heads, block_tokens, head_dim)
+        self._hold(torch.zeros(shape, dtype=torch.int8, device=device),
+                   torch.zeros(shape, dtype=torch.int8, device=device),
+                   torch.zeros(shape[:2], dtype=torch.float32, device=device),
+                   torch.zeros(shape[:2], dtype=torch.float32, device=device))
+
+    @classmethod
+    def of(cls, k, v, k_scale, v_scale):
+        """A cache in the caller's tensors: int8 [pages, kv_heads,
+        block_tokens, head_dim] and float32 [pages, kv_heads]."""
+        self = cls.__new__(cls)
+        self._hold(k, v, k_scale, v_scale)
+        return self
+
+    def _hold(self, k, v, k_scale, v_scale):
+        torch = _torch()
+        for t, dtype, shape in ((k, torch.int8, k.shape), (v, torch.int8, k.shape),
+                                (k_scale, torch.float32, k.shape[:2]), (v_scale, torch.float32, k.shape[:2])):
+            if not t.is_cuda or t.dtype != dtype or t.shape != shape or t.device != k.device or not t.is_contiguous():
+                raise ValueError(f"expected a contiguous {dtype} tensor of shape {tuple(shape)} on {k.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        pages, self.kv_heads, self.block_tokens, self.head_dim = k.shape
+        self._desc = Kv8Desc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
+                             self.kv_heads, self.head_dim, self.block_tokens)
+
+    def append(self, k, v, block_table, starts, counts=None, stream=None):
+        """Tokens starts[b] .. of each sequence from k and v [batch, tokens,
+        kv_heads, head_dim]: all of them, or the first counts[b]."""
+        b, n = k.shape[:2]
+        code = _elem(k, v)
+        if tuple(k.shape) != (b, n, self.kv_heads, self.head_dim) or v.shape != k.shape or k.device != self.k.device:
+            raise ValueError(f"k and v have to have shape [batch, tokens, {self.kv_heads}, {self.head_dim}] on {self.k.device}")
+        pages = block_table.shape[-1]
+        check(load().nhip_kv8_append(self._desc, code, k.data_ptr(), _strides(k.stride()[:3]), v.data_ptr(),
+                                     _strides(v.stride()[:3]), b, n,
+                                     _ints(block_table, k.device, (b, pages), "block_table"), pages,
+                                     _ints(starts, k.device, (b,), "starts"),
+                                     None if counts is None else _ints(counts, k.device, (b,), "counts"),
+                                     _stream(stream)))
+
+    def read(self, block_table, starts, tokens, dtype, out=None, stream=None):
+        """Values of tokens starts[b] .. starts[b] + tokens - 1: (k, v), each
+        [batch, tokens, kv_heads, head_dim]."""
+        b, pages = block_table.shape
+        shape = (b, tokens, self.kv_heads, self.head_dim)
+        k, v = (_output(o, self.k, shape, stream, dtype) for o in (out or (None, None)))
+        check(load().nhip_kv8_read(self._desc, _elem(k, v), b, tokens,
+                                   _ints(block_table, self.k.device, (b, pages), "block_table"), pages,
+                                   _ints(starts, self.k.device, (b,), "starts"), k.data_ptr(), v.data_ptr(),
+                                   _stream(stream)))
+        return k, v
+
+    def attention(self, q, block_table, lengths, max_length=None, causal=False, scale=None, out=None, workspace=None,
+                  stream=None):
+        """Attention of q [batch, queries, heads, head_dim] to the first
+        lengths[b] cached tokens (at most max_length; default what the block
+        table holds).  causal: the queries are the last tokens."""
+        b, lq, h, d = q.shape
+        code = _elem(q)
+        if d != self.head_dim or q.device != self.k.device:
+            raise ValueError(f"q has to have {self.head_dim} channels to a head, on {self.k.device}")
+        pages = block_table.shape[-1]
+        if max_length is None:
+            max_length = pages * self.block_tokens
+        desc, need = _attention(code, b, lq, max_length, h, self.kv_heads, d, scale)
+        out = _output(out, q, q.shape, stream)
+        ws, ptr, nbytes = _scratch(workspace, need, q.device, stream)
+        check(load().nhip_kv8_attention_forward(desc, self._desc, q.data_ptr(), _strides(q.stride()[:3]),
+                                                _ints(block_table, q.device, (b, pages), "block_table"), pages,
+                                                _ints(lengths, q.device, (b,), "lengths"), 1 if causal else 0,
+                                                out.data_ptr(), ptr, nbytes, _stream(stream)))
+        return out
+
 
 
 class Graph:
