@@ -26,6 +26,7 @@ struct AttnArgs {
   int64_t mask_stride;
   int32_t batch, queries, keys, heads, kv_heads, group, d, causal;
   int32_t rows;       // queries * group
+  int32_t tiles;      // the kernel of many rows
   int32_t row_tiles;  // row tiles of a key/value head
   int32_t splits;     // parts of a sequence's keys
   float scale_log2;   // scale / ln 2
@@ -45,6 +46,7 @@ namespace attn {
 constexpr int kRowTile = 16;   // query rows of a workgroup
 constexpr int kKeyTile = 32;   // keys of a wave's step
 constexpr int kWaves = 4;
+constexpr int kTilesRows = 32 * kWaves;  // query rows of a workgroup, many rows
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 
@@ -585,27 +587,42 @@ int rows_launch(const AttnArgs& a, hipStream_t s) {
   if (bytes > 65536) NHIP_TRY(ensure_dynamic_lds((const void*)attn_rows_kernel<T, DP, SRC>, bytes));
   const uint32_t wgs = (uint32_t)((int64_t)a.batch * a.kv_heads * a.splits * a.row_tiles);
   NHIP_LAUNCH("attention_rows", (attn_rows_kernel<T, DP, SRC>), dim3(wgs), dim3(kWaves * 64), bytes, s, a);
-  NHIP_TRY(check_launch("attention_rows"));
-  if (a.splits == 1) return ok();
-  const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
-  NHIP_LAUNCH("attention_join", attn_join_kernel<T>, dim3((uint32_t)ceil_div(rows, 4)), dim3(256), 0, s, a);
-  return check_launch("attention_join");
+  return check_launch("attention_rows");
+}
+
+}  // namespace attn
+}  // namespace nhip
+
+#include "attn_tiles.h"
+
+namespace nhip {
+namespace attn {
+
+template <class T, int DP, int SRC>
+int launch(const AttnArgs& a, hipStream_t s) {
+  if constexpr (SRC != kSrcAny) {
+    if (a.tiles) return tiles_launch<T, DP, SRC>(a, s);
+  }
+  return rows_launch<T, DP, SRC>(a, s);
 }
 
 template <class T, int SRC>
-int rows_by_dim(const AttnArgs& a, hipStream_t s) {
-  if (a.d <= 64) return rows_launch<T, 64, SRC>(a, s);
-  if (a.d <= 128) return rows_launch<T, 128, SRC>(a, s);
-  return rows_launch<T, 256, SRC>(a, s);
+int launch_by_dim(const AttnArgs& a, hipStream_t s) {
+  if (a.d <= 64) return launch<T, 64, SRC>(a, s);
+  if (a.d <= 128) return launch<T, 128, SRC>(a, s);
+  return launch<T, 256, SRC>(a, s);
 }
 
 template <class T>
 int run(const AttnArgs& a, int src, hipStream_t s) {
-  switch (src) {
-    case kSrcVec: return rows_by_dim<T, kSrcVec>(a, s);
-    case kSrcAny: return rows_by_dim<T, kSrcAny>(a, s);
-    default: return rows_by_dim<T, kSrcInt8>(a, s);
-  }
+  const int st = src == kSrcVec   ? launch_by_dim<T, kSrcVec>(a, s)
+                 : src == kSrcAny ? launch_by_dim<T, kSrcAny>(a, s)
+                                  : launch_by_dim<T, kSrcInt8>(a, s);
+  NHIP_TRY(st);
+  if (a.splits == 1) return ok();
+  const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
+  NHIP_LAUNCH("attention_join", attn_join_kernel<T>, dim3((uint32_t)ceil_div(rows, 4)), dim3(256), 0, s, a);
+  return check_launch("attention_join");
 }
 
 }  // namespace attn

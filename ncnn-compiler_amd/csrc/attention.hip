@@ -8,8 +8,9 @@
 namespace nhip {
 namespace {
 
-// Checks the sizes and fills them in; the number of parts of the keys.
-int attn_args(const nhip_attention_desc* d, AttnArgs* a) {
+// Checks the sizes and fills them in, chooses the kernel (vec: rows that the
+// one for many rows takes) and the number of parts of the keys.
+int attn_args(const nhip_attention_desc* d, bool vec, AttnArgs* a) {
   if (!d) return fail(NHIP_STATUS_NULL_POINTER, "attention: null descriptor");
   if (!elem_size(d->dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "attention: dtype has to be F32, F16 or BF16");
   if (d->batch < 0 || d->queries < 0 || d->keys < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative extent");
@@ -30,20 +31,33 @@ int attn_args(const nhip_attention_desc* d, AttnArgs* a) {
   if (d->keys > most || (int64_t)d->queries * a->group > most)
     return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: at most 2^30 keys, and rows of a key/value head");
   a->rows = d->queries * a->group;
-  a->row_tiles = (int)ceil_div(std::max(a->rows, 1), attn::kRowTile);
-  // few rows: the keys are split until there are two workgroups for every CU,
-  // each part with at least 128 keys
+  a->tiles = vec && a->rows > 64;
+  const int tile = a->tiles ? attn::kTilesRows : attn::kRowTile;
+  a->row_tiles = (int)ceil_div(std::max(a->rows, 1), tile);
+  // few workgroups: the keys are split until there are two for every CU, each
+  // part with at least 128 keys
   const int64_t heads = (int64_t)d->batch * d->kv_heads;
-  if (heads > 0x7fffffff / a->row_tiles) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: too many rows");
+  if (heads > 0x7fffff00 / a->row_tiles) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: too many rows");
   const int64_t wgs = std::max<int64_t>(1, heads * a->row_tiles);
   const int64_t want = std::max<int64_t>(1, 2 * cu_count() / wgs);
   a->splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(d->keys, 128), 64}));
   return ok();
 }
 
-uint64_t attn_workspace(const AttnArgs& a) {
+uint64_t workspace_of(const AttnArgs& a) {
   if (a.splits == 1) return 0;
   return (uint64_t)a.batch * a.kv_heads * a.rows * a.splits * (a.d * sizeof(float) + sizeof(float2));
+}
+
+// The most that a call with this descriptor needs, whatever its strides.
+int attn_workspace(const nhip_attention_desc* d, uint64_t* bytes) {
+  *bytes = 0;
+  for (bool vec : {false, true}) {
+    AttnArgs a{};
+    NHIP_TRY(attn_args(d, vec, &a));
+    *bytes = std::max(*bytes, workspace_of(a));
+  }
+  return ok();
 }
 
 int attn_forward(AttnArgs& a, const nhip_attention_desc* d, int src, const void* query, const int64_t* qs, void* out,
@@ -57,7 +71,7 @@ int attn_forward(AttnArgs& a, const nhip_attention_desc* d, int src, const void*
     if (qs[i] < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative stride");
     a.qs[i] = qs[i];
   }
-  const uint64_t need = attn_workspace(a);
+  const uint64_t need = workspace_of(a);
   if (need) {
     if (!workspace) return fail(NHIP_STATUS_NULL_POINTER, "attention: null workspace");
     if (workspace_bytes < need || !aligned_to(workspace, 16))
@@ -88,10 +102,7 @@ extern "C" {
 
 int nhip_cross_attention_workspace_size(const nhip_attention_desc* desc, uint64_t* bytes) {
   if (!bytes) return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
-  AttnArgs a{};
-  NHIP_TRY(attn_args(desc, &a));
-  *bytes = attn_workspace(a);
-  return ok();
+  return attn_workspace(desc, bytes);
 }
 
 int nhip_cross_attention_forward(const nhip_attention_desc* desc, const void* query, const int64_t* query_strides,
@@ -100,7 +111,7 @@ int nhip_cross_attention_forward(const nhip_attention_desc* desc, const void* qu
                                  int64_t mask_stride, void* out, void* workspace, uint64_t workspace_bytes,
                                  void* stream) {
   AttnArgs a{};
-  NHIP_TRY(attn_args(desc, &a));
+  NHIP_TRY(attn_args(desc, false, &a));
   if (desc->batch == 0 || desc->queries == 0) return ok();
   if (!query || !query_strides || !out || !key_strides || !value_strides || (desc->keys && (!key || !value)))
     return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
@@ -120,15 +131,13 @@ int nhip_cross_attention_forward(const nhip_attention_desc* desc, const void* qu
   a.mask_stride = mask_stride;
   const bool vec = desc->head_dim % (16 / es) == 0 && vec_rows(query, query_strides, es) &&
                    vec_rows(key, key_strides, es) && vec_rows(value, value_strides, es);
+  NHIP_TRY(attn_args(desc, vec, &a));
   return attn_forward(a, desc, vec ? kSrcVec : kSrcAny, query, query_strides, out, workspace, workspace_bytes, stream);
 }
 
 int nhip_kv8_attention_workspace_size(const nhip_attention_desc* desc, const nhip_kv8_cache* cache, uint64_t* bytes) {
   if (!bytes || !cache) return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
-  AttnArgs a{};
-  NHIP_TRY(attn_args(desc, &a));
-  *bytes = attn_workspace(a);
-  return ok();
+  return attn_workspace(desc, bytes);
 }
 
 int nhip_kv8_attention_forward(const nhip_attention_desc* desc, const nhip_kv8_cache* cache, const void* query,
@@ -136,7 +145,7 @@ int nhip_kv8_attention_forward(const nhip_attention_desc* desc, const nhip_kv8_c
                                const int32_t* lengths, int32_t causal, void* out, void* workspace,
                                uint64_t workspace_bytes, void* stream) {
   AttnArgs a{};
-  NHIP_TRY(attn_args(desc, &a));
+  NHIP_TRY(attn_args(desc, true, &a));
   NHIP_TRY(kv8_args(cache, block_table, table_pages, &a.cache));
   if (cache->kv_heads != desc->kv_heads || cache->head_dim != desc->head_dim)
     return fail(NHIP_STATUS_INVALID_SHAPE, "attention: the cache has other heads");

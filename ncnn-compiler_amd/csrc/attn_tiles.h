@@ -1,0 +1,277 @@
+// Attention of many query rows: 128 rows to a workgroup, 32 to a wave, tiles
+// of keys and values staged in LDS for all of them.  (Included by attention.h.)
+
+namespace nhip {
+namespace attn {
+
+// Sizes of the kernel for channels padded to DP.
+template <class T, int DP, int SRC>
+struct TilesShape {
+  typedef typename Second<T, SRC>::type P;
+  static constexpr int KT = DP == 256 ? 32 : 64;                        // keys of a tile: two buffers fit the LDS, one the registers
+  static constexpr int E = SRC == kSrcInt8 ? 16 : 16 / (int)sizeof(T);  // channels of a 16-byte load
+  static constexpr int L = KT * DP / E / (kWaves * 64);                 // loads of a thread, keys and values each
+  // Rows padded so that the eight rows of a 16-byte read, and the four of a
+  // transposing read, lie in different banks.
+  static constexpr int SK = DP + 16 / (int)sizeof(T);
+  static constexpr int SV = DP + (sizeof(P) == 2 ? 32 : 8);
+  static constexpr int kbytes = KT * SK * (int)sizeof(T), vbytes = KT * SV * (int)sizeof(P);
+  static constexpr int bytes = 2 * (kbytes + vbytes);
+};
+
+// The next tile on its way, spread over the workgroup.
+template <class T, int DP, int SRC>
+struct TilesLoad {
+  typedef TilesShape<T, DP, SRC> S;
+  typedef typename S::P P;
+  int4 k[S::L], v[S::L];
+  __device__ __forceinline__ void load(const AttnArgs& a, const T* kbase, const T* vbase, const TileKeys& keys, int kvh, int key0, int wave, int lane) {
+    constexpr int per = DP / S::E;
+#pragma unroll
+    for (int i = 0; i < S::L; ++i) {
+      const int first = (wave * 64 + i * kWaves * 64) / per;  // a wave's 64 pieces lie inside 16 rows of a page
+      const int at = wave * 64 + lane + i * kWaves * 64, r = at / per, c = at % per * S::E;
+      const int64_t page = SRC == kSrcInt8 ? lane_page(keys, first & ~15) : 0;
+      const bool on = keys.counts >> r & 1;
+      k[i] = load_row16<T, SRC>(a, kbase, a.ks[1], a.cache.k, kvh, page, key0, r, c, on);
+      v[i] = load_row16<T, SRC>(a, vbase, a.vs[1], a.cache.v, kvh, page, key0, r, c, on);
+    }
+  }
+  __device__ __forceinline__ void store(char* lds, int wave, int lane) const {
+    constexpr int per = DP / S::E;
+#pragma unroll
+    for (int i = 0; i < S::L; ++i) {
+      const int at = wave * 64 + lane + i * kWaves * 64, r = at / per, c = at % per * S::E;
+      T* kt = reinterpret_cast<T*>(lds) + r * S::SK + c;
+      P* vt = reinterpret_cast<P*>(lds + S::kbytes) + r * S::SV + c;
+      if constexpr (SRC == kSrcInt8) {
+        *reinterpret_cast<typename Frag<T>::type*>(kt) = codes8<T>(k[i].x, k[i].y);
+        *reinterpret_cast<typename Frag<T>::type*>(kt + 8) = codes8<T>(k[i].z, k[i].w);
+        *reinterpret_cast<typename Frag<P>::type*>(vt) = codes8<P>(v[i].x, v[i].y);
+        *reinterpret_cast<typename Frag<P>::type*>(vt + 8) = codes8<P>(v[i].z, v[i].w);
+      } else {
+        *reinterpret_cast<int4*>(kt) = k[i];
+        *reinterpret_cast<int4*>(vt) = v[i];
+      }
+    }
+  }
+};
+
+// A lane's eight summed values down channel c0 + (l & 31) of V in LDS: keys
+// 8 u + 4 h .. + 3 for u = 0, 1 (h = lane / 32), as eight of a score tile's
+// sums lie in a lane.
+template <class T, int STRIDE>
+__device__ __forceinline__ typename Frag<T>::type load_v32(const T* tile, int c0, int lane) {
+  const int h = lane >> 5;
+  typename Frag<T>::type f;
+  if constexpr (sizeof(T) == 2) {
+    const int j = lane & 15;
+    const T* at = tile + (4 * h + (j >> 2)) * STRIDE + c0 + (lane & 16) + (j & 3) * 4;
+    typedef __attribute__((address_space(3))) v4s lds4;
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at);
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(at + 8 * STRIDE));
+    f = __builtin_bit_cast(typename Frag<T>::type, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = tile[(8 * (i >> 2) + 4 * h + (i & 3)) * STRIDE + c0 + (lane & 31)];
+  }
+  return f;
+}
+
+// One workgroup: kTilesRows query rows of one key/value head over one part of
+// the keys.  Scores, probabilities and sums stay in registers from one product
+// to the other; while a tile is worked on, the next one's loads are under way,
+// and it goes into the other of two LDS buffers: one barrier a tile.
+template <class T, int DP, int SRC>
+__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void attn_tiles_kernel(AttnArgs a, uint32_t wgs) {
+  typedef TilesShape<T, DP, SRC> S;
+  typedef typename S::P P;
+  typedef typename Frag<T>::type FT;
+  typedef typename Frag<P>::type FP;
+  constexpr int KT = S::KT, NT = KT / 32, KS = DP / 16, DT = DP / 32, PARTS = Second<T, SRC>::parts;
+  extern __shared__ char lds[];
+  const int lane = threadIdx.x & 63, wave = wave_id(), h = lane >> 5, col = lane & 31;
+  // workgroups go to the eight dies in turn: each die gets a run of them, so
+  // that those of one head meet in its L2
+  uint32_t at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (at >= wgs) return;
+  const int rt = at % a.row_tiles;
+  at /= a.row_tiles;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int kvh = at % a.kv_heads, b = at / a.kv_heads;
+
+  const int length = a.lengths ? max(0, min(a.lengths[b], a.keys)) : a.keys;
+  const int row = rt * kTilesRows + wave * 32 + col;
+  const int qi = row / a.group, head = kvh * a.group + row % a.group;
+  int sees = length, all_see = length, visible = length, begin, end;
+  if (a.causal) {
+    const int last = min(rt * kTilesRows + kTilesRows - 1, a.rows - 1) / a.group;
+    const int first = (rt * kTilesRows + wave * 32) / a.group;
+    sees = max(0, length - a.queries + 1 + qi);
+    all_see = max(0, length - a.queries + 1 + first);
+    visible = max(0, min(length, length - a.queries + 1 + last));
+  }
+  part_of(a, length, visible, split, KT, begin, end);
+
+  FT qf[KS];
+  const T* qrow = (const T*)a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    qf[s] = row < a.rows ? load_q<T, true>(qrow, s * 16 + h * 8, a.d) : zero_frag<T>();
+    if (a.scale_log2 < 0.f) qf[s] = -qf[s];
+  }
+
+  v16f acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  bool seen = false;
+  const T* kbase = (const T*)a.k + b * a.ks[0] + kvh * a.ks[2];
+  const T* vbase = (const T*)a.v + b * a.vs[0] + kvh * a.vs[2];
+
+  if (begin < end) {
+    TilesLoad<T, DP, SRC> next;
+    TileKeys keys = know_tile<SRC, KT>(a, ask_tile<SRC, KT>(a, b, begin, lane), kvh, begin, end, lane);
+    next.load(a, kbase, vbase, keys, kvh, begin, wave, lane);
+    TileAsk ask = ask_tile<SRC, KT>(a, b, min(begin + KT, a.keys), lane);
+    next.store(lds, wave, lane);
+    __syncthreads();
+    int buf = 0;
+    for (int key0 = begin; key0 < end; key0 += KT) {
+      // the next tile (past the end: nothing counts, nothing is read)
+      const int key1 = min(key0 + KT, a.keys);
+      const TileKeys soon = know_tile<SRC, KT>(a, ask, kvh, key0 + KT, end, lane);
+      next.load(a, kbase, vbase, soon, kvh, key1, wave, lane);
+      ask = ask_tile<SRC, KT>(a, b, min(key1 + KT, a.keys), lane);
+
+      const T* kt = reinterpret_cast<const T*>(lds + buf * (S::kbytes + S::vbytes));
+      const P* vt = reinterpret_cast<const P*>(lds + buf * (S::kbytes + S::vbytes) + S::kbytes);
+      v16f s[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+          s[t] = mma32(*reinterpret_cast<const FT*>(kt + (t * 32 + col) * S::SK + i * 16 + h * 8), qf[i], s[t]);
+      }
+      if constexpr (NT == 2)
+        settle(s[0], s[1]);
+      else
+        settle(s[0]);
+
+      // over the cache: scores in units of ln 2, a page's scale included; else
+      // the factor goes into the exponent
+      if constexpr (SRC == kSrcInt8) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[t][i] *= fabsf(a.scale_log2) * lane_float(keys.kscale, t * 32 + (i >> 3) * 16);
+      }
+      // (of a scale of 0, too, -infinity stays what it is)
+      const float factor = SRC == kSrcInt8 ? 1.f : fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
+      constexpr uint64_t every = KT == 64 ? ~0ull : 0xffffffffull;
+      const bool whole = (keys.counts & every) == every && key0 + KT <= all_see;  // uniform
+      uint64_t on = every;
+      if (!whole) {
+        const int n = min(max(sees - key0, 0), KT);
+        on = keys.counts & (n >= 64 ? ~0ull : (1ull << n) - 1);
+        const uint64_t mine = on >> (4 * h);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!(mine >> (t * 32 + (i >> 2) * 8 + (i & 3)) & 1)) s[t][i] = -INFINITY;
+      }
+      seen |= on != 0;
+      // The reference point of the exponent need not be the row's maximum: it
+      // moves only where a score lies more than 8 above it (probabilities up
+      // to 2^8, sums in fp32), which spares most tiles the scaling of the sums.
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+      top = max32(top);
+      top *= factor;
+      if (__any(top > m + 8.f)) {
+        const float to = fmaxf(m, top);
+        const float keep = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= keep;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[t][i] *= keep;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      FP pf[NT][2][PARTS];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[t][i], factor, -base));
+          l += p;
+          if constexpr (SRC == kSrcInt8) p *= lane_float(keys.vscale, t * 32 + (i >> 3) * 16);
+          pf[t][i >> 3][0][i & 7] = (P)p;
+          if constexpr (PARTS == 2) pf[t][i >> 3][1][i & 7] = (P)(p - (float)pf[t][i >> 3][0][i & 7]);
+        }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c = 0; c < DT; ++c) {
+            const FP vf = load_v32<P, S::SV>(vt + (t * 32 + u * 16) * S::SV, c * 32, lane);
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) acc[c] = mma32(vf, pf[t][u][i], acc[c]);
+          }
+      buf ^= 1;
+      next.store(lds + buf * (S::kbytes + S::vbytes), wave, lane);
+      keys = soon;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) settle(acc[t]);
+  }
+  l += __shfl_xor(l, 32);
+  if (l != l) m = INFINITY;                         // NaN to whoever joins this
+  else if (m == -INFINITY) l = seen ? -1.f : 0.f;  // scores of -infinity alone: 0 / 0, told from a row that sees nothing
+  if (row >= a.rows) return;
+  const int64_t prow = (((int64_t)b * a.kv_heads + kvh) * a.rows + row) * a.splits + split;
+  float* part = a.part_o + prow * a.d;
+  T* out = (T*)a.o + (((int64_t)b * a.queries + qi) * a.heads + head) * a.d;
+  const float scale = m == -INFINITY ? (l < 0.f ? NAN : 0.f) : 1.f / l;
+  if (a.splits > 1 && h == 0) a.part_ml[prow] = make_float2(m, l);
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int c = t * 32 + (i >> 2) * 8 + 4 * h;
+      if (c < a.d) {
+        float o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = a.splits > 1 ? acc[t][i + j] : acc[t][i + j] * scale;
+        if (a.splits > 1)
+          *reinterpret_cast<v4f*>(part + c) = v4f{o[0], o[1], o[2], o[3]};
+        else
+          Vec<T, 4>::store(out + c, o);
+      }
+    }
+}
+
+template <class T, int DP, int SRC>
+int tiles_launch(const AttnArgs& a, hipStream_t s) {
+  constexpr int bytes = TilesShape<T, DP, SRC>::bytes;
+  static_assert(bytes <= 160 * 1024, "two tiles fit the LDS");
+  if (bytes > 65536) NHIP_TRY(ensure_dynamic_lds((const void*)attn_tiles_kernel<T, DP, SRC>, bytes));
+  const uint32_t wgs = (uint32_t)((int64_t)a.batch * a.kv_heads * a.splits * a.row_tiles);
+  NHIP_LAUNCH("attention_tiles", (attn_tiles_kernel<T, DP, SRC>), dim3((wgs + 7) / 8 * 8), dim3(kWaves * 64), bytes, s, a, wgs);
+  return check_launch("attention_tiles");
+}
+
+}  // namespace attn
+}  // namespace nhip
