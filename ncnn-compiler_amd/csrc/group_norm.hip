@@ -30,8 +30,10 @@ namespace nhip {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kOneThreads = 512;   // of a workgroup that does its groups alone
 constexpr int kMaxChannels = 4096;
-constexpr int kMaxChunks = 128;  // parts of an image: what each workgroup of the second pass merges
+constexpr int kMaxChunks = 256;  // parts of an image: what each workgroup of the second pass merges
+constexpr int kDeep = 4;         // vectors of a thread under way at once
 constexpr int kTile = 64;        // pixels and channels of a transposed tile (blobs)
 
 struct NormArgs {
@@ -41,7 +43,7 @@ struct NormArgs {
   const float* affine;
   int64_t pixels, image_stride, row_stride;
   int channels, groups, cpg, act;
-  int chunks;           // of an image
+  int chunks;           // of an image; 0: one launch
   int64_t chunk;        // pixels of a chunk (the last may have fewer)
   float eps;
 };
@@ -55,9 +57,10 @@ __device__ __forceinline__ float activate(float y) {
 
 // Lanes of a wave that share one group: a power of two, so that their sums
 // are butterflies inside the wave.
+template <int TH>
 __device__ __forceinline__ int team_of(int groups) {
   int t = 64;
-  while (t > 1 && (kThreads / t) < groups) t >>= 1;
+  while (t > 1 && (TH / t) < groups) t >>= 1;
   return t;
 }
 template <class S>
@@ -91,7 +94,7 @@ __device__ __forceinline__ double2 moments(double s1, float s2, float shift, dou
 // Merges the chunks of image `n` for groups [g0, g1): mean and 1/sqrt(var + eps)
 // to stat[g - g0].
 __device__ void merge_chunks(const NormArgs& a, int n, int g0, int g1, float2* stat) {
-  const int team = team_of(g1 - g0), lane = threadIdx.x & (team - 1);
+  const int team = team_of<kThreads>(g1 - g0), lane = threadIdx.x & (team - 1);
   const double2* part = a.part + (int64_t)n * a.chunks * a.groups;
   const double last = (double)(a.pixels - (int64_t)(a.chunks - 1) * a.chunk), total = (double)a.pixels;
   for (int gb = g0; gb < g1; gb += kThreads / team) {  // uniform: all lanes of a team stay in the butterflies
@@ -112,37 +115,48 @@ __device__ void merge_chunks(const NormArgs& a, int n, int g0, int g1, float2* s
   }
 }
 
-// Statistics of one chunk of one image, channels last.  A thread keeps its V
-// channels and walks pixels; channels are merged into groups through LDS.
-template <class T, int V>
-__global__ __launch_bounds__(kThreads) void norm_stats_tokens_kernel(NormArgs a) {
+// Means and squared deviations of channels [c0, c0 + cn) over pixels [p0, p1)
+// of one image (x: its first pixel), channels last, to ch[0, cn).  A thread
+// keeps its V channels and walks pixels; `red` holds the threads' sums: those
+// of a channel are added by as many threads as there are for it, then by one.
+template <class T, int V, int TH>
+__device__ void channel_moments(const NormArgs& a, const T* x, int c0, int cn, int64_t p0, int64_t p1, double2* ch, void* red) {
   typedef typename First<T>::type S;
-  extern __shared__ double2 lds[];  // [channels] mean, deviations; then [threads][V] first, [threads][V] second sums
-  S* red1 = reinterpret_cast<S*>(lds + a.channels);
-  float* red2 = reinterpret_cast<float*>(red1 + kThreads * V);
-  const int n = blockIdx.x / a.chunks, k = blockIdx.x % a.chunks;
-  const int64_t p0 = (int64_t)k * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
-  const T* x = (const T*)a.x + n * a.image_stride;
-  const int vecs = a.channels / V;
-  const double count = (double)(p1 - p0);
-  for (int v0 = 0; v0 < vecs; v0 += kThreads) {
-    const int cols = min(kThreads, vecs - v0), rows = kThreads / cols;
+  S* red1 = reinterpret_cast<S*>(red);
+  S* more1 = red1 + TH * V;
+  float* red2 = reinterpret_cast<float*>(more1 + TH);
+  float* more2 = red2 + TH * V;
+  const int vecs = cn / V;
+  for (int v0 = 0; v0 < vecs; v0 += TH) {
+    const int cols = min(TH, vecs - v0), rows = TH / cols;
     const int col = threadIdx.x % cols, row = threadIdx.x / cols;
     S s1[V] = {};
     float s2[V] = {}, shift[V];
     if (row < rows) {
-      const T* px = x + (int64_t)(v0 + col) * V;
+      const T* px = x + c0 + (int64_t)(v0 + col) * V;
       Vec<T, V>::load(px + p0 * a.row_stride, shift);
-#pragma unroll 4
-      for (int64_t p = p0 + row; p < p1; p += rows) {
-        float t[V];
-        Vec<T, V>::load(px + p * a.row_stride, t);
+      const auto add = [&](const float(&t)[V]) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float d = t[i] - shift[i];
           s1[i] += first_power(t[i], d, S());
           s2[i] = fmaf(d, d, s2[i]);
         }
+      };
+      const int64_t step = rows * a.row_stride;
+      int64_t p = p0 + row;
+      const T* at = px + p * a.row_stride;
+      for (; p + (kDeep - 1) * rows < p1; p += kDeep * rows, at += kDeep * step) {
+        float t[kDeep][V];
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) Vec<T, V>::load(at + u * step, t[u]);
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) add(t[u]);
+      }
+      for (; p < p1; p += rows, at += step) {
+        float t[V];
+        Vec<T, V>::load(at, t);
+        add(t);
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -151,87 +165,162 @@ __global__ __launch_bounds__(kThreads) void norm_stats_tokens_kernel(NormArgs a)
       }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < cols * V; c += kThreads) {
+    const int cv = cols * V, parts = max(1, TH / cv);
+    for (int i = threadIdx.x; i < cv * parts; i += TH) {  // parts > 1: one step
+      const int c = i % cv;
       S u1 = 0;
       float u2 = 0.f;
-      for (int r = 0; r < rows; ++r) {
-        u1 += red1[r * cols * V + c];
-        u2 += red2[r * cols * V + c];
+      for (int r = i / cv; r < rows; r += parts) {
+        u1 += red1[r * cv + c];
+        u2 += red2[r * cv + c];
       }
-      lds[v0 * V + c] = moments(u1, u2, (float)x[p0 * a.row_stride + v0 * V + c], count);
+      if (parts == 1) {
+        ch[v0 * V + c] = moments(u1, u2, (float)x[p0 * a.row_stride + c0 + v0 * V + c], (double)(p1 - p0));
+      } else {
+        more1[i] = u1;
+        more2[i] = u2;
+      }
     }
     __syncthreads();
+    if (parts > 1) {  // uniform
+      if (threadIdx.x < cv) {
+        S u1 = 0;
+        float u2 = 0.f;
+        for (int q = 0; q < parts; ++q) {
+          u1 += more1[q * cv + threadIdx.x];
+          u2 += more2[q * cv + threadIdx.x];
+        }
+        ch[v0 * V + threadIdx.x] = moments(u1, u2, (float)x[p0 * a.row_stride + c0 + v0 * V + threadIdx.x], (double)(p1 - p0));
+      }
+      __syncthreads();
+    }
   }
-  const int team = team_of(a.groups), lane = threadIdx.x & (team - 1);
-  for (int gb = 0; gb < a.groups; gb += kThreads / team) {
+}
+
+// Merges channels of `count` values each into `groups` groups: calls
+// done(group, mean, squared deviations) in one lane for each.
+template <int TH, class F>
+__device__ __forceinline__ void merge_channels(const NormArgs& a, const double2* ch, int groups, double count, F done) {
+  const int team = team_of<TH>(groups), lane = threadIdx.x & (team - 1);
+  for (int gb = 0; gb < groups; gb += TH / team) {
     const int g = gb + threadIdx.x / team;
-    const bool in = g < a.groups;
-    const double2* ch = lds + g * a.cpg;
+    const bool in = g < groups;
+    const double2* of = ch + g * a.cpg;
     double m = 0.0;
-    for (int c = lane; in && c < a.cpg; c += team) m += ch[c].x;
+    for (int c = lane; in && c < a.cpg; c += team) m += of[c].x;
     m = team_sum(m, team) / a.cpg;
     double v = 0.0;
     for (int c = lane; in && c < a.cpg; c += team) {
-      const double d = ch[c].x - m;
-      v += ch[c].y + count * d * d;
+      const double d = of[c].x - m;
+      v += of[c].y + count * d * d;
     }
     v = team_sum(v, team);
-    if (in && lane == 0) a.part[(int64_t)blockIdx.x * a.groups + g] = make_double2(m, v);
+    if (in && lane == 0) done(g, m, v);
   }
 }
 
-template <class T, int V, int ACT>
-__global__ __launch_bounds__(kThreads) void norm_apply_tokens_kernel(NormArgs a) {
-  extern __shared__ float2 stats[];  // [groups]
-  const int n = blockIdx.x / a.chunks, k = blockIdx.x % a.chunks;
-  merge_chunks(a, n, 0, a.groups, stats);
-  __syncthreads();
-  const int64_t p0 = (int64_t)k * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
-  const T* x = (const T*)a.x + n * a.image_stride;
-  T* y = (T*)a.y + n * a.pixels * a.channels;
-  const int vecs = a.channels / V;
-  for (int v0 = 0; v0 < vecs; v0 += kThreads) {
-    const int cols = min(kThreads, vecs - v0), rows = kThreads / cols;
+// y of channels [c0, c0 + cn) over pixels [p0, p1), channels last; stat: of
+// the groups from the one that c0 begins.
+template <class T, int V, int ACT, int TH>
+__device__ void apply_tokens(const NormArgs& a, const T* x, T* y, int c0, int cn, int64_t p0, int64_t p1, const float2* stat) {
+  const int vecs = cn / V;
+  for (int v0 = 0; v0 < vecs; v0 += TH) {
+    const int cols = min(TH, vecs - v0), rows = TH / cols;
     const int col = threadIdx.x % cols, row = threadIdx.x / cols;
     if (row >= rows) continue;
-    const int c0 = (v0 + col) * V;
+    const int c = (v0 + col) * V;
     float mean[V], scale[V], beta[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float2 s = stats[(c0 + i) / a.cpg];
+      const float2 s = stat[(c + i) / a.cpg];
       mean[i] = s.x;
-      scale[i] = s.y * a.affine[c0 + i];
-      beta[i] = a.affine[a.channels + c0 + i];
+      scale[i] = s.y * a.affine[c0 + c + i];
+      beta[i] = a.affine[a.channels + c0 + c + i];
     }
-#pragma unroll 4
-    for (int64_t p = p0 + row; p < p1; p += rows) {
-      float t[V];
-      Vec<T, V>::load(x + p * a.row_stride + c0, t);
+    const auto result = [&](float(&t)[V]) {
 #pragma unroll
       for (int i = 0; i < V; ++i) t[i] = activate<ACT>(fmaf(t[i] - mean[i], scale[i], beta[i]));
-      Vec<T, V>::store(y + p * a.channels + c0, t);
+    };
+    const int64_t in = rows * a.row_stride, out = (int64_t)rows * a.channels;
+    int64_t p = p0 + row;
+    const T* from = x + p * a.row_stride + c0 + c;
+    T* to = y + p * a.channels + c0 + c;
+    for (; p + (kDeep - 1) * rows < p1; p += kDeep * rows, from += kDeep * in, to += kDeep * out) {
+      float t[kDeep][V];
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) Vec<T, V>::load(from + u * in, t[u]);
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        result(t[u]);
+        Vec<T, V>::store(to + u * out, t[u]);
+      }
+    }
+    for (; p < p1; p += rows, from += in, to += out) {
+      float t[V];
+      Vec<T, V>::load(from, t);
+      result(t);
+      Vec<T, V>::store(to, t);
     }
   }
 }
 
-// Statistics of one chunk of pixels of one group, channels first.
+// Statistics of one chunk of one image, channels last.
 template <class T, int V>
-__global__ __launch_bounds__(kThreads) void norm_stats_blobs_kernel(NormArgs a) {
-  typedef typename First<T>::type S;
-  __shared__ S red1[kThreads / 64];
-  __shared__ float red2[kThreads / 64];
-  const int g = blockIdx.x % a.groups, nk = blockIdx.x / a.groups;
-  const int n = nk / a.chunks, k = nk % a.chunks;
+__global__ __launch_bounds__(kThreads) void norm_stats_tokens_kernel(NormArgs a) {
+  extern __shared__ double2 lds[];  // [channels] mean, deviations; then the threads' sums
+  const int n = blockIdx.x / a.chunks, k = blockIdx.x % a.chunks;
   const int64_t p0 = (int64_t)k * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
-  const T* x = (const T*)a.x + n * a.image_stride + (int64_t)g * a.cpg * a.row_stride;
+  channel_moments<T, V, kThreads>(a, (const T*)a.x + n * a.image_stride, 0, a.channels, p0, p1, lds, lds + a.channels);
+  merge_channels<kThreads>(a, lds, a.groups, (double)(p1 - p0),
+                 [&](int g, double m, double v) { a.part[(int64_t)blockIdx.x * a.groups + g] = make_double2(m, v); });
+}
+
+// Result of `each` groups over `run` chunks of pixels.
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kThreads) void norm_apply_tokens_kernel(NormArgs a, int each, int run, int runs) {
+  extern __shared__ float2 stats[];  // [each]
+  const int k = blockIdx.x % runs, rest = blockIdx.x / runs;
+  const int g0 = rest % (a.groups / each) * each, n = rest / (a.groups / each);
+  merge_chunks(a, n, g0, g0 + each, stats);
+  __syncthreads();
+  const int64_t p0 = (int64_t)k * run * a.chunk, p1 = min(p0 + run * a.chunk, a.pixels);
+  apply_tokens<T, V, ACT, kThreads>(a, (const T*)a.x + n * a.image_stride, (T*)a.y + n * a.pixels * a.channels,
+                                    g0 * a.cpg, each * a.cpg, p0, p1, stats);
+}
+
+// Small images in one launch: a workgroup does a few whole groups of an
+// image, statistics and result.
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kOneThreads) void norm_one_tokens_kernel(NormArgs a, int groups) {
+  extern __shared__ double2 lds[];  // [channels of the groups]; then the threads' sums, and in their place the statistics
+  const int parts = a.groups / groups, n = blockIdx.x / parts, g0 = blockIdx.x % parts * groups;
+  const T* x = (const T*)a.x + n * a.image_stride;
+  const int cn = groups * a.cpg;
+  channel_moments<T, V, kOneThreads>(a, x, g0 * a.cpg, cn, 0, a.pixels, lds, lds + cn);
+  float2* stats = reinterpret_cast<float2*>(lds + cn);
+  const double all = (double)a.pixels * a.cpg, eps = a.eps;
+  merge_channels<kOneThreads>(a, lds, groups, (double)a.pixels,
+                 [&](int g, double m, double v) { stats[g] = make_float2((float)m, (float)(1.0 / sqrt(v / all + eps))); });
+  __syncthreads();
+  apply_tokens<T, V, ACT, kOneThreads>(a, x, (T*)a.y + n * a.pixels * a.channels, g0 * a.cpg, cn, 0, a.pixels, stats);
+}
+
+// Mean and squared deviations of pixels [p0, p1) of one group's channels,
+// channels first (x: the group's first channel); valid in thread 0.
+template <class T, int V, int TH>
+__device__ double2 group_moments(const NormArgs& a, const T* x, int64_t p0, int64_t p1) {
+  typedef typename First<T>::type S;
+  __shared__ S red1[TH / 64];
+  __shared__ float red2[TH / 64];
   const float shift = (float)x[p0];
   const int vecs = (int)((p1 - p0) / V);
   S s1 = 0;
   float s2 = 0.f;
-  const int lanes = min(kThreads, (vecs + 63) / 64 * 64);
-  const int rows = kThreads / lanes, row = threadIdx.x / lanes, col = threadIdx.x % lanes;
+  const int lanes = min(TH, (vecs + 63) / 64 * 64);
+  const int rows = TH / lanes, row = threadIdx.x / lanes, col = threadIdx.x % lanes;
   if (row < rows)
     for (int c = row; c < a.cpg; c += rows)
+#pragma unroll 4
       for (int v = col; v < vecs; v += lanes) {
         float t[V];
         Vec<T, V>::load(x + c * a.row_stride + p0 + (int64_t)v * V, t);
@@ -249,14 +338,42 @@ __global__ __launch_bounds__(kThreads) void norm_stats_blobs_kernel(NormArgs a) 
     red2[threadIdx.x / 64] = s2;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    S u1 = 0;
-    float u2 = 0.f;
-    for (int i = 0; i < kThreads / 64; ++i) {
-      u1 += red1[i];
-      u2 += red2[i];
-    }
-    a.part[(int64_t)nk * a.groups + g] = moments(u1, u2, shift, (double)(p1 - p0) * a.cpg);
+  S u1 = 0;
+  float u2 = 0.f;
+  for (int i = 0; i < TH / 64; ++i) {
+    u1 += red1[i];
+    u2 += red2[i];
+  }
+  return moments(u1, u2, shift, (double)(p1 - p0) * a.cpg);
+}
+
+// Statistics of one chunk of pixels of one group, channels first.
+template <class T, int V>
+__global__ __launch_bounds__(kThreads) void norm_stats_blobs_kernel(NormArgs a) {
+  const int g = blockIdx.x % a.groups, nk = blockIdx.x / a.groups;
+  const int n = nk / a.chunks, k = nk % a.chunks;
+  const int64_t p0 = (int64_t)k * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
+  const double2 m = group_moments<T, V, kThreads>(a, (const T*)a.x + n * a.image_stride + (int64_t)g * a.cpg * a.row_stride, p0, p1);
+  if (threadIdx.x == 0) a.part[(int64_t)nk * a.groups + g] = m;
+}
+
+// Small images in one launch, channels first: a workgroup does one group of
+// an image.  Lanes run along the group's channels, then pixels: results leave
+// in pieces of a group's channels, values come in runs of 64 / channels pixels.
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kOneThreads) void norm_one_blobs_kernel(NormArgs a, FastDiv by_cpg) {
+  const int g = blockIdx.x % a.groups, n = blockIdx.x / a.groups;
+  const T* x = (const T*)a.x + n * a.image_stride + (int64_t)g * a.cpg * a.row_stride;
+  T* y = (T*)a.y + n * a.pixels * a.channels + g * a.cpg;
+  const double2 s = group_moments<T, V, kOneThreads>(a, x, 0, a.pixels);
+  const float mean = (float)s.x, rstd = (float)(1.0 / sqrt(s.y / ((double)a.pixels * a.cpg) + (double)a.eps));
+  const int all = (int)a.pixels * a.cpg;
+  const float* gamma = a.affine + g * a.cpg;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < all; i += kOneThreads) {
+    const int p = fdiv(i, by_cpg), c = i - p * a.cpg;
+    const float v = (float)x[c * a.row_stride + p];
+    y[(int64_t)p * a.channels + c] = (T)activate<ACT>(fmaf(v - mean, rstd * gamma[c], gamma[a.channels + c]));
   }
 }
 
@@ -287,18 +404,40 @@ __global__ __launch_bounds__(kThreads) void norm_apply_blobs_kernel(NormArgs a, 
     y[(int64_t)p * a.channels + lane] = (T)activate<ACT>(fmaf(tile[lane][p] - s.x, scale, beta));
 }
 
-// Chunks of an image: enough workgroups for four to a CU, each of at least
-// 8192 values, and few enough to be merged by every workgroup of the second
-// pass.
+// Groups that one workgroup of the single launch does: those whose channels
+// fill 64 bytes of a pixel (tokens), one (blobs).  0: two launches.
+//
+// One launch spares the second's 4 us where the call is bound by launches; but
+// a workgroup walks its groups' pixels alone.  Measured, us a call (two
+// launches / one): tokens of 50 KB to a workgroup 11.8 / 9.0 (784 x 512 bf16)
+// and 12.8 / 8.2 (fp32), of 200 KB 12.7 / 13.1 (fp32) and 11.5 / 17.4 (bf16);
+// blobs of 3136 values 12 / 8, of 12544 12.0 / 10.2, of 25088 12.4 / 16.3.
+int groups_of_one(int channels, int groups, int layout, int es, int64_t n, int64_t pixels) {
+  const int cpg = channels / groups;
+  int each = 1;
+  if (layout == NHIP_LAYOUT_TOKENS)
+    while (each * cpg * es < 64 && groups % (2 * each) == 0) each *= 2;
+  const int64_t values = pixels * each * cpg;
+  const int force = setting_int("NHIP_NORM_ONE", -1);
+  if (force == 0 || values > (1 << 28) || n * (groups / each) > 0x7fffffff) return 0;
+  return force == 1 || (layout == NHIP_LAYOUT_TOKENS ? values * es <= 65536 : values <= 16384) ? each : 0;
+}
+
+// Chunks of an image: enough workgroups for two to a CU (tokens) or four
+// (blobs, smaller ones), each of at least 8192 values, and few enough to be
+// merged by every workgroup of the second pass.  Tokens, us a call at 2 / 3 / 4
+// to a CU: 32 x 3136 x 256 bf16 32.7 / 33.7 / 34.7, 8 x 50175 x 320 f16 172 /
+// 180 / 179; one image of 12544 x 320 fp32 in 128 / 256 / 512 chunks 23.6 /
+// 19.8 / 25.4.
 void chunks_of(int channels, int64_t n, int64_t pixels, int per_image, NormArgs* a) {
-  const int64_t want = ceil_div((int64_t)4 * cu_count(), n * per_image);
+  const int64_t want = ceil_div((int64_t)(per_image == 1 ? 2 : 4) * cu_count(), n * per_image);
   const int64_t fit = std::max<int64_t>(1, pixels * channels / per_image / 8192);
   int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({want, fit, (int64_t)kMaxChunks, pixels}));
   a->chunk = round_up(ceil_div(pixels, chunks), 8);  // whole vectors along the pixels (blobs)
   a->chunks = (int)ceil_div(pixels, a->chunk);
 }
 
-int norm_args(const nhip_norm_plan* p, int32_t dtype, int32_t layout, int32_t n, int64_t pixels, NormArgs* a) {
+int norm_args(const nhip_norm_plan* p, int32_t dtype, int32_t layout, int32_t n, int64_t pixels, NormArgs* a, int* one) {
   if (!p) return fail(NHIP_STATUS_NULL_POINTER, "group norm: null plan");
   if (!elem_size(dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "group norm: dtype has to be F32, F16 or BF16");
   if (layout != NHIP_LAYOUT_TOKENS && layout != NHIP_LAYOUT_BLOBS)
@@ -313,7 +452,8 @@ int norm_args(const nhip_norm_plan* p, int32_t dtype, int32_t layout, int32_t n,
   a->act = p->act;
   a->eps = p->eps;
   a->affine = p->affine;
-  if (n && pixels) {
+  *one = n && pixels ? groups_of_one(p->channels, p->groups, layout, elem_size(dtype), n, pixels) : 0;
+  if (n && pixels && !*one) {
     chunks_of(p->channels, n, pixels, layout == NHIP_LAYOUT_BLOBS ? p->groups : 1, a);
     const int64_t wgs = std::max<int64_t>((int64_t)n * a->chunks * p->groups,
                                           ceil_div(pixels, kTile) * ceil_div(p->channels, kTile) * n);
@@ -328,28 +468,63 @@ int norm_apply(const NormArgs& a, int layout, int n, bool vec, hipStream_t s) {
     const int pt = (int)ceil_div(a.pixels, kTile), ct = (int)ceil_div(a.channels, kTile);
     NHIP_LAUNCH("group_norm_apply", (norm_apply_blobs_kernel<T, ACT>), dim3((uint32_t)((int64_t)pt * ct * n)),
                 dim3(kThreads), 0, s, a, pt, ct);
-  } else if (vec) {
-    NHIP_LAUNCH("group_norm_apply", (norm_apply_tokens_kernel<T, kVec<T>, ACT>), dim3((uint32_t)(n * a.chunks)),
-                dim3(kThreads), a.groups * sizeof(float2), s, a);
   } else {
-    NHIP_LAUNCH("group_norm_apply", (norm_apply_tokens_kernel<T, 1, ACT>), dim3((uint32_t)(n * a.chunks)),
-                dim3(kThreads), a.groups * sizeof(float2), s, a);
+    // Many chunks to merge: a workgroup takes fewer groups (of 256 bytes of a
+    // pixel at least) and as many more chunks.  us a call without / with this:
+    // 4 x 4096 x 320 bf16 (128 chunks) 22.6 / 19.0, 1 x 12544 x 320 fp32 (256)
+    // 27.5 / 19.8; of 64 chunks 8 x 50175 x 320 172 / 180.
+    constexpr int V = kVec<T>;
+    int each = a.groups;
+    if (a.chunks > 64)
+      while (each % 2 == 0 && each / 2 * a.cpg * (int)sizeof(T) >= 256 && (!vec || each / 2 * a.cpg % V == 0)) each /= 2;
+    const int run = a.groups / each, runs = (int)ceil_div(a.chunks, run);
+    const dim3 grid((uint32_t)((int64_t)n * runs * run));
+    if (vec)
+      NHIP_LAUNCH("group_norm_apply", (norm_apply_tokens_kernel<T, V, ACT>), grid, dim3(kThreads), each * sizeof(float2), s, a,
+                  each, run, runs);
+    else
+      NHIP_LAUNCH("group_norm_apply", (norm_apply_tokens_kernel<T, 1, ACT>), grid, dim3(kThreads), each * sizeof(float2), s, a,
+                  each, run, runs);
   }
   return check_launch("group_norm_apply");
 }
 
 template <class T>
-size_t stats_lds(int channels, int v) {
-  return channels * sizeof(double2) + kThreads * v * (sizeof(typename First<T>::type) + sizeof(float));
+size_t stats_lds(int channels, int v, int threads) {
+  return channels * sizeof(double2) + threads * (v + 1) * (sizeof(typename First<T>::type) + sizeof(float));
+}
+
+template <class T, int ACT>
+int norm_one(const NormArgs& a, int layout, int n, int groups, bool vec, hipStream_t s) {
+  constexpr int V = kVec<T>;
+  const dim3 grid((uint32_t)((int64_t)n * (a.groups / groups)));
+  if (layout == NHIP_LAYOUT_BLOBS) {
+    if (vec)
+      NHIP_LAUNCH("group_norm_one", (norm_one_blobs_kernel<T, V, ACT>), grid, dim3(kOneThreads), 0, s, a, fast_div(a.cpg));
+    else
+      NHIP_LAUNCH("group_norm_one", (norm_one_blobs_kernel<T, 1, ACT>), grid, dim3(kOneThreads), 0, s, a, fast_div(a.cpg));
+  } else if (vec && groups * a.cpg % V == 0) {
+    NHIP_LAUNCH("group_norm_one", (norm_one_tokens_kernel<T, V, ACT>), grid, dim3(kOneThreads),
+                stats_lds<T>(groups * a.cpg, V, kOneThreads), s, a, groups);
+  } else {
+    NHIP_LAUNCH("group_norm_one", (norm_one_tokens_kernel<T, 1, ACT>), grid, dim3(kOneThreads),
+                stats_lds<T>(groups * a.cpg, 1, kOneThreads), s, a, groups);
+  }
+  return check_launch("group_norm_one");
 }
 
 template <class T>
-int norm_run(const NormArgs& a, int layout, int n, hipStream_t s) {
+int norm_run(const NormArgs& a, int layout, int n, int one, hipStream_t s) {
   constexpr int V = kVec<T>;
   const bool blobs = layout == NHIP_LAYOUT_BLOBS;
   // whole 16-byte vectors: along the pixels (blobs) or the channels (tokens)
   const bool vec = aligned_to(a.x, 16) && a.image_stride % V == 0 && a.row_stride % V == 0 &&
                    (blobs ? a.pixels % V == 0 : a.channels % V == 0 && aligned_to(a.y, 16));
+  if (one) switch (a.act) {
+      case NHIP_ACT_RELU: return norm_one<T, NHIP_ACT_RELU>(a, layout, n, one, vec, s);
+      case NHIP_ACT_SILU: return norm_one<T, NHIP_ACT_SILU>(a, layout, n, one, vec, s);
+      default: return norm_one<T, NHIP_ACT_NONE>(a, layout, n, one, vec, s);
+    }
   if (blobs) {
     const dim3 grid((uint32_t)((int64_t)n * a.chunks * a.groups));
     if (vec)
@@ -360,10 +535,10 @@ int norm_run(const NormArgs& a, int layout, int n, hipStream_t s) {
     const dim3 grid((uint32_t)(n * a.chunks));
     if (vec)
       NHIP_LAUNCH("group_norm_stats", (norm_stats_tokens_kernel<T, V>), grid, dim3(kThreads),
-                  stats_lds<T>(a.channels, V), s, a);
+                  stats_lds<T>(a.channels, V, kThreads), s, a);
     else
       NHIP_LAUNCH("group_norm_stats", (norm_stats_tokens_kernel<T, 1>), grid, dim3(kThreads),
-                  stats_lds<T>(a.channels, 1), s, a);
+                  stats_lds<T>(a.channels, 1, kThreads), s, a);
   }
   NHIP_TRY(check_launch("group_norm_stats"));
   switch (a.act) {
@@ -423,7 +598,8 @@ int nhip_group_norm_workspace_size(nhip_norm_t plan, int32_t dtype, int32_t layo
                                    uint64_t* bytes) {
   if (!bytes) return fail(NHIP_STATUS_NULL_POINTER, "group norm: null pointer");
   NormArgs a{};
-  NHIP_TRY(norm_args(plan, dtype, layout, n, pixels, &a));
+  int one;
+  NHIP_TRY(norm_args(plan, dtype, layout, n, pixels, &a, &one));
   *bytes = (uint64_t)n * a.chunks * a.groups * sizeof(double2);
   return ok();
 }
@@ -432,7 +608,8 @@ int nhip_group_norm_forward(nhip_norm_t plan, const void* input, int32_t dtype, 
                             int64_t pixels, int64_t image_stride, int64_t row_stride, void* output, void* workspace,
                             uint64_t workspace_bytes, void* stream) {
   NormArgs a{};
-  NHIP_TRY(norm_args(plan, dtype, layout, n, pixels, &a));
+  int one;
+  NHIP_TRY(norm_args(plan, dtype, layout, n, pixels, &a, &one));
   if (n == 0 || pixels == 0) return ok();
   if (!input || !output) return fail(NHIP_STATUS_NULL_POINTER, "group norm: null pointer");
   const int es = elem_size(dtype);
@@ -441,15 +618,15 @@ int nhip_group_norm_forward(nhip_norm_t plan, const void* input, int32_t dtype, 
   if (row_stride < (layout == NHIP_LAYOUT_BLOBS ? pixels : (int64_t)a.channels) || image_stride < 0)
     return fail(NHIP_STATUS_INVALID_SHAPE, "group norm: rows overlap");
   const uint64_t need = (uint64_t)n * a.chunks * a.groups * sizeof(double2);
-  if (!workspace) return fail(NHIP_STATUS_NULL_POINTER, "group norm: null workspace");
-  if (workspace_bytes < need || !aligned_to(workspace, 16))
+  if (need && !workspace) return fail(NHIP_STATUS_NULL_POINTER, "group norm: null workspace");
+  if (need && (workspace_bytes < need || !aligned_to(workspace, 16)))
     return fail(NHIP_STATUS_OUTPUT_CAPACITY_INSUFFICIENT, "group norm: workspace too small or not 16-byte aligned");
   a.x = input;
   a.y = output;
   a.part = (double2*)workspace;
   a.image_stride = image_stride;
   a.row_stride = row_stride;
-  return NHIP_FOR_ELEM(dtype, T, norm_run<T>(a, layout, n, as_stream(stream)));
+  return NHIP_FOR_ELEM(dtype, T, norm_run<T>(a, layout, n, one, as_stream(stream)));
 }
 
 int nhip_norm_destroy(nhip_norm_t plan) {

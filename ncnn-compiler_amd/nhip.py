@@ -93,6 +93,7 @@ class Kv8Desc(ctypes.Structure):
 
 
 _lib = None
+_settings = 0  # reloads: workspace sizes held from before one are asked for again
 _P = ctypes.c_void_p
 _Strides = ctypes.c_int64 * 3
 
@@ -212,7 +213,9 @@ def init(device: int = 0) -> None:
 def reload_settings() -> None:
     """Re-read the NHIP_* tuning / test switches from the environment (the
     library reads them once, at first use)."""
+    global _settings
     check(load().nhip_reload_settings())
+    _settings += 1
 
 
 def timer_start(kernel_filter: str = "") -> None:
@@ -667,59 +670,72 @@ def dequantize(x, scale, bias=None, stream=None):
 
 
 # ------------------------------------------------------------ token operators
-_ELEM = {}
+_ELEM = {}  # element types, filled with the first call
 
 
 def _elem(t, *like):
-    """The element type code of a device tensor whose channels are contiguous;
-    `like`: tensors that have to have its type and device."""
+    """(element type code, device index) of a device tensor whose channels
+    are contiguous; `like`: tensors that have to have its type and device.
+    Small calls are bound by the host, so the checks are the cheap forms of
+    themselves (2 us of a call's 9 before)."""
     torch = _torch()
     if not _ELEM:
         _ELEM.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16})
-    for x in (t, *like):
-        if not isinstance(x, torch.Tensor) or not x.is_cuda:
-            raise TypeError("nhip expects a CUDA (HIP) device tensor")
-        if x.dtype != t.dtype or x.device != t.device:
-            raise TypeError(f"expected {t.dtype} on {t.device}, got {x.dtype} on {x.device}")
-        if x.shape[-1] > 1 and x.stride(-1) != 1:
+    dev, dtype = t.get_device(), t.dtype
+    if dev < 0:
+        raise TypeError("nhip expects a CUDA (HIP) device tensor")
+    code = _ELEM.get(dtype)
+    if code is None:
+        raise TypeError(f"expected float32, float16 or bfloat16, got {dtype}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError("channels have to be contiguous")
+    for x in like:
+        if x.dtype != dtype or x.get_device() != dev:
+            raise TypeError(f"expected {dtype} on {t.device}, got {x.dtype} on {x.device}")
+        if x.stride(-1) != 1 and x.shape[-1] > 1:
             raise ValueError("channels have to be contiguous")
-    if t.device.index != torch._C._cuda_getDevice():
+    if dev != torch._C._cuda_getDevice():
         raise ValueError(f"{t.device} is not the current device")
-    if t.dtype not in _ELEM:
-        raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}")
-    return _ELEM[t.dtype]
+    return code, dev
 
 
-def _ints(t, device, shape, what):
-    """Pointer of a contiguous int32 device tensor of that shape."""
-    if t.dtype != _torch().int32 or t.device != device or not t.is_contiguous() or tuple(t.shape) != shape:
-        raise ValueError(f"{what} has to be a contiguous int32 tensor of shape {shape} on {device}")
+def _ints(t, dev, shape, what):
+    """Pointer of a contiguous int32 tensor of that shape on device `dev`."""
+    if t.shape != shape or t.dtype != _torch().int32 or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what} has to be a contiguous int32 tensor of shape {tuple(shape)} on device {dev}")
     return t.data_ptr()
 
 
 def _output(out, like, shape, stream, dtype=None):
     """`out`, checked, or a new tensor that `stream` may write."""
-    torch = _torch()
-    dtype = dtype or like.dtype
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=like.device)
+        torch = _torch()
+        if dtype is None and shape == like.shape and like.is_contiguous():
+            out = torch.empty_like(like)  # the cheapest of torch's allocations
+        else:
+            out = torch.empty(shape, dtype=dtype or like.dtype, device=like.device)
         if stream is not None:
             out.record_stream(stream)
-    elif out.dtype != dtype or out.device != like.device or not out.is_contiguous() or tuple(out.shape) != tuple(shape):
-        raise ValueError(f"out has to be a contiguous {dtype} tensor of shape {tuple(shape)} on {like.device}")
+    elif out.dtype != (dtype or like.dtype) or out.device != like.device or not out.is_contiguous() or out.shape != shape:
+        raise ValueError(f"out has to be a contiguous {dtype or like.dtype} tensor of shape {tuple(shape)} on {like.device}")
     return out
 
 
-def _scratch(workspace, nbytes, device, stream):
+def _scratch(workspace, nbytes, like, stream):
     """(tensor, pointer, bytes) of the caller's workspace or a new one, which
     stays allocated until `stream` is done with it."""
     if workspace is None:
         if not nbytes:
             return None, None, 0
-        workspace = _torch().empty(nbytes, dtype=_torch().uint8, device=device)
+        workspace = like.new_empty(nbytes, dtype=_torch().uint8)
         if stream is not None:
             workspace.record_stream(stream)
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _on(stream, dev):
+    """Handle of the given stream or of the device's current one."""
+    return stream.cuda_stream if stream is not None else _torch()._C._cuda_getCurrentRawStream(dev)
 
 
 @functools.lru_cache(4096)
@@ -744,7 +760,7 @@ class GroupNorm(_Plan):
         self._sizes = {}
 
     def workspace_size(self, dtype_code, n, pixels) -> int:
-        key = (dtype_code, n, pixels)
+        key = (_settings, dtype_code, n, pixels)
         if key not in self._sizes:
             b = ctypes.c_uint64()
             check(load().nhip_group_norm_workspace_size(self.handle, dtype_code, self.layout, n, pixels, ctypes.byref(b)))
@@ -765,14 +781,14 @@ class GroupNorm(_Plan):
             v = x if x.dim() == 3 else x.view(x.shape[0], -1, x.shape[3])
             n, pixels, c = v.shape
             shape = x.shape
-        code = _elem(v)
+        code, dev = _elem(v)
         if c != self.channels:
             raise ValueError(f"x has {c} channels, expected {self.channels}")
         out = _output(out, x, shape, stream)
-        ws, ptr, nbytes = _scratch(workspace, self.workspace_size(code, n, pixels), x.device, stream)
+        ws, ptr, nbytes = _scratch(workspace, self.workspace_size(code, n, pixels), x, stream)
         check(load().nhip_group_norm_forward(self.handle, v.data_ptr(), code, self.layout, n, pixels, v.stride(0),
                                              max(v.stride(1), v.shape[2]) if v.shape[1] == 1 else v.stride(1),
-                                             out.data_ptr(), ptr, nbytes, _stream(stream)))
+                                             out.data_ptr(), ptr, nbytes, _on(stream, dev)))
         return out
 
 
@@ -800,11 +816,11 @@ class Rotary(_Plan):
         b, n, h, d = x.shape
         if d != self.head_dim:
             raise ValueError(f"x has {d} channels to a head, expected {self.head_dim}")
-        code = _elem(x)
+        code, dev = _elem(x)
         per = positions.shape[0]
         if per not in (1, b):
             raise ValueError("positions have to have the batch's size or 1")
-        pos = _ints(positions, x.device, (per, n, self.axes), "positions")
+        pos = _ints(positions, dev, (per, n, self.axes), "positions")
         if out is None:
             out = _output(None, x, x.shape, stream)
         elif out.shape != x.shape:
@@ -813,7 +829,7 @@ class Rotary(_Plan):
             _elem(x, out)
         check(load().nhip_rotary_forward(self.handle, x.data_ptr(), code, b, n, h, _strides(x.stride()[:3]), pos,
                                          n * self.axes if per > 1 else 0, 1 if inverse else 0, out.data_ptr(),
-                                         _strides(out.stride()[:3]), _stream(stream)))
+                                         _strides(out.stride()[:3]), _on(stream, dev)))
         return out
 
 
@@ -834,11 +850,11 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, out=No
     torch = _torch()
     b, lq, h, d = q.shape
     lk, hkv = k.shape[1], k.shape[2]
-    code = _elem(q, k, v)
-    if tuple(k.shape) != (b, lk, hkv, d) or v.shape != k.shape:
+    code, dev = _elem(q, k, v)
+    if k.shape != (b, lk, hkv, d) or v.shape != k.shape:
         raise ValueError(f"k and v have shapes {tuple(k.shape)} and {tuple(v.shape)}: expected [{b}, keys, kv_heads, {d}]")
     desc, need = _attention(code, b, lq, lk, h, hkv, d, scale)
-    lengths = None if key_lengths is None else _ints(key_lengths, q.device, (b,), "key_lengths")
+    lengths = None if key_lengths is None else _ints(key_lengths, dev, (b,), "key_lengths")
     mask, mask_stride = None, 0
     if key_mask is not None:
         if key_mask.dtype != torch.bool or key_mask.device != q.device or tuple(key_mask.shape) not in ((b, lk), (lk,)):
@@ -847,10 +863,10 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, out=No
             raise ValueError("key_mask's keys have to be contiguous")
         mask, mask_stride = key_mask.data_ptr(), key_mask.stride(0) if key_mask.dim() == 2 else 0
     out = _output(out, q, q.shape, stream)
-    ws, ptr, nbytes = _scratch(workspace, need, q.device, stream)
+    ws, ptr, nbytes = _scratch(workspace, need, q, stream)
     check(load().nhip_cross_attention_forward(desc, q.data_ptr(), _strides(q.stride()[:3]), k.data_ptr(),
                                               _strides(k.stride()[:3]), v.data_ptr(), _strides(v.stride()[:3]),
-                                              lengths, mask, mask_stride, out.data_ptr(), ptr, nbytes, _stream(stream)))
+                                              lengths, mask, mask_stride, out.data_ptr(), ptr, nbytes, _on(stream, dev)))
     return out
 
 
@@ -883,6 +899,7 @@ class KvCache8:
             if not t.is_cuda or t.dtype != dtype or t.shape != shape or t.device != k.device or not t.is_contiguous():
                 raise ValueError(f"expected a contiguous {dtype} tensor of shape {tuple(shape)} on {k.device}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._dev = k.get_device()
         pages, self.kv_heads, self.block_tokens, self.head_dim = k.shape
         self._desc = Kv8Desc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
                              self.kv_heads, self.head_dim, self.block_tokens)
@@ -891,16 +908,16 @@ class KvCache8:
         """Tokens starts[b] .. of each sequence from k and v [batch, tokens,
         kv_heads, head_dim]: all of them, or the first counts[b]."""
         b, n = k.shape[:2]
-        code = _elem(k, v)
-        if tuple(k.shape) != (b, n, self.kv_heads, self.head_dim) or v.shape != k.shape or k.device != self.k.device:
+        code, dev = _elem(k, v)
+        if k.shape != (b, n, self.kv_heads, self.head_dim) or v.shape != k.shape or dev != self._dev:
             raise ValueError(f"k and v have to have shape [batch, tokens, {self.kv_heads}, {self.head_dim}] on {self.k.device}")
         pages = block_table.shape[-1]
         check(load().nhip_kv8_append(self._desc, code, k.data_ptr(), _strides(k.stride()[:3]), v.data_ptr(),
                                      _strides(v.stride()[:3]), b, n,
-                                     _ints(block_table, k.device, (b, pages), "block_table"), pages,
-                                     _ints(starts, k.device, (b,), "starts"),
-                                     None if counts is None else _ints(counts, k.device, (b,), "counts"),
-                                     _stream(stream)))
+                                     _ints(block_table, dev, (b, pages), "block_table"), pages,
+                                     _ints(starts, dev, (b,), "starts"),
+                                     None if counts is None else _ints(counts, dev, (b,), "counts"),
+                                     _on(stream, dev)))
 
     def read(self, block_table, starts, tokens, dtype, out=None, stream=None):
         """Values of tokens starts[b] .. starts[b] + tokens - 1: (k, v), each
@@ -908,10 +925,9 @@ class KvCache8:
         b, pages = block_table.shape
         shape = (b, tokens, self.kv_heads, self.head_dim)
         k, v = (_output(o, self.k, shape, stream, dtype) for o in (out or (None, None)))
-        check(load().nhip_kv8_read(self._desc, _elem(k, v), b, tokens,
-                                   _ints(block_table, self.k.device, (b, pages), "block_table"), pages,
-                                   _ints(starts, self.k.device, (b,), "starts"), k.data_ptr(), v.data_ptr(),
-                                   _stream(stream)))
+        code, dev = _elem(k, v)
+        check(load().nhip_kv8_read(self._desc, code, b, tokens, _ints(block_table, dev, (b, pages), "block_table"), pages,
+                                   _ints(starts, dev, (b,), "starts"), k.data_ptr(), v.data_ptr(), _on(stream, dev)))
         return k, v
 
     def attention(self, q, block_table, lengths, max_length=None, causal=False, scale=None, out=None, workspace=None,
@@ -920,19 +936,19 @@ class KvCache8:
         lengths[b] cached tokens (at most max_length; default what the block
         table holds).  causal: the queries are the last tokens."""
         b, lq, h, d = q.shape
-        code = _elem(q)
-        if d != self.head_dim or q.device != self.k.device:
+        code, dev = _elem(q)
+        if d != self.head_dim or dev != self._dev:
             raise ValueError(f"q has to have {self.head_dim} channels to a head, on {self.k.device}")
         pages = block_table.shape[-1]
         if max_length is None:
             max_length = pages * self.block_tokens
         desc, need = _attention(code, b, lq, max_length, h, self.kv_heads, d, scale)
         out = _output(out, q, q.shape, stream)
-        ws, ptr, nbytes = _scratch(workspace, need, q.device, stream)
+        ws, ptr, nbytes = _scratch(workspace, need, q, stream)
         check(load().nhip_kv8_attention_forward(desc, self._desc, q.data_ptr(), _strides(q.stride()[:3]),
-                                                _ints(block_table, q.device, (b, pages), "block_table"), pages,
-                                                _ints(lengths, q.device, (b,), "lengths"), 1 if causal else 0,
-                                                out.data_ptr(), ptr, nbytes, _stream(stream)))
+                                                _ints(block_table, dev, (b, pages), "block_table"), pages,
+                                                _ints(lengths, dev, (b,), "lengths"), 1 if causal else 0,
+                                                out.data_ptr(), ptr, nbytes, _on(stream, dev)))
         return out
 
 

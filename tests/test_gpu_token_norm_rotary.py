@@ -54,6 +54,16 @@ def test_group_norm(n, pixels, c, groups, dtype, blobs):
     check_norm(x.cuda(), groups, "silu", blobs)
 
 
+@pytest.mark.parametrize("one", ["0", "1"])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("blobs", [False, True])
+@pytest.mark.parametrize("n,pixels,c,groups", [(2, 9, 24, 3), (1, 1500, 96, 32), (3, 333, 20, 20), (2, 4097, 64, 1)])
+def test_group_norm_one_and_two_launches(n, pixels, c, groups, blobs, dtype, one, nhip_env):
+    nhip_env.setenv("NHIP_NORM_ONE", one)
+    x = randn(21, (n, c, pixels) if blobs else (n, pixels, c), dtype)
+    check_norm(x.cuda(), groups, "silu", blobs)
+
+
 @pytest.mark.parametrize("act", ["none", "relu"])
 @pytest.mark.parametrize("blobs", [False, True])
 def test_group_norm_activation_and_no_affine(act, blobs):
@@ -90,10 +100,10 @@ def test_group_norm_strides_and_alignment(dtype):
 
 
 def test_group_norm_in_place_and_given_workspace():
-    x = randn(7, (2, 33, 64), F16).cuda()
+    x = randn(7, (2, 3301, 64), F16).cuda()  # large enough for a workspace
     norm = nhip.GroupNorm(8, 64)
     want = norm.forward(x)
-    ws = torch.empty(norm.workspace_size(nhip.DTYPE_F16, 2, 33), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(norm.workspace_size(nhip.DTYPE_F16, 2, 3301), dtype=torch.uint8, device="cuda")
     y = x.clone()
     assert norm.forward(y, out=y, workspace=ws) is y
     assert torch.equal(y, want)
