@@ -9,6 +9,8 @@
 // O^T = V^T P^T takes its right operand.
 #pragma once
 
+#include <type_traits>
+
 #include "elem.h"
 #include "kv_cache8.h"
 
@@ -28,10 +30,12 @@ struct AttnArgs {
   int32_t rows;       // queries * group
   int32_t tiles;      // the kernel of many rows
   int32_t row_tiles;  // row tiles of a key/value head
-  int32_t splits;     // parts of a sequence's keys
+  int32_t splits;     // few rows: parts of a sequence's keys
+  int32_t workers;    // many rows: workgroups
+  int32_t units;      // and the parts of a row tile's keys that are dealt to them
   float scale_log2;   // scale / ln 2
-  float* part_o;      // [batch][kv_heads][rows][splits][d]
-  float2* part_ml;    // [batch][kv_heads][rows][splits]: maximum, sum
+  float* part_o;      // few rows: [batch][kv_heads][rows][splits][d]; many: [workers][2][128][d]
+  float2* part_ml;    // the same without [d]: maximum, sum
 };
 
 // Where keys and values come from.
@@ -167,12 +171,12 @@ __device__ __forceinline__ int4 load_row16(const AttnArgs& a, const void* base, 
     // a chunk may run past channel d into the next row, or past the page's end, where the buffer ends
     const uint32_t bytes = (uint32_t)a.d << a.cache.shift;
     const int8_t* at = codes + (page < 0 ? 0 : page * a.cache.kv_heads + kvh) * bytes;
-    const int slot = (key0 + r) & ((1 << a.cache.shift) - 1);
-    return buf_load_b128(make_rsrc(at, bytes), counts && c < a.d ? (uint32_t)(slot * a.d + c) : kBufOOB);
+    const uint32_t slot = (key0 + r) & ((1 << a.cache.shift) - 1), off = slot * a.d + c;
+    return buf_load_b128(make_rsrc(at, bytes), counts && c < a.d ? off : kBufOOB);
   } else {
     const T* at = (const T*)base + (int64_t)key0 * stride;
-    return buf_load_b128(make_rsrc(at, 0x7fffffffu),
-                         counts && c < a.d ? (uint32_t)((r * (int)stride + c) * (int)sizeof(T)) : kBufOOB);
+    const uint32_t off = (r * (uint32_t)stride + c) * (uint32_t)sizeof(T);
+    return buf_load_b128(make_rsrc(at, 0x7fffffffu), counts && c < a.d ? off : kBufOOB);
   }
 }
 
@@ -287,6 +291,16 @@ __device__ __forceinline__ typename Frag<T>::type load_v16(const T* tile, int c0
   }
   return f;
 }
+
+// The exponent's reference point need not be the row's largest score: it moves
+// only where a score lies more than kRoom above it, which spares most tiles the
+// scaling of the sums, and then to kBelow under that score.  fp16
+// probabilities lie high in their range (2^6 to 2^14 for the largest), so that
+// small ones keep their digits: they decide where the large ones meet values of 0.
+template <class P>
+constexpr float kRoom = std::is_same<P, f16>::value ? 14.f : 8.f;
+template <class P>
+constexpr float kBelow = std::is_same<P, f16>::value ? 6.f : 0.f;
 
 template <class P>
 constexpr int kPad16 = sizeof(P) == 2 ? 16 : 4;  // the rows that a read takes together lie in different banks
@@ -415,10 +429,11 @@ __global__ __launch_bounds__(kWaves * 64) void attn_rows_kernel(AttnArgs a) {
   const int row = rt * kRowTile + col;  // the lane's row
   const int qi = row / a.group, head = kvh * a.group + row % a.group;
   // keys that the lane's row sees, and that any row of the tile does
-  int sees = length, visible = length, begin, end;
+  int sees = length, all_see = length, visible = length, begin, end;
   if (a.causal) {
     const int last = min(rt * kRowTile + kRowTile - 1, a.rows - 1) / a.group;
     sees = max(0, length - a.queries + 1 + qi);
+    all_see = max(0, length - a.queries + 1 + rt * kRowTile / a.group);
     visible = max(0, min(length, length - a.queries + 1 + last));
   }
   part_of(a, length, visible, split, STEP, begin, end);
@@ -460,32 +475,44 @@ __global__ __launch_bounds__(kWaves * 64) void attn_rows_kernel(AttnArgs a) {
       tile.load(a, kbase, vbase, kvh, min(key0 + STEP, a.keys), begin, lane);
       ask = ask_tile<SRC, kKeyTile>(a, b, min(key0 + 2 * STEP, a.keys), lane);
 
-      // scores in units of ln 2; the running maximum of the row
-      float x[8], top = m;
-      bool on[8];
+      // scores in units of ln 2 (over the cache with the page's scale)
+      float x[8], top = -INFINITY;
       float vscale[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const float c = SRC == kSrcInt8 ? a.scale_log2 * lane_float(keys.kscale, t * 16) : a.scale_log2;
         vscale[t] = SRC == kSrcInt8 ? lane_float(keys.vscale, t * 16) : 1.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = t * 4 + j, r = t * 16 + 4 * g + j;
-          on[i] = (keys.counts >> r & 1) && key0 + r < sees;
-          x[i] = s[t][j] * c;
-          if (on[i]) top = fmaxf(top, x[i]);
-          seen |= on[i];
-        }
+        for (int j = 0; j < 4; ++j) x[t * 4 + j] = s[t][j] * c;
       }
+      if ((uint32_t)keys.counts == 0xffffffffu && key0 + kKeyTile <= all_see) {  // uniform
+        seen = true;
+      } else {
+        const int n = min(max(sees - key0, 0), kKeyTile);
+        const uint32_t on = (uint32_t)keys.counts & (uint32_t)((1ull << n) - 1), mine = on >> (4 * g);
+        seen |= on != 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (!(mine >> ((i >> 2) * 16 + (i & 3)) & 1)) x[i] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
       top = max32(max16(top));
-      const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet, or only scores of -infinity
-      const float keep = __builtin_amdgcn_exp2f(m - base);
-      m = top;
-      l *= keep;
+      if (__any(top > m + kRoom<P>)) {
+        const float to = fmaxf(m, top - kBelow<P>);
+        const float keep = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= keep;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] *= keep;
+      }
+      const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet, or only scores of -infinity
       FP pf[Second<T, SRC>::parts];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float p = on[i] ? __builtin_amdgcn_exp2f(x[i] - base) : 0.f;
+        float p = __builtin_amdgcn_exp2f(x[i] - base);
         l += p;
         if constexpr (SRC == kSrcInt8) p *= vscale[i >> 2];
         pf[0][i] = (P)p;
@@ -495,8 +522,6 @@ __global__ __launch_bounds__(kWaves * 64) void attn_rows_kernel(AttnArgs a) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] *= keep;
         const FP vf = load_v16<P, STRIDE>(vt, t * 16, lane);
 #pragma unroll
         for (int i = 0; i < Second<T, SRC>::parts; ++i) acc[t] = mma16(vf, pf[i], acc[t]);
@@ -554,31 +579,46 @@ __global__ __launch_bounds__(kWaves * 64) void attn_rows_kernel(AttnArgs a) {
   }
 }
 
-// Joins the parts of one row: one wave.
-template <class T>
+// Joins parts of one row's result for V of its channels: part i's maximum and
+// sum at ml(i), its sums at o(i).
+template <class T, int V, class ML, class O>
+__device__ __forceinline__ void join_parts(int parts, ML ml, O o, T* out) {
+  typedef float VF __attribute__((ext_vector_type(V)));
+  float top = -INFINITY, total = 0.f, sum[V] = {};
+  bool nan = false;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float2 p = ml(i);
+    const VF x = *reinterpret_cast<const VF*>(o(i));
+    nan |= p.y < 0.f;
+    const float to = fmaxf(top, p.x);
+    // -infinity: a part without a score above it has no weight
+    const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - to);
+    const float w = p.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p.x - to);
+    total = total * keep + (p.x == -INFINITY ? 0.f : w * p.y);
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = sum[j] * keep + (p.x == -INFINITY ? 0.f : w * x[j]);
+    top = to;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) sum[j] = top == -INFINITY ? (nan ? NAN : 0.f) : sum[j] / total;
+  Vec<T, V>::store(out, sum);
+}
+
+template <class T, int V>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-  const int64_t prow = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int cols = a.d / V, c = (int)(item % cols) * V;
+  const int64_t prow = item / cols;
   if (prow >= (int64_t)a.batch * a.kv_heads * a.rows) return;
   const int row = (int)(prow % a.rows);
   const int64_t bk = prow / a.rows;
   const int kvh = (int)(bk % a.kv_heads);
   const int64_t b = bk / a.kv_heads;
-  const float2* ml = a.part_ml + prow * a.splits;
-  float top = -INFINITY, total = 0.f;
-  bool nan = false;
-  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, ml[i].x);
-  for (int i = 0; i < a.splits; ++i) {
-    nan |= ml[i].y < 0.f;
-    if (ml[i].x != -INFINITY) total += __builtin_amdgcn_exp2f(ml[i].x - top) * ml[i].y;
-  }
-  T* out = (T*)a.o + ((b * a.queries + row / a.group) * a.heads + kvh * a.group + row % a.group) * a.d;
-  for (int c = lane; c < a.d; c += 64) {
-    float o = 0.f;
-    for (int i = 0; i < a.splits; ++i)
-      if (ml[i].x != -INFINITY) o += __builtin_amdgcn_exp2f(ml[i].x - top) * a.part_o[(prow * a.splits + i) * a.d + c];
-    out[c] = (T)(top == -INFINITY ? (nan ? NAN : 0.f) : o / total);
-  }
+  join_parts<T, V>(
+      a.splits, [&](int i) { return a.part_ml[prow * a.splits + i]; },
+      [&](int i) { return a.part_o + (prow * a.splits + i) * a.d + c; },
+      (T*)a.o + ((b * a.queries + row / a.group) * a.heads + kvh * a.group + row % a.group) * a.d + c);
 }
 
 template <class T, int DP, int SRC>
@@ -619,9 +659,12 @@ int run(const AttnArgs& a, int src, hipStream_t s) {
                  : src == kSrcAny ? launch_by_dim<T, kSrcAny>(a, s)
                                   : launch_by_dim<T, kSrcInt8>(a, s);
   NHIP_TRY(st);
-  if (a.splits == 1) return ok();
+  if (a.tiles || a.splits == 1) return ok();
   const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
-  NHIP_LAUNCH("attention_join", attn_join_kernel<T>, dim3((uint32_t)ceil_div(rows, 4)), dim3(256), 0, s, a);
+  if (a.d % 4 == 0 && aligned_to(a.o, 4 * sizeof(T)))
+    NHIP_LAUNCH("attention_join", (attn_join_kernel<T, 4>), dim3((uint32_t)ceil_div(rows * (a.d / 4), 256)), dim3(256), 0, s, a);
+  else
+    NHIP_LAUNCH("attention_join", (attn_join_kernel<T, 1>), dim3((uint32_t)ceil_div(rows * a.d, 256)), dim3(256), 0, s, a);
   return check_launch("attention_join");
 }
 

@@ -34,20 +34,39 @@ int attn_args(const nhip_attention_desc* d, bool vec, AttnArgs* a) {
   a->tiles = vec && a->rows > 64;
   const int tile = a->tiles ? attn::kTilesRows : attn::kRowTile;
   a->row_tiles = (int)ceil_div(std::max(a->rows, 1), tile);
-  // few workgroups: the keys are split until there are two for every CU, each
-  // part with at least 128 keys
   const int64_t heads = (int64_t)d->batch * d->kv_heads;
-  if (heads > 0x7fffff00 / a->row_tiles) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: too many rows");
+  if (heads > 0x7fffff00 / attn::kTilesRows / a->row_tiles)
+    return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: too many rows");
   const int64_t wgs = std::max<int64_t>(1, heads * a->row_tiles);
-  const int64_t want = std::max<int64_t>(1, 2 * cu_count() / wgs);
-  a->splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(d->keys, 128), 64}));
+  a->splits = 1;
+  if (!a->tiles) {
+    // few workgroups: the keys are split until there are two for every CU, each
+    // part with at least 128 keys
+    const int64_t want = std::max<int64_t>(1, 2 * cu_count() / wgs);
+    a->splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(d->keys, 128), 64}));
+    return ok();
+  }
+  // One row tile to a worker, unless that leaves over a tenth of the places on
+  // the CUs empty; then as many workers as there are places, the work dealt to
+  // them in equal runs of at least 256 keys.
+  const int keys = a->d > 128 ? 32 : 64;  // of a tile
+  const int64_t places = (int64_t)cu_count() * (a->d <= (d->dtype == NHIP_DTYPE_F32 ? 64 : 128) ? 2 : 1);
+  a->workers = (int)wgs;
+  a->units = std::max(1, (int)ceil_div(d->keys, keys));
+  if (wgs * 10 < ceil_div(wgs, places) * places * 9 && wgs * a->units < 0x7fffffff) {
+    const int64_t workers = std::min(places, wgs * a->units * keys / 256);
+    if (workers > wgs || workers == places) a->workers = (int)std::max<int64_t>(1, workers);
+  }
   return ok();
 }
 
-uint64_t workspace_of(const AttnArgs& a) {
-  if (a.splits == 1) return 0;
-  return (uint64_t)a.batch * a.kv_heads * a.rows * a.splits * (a.d * sizeof(float) + sizeof(float2));
+// Parts' (maximum, sum) pairs, an even number; their sums follow, 16-byte aligned.
+uint64_t parts_of(const AttnArgs& a) {
+  if (a.tiles) return a.workers == a.batch * a.kv_heads * a.row_tiles ? 0 : (uint64_t)a.workers * 2 * attn::kTilesRows;
+  return a.splits == 1 ? 0 : (uint64_t)round_up((int64_t)a.batch * a.kv_heads * a.rows * a.splits, 2);
 }
+
+uint64_t workspace_of(const AttnArgs& a) { return parts_of(a) * (a.d * sizeof(float) + sizeof(float2)); }
 
 // The most that a call with this descriptor needs, whatever its strides.
 int attn_workspace(const nhip_attention_desc* d, uint64_t* bytes) {
@@ -77,7 +96,7 @@ int attn_forward(AttnArgs& a, const nhip_attention_desc* d, int src, const void*
     if (workspace_bytes < need || !aligned_to(workspace, 16))
       return fail(NHIP_STATUS_OUTPUT_CAPACITY_INSUFFICIENT, "attention: workspace too small or not 16-byte aligned");
     a.part_ml = (float2*)workspace;
-    a.part_o = (float*)(a.part_ml + (uint64_t)a.batch * a.kv_heads * a.rows * a.splits);
+    a.part_o = (float*)(a.part_ml + parts_of(a));
   }
   switch (d->dtype) {
     case NHIP_DTYPE_F32: return attn_run_f32(a, src, as_stream(stream));
@@ -129,7 +148,7 @@ int nhip_cross_attention_forward(const nhip_attention_desc* desc, const void* qu
   a.mask = key_mask;
   if (mask_stride < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative stride");
   a.mask_stride = mask_stride;
-  const bool vec = desc->head_dim % (16 / es) == 0 && vec_rows(query, query_strides, es) &&
+  const bool vec = desc->head_dim % (16 / es) == 0 && aligned_to(out, 16) && vec_rows(query, query_strides, es) &&
                    vec_rows(key, key_strides, es) && vec_rows(value, value_strides, es);
   NHIP_TRY(attn_args(desc, vec, &a));
   return attn_forward(a, desc, vec ? kSrcVec : kSrcAny, query, query_strides, out, workspace, workspace_bytes, stream);
@@ -155,8 +174,8 @@ int nhip_kv8_attention_forward(const nhip_attention_desc* desc, const nhip_kv8_c
   a.lengths = lengths;
   a.causal = causal != 0;
   const int v = 16 / elem_size(desc->dtype);
-  if (!aligned_to(query, 16) || query_strides[0] % v || query_strides[1] % v || query_strides[2] % v)
-    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: query rows over the cache have to be 16-byte aligned");
+  if (!aligned_to(query, 16) || !aligned_to(out, 16) || query_strides[0] % v || query_strides[1] % v || query_strides[2] % v)
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: queries and results over the cache have to be 16-byte aligned");
   return attn_forward(a, desc, kSrcInt8, query, query_strides, out, workspace, workspace_bytes, stream);
 }
 

@@ -4,10 +4,15 @@
 namespace nhip {
 namespace attn {
 
+// Page scales of values below this add nothing to an fp16 result.
+constexpr float kLeastUnit = 0x1p-60f, kMostUnit = 0x1p60f;
+
 // Sizes of the kernel for channels padded to DP.
 template <class T, int DP, int SRC>
 struct TilesShape {
-  typedef typename Second<T, SRC>::type P;
+  typedef T P;  // probabilities and values in the second product
+  // fp16 over the cache: the sums count in units of the page's scale (below)
+  static constexpr bool units = SRC == kSrcInt8 && std::is_same<T, f16>::value;
   static constexpr int KT = DP == 256 ? 32 : 64;                        // keys of a tile: two buffers fit the LDS, one the registers
   static constexpr int E = SRC == kSrcInt8 ? 16 : 16 / (int)sizeof(T);  // channels of a 16-byte load
   static constexpr int L = KT * DP / E / (kWaves * 64);                 // loads of a thread, keys and values each
@@ -33,8 +38,9 @@ struct TilesLoad {
       const int at = wave * 64 + lane + i * kWaves * 64, r = at / per, c = at % per * S::E;
       const int64_t page = SRC == kSrcInt8 ? lane_page(keys, first & ~15) : 0;
       const bool on = keys.counts >> r & 1;
+      const bool von = on & !(S::units && lane_float(keys.vscale, first & ~15) < kLeastUnit);
       k[i] = load_row16<T, SRC>(a, kbase, a.ks[1], a.cache.k, kvh, page, key0, r, c, on);
-      v[i] = load_row16<T, SRC>(a, vbase, a.vs[1], a.cache.v, kvh, page, key0, r, c, on);
+      v[i] = load_row16<T, SRC>(a, vbase, a.vs[1], a.cache.v, kvh, page, key0, r, c, von);
     }
   }
   __device__ __forceinline__ void store(char* lds, int wave, int lane) const {
@@ -78,189 +84,277 @@ __device__ __forceinline__ typename Frag<T>::type load_v32(const T* tile, int c0
   return f;
 }
 
-// One workgroup: kTilesRows query rows of one key/value head over one part of
-// the keys.  Scores, probabilities and sums stay in registers from one product
+// l + the sum of eight probabilities as the second product takes them (exact,
+// summed in fp32), one instruction for two: fp16 over the cache, whose vector
+// unit converts codes besides (71 us for a chunk, 73 with 32 additions; without
+// codes to convert the additions were the faster, 700 us to 715).
+__device__ __forceinline__ float sum8(v8h p, float l) {
+  typedef f16 v2h __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2(v2h{p[i], p[i + 1]}, v2h{(f16)1.f, (f16)1.f}, l, false);
+  return l;
+}
+
+// The work of a launch is row tiles x units (a unit: one of `units` equal parts
+// of a row tile's keys; below 2^31 of them where they are dealt), dealt to the
+// workers in equal runs.  With as many workers as row tiles each does one; with
+// fewer or more, a run crosses row tiles or ends inside one.
+__device__ __forceinline__ uint32_t first_unit(const AttnArgs& a, uint32_t worker) {
+  const uint32_t work = (uint32_t)a.batch * a.kv_heads * a.row_tiles * a.units;
+  return (uint32_t)((uint64_t)worker * work / (uint32_t)a.workers);
+}
+__device__ __forceinline__ int worker_of(const AttnArgs& a, uint32_t unit) {
+  const uint32_t work = (uint32_t)a.batch * a.kv_heads * a.row_tiles * a.units;
+  return (int)((((uint64_t)unit + 1) * a.workers - 1) / work);
+}
+
+// One workgroup, kTilesRows query rows of one key/value head at a time.  Scores, probabilities and sums stay in registers from one product
 // to the other; while a tile is worked on, the next one's loads are under way,
 // and it goes into the other of two LDS buffers: one barrier a tile.
 template <class T, int DP, int SRC>
-__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void attn_tiles_kernel(AttnArgs a, uint32_t wgs) {
+__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void attn_tiles_kernel(AttnArgs a) {
   typedef TilesShape<T, DP, SRC> S;
   typedef typename S::P P;
   typedef typename Frag<T>::type FT;
   typedef typename Frag<P>::type FP;
-  constexpr int KT = S::KT, NT = KT / 32, KS = DP / 16, DT = DP / 32, PARTS = Second<T, SRC>::parts;
+  constexpr int KT = S::KT, NT = KT / 32, KS = DP / 16, DT = DP / 32;
+  constexpr int AHEAD = sizeof(T) == 4 ? 2 : KS < 8 ? KS : 8;  // operands read ahead of their products
   extern __shared__ char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id(), h = lane >> 5, col = lane & 31;
-  // workgroups go to the eight dies in turn: each die gets a run of them, so
+  // workgroups go to the eight dies in turn: each die gets a run of workers, so
   // that those of one head meet in its L2
-  uint32_t at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  if (at >= wgs) return;
-  const int rt = at % a.row_tiles;
-  at /= a.row_tiles;
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int kvh = at % a.kv_heads, b = at / a.kv_heads;
+  const uint32_t worker = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (worker >= (uint32_t)a.workers) return;
+  const bool dealt = a.workers != a.batch * a.kv_heads * a.row_tiles;
+  uint32_t unit = dealt ? first_unit(a, worker) : 0, unit_end = dealt ? first_unit(a, worker + 1) : (uint32_t)a.units;
+  while (unit < unit_end) {
+    // units [u0, u1) of one row tile
+    const uint32_t tile = dealt ? unit / (uint32_t)a.units : worker;
+    const int u0 = dealt ? (int)(unit - tile * a.units) : 0, u1 = min(a.units, u0 + (int)(unit_end - unit));
+    unit += u1 - u0;
+    const int rt = tile % a.row_tiles, kvh = tile / a.row_tiles % a.kv_heads, b = tile / a.row_tiles / a.kv_heads;
 
-  const int length = a.lengths ? max(0, min(a.lengths[b], a.keys)) : a.keys;
-  const int row = rt * kTilesRows + wave * 32 + col;
-  const int qi = row / a.group, head = kvh * a.group + row % a.group;
-  int sees = length, all_see = length, visible = length, begin, end;
-  if (a.causal) {
-    const int last = min(rt * kTilesRows + kTilesRows - 1, a.rows - 1) / a.group;
-    const int first = (rt * kTilesRows + wave * 32) / a.group;
-    sees = max(0, length - a.queries + 1 + qi);
-    all_see = max(0, length - a.queries + 1 + first);
-    visible = max(0, min(length, length - a.queries + 1 + last));
-  }
-  part_of(a, length, visible, split, KT, begin, end);
+    const int length = a.lengths ? max(0, min(a.lengths[b], a.keys)) : a.keys;
+    const int row = rt * kTilesRows + wave * 32 + col;
+    const int qi = row / a.group, head = kvh * a.group + row % a.group;
+    int sees = length, all_see = length, visible = length;
+    if (a.causal) {
+      const int last = min(rt * kTilesRows + kTilesRows - 1, a.rows - 1) / a.group;
+      const int first = (rt * kTilesRows + wave * 32) / a.group;
+      sees = max(0, length - a.queries + 1 + qi);
+      all_see = max(0, length - a.queries + 1 + first);
+      visible = max(0, min(length, length - a.queries + 1 + last));
+    }
+    int begin = u0 * KT, end = u1 * KT;
+    if (const int64_t tiles = (visible + KT - 1) / KT; tiles != a.units) {
+      begin = (int)(u0 * tiles / a.units) * KT;
+      end = (int)(u1 * tiles / a.units) * KT;
+    }
+    end = min(end, visible);
 
-  FT qf[KS];
-  const T* qrow = (const T*)a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
+    FT qf[KS];
+    const T* qrow = (const T*)a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    qf[s] = row < a.rows ? load_q<T, true>(qrow, s * 16 + h * 8, a.d) : zero_frag<T>();
-    if (a.scale_log2 < 0.f) qf[s] = -qf[s];
-  }
+    for (int s = 0; s < KS; ++s) {
+      qf[s] = row < a.rows ? load_q<T, true>(qrow, s * 16 + h * 8, a.d) : zero_frag<T>();
+      if (a.scale_log2 < 0.f) qf[s] = -qf[s];
+    }
 
-  v16f acc[DT];
+    v16f acc[DT];
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  bool seen = false;
-  const T* kbase = (const T*)a.k + b * a.ks[0] + kvh * a.ks[2];
-  const T* vbase = (const T*)a.v + b * a.vs[0] + kvh * a.vs[2];
+      for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    float in = 1.f;  // what one of the sums' units stands for
+    bool seen = false;
+    const T* kbase = (const T*)a.k + b * a.ks[0] + kvh * a.ks[2];
+    const T* vbase = (const T*)a.v + b * a.vs[0] + kvh * a.vs[2];
 
-  if (begin < end) {
-    TilesLoad<T, DP, SRC> next;
-    TileKeys keys = know_tile<SRC, KT>(a, ask_tile<SRC, KT>(a, b, begin, lane), kvh, begin, end, lane);
-    next.load(a, kbase, vbase, keys, kvh, begin, wave, lane);
-    TileAsk ask = ask_tile<SRC, KT>(a, b, min(begin + KT, a.keys), lane);
-    next.store(lds, wave, lane);
-    __syncthreads();
-    int buf = 0;
-    for (int key0 = begin; key0 < end; key0 += KT) {
-      // the next tile (past the end: nothing counts, nothing is read)
-      const int key1 = min(key0 + KT, a.keys);
-      const TileKeys soon = know_tile<SRC, KT>(a, ask, kvh, key0 + KT, end, lane);
-      next.load(a, kbase, vbase, soon, kvh, key1, wave, lane);
-      ask = ask_tile<SRC, KT>(a, b, min(key1 + KT, a.keys), lane);
-
-      const T* kt = reinterpret_cast<const T*>(lds + buf * (S::kbytes + S::vbytes));
-      const P* vt = reinterpret_cast<const P*>(lds + buf * (S::kbytes + S::vbytes) + S::kbytes);
-      v16f s[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < KS; ++i)
-          s[t] = mma32(*reinterpret_cast<const FT*>(kt + (t * 32 + col) * S::SK + i * 16 + h * 8), qf[i], s[t]);
-      }
-      if constexpr (NT == 2)
-        settle(s[0], s[1]);
-      else
-        settle(s[0]);
-
-      // over the cache: scores in units of ln 2, a page's scale included; else
-      // the factor goes into the exponent
-      if constexpr (SRC == kSrcInt8) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[t][i] *= fabsf(a.scale_log2) * lane_float(keys.kscale, t * 32 + (i >> 3) * 16);
-      }
-      // (of a scale of 0, too, -infinity stays what it is)
-      const float factor = SRC == kSrcInt8 ? 1.f : fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
-      constexpr uint64_t every = KT == 64 ? ~0ull : 0xffffffffull;
-      const bool whole = (keys.counts & every) == every && key0 + KT <= all_see;  // uniform
-      uint64_t on = every;
-      if (!whole) {
-        const int n = min(max(sees - key0, 0), KT);
-        on = keys.counts & (n >= 64 ? ~0ull : (1ull << n) - 1);
-        const uint64_t mine = on >> (4 * h);
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!(mine >> (t * 32 + (i >> 2) * 8 + (i & 3)) & 1)) s[t][i] = -INFINITY;
-      }
-      seen |= on != 0;
-      // The reference point of the exponent need not be the row's maximum: it
-      // moves only where a score lies more than 8 above it (probabilities up
-      // to 2^8, sums in fp32), which spares most tiles the scaling of the sums.
-      float top = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
-      top = max32(top);
-      top *= factor;
-      if (__any(top > m + 8.f)) {
-        const float to = fmaxf(m, top);
-        const float keep = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
-        m = to;
-        l *= keep;
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[t][i] *= keep;
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      FP pf[NT][2][PARTS];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[t][i], factor, -base));
-          l += p;
-          if constexpr (SRC == kSrcInt8) p *= lane_float(keys.vscale, t * 32 + (i >> 3) * 16);
-          pf[t][i >> 3][0][i & 7] = (P)p;
-          if constexpr (PARTS == 2) pf[t][i >> 3][1][i & 7] = (P)(p - (float)pf[t][i >> 3][0][i & 7]);
-        }
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int c = 0; c < DT; ++c) {
-            const FP vf = load_v32<P, S::SV>(vt + (t * 32 + u * 16) * S::SV, c * 32, lane);
-#pragma unroll
-            for (int i = 0; i < PARTS; ++i) acc[c] = mma32(vf, pf[t][u][i], acc[c]);
-          }
-      buf ^= 1;
-      next.store(lds + buf * (S::kbytes + S::vbytes), wave, lane);
-      keys = soon;
+    if (begin < end) {
+      TilesLoad<T, DP, SRC> next;
+      TileKeys keys = know_tile<SRC, KT>(a, ask_tile<SRC, KT>(a, b, begin, lane), kvh, begin, end, lane);
+      next.load(a, kbase, vbase, keys, kvh, begin, wave, lane);
+      TileAsk ask = ask_tile<SRC, KT>(a, b, min(begin + KT, a.keys), lane);
+      next.store(lds, wave, lane);
       __syncthreads();
-    }
+      int buf = 0;
+      for (int key0 = begin; key0 < end; key0 += KT) {
+        // the next tile (past the end: nothing counts, nothing is read)
+        const int key1 = min(key0 + KT, a.keys);
+        const TileKeys soon = know_tile<SRC, KT>(a, ask, kvh, key0 + KT, end, lane);
+        next.load(a, kbase, vbase, soon, kvh, key1, wave, lane);
+        ask = ask_tile<SRC, KT>(a, b, min(key1 + KT, a.keys), lane);
+
+        const T* kt = reinterpret_cast<const T*>(lds + buf * (S::kbytes + S::vbytes));
+        const P* vt = reinterpret_cast<const P*>(lds + buf * (S::kbytes + S::vbytes) + S::kbytes);
+        v16f s[NT];
 #pragma unroll
-    for (int t = 0; t < DT; ++t) settle(acc[t]);
-  }
-  l += __shfl_xor(l, 32);
-  if (l != l) m = INFINITY;                         // NaN to whoever joins this
-  else if (m == -INFINITY) l = seen ? -1.f : 0.f;  // scores of -infinity alone: 0 / 0, told from a row that sees nothing
-  if (row >= a.rows) return;
-  const int64_t prow = (((int64_t)b * a.kv_heads + kvh) * a.rows + row) * a.splits + split;
-  float* part = a.part_o + prow * a.d;
-  T* out = (T*)a.o + (((int64_t)b * a.queries + qi) * a.heads + head) * a.d;
-  const float scale = m == -INFINITY ? (l < 0.f ? NAN : 0.f) : 1.f / l;
-  if (a.splits > 1 && h == 0) a.part_ml[prow] = make_float2(m, l);
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
+          for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int c = t * 32 + (i >> 2) * 8 + 4 * h;
-      if (c < a.d) {
-        float o[4];
+          for (int i0 = 0; i0 < KS; i0 += AHEAD) {
+            FT kf[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = a.splits > 1 ? acc[t][i + j] : acc[t][i + j] * scale;
-        if (a.splits > 1)
-          *reinterpret_cast<v4f*>(part + c) = v4f{o[0], o[1], o[2], o[3]};
+            for (int i = 0; i < AHEAD; ++i) kf[i] = *reinterpret_cast<const FT*>(kt + (t * 32 + col) * S::SK + (i0 + i) * 16 + h * 8);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) s[t] = mma32(kf[i], qf[i0 + i], s[t]);
+          }
+        }
+        if constexpr (NT == 2)
+          settle(s[0], s[1]);
         else
-          Vec<T, 4>::store(out + c, o);
+          settle(s[0]);
+
+        // From scores to units of ln 2, over the cache with the scale of the 16
+        // keys' page; the factor goes into the exponent.  (Not 0, so that
+        // -infinity stays what it is.)
+        float factor[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            factor[t][u] = fmaxf(fabsf(a.scale_log2) * (SRC == kSrcInt8 ? lane_float(keys.kscale, t * 32 + u * 16) : 1.f), 1.17549435e-38f);
+        constexpr uint64_t every = KT == 64 ? ~0ull : 0xffffffffull;
+        const bool whole = (keys.counts & every) == every && key0 + KT <= all_see;  // uniform
+        uint64_t on = every;
+        if (!whole) {
+          const int n = min(max(sees - key0, 0), KT);
+          on = keys.counts & (n >= 64 ? ~0ull : (1ull << n) - 1);
+          const uint64_t mine = on >> (4 * h);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (!(mine >> (t * 32 + (i >> 2) * 8 + (i & 3)) & 1)) s[t][i] = -INFINITY;
+        }
+        seen |= on != 0;
+        float top = -INFINITY;
+        if constexpr (SRC != kSrcInt8) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+          top *= factor[0][0];
+        } else
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float most = s[t][u * 8];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) most = fmaxf(most, s[t][u * 8 + i]);
+            top = fmaxf(top, most * factor[t][u]);
+          }
+        top = max32(top);
+        if (__any(top > m + kRoom<P>)) {
+          const float to = fmaxf(m, top - kBelow<P>);
+          const float keep = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+          m = to;
+          l *= keep;
+#pragma unroll
+          for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[t][i] *= keep;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        FP pf[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float vscale = SRC == kSrcInt8 && !S::units ? lane_float(keys.vscale, t * 32 + u * 16) : 1.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float p = __builtin_amdgcn_exp2f(fmaf(s[t][u * 8 + i], factor[t][u], -base));
+              if constexpr (!S::units) l += p;
+              if constexpr (SRC == kSrcInt8 && !S::units) p *= vscale;
+              pf[t][u][i] = (P)p;
+            }
+            if constexpr (S::units) l = sum8(pf[t][u], l);
+          }
+        // (over the cache, whose other waves convert codes: 73 -> 71 us; else no gain)
+        if constexpr (SRC == kSrcInt8) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if constexpr (S::units) {
+              // probabilities times a page's scale may leave fp16's range, so
+              // the sums change to its units instead
+              const float now = fminf(fmaxf(lane_float(keys.vscale, t * 32 + u * 16), kLeastUnit), kMostUnit);
+              if (now != in) {
+                settle(acc[0]);
+                const float r = in * __builtin_amdgcn_rcpf(now);
+#pragma unroll
+                for (int c = 0; c < DT; ++c) {
+                  asm volatile("" : "+v"(acc[c]));  // after the wait
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) acc[c][i] *= r;
+                }
+                in = now;
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < DT; ++c) acc[c] = mma32(load_v32<P, S::SV>(vt + (t * 32 + u * 16) * S::SV, c * 32, lane), pf[t][u], acc[c]);
+          }
+        if constexpr (SRC == kSrcInt8) __builtin_amdgcn_s_setprio(0);
+        buf ^= 1;
+        next.store(lds + buf * (S::kbytes + S::vbytes), wave, lane);
+        keys = soon;
+        __syncthreads();
       }
+#pragma unroll
+      for (int t = 0; t < DT; ++t) settle(acc[t]);
     }
+    l += __shfl_xor(l, 32);
+    if (l != l) m = INFINITY;                         // NaN to whoever joins this
+    else if (m == -INFINITY) l = seen ? -1.f : 0.f;  // scores of -infinity alone: 0 / 0, told from a row that sees nothing
+    // a whole row tile's result, or a part: the one that begins the tile goes to
+    // the worker's second place, any other to its first
+    const bool whole_tile = u1 - u0 == a.units;
+    const int64_t prow = ((int64_t)worker * 2 + (u0 == 0)) * kTilesRows + wave * 32 + col;
+    float* part = a.part_o + prow * a.d;
+    T* out = (T*)a.o + (((int64_t)b * a.queries + qi) * a.heads + head) * a.d;
+    const float scale = m == -INFINITY ? (l < 0.f ? NAN : 0.f) : in / l;
+    if (row < a.rows) {
+      if (!whole_tile && h == 0) a.part_ml[prow] = make_float2(m, l);
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int c = t * 32 + (i >> 2) * 8 + 4 * h;
+          if (c < a.d) {
+            float o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = acc[t][i + j] * (whole_tile ? scale : in);
+            if (whole_tile)
+              Vec<T, 4>::store(out + c, o);
+            else
+              *reinterpret_cast<v4f*>(part + c) = v4f{o[0], o[1], o[2], o[3]};
+          }
+        }
+    }
+  }
+}
+
+// Joins the parts of the row tiles that several workers share.
+template <class T>
+__global__ __launch_bounds__(256) void attn_tiles_join_kernel(AttnArgs a) {
+  const int cols = a.d / 4, per = (kTilesRows * cols + 255) / 256;  // workgroups of a row tile
+  const uint32_t tile = blockIdx.x / per;
+  const int w0 = worker_of(a, tile * a.units), w1 = worker_of(a, (tile + 1) * a.units - 1);
+  if (w0 == w1) return;
+  const int item = blockIdx.x % per * 256 + threadIdx.x, in = item / cols, c = item % cols * 4;
+  const int row = tile % a.row_tiles * kTilesRows + in;
+  if (in >= kTilesRows || row >= a.rows) return;
+  const int kvh = tile / a.row_tiles % a.kv_heads, b = tile / a.row_tiles / a.kv_heads;
+  const auto place = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i == 0)) * kTilesRows + in; };
+  join_parts<T, 4>(
+      w1 - w0 + 1, [&](int i) { return a.part_ml[place(i)]; }, [&](int i) { return a.part_o + place(i) * a.d + c; },
+      (T*)a.o + (((int64_t)b * a.queries + row / a.group) * a.heads + kvh * a.group + row % a.group) * a.d + c);
 }
 
 template <class T, int DP, int SRC>
@@ -268,9 +362,14 @@ int tiles_launch(const AttnArgs& a, hipStream_t s) {
   constexpr int bytes = TilesShape<T, DP, SRC>::bytes;
   static_assert(bytes <= 160 * 1024, "two tiles fit the LDS");
   if (bytes > 65536) NHIP_TRY(ensure_dynamic_lds((const void*)attn_tiles_kernel<T, DP, SRC>, bytes));
-  const uint32_t wgs = (uint32_t)((int64_t)a.batch * a.kv_heads * a.splits * a.row_tiles);
-  NHIP_LAUNCH("attention_tiles", (attn_tiles_kernel<T, DP, SRC>), dim3((wgs + 7) / 8 * 8), dim3(kWaves * 64), bytes, s, a, wgs);
-  return check_launch("attention_tiles");
+  NHIP_LAUNCH("attention_tiles", (attn_tiles_kernel<T, DP, SRC>), dim3((uint32_t)ceil_div(a.workers, 8) * 8),
+              dim3(kWaves * 64), bytes, s, a);
+  NHIP_TRY(check_launch("attention_tiles"));
+  const int64_t tiles = (int64_t)a.batch * a.kv_heads * a.row_tiles;
+  if (a.workers == tiles) return ok();
+  NHIP_LAUNCH("attention_join", attn_tiles_join_kernel<T>, dim3((uint32_t)(tiles * ceil_div(kTilesRows * (a.d / 4), 256))),
+              dim3(256), 0, s, a);
+  return check_launch("attention_join");
 }
 
 }  // namespace attn
