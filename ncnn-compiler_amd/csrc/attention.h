@@ -305,6 +305,13 @@ constexpr float kBelow = std::is_same<P, f16>::value ? 6.f : 0.f;
 template <class P>
 constexpr int kPad16 = sizeof(P) == 2 ? 16 : 4;  // the rows that a read takes together lie in different banks
 
+// Workgroups that a CU is to hold, what the registers are dealt out for: few
+// rows over the cache wait for memory and convert codes in turn (a cached step
+// 79 us with two, 73 with three).
+constexpr int rows_per_cu(int size, int dp, int src) {
+  return src == kSrcInt8 ? (size == 2 && dp <= 128 ? 3 : 1) : (src == kSrcVec && size * dp <= 256 ? 2 : 1);
+}
+
 template <class T, int DP, int SRC>
 constexpr int rows_lds() {
   typedef typename Second<T, SRC>::type P;
@@ -410,7 +417,7 @@ struct RowsTile {
 // wave's own LDS, which turns them; the next tile's loads are under way while
 // one is worked on.
 template <class T, int DP, int SRC>
-__global__ __launch_bounds__(kWaves * 64) void attn_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, rows_per_cu(sizeof(T), DP, SRC)) void attn_rows_kernel(AttnArgs a) {
   typedef typename Second<T, SRC>::type P;
   typedef typename Frag<T>::type FT;
   typedef typename Frag<P>::type FP;

@@ -9,8 +9,9 @@ namespace nhip {
 namespace {
 
 // Checks the sizes and fills them in, chooses the kernel (vec: rows that the
-// one for many rows takes) and the number of parts of the keys.
-int attn_args(const nhip_attention_desc* d, bool vec, AttnArgs* a) {
+// one for many rows takes; cache: over the 8-bit cache) and the number of parts
+// of the keys.
+int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
   if (!d) return fail(NHIP_STATUS_NULL_POINTER, "attention: null descriptor");
   if (!elem_size(d->dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "attention: dtype has to be F32, F16 or BF16");
   if (d->batch < 0 || d->queries < 0 || d->keys < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative extent");
@@ -40,10 +41,13 @@ int attn_args(const nhip_attention_desc* d, bool vec, AttnArgs* a) {
   const int64_t wgs = std::max<int64_t>(1, heads * a->row_tiles);
   a->splits = 1;
   if (!a->tiles) {
-    // few workgroups: the keys are split until there are two for every CU, each
-    // part with at least 128 keys
-    const int64_t want = std::max<int64_t>(1, 2 * cu_count() / wgs);
-    a->splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(d->keys, 128), 64}));
+    // Few workgroups: the keys are split until there is one for every CU (three
+    // over the cache), each part with at least 512 keys.  us at 1 / 2 / 4 a CU:
+    // cross attention of 256 heads, 3136 keys 67.7 / 72.3 / 74.6; 2 / 3 / 4 over
+    // the cache, 128 heads, 12544 keys 77.4 / 72.8 / 81.5.  Parts of 128 / 512 /
+    // 1024 keys: 8 heads of 12544 keys 24.9 / 21.2 / 23.0, 4 of 500 13.1 / 9.1.
+    const int64_t want = ((cache ? 3 : 1) * cu_count() + wgs / 2) / wgs;
+    a->splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(d->keys, 512), 64}));
     return ok();
   }
   // One row tile to a worker, unless that leaves over a tenth of the places on
@@ -69,11 +73,11 @@ uint64_t parts_of(const AttnArgs& a) {
 uint64_t workspace_of(const AttnArgs& a) { return parts_of(a) * (a.d * sizeof(float) + sizeof(float2)); }
 
 // The most that a call with this descriptor needs, whatever its strides.
-int attn_workspace(const nhip_attention_desc* d, uint64_t* bytes) {
+int attn_workspace(const nhip_attention_desc* d, bool cache, uint64_t* bytes) {
   *bytes = 0;
   for (bool vec : {false, true}) {
     AttnArgs a{};
-    NHIP_TRY(attn_args(d, vec, &a));
+    NHIP_TRY(attn_args(d, vec, cache, &a));
     *bytes = std::max(*bytes, workspace_of(a));
   }
   return ok();
@@ -121,7 +125,7 @@ extern "C" {
 
 int nhip_cross_attention_workspace_size(const nhip_attention_desc* desc, uint64_t* bytes) {
   if (!bytes) return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
-  return attn_workspace(desc, bytes);
+  return attn_workspace(desc, false, bytes);
 }
 
 int nhip_cross_attention_forward(const nhip_attention_desc* desc, const void* query, const int64_t* query_strides,
@@ -130,7 +134,7 @@ int nhip_cross_attention_forward(const nhip_attention_desc* desc, const void* qu
                                  int64_t mask_stride, void* out, void* workspace, uint64_t workspace_bytes,
                                  void* stream) {
   AttnArgs a{};
-  NHIP_TRY(attn_args(desc, false, &a));
+  NHIP_TRY(attn_args(desc, false, false, &a));
   if (desc->batch == 0 || desc->queries == 0) return ok();
   if (!query || !query_strides || !out || !key_strides || !value_strides || (desc->keys && (!key || !value)))
     return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
@@ -150,13 +154,13 @@ int nhip_cross_attention_forward(const nhip_attention_desc* desc, const void* qu
   a.mask_stride = mask_stride;
   const bool vec = desc->head_dim % (16 / es) == 0 && aligned_to(out, 16) && vec_rows(query, query_strides, es) &&
                    vec_rows(key, key_strides, es) && vec_rows(value, value_strides, es);
-  NHIP_TRY(attn_args(desc, vec, &a));
+  NHIP_TRY(attn_args(desc, vec, false, &a));
   return attn_forward(a, desc, vec ? kSrcVec : kSrcAny, query, query_strides, out, workspace, workspace_bytes, stream);
 }
 
 int nhip_kv8_attention_workspace_size(const nhip_attention_desc* desc, const nhip_kv8_cache* cache, uint64_t* bytes) {
   if (!bytes || !cache) return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
-  return attn_workspace(desc, bytes);
+  return attn_workspace(desc, true, bytes);
 }
 
 int nhip_kv8_attention_forward(const nhip_attention_desc* desc, const nhip_kv8_cache* cache, const void* query,
@@ -164,7 +168,7 @@ int nhip_kv8_attention_forward(const nhip_attention_desc* desc, const nhip_kv8_c
                                const int32_t* lengths, int32_t causal, void* out, void* workspace,
                                uint64_t workspace_bytes, void* stream) {
   AttnArgs a{};
-  NHIP_TRY(attn_args(desc, true, &a));
+  NHIP_TRY(attn_args(desc, true, true, &a));
   NHIP_TRY(kv8_args(cache, block_table, table_pages, &a.cache));
   if (cache->kv_heads != desc->kv_heads || cache->head_dim != desc->head_dim)
     return fail(NHIP_STATUS_INVALID_SHAPE, "attention: the cache has other heads");

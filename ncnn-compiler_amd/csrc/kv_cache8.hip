@@ -21,6 +21,7 @@ struct AppendArgs {
   const int32_t* starts;
   const int32_t* counts;
   int32_t tokens, touch;  // pages that a sequence may touch
+  FastDiv by_vecs;        // vectors of a token's head
 };
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -30,11 +31,12 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 
 // One workgroup: one page of one sequence, one head, keys or values.  The new
-// tokens are read twice (the second time from the cache that the first filled):
-// for their largest magnitude and to be quantised.
-template <class T, int V>
-__global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
-  __shared__ float red[kThreads / 64];
+// tokens are wanted twice, for their largest magnitude and to be quantised: a
+// thread keeps its first kHeld vectors (a page of 64 tokens of 128 16-bit
+// channels) and reads others again.
+template <class T, int V, int TH>
+__global__ __launch_bounds__(TH) void kv8_append_kernel(AppendArgs a) {
+  constexpr int kHeld = 4;
   const int which = blockIdx.x & 1;
   const uint32_t rest = blockIdx.x >> 1;
   const int h = rest % a.c.kv_heads;
@@ -43,49 +45,71 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
   const int start = a.starts[b];
   const int count = a.counts ? min(a.counts[b], a.tokens) : a.tokens;
   if (start < 0 || count <= 0) return;
-  const int bt = 1 << a.c.shift;
   const int64_t page = (int64_t)(start >> a.c.shift) + j;
   const int64_t t0 = max((int64_t)start, page << a.c.shift);
   const int64_t t1 = min((int64_t)start + count, (page + 1) << a.c.shift);
   if (t0 >= t1) return;
-  const int64_t id = kv8_page(a.c, b, page);
-  if (id < 0) return;
   const int d = a.c.head_dim;
-  int8_t* code = (which ? a.c.v : a.c.k) + ((id * a.c.kv_heads + h) << a.c.shift) * d;
-  float* scale = (which ? a.c.v_scale : a.c.k_scale) + id * a.c.kv_heads + h;
   const T* x = (const T*)a.x[which] + b * a.xs[which][0] + (t0 - start) * a.xs[which][1] + h * a.xs[which][2];
   const int64_t xt = a.xs[which][1];
   const int vecs = d / V, fresh = (int)(t1 - t0) * vecs;
+  const auto load = [&](int i, float(&t)[V]) {
+    const int token = fdiv(i, a.by_vecs);
+    Vec<T, V>::load(x + token * xt + (i - token * vecs) * V, t);
+  };
+  float held[kHeld][V];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (const int i = threadIdx.x + k * TH; i < fresh) load(i, held[k]);
+  const int64_t id = kv8_page(a.c, b, page);
+  if (id < 0) return;
+  int8_t* code = (which ? a.c.v : a.c.k) + ((id * a.c.kv_heads + h) << a.c.shift) * d;
+  float* scale = (which ? a.c.v_scale : a.c.k_scale) + id * a.c.kv_heads + h;
   const int had = (int)(t0 - (page << a.c.shift));  // tokens that the page holds
+  const float stood = *scale;
 
   float most = 0.f;
-  for (int i = threadIdx.x; i < fresh; i += kThreads) {
-    float t[V];
-    Vec<T, V>::load(x + i / vecs * xt + i % vecs * V, t);
+  const auto widest = [&](const float(&t)[V]) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float m = fabsf(t[e]);
       most = m <= 3.402823466e38f ? fmaxf(most, m) : most;  // NaN and infinities do not count
     }
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (threadIdx.x + k * TH < fresh) widest(held[k]);
+  for (int i = threadIdx.x + kHeld * TH; i < fresh; i += TH) {
+    float t[V];
+    load(i, t);
+    widest(t);
   }
   most = wave_max(most);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = most;
-  __syncthreads();
-  most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float was = had ? *scale : 0.f;
+  if constexpr (TH > 64) {
+    __shared__ float red[TH / 64];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TH / 64; ++i) most = fmaxf(most, red[i]);
+  }
+  const float was = had ? stood : 0.f;
   const float want = most > 0.f ? fmaxf(most * (1.0f / 127.0f), kScaleLeast) : 0.f;
   const float now = fmaxf(want, was);
   const float inv = now > 0.f ? 1.0f / now : 0.f;
-  __syncthreads();  // everybody has read the scale
-  if (threadIdx.x == 0) *scale = now;
+  if (threadIdx.x == 0) *scale = now;  // (every lane's own read of it is done: `now` depends on it)
   if (now != was) {
     const float ratio = was * inv;
-    for (int i = threadIdx.x; i < had * d; i += kThreads) code[i] = quantize_i8((float)code[i], ratio);
+    uint2* old = reinterpret_cast<uint2*>(code);  // head_dim is a multiple of 8
+    for (int i = threadIdx.x; i < had * d / 8; i += TH) {
+      const uint2 c = old[i];
+      int q[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = quantize_q((float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3))), ratio);
+      old[i] = make_uint2(pack_i8x4(q[0], q[1], q[2], q[3]), pack_i8x4(q[4], q[5], q[6], q[7]));
+    }
   }
   int8_t* to = code + had * d;
-  for (int i = threadIdx.x; i < fresh; i += kThreads) {
-    float t[V];
-    Vec<T, V>::load(x + i / vecs * xt + i % vecs * V, t);
+  const auto put = [&](int i, const float(&t)[V]) {
     int q[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) q[e] = quantize_q(t[e], inv);
@@ -96,6 +120,14 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     } else {
       to[i] = (int8_t)q[0];
     }
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (const int i = threadIdx.x + k * TH; i < fresh) put(i, held[k]);
+  for (int i = threadIdx.x + kHeld * TH; i < fresh; i += TH) {
+    float t[V];
+    load(i, t);
+    put(i, t);
   }
 }
 
@@ -103,22 +135,21 @@ struct ReadArgs {
   Kv8 c;
   void* out[2];
   const int32_t* starts;
-  int64_t items;  // of keys: batch * tokens * kv_heads * head_dim / 8
-  int32_t tokens;
+  int32_t tokens, items, blocks;  // of a sequence's keys: 8-channel pieces, workgroups
+  FastDiv by_vecs, by_heads;
 };
 
+// A thread: eight channels of one token and head, keys or values.
 template <class T>
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(ReadArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int which = blockIdx.y;
+  const int which = blockIdx.x & 1;
+  const uint32_t block = blockIdx.x >> 1;
+  const int b = block / a.blocks;
+  const int i = (int)(block % a.blocks) * kThreads + threadIdx.x;
   if (i >= a.items) return;
-  const int vecs = a.c.head_dim / 8;
-  const int c = (int)(i % vecs) * 8;
-  const int64_t r = i / vecs;
-  const int h = (int)(r % a.c.kv_heads);
-  const int64_t bt = r / a.c.kv_heads;
-  const int b = (int)(bt / a.tokens);
-  const int64_t t = (int64_t)a.starts[b] + bt % a.tokens;
+  const int r = fdiv(i, a.by_vecs), c = (i - r * (a.c.head_dim / 8)) * 8;
+  const int at_token = fdiv(r, a.by_heads), h = r - at_token * a.c.kv_heads;
+  const int64_t t = (int64_t)a.starts[b] + at_token;
   const int64_t id = t < 0 ? -1 : kv8_page(a.c, b, t >> a.c.shift);
   float v[8] = {};
   if (id >= 0) {
@@ -128,23 +159,31 @@ __global__ __launch_bounds__(kThreads) void kv8_read_kernel(ReadArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3))) * s;
   }
-  T* out = (T*)a.out[which] + i * 8;
+  T* out = (T*)a.out[which] + ((int64_t)b * a.items + i) * 8;
 #pragma unroll
   for (int e = 0; e < 8; e += kVec<T>) Vec<T, kVec<T>>::store(out + e, reinterpret_cast<float(&)[kVec<T>]>(v[e]));
 }
 
-template <class T>
-int append_run(const AppendArgs& a, uint32_t wgs, bool vec, hipStream_t s) {
-  if (vec)
-    NHIP_LAUNCH("kv8_append", (kv8_append_kernel<T, kVec<T>>), dim3(wgs), dim3(kThreads), 0, s, a);
+template <class T, int V>
+int append_launch(AppendArgs a, uint32_t wgs, hipStream_t s) {
+  const int vecs = a.c.head_dim / V;
+  a.by_vecs = fast_div(vecs);
+  // a wave does where a call's tokens leave it no more than it holds
+  if ((int64_t)a.tokens * vecs <= 4 * 64)
+    NHIP_LAUNCH("kv8_append", (kv8_append_kernel<T, V, 64>), dim3(wgs), dim3(64), 0, s, a);
   else
-    NHIP_LAUNCH("kv8_append", (kv8_append_kernel<T, 1>), dim3(wgs), dim3(kThreads), 0, s, a);
+    NHIP_LAUNCH("kv8_append", (kv8_append_kernel<T, V, kThreads>), dim3(wgs), dim3(kThreads), 0, s, a);
   return check_launch("kv8_append");
 }
 
 template <class T>
-int read_run(const ReadArgs& a, hipStream_t s) {
-  NHIP_LAUNCH("kv8_read", kv8_read_kernel<T>, dim3((uint32_t)ceil_div(a.items, kThreads), 2), dim3(kThreads), 0, s, a);
+int append_run(const AppendArgs& a, uint32_t wgs, bool vec, hipStream_t s) {
+  return vec ? append_launch<T, kVec<T>>(a, wgs, s) : append_launch<T, 1>(a, wgs, s);
+}
+
+template <class T>
+int read_run(const ReadArgs& a, uint32_t wgs, hipStream_t s) {
+  NHIP_LAUNCH("kv8_read", kv8_read_kernel<T>, dim3(wgs), dim3(kThreads), 0, s, a);
   return check_launch("kv8_read");
 }
 
@@ -225,11 +264,15 @@ int nhip_kv8_read(const nhip_kv8_cache* cache, int32_t dtype, int32_t batch, int
   a.out[1] = value;
   a.starts = starts;
   a.tokens = tokens;
-  const int64_t rows = (int64_t)batch * tokens;
-  if (rows > (int64_t(0x7fffffff) * kThreads) / a.c.kv_heads / a.c.head_dim)
+  const int64_t items = (int64_t)tokens * a.c.kv_heads * (a.c.head_dim / 8);
+  if (tokens > (0x7fffffff - kThreads) / a.c.kv_heads / (a.c.head_dim / 8) ||
+      batch > 0x7fffffff / 2 / ceil_div(items, kThreads))
     return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "kv8: too many tokens in one call");
-  a.items = rows * a.c.kv_heads * (a.c.head_dim / 8);
-  return NHIP_FOR_ELEM(dtype, T, read_run<T>(a, as_stream(stream)));
+  a.items = (int32_t)items;
+  a.blocks = (int32_t)ceil_div(items, kThreads);
+  a.by_vecs = fast_div(a.c.head_dim / 8);
+  a.by_heads = fast_div(a.c.kv_heads);
+  return NHIP_FOR_ELEM(dtype, T, read_run<T>(a, (uint32_t)batch * a.blocks * 2, as_stream(stream)));
 }
 
 }  // extern "C"

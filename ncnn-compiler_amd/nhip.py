@@ -834,11 +834,14 @@ class Rotary(_Plan):
 
 
 @functools.lru_cache(4096)
-def _attention(code, b, lq, lk, h, hkv, d, scale):
+def _attention(code, b, lq, lk, h, hkv, d, scale, cached=False):
     """(descriptor, workspace bytes)."""
     desc = AttentionDesc(code, b, lq, lk, h, hkv, d, float(d) ** -0.5 if scale is None else float(scale))
     n = ctypes.c_uint64()
-    check(load().nhip_cross_attention_workspace_size(ctypes.byref(desc), ctypes.byref(n)))
+    if cached:  # the size goes by the descriptor alone
+        check(load().nhip_kv8_attention_workspace_size(ctypes.byref(desc), ctypes.byref(Kv8Desc()), ctypes.byref(n)))
+    else:
+        check(load().nhip_cross_attention_workspace_size(ctypes.byref(desc), ctypes.byref(n)))
     return desc, n.value
 
 
@@ -942,7 +945,7 @@ class KvCache8:
         pages = block_table.shape[-1]
         if max_length is None:
             max_length = pages * self.block_tokens
-        desc, need = _attention(code, b, lq, max_length, h, self.kv_heads, d, scale)
+        desc, need = _attention(code, b, lq, max_length, h, self.kv_heads, d, scale, True)
         out = _output(out, q, q.shape, stream)
         ws, ptr, nbytes = _scratch(workspace, need, q, stream)
         check(load().nhip_kv8_attention_forward(desc, self._desc, q.data_ptr(), _strides(q.stride()[:3]),
