@@ -32,7 +32,18 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
   if (d->keys > most || (int64_t)d->queries * a->group > most)
     return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: at most 2^30 keys, and rows of a key/value head");
   a->rows = d->queries * a->group;
-  a->tiles = vec && a->rows > 64;
+  // The kernel of few rows reads all keys and values for every 16 of them, some
+  // 8 TB/s from the L2s; the one of many reads them once for 128, and its parts
+  // are joined in a launch of their own (5 us).  So the second where the first
+  // would read 8 us longer, unless its workgroups leave most CUs idle.  us, few
+  // / many: 64 heads of 3136 keys of 128 bf16, 32 rows 38.1 / 30.9; 192 of 800
+  // of 64, 32 rows 16.4 / 21.0, 64 rows 24.3 / 22.2; 1 of 12544 of 128, 256 rows
+  // 22.8 / 25.4; over the cache 64 heads, 32 rows 31.7 / 34.5, 64 rows 45.0 / 36.5.
+  const int64_t kv_heads = (int64_t)d->batch * d->kv_heads, tiles16 = ceil_div(std::max(a->rows, 1), attn::kRowTile);
+  const double bytes = (double)kv_heads * d->keys * d->head_dim * 2 * (cache ? 1 : elem_size(d->dtype));
+  const int force = setting_int("NHIP_ATTN_TILES", -1);
+  a->tiles = vec && force != 0 &&
+             (force == 1 || kv_heads * tiles16 > 4 * cu_count() || (kv_heads * tiles16 > cu_count() / 4 && (tiles16 - 1) * bytes > 64e6));
   const int tile = a->tiles ? attn::kTilesRows : attn::kRowTile;
   a->row_tiles = (int)ceil_div(std::max(a->rows, 1), tile);
   const int64_t heads = (int64_t)d->batch * d->kv_heads;

@@ -834,7 +834,7 @@ class Rotary(_Plan):
 
 
 @functools.lru_cache(4096)
-def _attention(code, b, lq, lk, h, hkv, d, scale, cached=False):
+def _attention(settings, code, b, lq, lk, h, hkv, d, scale, cached=False):
     """(descriptor, workspace bytes)."""
     desc = AttentionDesc(code, b, lq, lk, h, hkv, d, float(d) ** -0.5 if scale is None else float(scale))
     n = ctypes.c_uint64()
@@ -856,7 +856,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, out=No
     code, dev = _elem(q, k, v)
     if k.shape != (b, lk, hkv, d) or v.shape != k.shape:
         raise ValueError(f"k and v have shapes {tuple(k.shape)} and {tuple(v.shape)}: expected [{b}, keys, kv_heads, {d}]")
-    desc, need = _attention(code, b, lq, lk, h, hkv, d, scale)
+    desc, need = _attention(_settings, code, b, lq, lk, h, hkv, d, scale)
     lengths = None if key_lengths is None else _ints(key_lengths, dev, (b,), "key_lengths")
     mask, mask_stride = None, 0
     if key_mask is not None:
@@ -945,7 +945,7 @@ class KvCache8:
         pages = block_table.shape[-1]
         if max_length is None:
             max_length = pages * self.block_tokens
-        desc, need = _attention(code, b, lq, max_length, h, self.kv_heads, d, scale, True)
+        desc, need = _attention(_settings, code, b, lq, max_length, h, self.kv_heads, d, scale, True)
         out = _output(out, q, q.shape, stream)
         ws, ptr, nbytes = _scratch(workspace, need, q, stream)
         check(load().nhip_kv8_attention_forward(desc, self._desc, q.data_ptr(), _strides(q.stride()[:3]),
