@@ -64,7 +64,7 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
   // One row tile to a worker, unless that leaves over a tenth of the places on
   // the CUs empty; then as many workers as there are places, the work dealt to
   // them in equal runs of at least 256 keys.
-  const int keys = a->d > 128 ? 32 : 64;  // of a tile
+  const int keys = a->d > (d->dtype == NHIP_DTYPE_F32 ? 64 : 128) ? 32 : 64;  // of a tile
   const int64_t places = (int64_t)cu_count() * (a->d <= (d->dtype == NHIP_DTYPE_F32 ? 64 : 128) ? 2 : 1);
   a->workers = (int)wgs;
   a->units = std::max(1, (int)ceil_div(d->keys, keys));

@@ -7,28 +7,64 @@ namespace attn {
 // Page scales of values below this add nothing to an fp16 result.
 constexpr float kLeastUnit = 0x1p-60f, kMostUnit = 0x1p60f;
 
+// fp32 values as sums of bf16 pieces, largest first: x = hi + mid + lo exactly
+// (each rounding leaves at most 16, then 8 significant bits) while lo is above
+// bf16's smallest normal number and hi below its largest.  A product of two
+// such sums without the products of mid and lo, lo and mid, lo and lo, below
+// 2^-25 of it: six matrix instructions on bf16 in place of eight on fp32 that
+// take twice as long each.
+constexpr float kPieceMost = 3.38e38f;
+constexpr uint32_t kPieceLeast = (127 - 100) << 24;  // of 2^-100, the bits without the sign's place
+__device__ __forceinline__ void split8(v8f x, v8b (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[0][i] = (bf16)x[i];
+    const float r = x[i] - (float)p[0][i];
+    p[1][i] = (bf16)r;
+    p[2][i] = (bf16)(r - (float)p[1][i]);
+  }
+}
+// Whether pieces would not hold some value that was shown to it.
+struct PieceRange {
+  float most = 0.f;
+  uint32_t least = 0xffffffffu;
+  __device__ __forceinline__ void show(float x) {
+    most = fmaxf(most, fabsf(x));  // NaN passes: its pieces are NaN
+    least = min(least, (__builtin_bit_cast(uint32_t, x) << 1) - 1u);  // 0 wraps around
+  }
+  __device__ __forceinline__ bool missed() const { return most > kPieceMost || least < kPieceLeast - 1u; }
+};
+
 // Sizes of the kernel for channels padded to DP.
 template <class T, int DP, int SRC>
 struct TilesShape {
-  typedef T P;  // probabilities and values in the second product
+  static constexpr bool split = sizeof(T) == 4;
+  typedef typename std::conditional<split, bf16, T>::type M;  // what the matrix instructions take
+  static constexpr int KP = split && SRC != kSrcInt8 ? 3 : 1;  // pieces of a key or value (codes are exact in one)
+  static constexpr int QP = split ? 3 : 1;                     // of a query or probability
   // fp16 over the cache: the sums count in units of the page's scale (below)
   static constexpr bool units = SRC == kSrcInt8 && std::is_same<T, f16>::value;
-  static constexpr int KT = DP == 256 ? 32 : 64;                        // keys of a tile: two buffers fit the LDS, one the registers
-  static constexpr int E = SRC == kSrcInt8 ? 16 : 16 / (int)sizeof(T);  // channels of a 16-byte load
-  static constexpr int L = KT * DP / E / (kWaves * 64);                 // loads of a thread, keys and values each
+  static constexpr int KT = DP == 256 || (split && DP == 128) ? 32 : 64;  // keys of a tile
+  static constexpr int E = SRC == kSrcInt8 ? 16 : 16 / (int)sizeof(T);    // channels of a 16-byte load
+  static constexpr int L = KT * DP / E / (kWaves * 64);                   // loads of a thread, keys and values each
   // Rows padded so that the eight rows of a 16-byte read, and the four of a
   // transposing read, lie in different banks.
-  static constexpr int SK = DP + 16 / (int)sizeof(T);
-  static constexpr int SV = DP + (sizeof(P) == 2 ? 32 : 8);
-  static constexpr int kbytes = KT * SK * (int)sizeof(T), vbytes = KT * SV * (int)sizeof(P);
-  static constexpr int bytes = 2 * (kbytes + vbytes);
+  static constexpr int SK = DP + 8, SV = DP + 32;
+  static constexpr int kplane = KT * SK, vplane = KT * SV;  // values of one piece
+  static constexpr int buffer = KP * (kplane + vplane) * 2;
+  // Pieces leave room for one buffer where two workgroups share a CU: a
+  // second barrier a tile, and two words that say which tile they do not hold.
+  static constexpr int buffers = KP == 3 ? 1 : 2;
+  static constexpr int bytes = buffers * buffer + (KP == 3 ? 16 : 0);
+  static constexpr int per_cu = (split ? DP == 64 : DP <= 128) ? 2 : 1;
 };
 
 // The next tile on its way, spread over the workgroup.
 template <class T, int DP, int SRC>
 struct TilesLoad {
   typedef TilesShape<T, DP, SRC> S;
-  typedef typename S::P P;
+  typedef typename S::M M;
+  typedef typename Frag<M>::type FM;
   int4 k[S::L], v[S::L];
   __device__ __forceinline__ void load(const AttnArgs& a, const T* kbase, const T* vbase, const TileKeys& keys, int kvh, int key0, int wave, int lane) {
     constexpr int per = DP / S::E;
@@ -43,45 +79,69 @@ struct TilesLoad {
       v[i] = load_row16<T, SRC>(a, vbase, a.vs[1], a.cache.v, kvh, page, key0, r, c, von);
     }
   }
-  __device__ __forceinline__ void store(char* lds, int wave, int lane) const {
+  // To LDS; whether pieces miss some value of this thread.
+  __device__ __forceinline__ bool store(char* lds, int wave, int lane) const {
     constexpr int per = DP / S::E;
+    PieceRange range;
 #pragma unroll
     for (int i = 0; i < S::L; ++i) {
       const int at = wave * 64 + lane + i * kWaves * 64, r = at / per, c = at % per * S::E;
-      T* kt = reinterpret_cast<T*>(lds) + r * S::SK + c;
-      P* vt = reinterpret_cast<P*>(lds + S::kbytes) + r * S::SV + c;
+      M* kt = reinterpret_cast<M*>(lds) + r * S::SK + c;
+      M* vt = reinterpret_cast<M*>(lds) + S::KP * S::kplane + r * S::SV + c;
       if constexpr (SRC == kSrcInt8) {
-        *reinterpret_cast<typename Frag<T>::type*>(kt) = codes8<T>(k[i].x, k[i].y);
-        *reinterpret_cast<typename Frag<T>::type*>(kt + 8) = codes8<T>(k[i].z, k[i].w);
-        *reinterpret_cast<typename Frag<P>::type*>(vt) = codes8<P>(v[i].x, v[i].y);
-        *reinterpret_cast<typename Frag<P>::type*>(vt + 8) = codes8<P>(v[i].z, v[i].w);
+        *reinterpret_cast<FM*>(kt) = codes8<M>(k[i].x, k[i].y);
+        *reinterpret_cast<FM*>(kt + 8) = codes8<M>(k[i].z, k[i].w);
+        *reinterpret_cast<FM*>(vt) = codes8<M>(v[i].x, v[i].y);
+        *reinterpret_cast<FM*>(vt + 8) = codes8<M>(v[i].z, v[i].w);
+      } else if constexpr (S::split) {
+        typedef bf16 v4b __attribute__((ext_vector_type(4)));
+        const v4f kx = __builtin_bit_cast(v4f, k[i]), vx = __builtin_bit_cast(v4f, v[i]);
+        v8f x;
+        v8b p[3];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = kx[j];
+          x[4 + j] = vx[j];
+          range.show(kx[j]);
+          range.show(vx[j]);
+        }
+        split8(x, p);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          *reinterpret_cast<v4b*>(kt + j * S::kplane) = v4b{p[j][0], p[j][1], p[j][2], p[j][3]};
+          *reinterpret_cast<v4b*>(vt + j * S::vplane) = v4b{p[j][4], p[j][5], p[j][6], p[j][7]};
+        }
       } else {
         *reinterpret_cast<int4*>(kt) = k[i];
         *reinterpret_cast<int4*>(vt) = v[i];
       }
     }
+    return S::KP == 3 && range.missed();
   }
 };
+
+// c + the product of two sums of pieces, smallest products first.
+template <int KP, int QP, class F>
+__device__ __forceinline__ v16f mma32_pieces(const F (&k)[KP], const F (&q)[QP], v16f c) {
+#pragma unroll
+  for (int n = QP - 1; n >= 0; --n)
+#pragma unroll
+    for (int i = 0; i < KP; ++i)
+      if (n - i >= 0 && n - i < QP) c = mma32(k[i], q[n - i], c);
+  return c;
+}
 
 // A lane's eight summed values down channel c0 + (l & 31) of V in LDS: keys
 // 8 u + 4 h .. + 3 for u = 0, 1 (h = lane / 32), as eight of a score tile's
 // sums lie in a lane.
 template <class T, int STRIDE>
 __device__ __forceinline__ typename Frag<T>::type load_v32(const T* tile, int c0, int lane) {
-  const int h = lane >> 5;
-  typename Frag<T>::type f;
-  if constexpr (sizeof(T) == 2) {
-    const int j = lane & 15;
-    const T* at = tile + (4 * h + (j >> 2)) * STRIDE + c0 + (lane & 16) + (j & 3) * 4;
-    typedef __attribute__((address_space(3))) v4s lds4;
-    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at);
-    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(at + 8 * STRIDE));
-    f = __builtin_bit_cast(typename Frag<T>::type, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = tile[(8 * (i >> 2) + 4 * h + (i & 3)) * STRIDE + c0 + (lane & 31)];
-  }
-  return f;
+  const int h = lane >> 5, j = lane & 15;
+  const T* at = tile + (4 * h + (j >> 2)) * STRIDE + c0 + (lane & 16) + (j & 3) * 4;
+  typedef __attribute__((address_space(3))) v4s lds4;
+  const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at);
+  const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(at + 8 * STRIDE));
+  return __builtin_bit_cast(typename Frag<T>::type, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // l + the sum of eight probabilities as the second product takes them (exact,
@@ -108,17 +168,17 @@ __device__ __forceinline__ int worker_of(const AttnArgs& a, uint32_t unit) {
   return (int)((((uint64_t)unit + 1) * a.workers - 1) / work);
 }
 
-// One workgroup, kTilesRows query rows of one key/value head at a time.  Scores, probabilities and sums stay in registers from one product
-// to the other; while a tile is worked on, the next one's loads are under way,
-// and it goes into the other of two LDS buffers: one barrier a tile.
+// One workgroup, kTilesRows query rows of one key/value head at a time.  Scores,
+// probabilities and sums stay in registers from one product to the other; while
+// a tile is worked on, the next one's loads are under way, and it goes into the
+// other of two LDS buffers: one barrier a tile.
 template <class T, int DP, int SRC>
-__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void attn_tiles_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, (TilesShape<T, DP, SRC>::per_cu)) void attn_tiles_kernel(AttnArgs a) {
   typedef TilesShape<T, DP, SRC> S;
-  typedef typename S::P P;
-  typedef typename Frag<T>::type FT;
-  typedef typename Frag<P>::type FP;
-  constexpr int KT = S::KT, NT = KT / 32, KS = DP / 16, DT = DP / 32;
-  constexpr int AHEAD = sizeof(T) == 4 ? 2 : KS < 8 ? KS : 8;  // operands read ahead of their products
+  typedef typename S::M M;
+  typedef typename Frag<M>::type FM;
+  constexpr int KT = S::KT, NT = KT / 32, KS = DP / 16, DT = DP / 32, KP = S::KP, QP = S::QP;
+  constexpr int AHEAD = S::split ? 1 : KS < 8 ? KS : 8;  // operands read ahead of their products
   extern __shared__ char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id(), h = lane >> 5, col = lane & 31;
   // workgroups go to the eight dies in turn: each die gets a run of workers, so
@@ -152,13 +212,31 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) v
     }
     end = min(end, visible);
 
-    FT qf[KS];
+    // (pieces of more than 128 channels would not fit the registers: split at each use)
+    constexpr bool LATE = S::split && DP == 256;
+    FM qf[LATE ? 1 : KS][QP];
+    v8f qx[LATE ? KS : 1];
     const T* qrow = (const T*)a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
+    const auto query = [&](int s) {
+      auto q = row < a.rows ? load_q<T, true>(qrow, s * 16 + h * 8, a.d) : zero_frag<T>();
+      return a.scale_log2 < 0.f ? -q : q;
+    };
+    PieceRange qrange;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      qf[s] = row < a.rows ? load_q<T, true>(qrow, s * 16 + h * 8, a.d) : zero_frag<T>();
-      if (a.scale_log2 < 0.f) qf[s] = -qf[s];
+      if constexpr (S::split) {
+        const v8f q = query(s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qrange.show(q[i]);
+        if constexpr (LATE)
+          qx[s] = q;
+        else
+          split8(q, qf[s]);
+      } else {
+        qf[s][0] = query(s);
+      }
     }
+    const bool qmissed = KP == 3 && __any(qrange.missed());
 
     v16f acc[DT];
 #pragma unroll
@@ -176,9 +254,14 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) v
       TileKeys keys = know_tile<SRC, KT>(a, ask_tile<SRC, KT>(a, b, begin, lane), kvh, begin, end, lane);
       next.load(a, kbase, vbase, keys, kvh, begin, wave, lane);
       TileAsk ask = ask_tile<SRC, KT>(a, b, min(begin + KT, a.keys), lane);
-      next.store(lds, wave, lane);
+      int* missed = reinterpret_cast<int*>(lds + S::buffers * S::buffer);  // [2], tiles by turns
+      if constexpr (KP == 3) {
+        if (threadIdx.x < 2) missed[threadIdx.x] = 0;
+        __syncthreads();
+      }
+      if (__any(next.store(lds, wave, lane)) && lane == 0) missed[0] = 1;
       __syncthreads();
-      int buf = 0;
+      int turn = 0;
       for (int key0 = begin; key0 < end; key0 += KT) {
         // the next tile (past the end: nothing counts, nothing is read)
         const int key1 = min(key0 + KT, a.keys);
@@ -186,22 +269,55 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) v
         next.load(a, kbase, vbase, soon, kvh, key1, wave, lane);
         ask = ask_tile<SRC, KT>(a, b, min(key1 + KT, a.keys), lane);
 
-        const T* kt = reinterpret_cast<const T*>(lds + buf * (S::kbytes + S::vbytes));
-        const P* vt = reinterpret_cast<const P*>(lds + buf * (S::kbytes + S::vbytes) + S::kbytes);
+        const M* kt = reinterpret_cast<const M*>(lds + (S::buffers == 2 ? turn : 0) * S::buffer);
+        const M* vt = kt + KP * S::kplane;
+        const bool exact = KP == 3 && (qmissed || __builtin_amdgcn_readfirstlane(missed[turn]));
         v16f s[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+        if (KP == 3 && __builtin_expect(exact, false)) {
+          // values that pieces do not hold: fp32 products of the keys as they stand in memory
+          if constexpr (KP == 3) {
+            int kcol = col;
+            asm volatile("" : "+v"(kcol));  // addresses are formed here, not kept through the loop
+#pragma unroll 1
+            for (int i = 0; i < KS; ++i) {
+              const v8f q = query(i);
 #pragma unroll
-          for (int i0 = 0; i0 < KS; i0 += AHEAD) {
-            FT kf[AHEAD];
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) kf[i] = *reinterpret_cast<const FT*>(kt + (t * 32 + col) * S::SK + (i0 + i) * 16 + h * 8);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) s[t] = mma32(kf[i], qf[i0 + i], s[t]);
+              for (int t = 0; t < NT; ++t) {
+                const bool counts = keys.counts >> (t * 32 + kcol) & 1;
+                struct { int4 lo, hi; } both;
+                both.lo = load_row16<T, SRC>(a, kbase, a.ks[1], nullptr, 0, 0, key0, t * 32 + kcol, i * 16 + h * 8, counts);
+                both.hi = load_row16<T, SRC>(a, kbase, a.ks[1], nullptr, 0, 0, key0, t * 32 + kcol, i * 16 + h * 8 + 4, counts);
+                s[t] = mma32(__builtin_bit_cast(v8f, both), q, s[t]);
+              }
+            }
           }
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i0 = 0; i0 < KS; i0 += AHEAD) {
+              FM kf[AHEAD][KP];
+#pragma unroll
+              for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+                for (int p = 0; p < KP; ++p)
+                  kf[i][p] = *reinterpret_cast<const FM*>(kt + p * S::kplane + (t * 32 + col) * S::SK + (i0 + i) * 16 + h * 8);
+              if constexpr (!S::split) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+              for (int i = 0; i < AHEAD; ++i) {
+                if constexpr (LATE) {
+                  v8b q[3];
+                  split8(qx[i0 + i], q);
+                  s[t] = mma32_pieces(kf[i], q, s[t]);
+                } else {
+                  s[t] = mma32_pieces(kf[i], qf[i0 + i], s[t]);
+                }
+              }
+            }
         }
         if constexpr (NT == 2)
           settle(s[0], s[1]);
@@ -249,8 +365,8 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) v
             top = fmaxf(top, most * factor[t][u]);
           }
         top = max32(top);
-        if (__any(top > m + kRoom<P>)) {
-          const float to = fmaxf(m, top - kBelow<P>);
+        if (__any(top > m + kRoom<M>)) {
+          const float to = fmaxf(m, top - kBelow<M>);
           const float keep = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
           m = to;
           l *= keep;
@@ -260,21 +376,48 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) v
             for (int i = 0; i < 16; ++i) acc[t][i] *= keep;
         }
         const float base = m == -INFINITY ? 0.f : m;
-        FP pf[NT][2];
+        typename std::conditional<S::split, v8f, FM>::type pf[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const float vscale = SRC == kSrcInt8 && !S::units ? lane_float(keys.vscale, t * 32 + u * 16) : 1.f;
+            v8f p;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              float p = __builtin_amdgcn_exp2f(fmaf(s[t][u * 8 + i], factor[t][u], -base));
-              if constexpr (!S::units) l += p;
-              if constexpr (SRC == kSrcInt8 && !S::units) p *= vscale;
-              pf[t][u][i] = (P)p;
+              p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][u * 8 + i], factor[t][u], -base));
+              if constexpr (!S::units) l += p[i];
+              if constexpr (SRC == kSrcInt8 && !S::units) p[i] *= vscale;
+              if constexpr (!S::split) pf[t][u][i] = (M)p[i];
             }
+            if constexpr (S::split) pf[t][u] = p;
             if constexpr (S::units) l = sum8(pf[t][u], l);
           }
+        if (KP == 3 && __builtin_expect(exact, false)) {
+          if constexpr (KP == 3) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int c = 0; c < DT; ++c) {
+                  const __amdgpu_buffer_rsrc_t rows = make_rsrc(vbase + (int64_t)key0 * a.vs[1], 0x7fffffffu);
+                  int vcol = col;
+                  asm volatile("" : "+v"(vcol));
+                  v8f vf;
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) {
+                    const int r = t * 32 + u * 16 + 8 * (i >> 2) + 4 * h + (i & 3), ch = c * 32 + vcol;
+                    const bool counts = (keys.counts >> r & 1) && ch < a.d;
+                    vf[i] = buf_load_f32(rows, counts ? (r * (uint32_t)a.vs[1] + ch) * 4u : kBufOOB);
+                  }
+                  acc[c] = mma32(vf, pf[t][u], acc[c]);
+                  __builtin_amdgcn_sched_barrier(0);
+                }
+          }
+#pragma unroll
+          for (int c = 0; c < DT; ++c) settle(acc[c]);
+        } else {
         // (over the cache, whose other waves convert codes: 73 -> 71 us; else no gain)
         if constexpr (SRC == kSrcInt8) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -297,12 +440,27 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 && DP <= 128 ? 2 : 1) v
                 in = now;
               }
             }
+            FM pp[QP];
+            if constexpr (S::split)
+              split8(pf[t][u], pp);
+            else
+              pp[0] = pf[t][u];
 #pragma unroll
-            for (int c = 0; c < DT; ++c) acc[c] = mma32(load_v32<P, S::SV>(vt + (t * 32 + u * 16) * S::SV, c * 32, lane), pf[t][u], acc[c]);
+            for (int c = 0; c < DT; ++c) {
+              FM vf[KP];
+#pragma unroll
+              for (int p = 0; p < KP; ++p) vf[p] = load_v32<M, S::SV>(vt + p * S::vplane + (t * 32 + u * 16) * S::SV, c * 32, lane);
+              acc[c] = mma32_pieces(vf, pp, acc[c]);
+            }
           }
+        }
         if constexpr (SRC == kSrcInt8) __builtin_amdgcn_s_setprio(0);
-        buf ^= 1;
-        next.store(lds + buf * (S::kbytes + S::vbytes), wave, lane);
+        if constexpr (S::buffers == 1) {
+          __syncthreads();
+          if (threadIdx.x == 0) missed[turn] = 0;  // everybody has read it; next set in the tile after the next
+        }
+        turn ^= 1;
+        if (__any(next.store(lds + (S::buffers == 2 ? turn : 0) * S::buffer, wave, lane)) && lane == 0) missed[turn] = 1;
         keys = soon;
         __syncthreads();
       }
