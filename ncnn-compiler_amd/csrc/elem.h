@@ -24,7 +24,9 @@ inline int elem_size(int dtype) {
 inline bool aligned_to(const void* p, uint64_t bytes) { return reinterpret_cast<uint64_t>(p) % bytes == 0; }
 
 // N consecutive elements: one 16-byte access (4 fp32 or 8 16-bit elements) or
-// a single element.  The pointer is aligned to the whole access.
+// a single element.  The pointer is aligned to the whole access.  STREAM: a
+// store that takes no place in the caches, of a result that is too large for
+// them to hold it until its use.
 template <class T, int N>
 struct Vec {
   typedef T type __attribute__((ext_vector_type(N)));
@@ -33,18 +35,24 @@ struct Vec {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = (float)v[i];
   }
+  template <bool STREAM = false>
   __device__ __forceinline__ static void store(T* p, const float (&x)[N]) {
     type v;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (T)x[i];
-    *reinterpret_cast<type*>(p) = v;
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(v, reinterpret_cast<type*>(p));
+    else
+      *reinterpret_cast<type*>(p) = v;
   }
 };
 template <class T>
 struct Vec<T, 1> {
   __device__ __forceinline__ static void load(const T* p, float (&x)[1]) { x[0] = (float)*p; }
+  template <bool STREAM = false>
   __device__ __forceinline__ static void store(T* p, const float (&x)[1]) { *p = (T)x[0]; }
 };
+constexpr int64_t kStreamBytes = 64 << 20;  // results past this are stored with STREAM
 template <class T>
 constexpr int kVec = 16 / sizeof(T);
 

@@ -29,7 +29,8 @@ struct nhip_norm_plan {
 namespace nhip {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;      // of a workgroup, tokens
+constexpr int kBlobThreads = 256;  // blobs, two launches
 constexpr int kOneThreads = 512;   // of a workgroup that does its groups alone
 constexpr int kMaxChannels = 4096;
 constexpr int kMaxChunks = 256;  // parts of an image: what each workgroup of the second pass merges
@@ -93,11 +94,12 @@ __device__ __forceinline__ double2 moments(double s1, float s2, float shift, dou
 
 // Merges the chunks of image `n` for groups [g0, g1): mean and 1/sqrt(var + eps)
 // to stat[g - g0].
+template <int TH>
 __device__ void merge_chunks(const NormArgs& a, int n, int g0, int g1, float2* stat) {
-  const int team = team_of<kThreads>(g1 - g0), lane = threadIdx.x & (team - 1);
+  const int team = team_of<TH>(g1 - g0), lane = threadIdx.x & (team - 1);
   const double2* part = a.part + (int64_t)n * a.chunks * a.groups;
   const double last = (double)(a.pixels - (int64_t)(a.chunks - 1) * a.chunk), total = (double)a.pixels;
-  for (int gb = g0; gb < g1; gb += kThreads / team) {  // uniform: all lanes of a team stay in the butterflies
+  for (int gb = g0; gb < g1; gb += TH / team) {  // uniform: all lanes of a team stay in the butterflies
     const int g = gb + threadIdx.x / team;
     const bool in = g < g1;
     double m = 0.0;
@@ -221,7 +223,7 @@ __device__ __forceinline__ void merge_channels(const NormArgs& a, const double2*
 
 // y of channels [c0, c0 + cn) over pixels [p0, p1), channels last; stat: of
 // the groups from the one that c0 begins.
-template <class T, int V, int ACT, int TH>
+template <class T, int V, int ACT, int TH, bool STREAM>
 __device__ void apply_tokens(const NormArgs& a, const T* x, T* y, int c0, int cn, int64_t p0, int64_t p1, const float2* stat) {
   const int vecs = cn / V;
   for (int v0 = 0; v0 < vecs; v0 += TH) {
@@ -252,14 +254,14 @@ __device__ void apply_tokens(const NormArgs& a, const T* x, T* y, int c0, int cn
 #pragma unroll
       for (int u = 0; u < kDeep; ++u) {
         result(t[u]);
-        Vec<T, V>::store(to + u * out, t[u]);
+        Vec<T, V>::template store<STREAM>(to + u * out, t[u]);
       }
     }
     for (; p < p1; p += rows, from += in, to += out) {
       float t[V];
       Vec<T, V>::load(from, t);
       result(t);
-      Vec<T, V>::store(to, t);
+      Vec<T, V>::template store<STREAM>(to, t);
     }
   }
 }
@@ -276,15 +278,15 @@ __global__ __launch_bounds__(kThreads) void norm_stats_tokens_kernel(NormArgs a)
 }
 
 // Result of `each` groups over `run` chunks of pixels.
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, bool STREAM>
 __global__ __launch_bounds__(kThreads) void norm_apply_tokens_kernel(NormArgs a, int each, int run, int runs) {
   extern __shared__ float2 stats[];  // [each]
   const int k = blockIdx.x % runs, rest = blockIdx.x / runs;
   const int g0 = rest % (a.groups / each) * each, n = rest / (a.groups / each);
-  merge_chunks(a, n, g0, g0 + each, stats);
+  merge_chunks<kThreads>(a, n, g0, g0 + each, stats);
   __syncthreads();
   const int64_t p0 = (int64_t)k * run * a.chunk, p1 = min(p0 + run * a.chunk, a.pixels);
-  apply_tokens<T, V, ACT, kThreads>(a, (const T*)a.x + n * a.image_stride, (T*)a.y + n * a.pixels * a.channels,
+  apply_tokens<T, V, ACT, kThreads, STREAM>(a, (const T*)a.x + n * a.image_stride, (T*)a.y + n * a.pixels * a.channels,
                                     g0 * a.cpg, each * a.cpg, p0, p1, stats);
 }
 
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(kOneThreads) void norm_one_tokens_kernel(NormArgs a
   merge_channels<kOneThreads>(a, lds, groups, (double)a.pixels,
                  [&](int g, double m, double v) { stats[g] = make_float2((float)m, (float)(1.0 / sqrt(v / all + eps))); });
   __syncthreads();
-  apply_tokens<T, V, ACT, kOneThreads>(a, x, (T*)a.y + n * a.pixels * a.channels, g0 * a.cpg, cn, 0, a.pixels, stats);
+  apply_tokens<T, V, ACT, kOneThreads, false>(a, x, (T*)a.y + n * a.pixels * a.channels, g0 * a.cpg, cn, 0, a.pixels, stats);
 }
 
 // Mean and squared deviations of pixels [p0, p1) of one group's channels,
@@ -349,11 +351,11 @@ __device__ double2 group_moments(const NormArgs& a, const T* x, int64_t p0, int6
 
 // Statistics of one chunk of pixels of one group, channels first.
 template <class T, int V>
-__global__ __launch_bounds__(kThreads) void norm_stats_blobs_kernel(NormArgs a) {
+__global__ __launch_bounds__(kBlobThreads) void norm_stats_blobs_kernel(NormArgs a) {
   const int g = blockIdx.x % a.groups, nk = blockIdx.x / a.groups;
   const int n = nk / a.chunks, k = nk % a.chunks;
   const int64_t p0 = (int64_t)k * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
-  const double2 m = group_moments<T, V, kThreads>(a, (const T*)a.x + n * a.image_stride + (int64_t)g * a.cpg * a.row_stride, p0, p1);
+  const double2 m = group_moments<T, V, kBlobThreads>(a, (const T*)a.x + n * a.image_stride + (int64_t)g * a.cpg * a.row_stride, p0, p1);
   if (threadIdx.x == 0) a.part[(int64_t)nk * a.groups + g] = m;
 }
 
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(kOneThreads) void norm_one_blobs_kernel(NormArgs a,
 // A tile of kTile channels x kTile pixels through LDS: read along the pixels,
 // written along the channels.
 template <class T, int ACT>
-__global__ __launch_bounds__(kThreads) void norm_apply_blobs_kernel(NormArgs a, int ptiles, int ctiles) {
+__global__ __launch_bounds__(kBlobThreads) void norm_apply_blobs_kernel(NormArgs a, int ptiles, int ctiles) {
   __shared__ float tile[kTile][kTile + 1];
   __shared__ float2 stat[kTile];
   const int pt = blockIdx.x % ptiles, rest = blockIdx.x / ptiles;
@@ -388,19 +390,19 @@ __global__ __launch_bounds__(kThreads) void norm_apply_blobs_kernel(NormArgs a, 
   const int64_t p0 = (int64_t)pt * kTile;
   const int cn = min(kTile, a.channels - c0), pn = (int)min((int64_t)kTile, a.pixels - p0);
   const int g0 = c0 / a.cpg, g1 = (c0 + cn - 1) / a.cpg + 1;
-  merge_chunks(a, n, g0, g1, stat);
+  merge_chunks<kBlobThreads>(a, n, g0, g1, stat);
   const T* x = (const T*)a.x + n * a.image_stride + p0;
   T* y = (T*)a.y + (n * a.pixels + p0) * a.channels + c0;
   const int lane = threadIdx.x % kTile, row = threadIdx.x / kTile;
 #pragma unroll 4
-  for (int c = row; c < cn; c += kThreads / kTile)
+  for (int c = row; c < cn; c += kBlobThreads / kTile)
     if (lane < pn) tile[c][lane] = (float)x[(int64_t)(c0 + c) * a.row_stride + lane];
   __syncthreads();
   if (lane >= cn) return;
   const float2 s = stat[(c0 + lane) / a.cpg - g0];
   const float scale = s.y * a.affine[c0 + lane], beta = a.affine[a.channels + c0 + lane];
 #pragma unroll 4
-  for (int p = row; p < pn; p += kThreads / kTile)
+  for (int p = row; p < pn; p += kBlobThreads / kTile)
     y[(int64_t)p * a.channels + lane] = (T)activate<ACT>(fmaf(tile[lane][p] - s.x, scale, beta));
 }
 
@@ -411,7 +413,9 @@ __global__ __launch_bounds__(kThreads) void norm_apply_blobs_kernel(NormArgs a, 
 // a workgroup walks its groups' pixels alone.  Measured, us a call (two
 // launches / one): tokens of 50 KB to a workgroup 11.8 / 9.0 (784 x 512 bf16)
 // and 12.8 / 8.2 (fp32), of 200 KB 12.7 / 13.1 (fp32) and 11.5 / 17.4 (bf16);
-// blobs of 3136 values 12 / 8, of 12544 12.0 / 10.2, of 25088 12.4 / 16.3.
+// blobs of 3136 values 12 / 8, of 12544 12.0 / 10.2, of 25088 12.4 / 16.3.  Of
+// tensors past 10 MB (tokens) or 16 MB (blobs) the launches no longer count:
+// 32 x 784 x 512 fp32 30 / 42.
 int groups_of_one(int channels, int groups, int layout, int es, int64_t n, int64_t pixels) {
   const int cpg = channels / groups;
   int each = 1;
@@ -420,7 +424,9 @@ int groups_of_one(int channels, int groups, int layout, int es, int64_t n, int64
   const int64_t values = pixels * each * cpg;
   const int force = setting_int("NHIP_NORM_ONE", -1);
   if (force == 0 || values > (1 << 28) || n * (groups / each) > 0x7fffffff) return 0;
-  return force == 1 || (layout == NHIP_LAYOUT_TOKENS ? values * es <= 65536 : values <= 16384) ? each : 0;
+  const int64_t bytes = n * pixels * channels * es;
+  return force == 1 || (layout == NHIP_LAYOUT_TOKENS ? values * es <= 65536 && bytes <= 10000000
+                                                     : values <= 16384 && bytes <= 16000000) ? each : 0;
 }
 
 // Chunks of an image: enough workgroups for two to a CU (tokens) or four
@@ -467,7 +473,7 @@ int norm_apply(const NormArgs& a, int layout, int n, bool vec, hipStream_t s) {
   if (layout == NHIP_LAYOUT_BLOBS) {
     const int pt = (int)ceil_div(a.pixels, kTile), ct = (int)ceil_div(a.channels, kTile);
     NHIP_LAUNCH("group_norm_apply", (norm_apply_blobs_kernel<T, ACT>), dim3((uint32_t)((int64_t)pt * ct * n)),
-                dim3(kThreads), 0, s, a, pt, ct);
+                dim3(kBlobThreads), 0, s, a, pt, ct);
   } else {
     // Many chunks to merge: a workgroup takes fewer groups (of 256 bytes of a
     // pixel at least) and as many more chunks.  us a call without / with this:
@@ -479,12 +485,14 @@ int norm_apply(const NormArgs& a, int layout, int n, bool vec, hipStream_t s) {
       while (each % 2 == 0 && each / 2 * a.cpg * (int)sizeof(T) >= 256 && (!vec || each / 2 * a.cpg % V == 0)) each /= 2;
     const int run = a.groups / each, runs = (int)ceil_div(a.chunks, run);
     const dim3 grid((uint32_t)((int64_t)n * runs * run));
+    const auto launch = [&](auto kernel) {
+      NHIP_LAUNCH("group_norm_apply", kernel, grid, dim3(kThreads), each * sizeof(float2), s, a, each, run, runs);
+    };
     if (vec)
-      NHIP_LAUNCH("group_norm_apply", (norm_apply_tokens_kernel<T, V, ACT>), grid, dim3(kThreads), each * sizeof(float2), s, a,
-                  each, run, runs);
+      // us without / with: 257 MB 165 / 144, 128 MB 87 / 73, 103 MB 69 / 57, 51 MB 33.0 / 32.7
+      n * a.pixels * a.channels * (int64_t)sizeof(T) > kStreamBytes ? launch(norm_apply_tokens_kernel<T, V, ACT, true>) : launch(norm_apply_tokens_kernel<T, V, ACT, false>);
     else
-      NHIP_LAUNCH("group_norm_apply", (norm_apply_tokens_kernel<T, 1, ACT>), grid, dim3(kThreads), each * sizeof(float2), s, a,
-                  each, run, runs);
+      launch(norm_apply_tokens_kernel<T, 1, ACT, false>);
   }
   return check_launch("group_norm_apply");
 }
@@ -503,12 +511,15 @@ int norm_one(const NormArgs& a, int layout, int n, int groups, bool vec, hipStre
       NHIP_LAUNCH("group_norm_one", (norm_one_blobs_kernel<T, V, ACT>), grid, dim3(kOneThreads), 0, s, a, fast_div(a.cpg));
     else
       NHIP_LAUNCH("group_norm_one", (norm_one_blobs_kernel<T, 1, ACT>), grid, dim3(kOneThreads), 0, s, a, fast_div(a.cpg));
-  } else if (vec && groups * a.cpg % V == 0) {
-    NHIP_LAUNCH("group_norm_one", (norm_one_tokens_kernel<T, V, ACT>), grid, dim3(kOneThreads),
-                stats_lds<T>(groups * a.cpg, V, kOneThreads), s, a, groups);
   } else {
-    NHIP_LAUNCH("group_norm_one", (norm_one_tokens_kernel<T, 1, ACT>), grid, dim3(kOneThreads),
-                stats_lds<T>(groups * a.cpg, 1, kOneThreads), s, a, groups);
+    const bool wide = vec && groups * a.cpg % V == 0;
+    const size_t lds = stats_lds<T>(groups * a.cpg, wide ? V : 1, kOneThreads);
+    const void* kernel = wide ? (const void*)norm_one_tokens_kernel<T, V, ACT> : (const void*)norm_one_tokens_kernel<T, 1, ACT>;
+    if (lds > 65536) NHIP_TRY(ensure_dynamic_lds(kernel, 160 * 1024));
+    if (wide)
+      NHIP_LAUNCH("group_norm_one", (norm_one_tokens_kernel<T, V, ACT>), grid, dim3(kOneThreads), lds, s, a, groups);
+    else
+      NHIP_LAUNCH("group_norm_one", (norm_one_tokens_kernel<T, 1, ACT>), grid, dim3(kOneThreads), lds, s, a, groups);
   }
   return check_launch("group_norm_one");
 }
@@ -528,17 +539,21 @@ int norm_run(const NormArgs& a, int layout, int n, int one, hipStream_t s) {
   if (blobs) {
     const dim3 grid((uint32_t)((int64_t)n * a.chunks * a.groups));
     if (vec)
-      NHIP_LAUNCH("group_norm_stats", (norm_stats_blobs_kernel<T, V>), grid, dim3(kThreads), 0, s, a);
+      NHIP_LAUNCH("group_norm_stats", (norm_stats_blobs_kernel<T, V>), grid, dim3(kBlobThreads), 0, s, a);
     else
-      NHIP_LAUNCH("group_norm_stats", (norm_stats_blobs_kernel<T, 1>), grid, dim3(kThreads), 0, s, a);
+      NHIP_LAUNCH("group_norm_stats", (norm_stats_blobs_kernel<T, 1>), grid, dim3(kBlobThreads), 0, s, a);
   } else {
     const dim3 grid((uint32_t)(n * a.chunks));
-    if (vec)
-      NHIP_LAUNCH("group_norm_stats", (norm_stats_tokens_kernel<T, V>), grid, dim3(kThreads),
-                  stats_lds<T>(a.channels, V, kThreads), s, a);
-    else
-      NHIP_LAUNCH("group_norm_stats", (norm_stats_tokens_kernel<T, 1>), grid, dim3(kThreads),
-                  stats_lds<T>(a.channels, 1, kThreads), s, a);
+    const size_t lds = stats_lds<T>(a.channels, vec ? V : 1, kThreads);
+    const auto launch = [&](auto kernel) {
+      if (lds > 65536) {
+        const int st = ensure_dynamic_lds((const void*)kernel, 160 * 1024);
+        if (st != NHIP_STATUS_SUCCESS) return st;
+      }
+      NHIP_LAUNCH("group_norm_stats", kernel, grid, dim3(kThreads), lds, s, a);
+      return ok();
+    };
+    NHIP_TRY(vec ? launch(norm_stats_tokens_kernel<T, V>) : launch(norm_stats_tokens_kernel<T, 1>));
   }
   NHIP_TRY(check_launch("group_norm_stats"));
   switch (a.act) {

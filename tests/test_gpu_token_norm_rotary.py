@@ -232,3 +232,27 @@ def test_wrapper_refusals():
             rot.forward(t, bad)
     with pytest.raises(nhip.NhipError):  # an output whose tokens overlap
         rot.forward(t, p, out=torch.zeros((2, 1, 1, 16), device="cuda").expand(2, 3, 1, 16))
+
+
+# ------------------------------------------------- past the last-level cache
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_group_norm_past_the_cache(dtype):
+    n, pixels, c = 36, 6007, 256 if dtype == BF16 else 128
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((n, pixels, c), generator=g, device="cuda").to(dtype)
+    gamma, beta = affine(c)
+    y = nhip.GroupNorm(16, c, gamma, beta, act=nhip.ACT_RELU).forward(x)
+    for i in (0, 17, 35):
+        want, bound = ref.group_norm(x[i:i + 1], 16, gamma, beta, 1e-5, "relu")
+        ref.assert_within(y[i:i + 1], want, bound)
+
+
+@pytest.mark.parametrize("neighbours", [False, True])
+def test_rotary_past_the_cache(neighbours):
+    n = 80001
+    x = torch.randn((1, n, 8, 128), generator=torch.Generator(device="cuda").manual_seed(4), device="cuda", dtype=F16)
+    pos = positions(5, 1, n, 2).cuda()
+    rot = nhip.Rotary(128, (20, 20), neighbours=neighbours)
+    y = rot.forward(x, pos)
+    for a, b in ((0, 777), (40000, 40100), (n - 5, n)):
+        assert torch.equal(y[:, a:b], rot.forward(x[:, a:b], pos[:, a:b].contiguous()))
