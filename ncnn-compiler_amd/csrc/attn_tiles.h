@@ -402,12 +402,12 @@ __global__ __launch_bounds__(kWaves * 64, (TilesShape<T, DP, SRC>::per_cu)) void
 #pragma unroll
                 for (int c = 0; c < DT; ++c) {
                   const __amdgpu_buffer_rsrc_t rows = make_rsrc(vbase + (int64_t)key0 * a.vs[1], 0x7fffffffu);
-                  int vcol = col;
-                  asm volatile("" : "+v"(vcol));
+                  int vcol = col, vh = h;
+                  asm volatile("" : "+v"(vcol), "+v"(vh));
                   v8f vf;
 #pragma unroll
                   for (int i = 0; i < 8; ++i) {
-                    const int r = t * 32 + u * 16 + 8 * (i >> 2) + 4 * h + (i & 3), ch = c * 32 + vcol;
+                    const int r = t * 32 + u * 16 + 8 * (i >> 2) + 4 * vh + (i & 3), ch = c * 32 + vcol;
                     const bool counts = (keys.counts >> r & 1) && ch < a.d;
                     vf[i] = buf_load_f32(rows, counts ? (r * (uint32_t)a.vs[1] + ch) * 4u : kBufOOB);
                   }
