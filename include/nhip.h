@@ -349,7 +349,10 @@ int nhip_dequantize_i32_f32(const int32_t* input, float* output, int32_t n,
  * integer ones.  Sums, softmax statistics and angles are held in fp32 or
  * more, results rounded once.  Strides count elements; channels and head
  * channels are always contiguous.  Tensors may have any alignment that their
- * type needs; 16-byte aligned rows take the wide loads.  The calls allocate
+ * type needs, and 16-byte aligned rows take the wide loads; but queries and
+ * results of the attention over the cache, values read from it and workspaces
+ * have to be 16-byte aligned.  A workspace is needed where its size is not 0;
+ * the size asked for covers any strides and alignment.  The calls allocate
  * nothing, so they may be recorded into a HIP graph.
  * ------------------------------------------------------------------------- */
 
@@ -438,10 +441,11 @@ int nhip_cross_attention_forward(
  * one sequence: codes k, v int8 [pages][kv_heads][block_tokens][head_dim] and
  * a scale for each page and head, k_scale, v_scale fp32 [pages][kv_heads]; a
  * code q stands for q * scale.  block_tokens: 16, 32, 64, 128 or 256;
- * head_dim a multiple of 8, at most 256; codes 16-byte aligned.  Which pages a sequence has
- * stands in its row of a block table: int32 [batch][table_pages], token t in
- * page table[b][t / block_tokens].  Tokens of a page number outside
- * 0..pages-1, or past the table, are not written, read as 0 and not seen. */
+ * head_dim a multiple of 8, at most 256; codes 16-byte aligned; codes of a
+ * page whose scale is 0 are 0.  Which pages a sequence has stands in its row
+ * of a block table: int32 [batch][table_pages], token t in page
+ * table[b][t / block_tokens].  Tokens of a page number outside 0..pages-1, or
+ * past the table, are not written, read as 0 and not seen. */
 typedef struct nhip_kv8_cache {
   int8_t* k;
   int8_t* v;

@@ -5,6 +5,12 @@
 // (a mean and a sum of squared deviations each), and a pass that merges them
 // and writes y.  Both stream the tensor, so bytes bound them: x is read
 // twice, the second time from the last-level cache where the tensor fits.
+// Measured: 32 x 3136 x 256 bf16 32 us a call (statistics 12, result 20: 5.1
+// TB/s, as a large copy); 8 x 50175 x 320 f16 129-139 us (47 and 83-94; floor
+// with one reading 99).  Images two at a time, so that the second reading stays
+// in the last-level cache, were no faster (153).  Small tensors take one launch
+// (5.5 us on the device at 1 x 128 x 28 x 28 fp32 blobs; a call is bound by the
+// host's 7.1).
 //
 // Statistics: sums of x - s and (x - s)^2 with s one of the values summed, over
 // at most a few hundred terms of a thread; means and squared deviations of

@@ -11,6 +11,8 @@
 //
 // Bytes bound it: every element is read and written once.  A thread forms the
 // sines and cosines of its pairs once and walks a few heads with them.
+// Measured: 2 x 25088 tokens, 16 heads of 128 bf16 (411 MB) 78 us, 5.3 TB/s, what
+// a large copy reaches; 32 single tokens 4 us on the device, 7.2 a call.
 #include <algorithm>
 #include <cmath>
 #include <new>

@@ -10,6 +10,10 @@ Layer objects mirror the reference's ncnn layer parameters
 (include/ncnn-mlir/Graph/graph.hpp:73-150) and its lowering semantics
 (lib/Conversion/NCNNToTosa/NCNNToTosa.cpp); batches are [N,C,H,W] stacks of the
 reference's single-image [C,H,W] blobs.
+
+Behind the layers stand the token operators, for a decoder that reads a
+network's features: GroupNorm, Rotary, cross_attention and KvCache8 (float32,
+float16 and bfloat16; no counterpart in the reference).
 """
 from __future__ import annotations
 
