@@ -1,16 +1,18 @@
 // Group norm with an activation into channels-last tokens:
 //   y = act((x - mean_g) / sqrt(var_g + eps) * gamma_c + beta_c).
 //
-// Two launches: the statistics of every (image, group) over chunks of pixels
-// (a mean and a sum of squared deviations each), and a pass that merges them
-// and writes y.  Both stream the tensor, so bytes bound them: x is read
-// twice, the second time from the last-level cache where the tensor fits.
-// Measured: 32 x 3136 x 256 bf16 32 us a call (statistics 12, result 20: 5.1
-// TB/s, as a large copy); 8 x 50175 x 320 f16 129-139 us (47 and 83-94; floor
-// with one reading 99).  Images two at a time, so that the second reading stays
-// in the last-level cache, were no faster (153).  Small tensors take one launch
-// (5.5 us on the device at 1 x 128 x 28 x 28 fp32 blobs; a call is bound by the
-// host's 7.1).
+// Bytes bound it.  Where a few groups of an image fit a workgroup's registers,
+// it reads them once, sums, and writes y.  Else two launches: the statistics of
+// every (image, group) over chunks of pixels (a mean and a sum of squared
+// deviations each), and a pass that merges them and writes y: x is read twice,
+// the second time from the last-level cache where the tensor fits.
+// Measured: 32 x 3136 x 256 bf16 25 us a call (103 MB moved, 4.1 TB/s; two
+// launches 31.4), 128 x 784 x 512 bf16 39 us (5.3 TB/s, as a large copy; two
+// launches 54); 8 x 50175 x 320 f16, in two launches, 129-139 us (47 and 83-94;
+// floor with one reading 99).  Images two at a time, so that the second
+// reading stays in the last-level cache, were no faster (153).  Small tensors
+// take one launch that reads twice (5.5 us on the device at 1 x 128 x 28 x 28
+// fp32 blobs; a call is bound by the host's 7.1).
 //
 // Statistics: sums of x - s and (x - s)^2 with s one of the values summed, over
 // at most a few hundred terms of a thread; means and squared deviations of
@@ -38,6 +40,7 @@ namespace {
 constexpr int kThreads = 512;      // of a workgroup, tokens
 constexpr int kBlobThreads = 256;  // blobs, two launches
 constexpr int kOneThreads = 512;   // of a workgroup that does its groups alone
+constexpr int kHeld = 16;  // vectors that a thread holds at most (single reading)
 constexpr int kMaxChannels = 4096;
 constexpr int kMaxChunks = 256;  // parts of an image: what each workgroup of the second pass merges
 constexpr int kDeep = 4;         // vectors of a thread under way at once
@@ -123,17 +126,78 @@ __device__ void merge_chunks(const NormArgs& a, int n, int g0, int g1, float2* s
   }
 }
 
+// Where the threads' sums stand: first powers, second, and each channel's of
+// several threads.
+template <class T, int V, int TH>
+struct Sums {
+  typedef typename First<T>::type S;
+  S *red1, *more1;
+  float *red2, *more2;
+  __device__ __forceinline__ explicit Sums(void* red) {
+    red1 = reinterpret_cast<S*>(red);
+    more1 = red1 + TH * V;
+    red2 = reinterpret_cast<float*>(more1 + TH);
+    more2 = red2 + TH * V;
+  }
+  __device__ __forceinline__ void put(int thread, const S (&s1)[V], const float (&s2)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      red1[thread * V + i] = s1[i];
+      red2[thread * V + i] = s2[i];
+    }
+  }
+};
+
+// Adds the sums of `rows` threads for each of `cols` vectors of channels, those
+// of a channel by as many threads as there are for it, then by one: means and
+// squared deviations of `count` values each to ch.  shift: what each channel's
+// values were taken from.
+template <class T, int V, int TH>
+__device__ void sum_channels(const T* shift, int cols, int rows, double count, double2* ch, const Sums<T, V, TH>& sums) {
+  typedef typename First<T>::type S;
+  const S* red1 = sums.red1;
+  S* more1 = sums.more1;
+  const float* red2 = sums.red2;
+  float* more2 = sums.more2;
+  __syncthreads();
+  const int cv = cols * V, parts = max(1, TH / cv);
+  for (int i = threadIdx.x; i < cv * parts; i += TH) {  // parts > 1: one step
+    const int c = i % cv;
+    S u1 = 0;
+    float u2 = 0.f;
+    for (int r = i / cv; r < rows; r += parts) {
+      u1 += red1[r * cv + c];
+      u2 += red2[r * cv + c];
+    }
+    if (parts == 1) {
+      ch[c] = moments(u1, u2, (float)shift[c], count);
+    } else {
+      more1[i] = u1;
+      more2[i] = u2;
+    }
+  }
+  __syncthreads();
+  if (parts > 1) {  // uniform
+    if (threadIdx.x < cv) {
+      S u1 = 0;
+      float u2 = 0.f;
+      for (int q = 0; q < parts; ++q) {
+        u1 += more1[q * cv + threadIdx.x];
+        u2 += more2[q * cv + threadIdx.x];
+      }
+      ch[threadIdx.x] = moments(u1, u2, (float)shift[threadIdx.x], count);
+    }
+    __syncthreads();
+  }
+}
+
 // Means and squared deviations of channels [c0, c0 + cn) over pixels [p0, p1)
 // of one image (x: its first pixel), channels last, to ch[0, cn).  A thread
-// keeps its V channels and walks pixels; `red` holds the threads' sums: those
-// of a channel are added by as many threads as there are for it, then by one.
+// keeps its V channels and walks pixels; `red` holds the threads' sums.
 template <class T, int V, int TH>
 __device__ void channel_moments(const NormArgs& a, const T* x, int c0, int cn, int64_t p0, int64_t p1, double2* ch, void* red) {
   typedef typename First<T>::type S;
-  S* red1 = reinterpret_cast<S*>(red);
-  S* more1 = red1 + TH * V;
-  float* red2 = reinterpret_cast<float*>(more1 + TH);
-  float* more2 = red2 + TH * V;
+  const Sums<T, V, TH> sums(red);
   const int vecs = cn / V;
   for (int v0 = 0; v0 < vecs; v0 += TH) {
     const int cols = min(TH, vecs - v0), rows = TH / cols;
@@ -166,42 +230,9 @@ __device__ void channel_moments(const NormArgs& a, const T* x, int c0, int cn, i
         Vec<T, V>::load(at, t);
         add(t);
       }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        red1[(row * cols + col) * V + i] = s1[i];
-        red2[(row * cols + col) * V + i] = s2[i];
-      }
+      sums.put(row * cols + col, s1, s2);
     }
-    __syncthreads();
-    const int cv = cols * V, parts = max(1, TH / cv);
-    for (int i = threadIdx.x; i < cv * parts; i += TH) {  // parts > 1: one step
-      const int c = i % cv;
-      S u1 = 0;
-      float u2 = 0.f;
-      for (int r = i / cv; r < rows; r += parts) {
-        u1 += red1[r * cv + c];
-        u2 += red2[r * cv + c];
-      }
-      if (parts == 1) {
-        ch[v0 * V + c] = moments(u1, u2, (float)x[p0 * a.row_stride + c0 + v0 * V + c], (double)(p1 - p0));
-      } else {
-        more1[i] = u1;
-        more2[i] = u2;
-      }
-    }
-    __syncthreads();
-    if (parts > 1) {  // uniform
-      if (threadIdx.x < cv) {
-        S u1 = 0;
-        float u2 = 0.f;
-        for (int q = 0; q < parts; ++q) {
-          u1 += more1[q * cv + threadIdx.x];
-          u2 += more2[q * cv + threadIdx.x];
-        }
-        ch[v0 * V + threadIdx.x] = moments(u1, u2, (float)x[p0 * a.row_stride + c0 + v0 * V + threadIdx.x], (double)(p1 - p0));
-      }
-      __syncthreads();
-    }
+    sum_channels<T, V, TH>(x + p0 * a.row_stride + c0 + v0 * V, cols, rows, (double)(p1 - p0), ch + v0 * V, sums);
   }
 }
 
@@ -311,6 +342,68 @@ __global__ __launch_bounds__(kOneThreads) void norm_one_tokens_kernel(NormArgs a
                  [&](int g, double m, double v) { stats[g] = make_float2((float)m, (float)(1.0 / sqrt(v / all + eps))); });
   __syncthreads();
   apply_tokens<T, V, ACT, kOneThreads, false>(a, x, (T*)a.y + n * a.pixels * a.channels, g0 * a.cpg, cn, 0, a.pixels, stats);
+}
+
+// A workgroup does a few whole groups of an image whose values its threads
+// hold, so that x is read once: all loads first, then the statistics, then the
+// results.  (At most kHeld times the workgroup's rows of pixels; whole vectors.)
+template <class T, int V, int ACT, int TH, bool STREAM>
+__global__ __launch_bounds__(TH) void norm_held_tokens_kernel(NormArgs a, int groups, int wgs) {
+  typedef typename First<T>::type S;
+  extern __shared__ double2 lds[];  // as norm_one_tokens_kernel's
+  // workgroups go to the eight dies in turn: an image's parts, which share
+  // lines of memory, to one of them
+  const int wg = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (wg >= wgs) return;
+  const int parts = a.groups / groups, n = wg / parts, c0 = wg % parts * groups * a.cpg;
+  const int cn = groups * a.cpg, cols = cn / V, rows = TH / cols, pixels = (int)a.pixels;
+  const int col = threadIdx.x % cols, row = threadIdx.x / cols;
+  const T* x = (const T*)a.x + n * a.image_stride + c0;
+  typename Vec<T, V>::type held[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)  // (past the last pixel: that one again)
+    if (u * rows < pixels) held[u] = *reinterpret_cast<const typename Vec<T, V>::type*>(x + min(row + u * rows, pixels - 1) * a.row_stride + col * V);
+  float shift[V];
+  Vec<T, V>::load(x + col * V, shift);
+  const int mine = row < rows ? (pixels - row + rows - 1) / rows : 0;  // vectors that count
+  const Sums<T, V, TH> sums(lds + cn);
+  {
+    S s1[V] = {};
+    float s2[V] = {};
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+      if (u < mine)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float t = (float)held[u][i], d = t - shift[i];
+          s1[i] += first_power(t, d, S());
+          s2[i] = fmaf(d, d, s2[i]);
+        }
+    if (row < rows) sums.put(row * cols + col, s1, s2);
+  }
+  sum_channels<T, V, TH>(x, cols, rows, (double)a.pixels, lds, sums);
+  float2* stats = reinterpret_cast<float2*>(lds + cn);
+  const double all = (double)a.pixels * a.cpg, eps = a.eps;
+  merge_channels<TH>(a, lds, groups, (double)a.pixels,
+                 [&](int g, double m, double v) { stats[g] = make_float2((float)m, (float)(1.0 / sqrt(v / all + eps))); });
+  __syncthreads();
+  float mean[V], scale[V], beta[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float2 s = stats[(col * V + i) / a.cpg];
+    mean[i] = s.x;
+    scale[i] = s.y * a.affine[c0 + col * V + i];
+    beta[i] = a.affine[a.channels + c0 + col * V + i];
+  }
+  T* y = (T*)a.y + (n * a.pixels + row) * a.channels + c0 + col * V;
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (u < mine) {
+      float t[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) t[i] = activate<ACT>(fmaf((float)held[u][i] - mean[i], scale[i], beta[i]));
+      Vec<T, V>::template store<STREAM>(y + (int64_t)u * rows * a.channels, t);
+    }
 }
 
 // Mean and squared deviations of pixels [p0, p1) of one group's channels,
@@ -429,7 +522,7 @@ int groups_of_one(int channels, int groups, int layout, int es, int64_t n, int64
     while (each * cpg * es < 64 && groups % (2 * each) == 0) each *= 2;
   const int64_t values = pixels * each * cpg;
   const int force = setting_int("NHIP_NORM_ONE", -1);
-  if (force == 0 || values > (1 << 28) || n * (groups / each) > 0x7fffffff) return 0;
+  if (force == 0 || force == 2 || values > (1 << 28) || n * (groups / each) > 0x7fffffff) return 0;
   const int64_t bytes = n * pixels * channels * es;
   return force == 1 || (layout == NHIP_LAYOUT_TOKENS ? values * es <= 65536 && bytes <= 10000000
                                                      : values <= 16384 && bytes <= 16000000) ? each : 0;
@@ -530,6 +623,70 @@ int norm_one(const NormArgs& a, int layout, int n, int groups, bool vec, hipStre
   return check_launch("group_norm_one");
 }
 
+// Groups that a workgroup which holds their values does, and its threads
+// (tokens of whole 16-byte vectors): groups whose channels fill 64 bytes of a
+// pixel, more of them where threads and workgroups are left.  0: not here.
+//
+// us a call, two launches / held.  Of 256 or 512 threads, several to a CU: 64 x
+// 784 x 512 bf16 32.6 / 23.9, 128 x 53.7 / 39.0, 32 x fp32 29.8 / 20.5, 16 x
+// 1024 x 1280 f16 29.2 / 21.4; of 512 threads and 8 / 64 workgroups 11.2 / 12.0,
+// 14.9 / 12.6.  Rows that are no whole 64 bytes share lines with their
+// neighbours, which costs where results are past the caches: 1024 x 640 f16 of 42
+// / 84 MB 28.0 / 21.5, 45.7 / 55.2.  Of 1024 threads, one to a CU, with nothing
+// beside its waits: 3136 x 256 bf16 of 128 / 192 / 256 / 384 / 512 / 1024
+// workgroups 20.9 / 22.0, 29.4 / 23.4, 31.4 / 25.0, 49.0 / 45.0, 53.0 / 50.8, 112 / 118.
+struct Held {
+  int groups, threads;
+};
+Held groups_held(const NormArgs& a, int n, int es) {
+  const int force = setting_int("NHIP_NORM_ONE", -1);
+  if (force == 0 || force == 1) return {0, 0};
+  const auto threads_of = [&](int each) {
+    const int cols = each * a.cpg * es / 16;
+    for (int th : {256, 512, 1024})
+      if (cols <= th && a.pixels <= (int64_t)kHeld * (th / cols)) return th;
+    return 0;
+  };
+  int each = 1;
+  while ((each * a.cpg * es < 64 || each * a.cpg * es % 16) && a.groups % (2 * each) == 0) each *= 2;
+  if (each * a.cpg * es % 16 || !threads_of(each)) return {0, 0};
+  while (a.groups % (2 * each) == 0 && threads_of(2 * each) == 256 && (int64_t)n * (a.groups / (2 * each)) >= 4 * cu_count()) each *= 2;
+  const int64_t wgs = (int64_t)n * (a.groups / each);
+  if (wgs > 0x7fffff00) return {0, 0};
+  const Held held{each, threads_of(each)};
+  if (force == 2) return held;
+  if (each * a.cpg * es % 64 && n * a.pixels * a.channels * es > kStreamBytes) return {0, 0};
+  if (held.threads == 512 && wgs * 4 < cu_count()) return {0, 0};
+  if (held.threads == 1024 && (wgs * 4 < 3 * cu_count() || wgs > 2 * cu_count())) return {0, 0};
+  return held;
+}
+
+template <class T, int ACT, int TH>
+int norm_held(const NormArgs& a, int n, int groups, hipStream_t s) {
+  constexpr int V = kVec<T>;
+  const int wgs = n * (a.groups / groups);
+  const size_t lds = stats_lds<T>(groups * a.cpg, V, TH);
+  const auto launch = [&](auto kernel) {
+    if (lds > 65536) {
+      const int st = ensure_dynamic_lds((const void*)kernel, 160 * 1024);
+      if (st != NHIP_STATUS_SUCCESS) return st;
+    }
+    NHIP_LAUNCH("group_norm_held", kernel, dim3((uint32_t)ceil_div(wgs, 8) * 8), dim3(TH), lds, s, a, groups, wgs);
+    return check_launch("group_norm_held");
+  };
+  const bool stream = n * a.pixels * a.channels * (int64_t)sizeof(T) > kStreamBytes && groups * a.cpg * sizeof(T) % 64 == 0;
+  return stream ? launch(norm_held_tokens_kernel<T, V, ACT, TH, true>) : launch(norm_held_tokens_kernel<T, V, ACT, TH, false>);
+}
+
+template <class T, int ACT>
+int norm_held(const NormArgs& a, int n, Held held, hipStream_t s) {
+  switch (held.threads) {
+    case 256: return norm_held<T, ACT, 256>(a, n, held.groups, s);
+    case 512: return norm_held<T, ACT, 512>(a, n, held.groups, s);
+    default: return norm_held<T, ACT, 1024>(a, n, held.groups, s);
+  }
+}
+
 template <class T>
 int norm_run(const NormArgs& a, int layout, int n, int one, hipStream_t s) {
   constexpr int V = kVec<T>;
@@ -541,6 +698,11 @@ int norm_run(const NormArgs& a, int layout, int n, int one, hipStream_t s) {
       case NHIP_ACT_RELU: return norm_one<T, NHIP_ACT_RELU>(a, layout, n, one, vec, s);
       case NHIP_ACT_SILU: return norm_one<T, NHIP_ACT_SILU>(a, layout, n, one, vec, s);
       default: return norm_one<T, NHIP_ACT_NONE>(a, layout, n, one, vec, s);
+    }
+  if (const Held held = !blobs && vec ? groups_held(a, n, sizeof(T)) : Held{0, 0}; held.groups) switch (a.act) {
+      case NHIP_ACT_RELU: return norm_held<T, NHIP_ACT_RELU>(a, n, held, s);
+      case NHIP_ACT_SILU: return norm_held<T, NHIP_ACT_SILU>(a, n, held, s);
+      default: return norm_held<T, NHIP_ACT_NONE>(a, n, held, s);
     }
   if (blobs) {
     const dim3 grid((uint32_t)((int64_t)n * a.chunks * a.groups));
