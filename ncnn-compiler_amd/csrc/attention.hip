@@ -65,9 +65,15 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
   // the CUs empty; then as many workers as there are places, the work dealt to
   // them in equal runs of at least 256 keys.
   const int keys = a->d > (d->dtype == NHIP_DTYPE_F32 ? 64 : 128) ? 32 : 64;  // of a tile
-  const int64_t places = (int64_t)cu_count() * (a->d <= (d->dtype == NHIP_DTYPE_F32 ? 64 : 128) ? 2 : 1);
+  int64_t places = (int64_t)cu_count() * (a->d <= (d->dtype == NHIP_DTYPE_F32 ? 64 : 128) ? 2 : 1);
   a->workers = (int)wgs;
   a->units = std::max(1, (int)ceil_div(d->keys, keys));
+  // Over the cache, where loads and codes are waited for, heads of 64 have room
+  // for a third workgroup on a CU: us at 2 / 3, 16 heads on 4 of 509 rows to
+  // 6272 keys 69.2 / 65; not in runs below 512 keys, 4 x 256 rows to 2048 keys 30.6 /
+  // 32.2; nor without codes, 1024 rows and keys, 128 heads 52.0 / 70.
+  if (cache && a->d <= 64 && d->dtype != NHIP_DTYPE_F32 && wgs * a->units * keys >= 512 * 3 * (int64_t)cu_count())
+    places = 3 * (int64_t)cu_count();
   if (wgs * 10 < ceil_div(wgs, places) * places * 9 && wgs * a->units < 0x7fffffff) {
     const int64_t workers = std::min(places, wgs * a->units * keys / 256);
     if (workers > wgs || workers == places) a->workers = (int)std::max<int64_t>(1, workers);

@@ -56,7 +56,7 @@ struct TilesShape {
   // second barrier a tile, and two words that say which tile they do not hold.
   static constexpr int buffers = KP == 3 ? 1 : 2;
   static constexpr int bytes = buffers * buffer + (KP == 3 ? 16 : 0);
-  static constexpr int per_cu = (split ? DP == 64 : DP <= 128) ? 2 : 1;
+  static constexpr int per_cu = split ? (DP == 64 ? 2 : 1) : DP == 64 && SRC == kSrcInt8 ? 3 : DP <= 128 ? 2 : 1;
 };
 
 // The next tile on its way, spread over the workgroup.
@@ -177,8 +177,9 @@ __device__ __forceinline__ int worker_of(const AttnArgs& a, uint32_t unit) {
 // TFLOP/s, 21 us of it the join), 4096 rows and keys, whose row tiles fill the
 // CUs evenly, 281-287 us (957-978; a library product of matrices alone 1130).  The
 // rest is the softmax: vector instructions of one wave beside another's products.
-// fp16 over the cache: 2 x 509 rows of 16 heads of 64 to 6272 keys 65 us: half
-// the products to a score and codes to convert, so vector instructions bound it.
+// fp16 over the cache: 2 x 509 rows of 16 heads of 64 to 6272 keys 60 us: half
+// the products to a score and codes to convert, so the waves' other instructions
+// bound it.
 // fp32: 4 x 784 rows of 12 heads of 64 to 197 keys 32 us, of which 12 pass before
 // the first tile and after the last; 2 x 2048 of 16 to 4096 keys 380-390 us (180
 // TFLOP/s; the fp32 instructions' rate is 154), some 1000 vector instructions
