@@ -61,9 +61,15 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
     a->splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(d->keys, 512), 64}));
     return ok();
   }
-  // One row tile to a worker, unless that leaves over a tenth of the places on
-  // the CUs empty; then as many workers as there are places, the work dealt to
-  // them in equal runs of at least 256 keys.
+  // One row tile to a worker, or as many workers as there are places on the
+  // CUs, the work dealt to them in equal runs of at least 256 keys, if that
+  // saves more than it costs: the parts' way through memory and the launch that
+  // joins them, and of each worker's pace a seventh (two row tiles' queries, all
+  // CUs busy).  us, one each / dealt: 4 x 784 rows of 12 heads of 64 bf16 (336
+  // row tiles) to 784 / 1500 / 3136 keys 23.5 / 33.5, 37.2 / 41.4, 68.3 / 63.7, of
+  // 128 35.3 / 48.4, 55.7 / 64.3, 100 / 101, of 64 fp32 76.6 / 75.9, 132 / 116, 257 /
+  // 215; 128, 256, 640 row tiles of 1024 keys of 64 bf16 20.7 / 23.3, 21.8 / 28.0,
+  // 37.6 / 47.9, fp32 63.6 / 43.9, 67.9 / 67.4, 151 / 144; 784 of 12544 of 128 bf16 780 / 703.
   const int keys = a->d > (d->dtype == NHIP_DTYPE_F32 ? 64 : 128) ? 32 : 64;  // of a tile
   int64_t places = (int64_t)cu_count() * (a->d <= (d->dtype == NHIP_DTYPE_F32 ? 64 : 128) ? 2 : 1);
   a->workers = (int)wgs;
@@ -74,7 +80,15 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
   // 32.2; nor without codes, 1024 rows and keys, 128 heads 52.0 / 70.
   if (cache && a->d <= 64 && d->dtype != NHIP_DTYPE_F32 && wgs * a->units * keys >= 512 * 3 * (int64_t)cu_count())
     places = 3 * (int64_t)cu_count();
-  if (wgs * 10 < ceil_div(wgs, places) * places * 9 && wgs * a->units < 0x7fffffff) {
+  // TFLOP/s of a CU, measured; a workgroup alone on a CU with room for two has
+  // 3/4 of what both have together (fp32: 5/8)
+  const bool f32 = d->dtype == NHIP_DTYPE_F32, two = places > cu_count();
+  const double rate = f32 ? (a->d <= 64 ? 0.84 : 0.55) : a->d <= 64 ? (cache ? 2.2 : 3.3) : a->d <= 128 ? 4.3 : 2.0;
+  const double unit = 4e-6 * attn::kTilesRows * keys * a->d / rate;  // us
+  const int64_t rounds = ceil_div(wgs, cu_count());
+  const double each = rounds + (two && rounds % 2 ? (f32 ? 0.6 : 0.33) : 0.0), dealt = 1.15 * wgs / cu_count();
+  const double join = 5 + 2.6 * places * attn::kTilesRows * a->d * sizeof(float) / 5e6;
+  if (a->units * unit * (each - dealt) > join && wgs * a->units < 0x7fffffff) {
     const int64_t workers = std::min(places, wgs * a->units * keys / 256);
     if (workers > wgs || workers == places) a->workers = (int)std::max<int64_t>(1, workers);
   }
