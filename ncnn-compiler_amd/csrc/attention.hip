@@ -35,15 +35,23 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
   // The kernel of few rows reads all keys and values for every 16 of them, some
   // 8 TB/s from the L2s; the one of many reads them once for 128, and its parts
   // are joined in a launch of their own (5 us).  So the second where the first
-  // would read 8 us longer, unless its workgroups leave most CUs idle.  us, few
-  // / many: 64 heads of 3136 keys of 128 bf16, 32 rows 38.1 / 30.9; 192 of 800
-  // of 64, 32 rows 16.4 / 21.0, 64 rows 24.3 / 22.2; 1 of 12544 of 128, 256 rows
-  // 22.8 / 25.4; over the cache 64 heads, 32 rows 31.7 / 34.5, 64 rows 45.0 / 36.5.
+  // would read longer than the second computes, unless its workgroups leave most
+  // CUs idle; and where the first would have several workgroups a CU, each with
+  // its own start.  The bounds are the best over 192 shapes each of 4 to 784 rows,
+  // 197 to 4096 keys (slower than the better kernel by 0.7 and 0.8% in the mean).
+  // us, few / many: 64 heads of 3136 keys of 128 bf16, 32 rows 38.1 / 30.9; 16 heads
+  // of 784 keys of 64 fp32, 256 rows 20.5 / 31.8, of 3136 of 128 102.6 / 64.8; 64
+  // heads of 197 keys, 256 rows of 64 bf16 13.4 / 9.9, of 128 24.3 / 13.6; over the
+  // cache 8 heads of 1024 of 128, 512 rows bf16 22.8 / 39.7, fp32 39.6 / 32.9.
   const int64_t kv_heads = (int64_t)d->batch * d->kv_heads, tiles16 = ceil_div(std::max(a->rows, 1), attn::kRowTile);
+  const bool f32 = d->dtype == NHIP_DTYPE_F32;
   const double bytes = (double)kv_heads * d->keys * d->head_dim * 2 * (cache ? 1 : elem_size(d->dtype));
   const int force = setting_int("NHIP_ATTN_TILES", -1);
+  const int full = cache ? (f32 ? 6 : 8) : f32 || d->head_dim <= 64 ? 6 : 3;  // halves of a CU
+  const double again = cache ? (f32 ? 28e6 : 90e6) : f32 ? 215e6 : 64e6;        // bytes
   a->tiles = vec && force != 0 &&
-             (force == 1 || kv_heads * tiles16 > 4 * cu_count() || (kv_heads * tiles16 > cu_count() / 4 && (tiles16 - 1) * bytes > 64e6));
+             (force == 1 || kv_heads * tiles16 * 2 >= full * cu_count() ||
+              (kv_heads * tiles16 >= cu_count() / 4 && (tiles16 - 1) * bytes > again));
   const int tile = a->tiles ? attn::kTilesRows : attn::kRowTile;
   a->row_tiles = (int)ceil_div(std::max(a->rows, 1), tile);
   const int64_t heads = (int64_t)d->batch * d->kv_heads;
@@ -82,7 +90,7 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
     places = 3 * (int64_t)cu_count();
   // TFLOP/s of a CU, measured; a workgroup alone on a CU with room for two has
   // 3/4 of what both have together (fp32: 5/8)
-  const bool f32 = d->dtype == NHIP_DTYPE_F32, two = places > cu_count();
+  const bool two = places > cu_count();
   const double rate = f32 ? (a->d <= 64 ? 0.84 : 0.55) : a->d <= 64 ? (cache ? 2.2 : 3.3) : a->d <= 128 ? 4.3 : 2.0;
   const double unit = 4e-6 * attn::kTilesRows * keys * a->d / rate;  // us
   const int64_t rounds = ceil_div(wgs, cu_count());
