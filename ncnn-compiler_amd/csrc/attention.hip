@@ -37,21 +37,22 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
   // are joined in a launch of their own (5 us).  So the second where the first
   // would read longer than the second computes, unless its workgroups leave most
   // CUs idle; and where the first would have several workgroups a CU, each with
-  // its own start.  The bounds are the best over 192 shapes each of 4 to 784 rows,
-  // 197 to 4096 keys (slower than the better kernel by 0.7 and 0.8% in the mean).
+  // its own start.  The bounds are the best over 330 shapes, and 192 over the
+  // cache, of 4 to 784 rows, 8 to 4096 keys (slower than the better kernel by 0.5
+  // and 0.8% in the mean).
   // us, few / many: 64 heads of 3136 keys of 128 bf16, 32 rows 38.1 / 30.9; 16 heads
   // of 784 keys of 64 fp32, 256 rows 20.5 / 31.8, of 3136 of 128 102.6 / 64.8; 64
-  // heads of 197 keys, 256 rows of 64 bf16 13.4 / 9.9, of 128 24.3 / 13.6; over the
-  // cache 8 heads of 1024 of 128, 512 rows bf16 22.8 / 39.7, fp32 39.6 / 32.9.
+  // heads of 197 keys, 256 rows of 64 bf16 13.4 / 9.9, of 128 24.3 / 13.6; 40 of 32
+  // keys, 198 rows of 128 fp32 28.7 / 15.3; over the cache 8 heads of 1024 of 128,
+  // 512 rows bf16 22.8 / 39.7, fp32 39.6 / 32.9.
   const int64_t kv_heads = (int64_t)d->batch * d->kv_heads, tiles16 = ceil_div(std::max(a->rows, 1), attn::kRowTile);
   const bool f32 = d->dtype == NHIP_DTYPE_F32;
   const double bytes = (double)kv_heads * d->keys * d->head_dim * 2 * (cache ? 1 : elem_size(d->dtype));
   const int force = setting_int("NHIP_ATTN_TILES", -1);
-  const int full = cache ? (f32 ? 6 : 8) : f32 || d->head_dim <= 64 ? 6 : 3;  // halves of a CU
-  const double again = cache ? (f32 ? 28e6 : 90e6) : f32 ? 215e6 : 64e6;        // bytes
-  a->tiles = vec && force != 0 &&
-             (force == 1 || kv_heads * tiles16 * 2 >= full * cu_count() ||
-              (kv_heads * tiles16 >= cu_count() / 4 && (tiles16 - 1) * bytes > again));
+  const double few = (double)kv_heads * tiles16 / cu_count();  // workgroups of the first to a CU
+  const bool full = cache ? few >= (f32 ? 3 : 4) : d->head_dim > 64 ? few >= 1.5 : f32 ? few > 2 : few >= 3;
+  const double again = cache ? (f32 ? 28e6 : 90e6) : f32 ? 215e6 : 64e6;  // bytes
+  a->tiles = vec && force != 0 && (force == 1 || full || (few >= 0.25 && (tiles16 - 1) * bytes > again));
   const int tile = a->tiles ? attn::kTilesRows : attn::kRowTile;
   a->row_tiles = (int)ceil_div(std::max(a->rows, 1), tile);
   const int64_t heads = (int64_t)d->batch * d->kv_heads;

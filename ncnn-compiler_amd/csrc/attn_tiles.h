@@ -173,7 +173,7 @@ __device__ __forceinline__ int worker_of(const AttnArgs& a, uint32_t unit) {
 // a tile is worked on, the next one's loads are under way, and it goes into the
 // other of two LDS buffers: one barrier a tile.
 //
-// Measured.  bf16: 2 x 3136 rows of 16 heads of 128 to 12544 keys 714 us (845
+// Measured.  bf16: 2 x 3136 rows of 16 heads of 128 to 12544 keys 703-729 us (827-858
 // TFLOP/s, 21 us of it the join), 4096 rows and keys, whose row tiles fill the
 // CUs evenly, 281-287 us (957-978; a library product of matrices alone 1130).  The
 // rest is the softmax: vector instructions of one wave beside another's products.
