@@ -5,6 +5,7 @@
 // Compiled with -ffp-contract=off: a code is the rounding of one separately
 // rounded product, so that it can be restated bit for bit.
 #include <algorithm>
+#include <type_traits>
 
 #include "elem.h"
 #include "kv_cache8.h"
@@ -12,7 +13,8 @@
 namespace nhip {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of a workgroup that reads
+constexpr int kHeld = 4;       // vectors that a thread appends without reading them again
 
 struct AppendArgs {
   Kv8 c;
@@ -32,14 +34,12 @@ __device__ __forceinline__ float wave_max(float v) {
 
 // One workgroup: one page of one sequence, one head, keys or values.  The new
 // tokens are wanted twice, for their largest magnitude and to be quantised: a
-// thread keeps its first kHeld vectors (a page of 64 tokens of 128 16-bit
-// channels) and reads others again.  Bytes bound it: 4 x 3136 tokens of 8 heads
-// of 128 bf16 21 us (77 MB, 3.7 TB/s: a workgroup's loads, its maximum and its
-// stores wait for each other, and 12 workgroups a CU end unevenly); one token to
-// each of 64 sequences 4.4 us, where a workgroup is one wave.
+// thread keeps its first kHeld vectors and reads others again.  Bytes bound
+// it: 4 x 3136 tokens of 8 heads of 128 bf16 17.5 us (77 MB, 4.4 TB/s; a
+// workgroup's loads, its maximum and its stores wait for each other); one token
+// to each of 64 sequences 4.4 us, where a workgroup is one wave.
 template <class T, int V, int TH>
 __global__ __launch_bounds__(TH) void kv8_append_kernel(AppendArgs a) {
-  constexpr int kHeld = 4;
   const int which = blockIdx.x & 1;
   const uint32_t rest = blockIdx.x >> 1;
   const int h = rest % a.c.kv_heads;
@@ -71,30 +71,38 @@ __global__ __launch_bounds__(TH) void kv8_append_kernel(AppendArgs a) {
   const int had = (int)(t0 - (page << a.c.shift));  // tokens that the page holds
   const float stood = *scale;
 
-  float most = 0.f;
-  const auto widest = [&](const float(&t)[V]) {
+  // the largest magnitude; NaN does not count, infinities only if asked for
+  const auto largest = [&](auto any) {
+    float most = 0.f;
+    const auto widest = [&](const float(&t)[V]) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float m = fabsf(t[e]);
-      most = m <= 3.402823466e38f ? fmaxf(most, m) : most;  // NaN and infinities do not count
+      for (int e = 0; e < V; ++e) {
+        const float m = fabsf(t[e]);
+        most = any() || m <= 3.402823466e38f ? fmaxf(most, m) : most;
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (threadIdx.x + k * TH < fresh) widest(held[k]);
+    for (int i = threadIdx.x + kHeld * TH; i < fresh; i += TH) {
+      float t[V];
+      load(i, t);
+      widest(t);
     }
+    most = wave_max(most);
+    if constexpr (TH > 64) {
+      __shared__ float red[TH / 64];
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = most;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < TH / 64; ++i) most = fmaxf(most, red[i]);
+    }
+    return most;
   };
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (threadIdx.x + k * TH < fresh) widest(held[k]);
-  for (int i = threadIdx.x + kHeld * TH; i < fresh; i += TH) {
-    float t[V];
-    load(i, t);
-    widest(t);
-  }
-  most = wave_max(most);
-  if constexpr (TH > 64) {
-    __shared__ float red[TH / 64];
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = most;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < TH / 64; ++i) most = fmaxf(most, red[i]);
-  }
+  // (two instructions less a value than without infinities at once: 19.9 -> 17.5 us)
+  float most = largest(std::true_type());
+  if (__builtin_expect(most > 3.402823466e38f, false)) most = largest(std::false_type());
   const float was = had ? stood : 0.f;
   const float want = most > 0.f ? fmaxf(most * (1.0f / 127.0f), kScaleLeast) : 0.f;
   const float now = fmaxf(want, was);
@@ -172,12 +180,20 @@ template <class T, int V>
 int append_launch(AppendArgs a, uint32_t wgs, hipStream_t s) {
   const int vecs = a.c.head_dim / V;
   a.by_vecs = fast_div(vecs);
-  // a wave does where a call's tokens leave it no more than it holds
-  if ((int64_t)a.tokens * vecs <= 4 * 64)
-    NHIP_LAUNCH("kv8_append", (kv8_append_kernel<T, V, 64>), dim3(wgs), dim3(64), 0, s, a);
-  else
-    NHIP_LAUNCH("kv8_append", (kv8_append_kernel<T, V, kThreads>), dim3(wgs), dim3(kThreads), 0, s, a);
-  return check_launch("kv8_append");
+  // As many threads as hold a page's new tokens, 1024 at most; a wave where a
+  // call's tokens leave it no more than it holds.  us at 256 / 512 / 1024
+  // threads: 4 x 3136 tokens of 8 heads of 128 bf16, pages of 64 (1024 vectors) 17.5 /
+  // 19.1 / 28.2; fp32 (2048) 28.2 / 23.3 / 28.2; 2 x 6000 of 4 heads of 256 bf16, pages of
+  // 256 (8192) 30.5 / 20.6 / 17.5.
+  const int64_t fresh = std::min<int64_t>(a.tokens, int64_t(1) << a.c.shift) * vecs;
+  const auto launch = [&](auto kernel, int threads) {
+    NHIP_LAUNCH("kv8_append", kernel, dim3(wgs), dim3(threads), 0, s, a);
+    return check_launch("kv8_append");
+  };
+  if ((int64_t)a.tokens * vecs <= kHeld * 64) return launch(kv8_append_kernel<T, V, 64>, 64);
+  if (fresh <= kHeld * 256) return launch(kv8_append_kernel<T, V, 256>, 256);
+  if (fresh <= kHeld * 512) return launch(kv8_append_kernel<T, V, 512>, 512);
+  return launch(kv8_append_kernel<T, V, 1024>, 1024);
 }
 
 template <class T>
