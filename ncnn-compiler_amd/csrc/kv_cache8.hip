@@ -146,16 +146,17 @@ struct ReadArgs {
   Kv8 c;
   void* out[2];
   const int32_t* starts;
-  int32_t tokens, items, blocks;  // of a sequence's keys: 8-channel pieces, workgroups
+  int32_t tokens, items, blocks;  // of a sequence: 8-channel pieces, workgroups
   FastDiv by_vecs, by_heads;
 };
 
-// A thread: eight channels of one token and head, keys or values.  Bytes bound
-// it: 4 x 3136 tokens of 8 heads of 128 to bf16 16.4 us (77 MB, 4.7 TB/s).
+// A thread: eight channels of one token and head, keys and values, for which
+// the page is found once (us with a thread for each / for both: bf16 15.7 / 14.9,
+// fp32 23.7 / 24.4, small reads 9.1 / 8.6).  Bytes bound it: 4 x 3136 tokens of 8
+// heads of 128 to bf16 15 us (77 MB, 5.1 TB/s, as a large copy).
 template <class T>
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(ReadArgs a) {
-  const int which = blockIdx.x & 1;
-  const uint32_t block = blockIdx.x >> 1;
+  const uint32_t block = blockIdx.x;
   const int b = block / a.blocks;
   const int i = (int)(block % a.blocks) * kThreads + threadIdx.x;
   if (i >= a.items) return;
@@ -163,17 +164,23 @@ __global__ __launch_bounds__(kThreads) void kv8_read_kernel(ReadArgs a) {
   const int at_token = fdiv(r, a.by_heads), h = r - at_token * a.c.kv_heads;
   const int64_t t = (int64_t)a.starts[b] + at_token;
   const int64_t id = t < 0 ? -1 : kv8_page(a.c, b, t >> a.c.shift);
-  float v[8] = {};
+  float v[2][8] = {};
   if (id >= 0) {
-    const int64_t at = (((id * a.c.kv_heads + h) << a.c.shift) + (t & ((1 << a.c.shift) - 1))) * a.c.head_dim + c;
-    const int2 q = *reinterpret_cast<const int2*>((which ? a.c.v : a.c.k) + at);
-    const float s = (which ? a.c.v_scale : a.c.k_scale)[id * a.c.kv_heads + h];
+    const int64_t page = id * a.c.kv_heads + h;
+    const int64_t at = ((page << a.c.shift) + (t & ((1 << a.c.shift) - 1))) * a.c.head_dim + c;
+    const int2 q[2] = {*reinterpret_cast<const int2*>(a.c.k + at), *reinterpret_cast<const int2*>(a.c.v + at)};
+    const float s[2] = {a.c.k_scale[page], a.c.v_scale[page]};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3))) * s;
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[w][e] = (float)(int8_t)((e < 4 ? q[w].x : q[w].y) >> (8 * (e & 3))) * s[w];
   }
-  T* out = (T*)a.out[which] + ((int64_t)b * a.items + i) * 8;
 #pragma unroll
-  for (int e = 0; e < 8; e += kVec<T>) Vec<T, kVec<T>>::store(out + e, reinterpret_cast<float(&)[kVec<T>]>(v[e]));
+  for (int w = 0; w < 2; ++w) {
+    T* out = (T*)a.out[w] + ((int64_t)b * a.items + i) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; e += kVec<T>) Vec<T, kVec<T>>::store(out + e, reinterpret_cast<float(&)[kVec<T>]>(v[w][e]));
+  }
 }
 
 template <class T, int V>
@@ -286,13 +293,13 @@ int nhip_kv8_read(const nhip_kv8_cache* cache, int32_t dtype, int32_t batch, int
   a.tokens = tokens;
   const int64_t items = (int64_t)tokens * a.c.kv_heads * (a.c.head_dim / 8);
   if (tokens > (0x7fffffff - kThreads) / a.c.kv_heads / (a.c.head_dim / 8) ||
-      batch > 0x7fffffff / 2 / ceil_div(items, kThreads))
+      batch > 0x7fffffff / ceil_div(items, kThreads))
     return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "kv8: too many tokens in one call");
   a.items = (int32_t)items;
   a.blocks = (int32_t)ceil_div(items, kThreads);
   a.by_vecs = fast_div(a.c.head_dim / 8);
   a.by_heads = fast_div(a.c.kv_heads);
-  return NHIP_FOR_ELEM(dtype, T, read_run<T>(a, (uint32_t)batch * a.blocks * 2, as_stream(stream)));
+  return NHIP_FOR_ELEM(dtype, T, read_run<T>(a, (uint32_t)batch * a.blocks, as_stream(stream)));
 }
 
 }  // extern "C"

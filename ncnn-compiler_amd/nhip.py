@@ -917,6 +917,8 @@ class KvCache8:
 
     def _hold(self, k, v, k_scale, v_scale):
         torch = _torch()
+        if not _ELEM:
+            _begin()
         for t, dtype, shape in ((k, torch.int8, k.shape), (v, torch.int8, k.shape),
                                 (k_scale, torch.float32, k.shape[:2]), (v_scale, torch.float32, k.shape[:2])):
             if not t.is_cuda or t.dtype != dtype or t.shape != shape or t.device != k.device or not t.is_contiguous():
@@ -947,8 +949,10 @@ class KvCache8:
         [batch, tokens, kv_heads, head_dim]."""
         b, pages = block_table.shape
         shape = (b, tokens, self.kv_heads, self.head_dim)
-        k, v = (_output(o, self.k, shape, stream, dtype) for o in (out or (None, None)))
-        code, dev = _elem(k, v)
+        k, v = out or (None, None)
+        k = _output(k, self.k, shape, stream, dtype)
+        code, dev = _elem(k)
+        v = _output(v, k, shape, stream)
         check(load().nhip_kv8_read(self._desc, code, b, tokens, _ints(block_table, dev, (b, pages), "block_table"), pages,
                                    _ints(starts, dev, (b,), "starts"), k.data_ptr(), v.data_ptr(), _on(stream, dev)))
         return k, v
