@@ -91,14 +91,17 @@ struct First<float> {
 // The value whose first powers are summed: x itself in 64 bits, else x - s.
 __device__ __forceinline__ float first_power(float x, float d, float) { return d; }
 __device__ __forceinline__ double first_power(float x, float d, double) { return (double)x; }
+// Squared deviations without what rounding may leave below 0.  NaN, of values
+// that are not all finite, stays.
+__device__ __forceinline__ double at_least_0(double v) { return v < 0.0 ? 0.0 : v; }
 // Mean and squared deviations of `count` values from their sums.
 __device__ __forceinline__ double2 moments(float s1, float s2, float shift, double count) {
   const double d = (double)s1 / count;
-  return make_double2((double)shift + d, fmax((double)s2 - (double)s1 * d, 0.0));
+  return make_double2((double)shift + d, at_least_0((double)s2 - (double)s1 * d));
 }
 __device__ __forceinline__ double2 moments(double s1, float s2, float shift, double count) {
   const double mean = s1 / count, d = mean - (double)shift;
-  return make_double2(mean, fmax((double)s2 - count * d * d, 0.0));
+  return make_double2(mean, at_least_0((double)s2 - count * d * d));
 }
 
 // Merges the chunks of image `n` for groups [g0, g1): mean and 1/sqrt(var + eps)
