@@ -6,24 +6,25 @@
 // every (image, group) over chunks of pixels (a mean and a sum of squared
 // deviations each), and a pass that merges them and writes y: x is read twice,
 // the second time from the last-level cache where the tensor fits.
-// Measured: 32 x 3136 x 256 bf16 25 us a call (103 MB moved, 4.1 TB/s; two
-// launches 31.4), 128 x 784 x 512 bf16 39 us (5.3 TB/s, as a large copy; two
-// launches 54); 8 x 50175 x 320 f16, in two launches, 129-139 us (47 and 83-94;
+// Measured: 32 x 3136 x 256 bf16 26.6 us a call (103 MB moved, 3.9 TB/s; two
+// launches 32), 128 x 784 x 512 bf16 39.6 us (5.2 TB/s, as a large copy; two
+// launches 54); 8 x 50175 x 320 f16, in two launches, 136-142 us (some 48 and 83-94;
 // floor with one reading 99).  Images two at a time, so that the second
 // reading stays in the last-level cache, were no faster (153).  Small tensors
 // take one launch that reads twice (5.5 us on the device at 1 x 128 x 28 x 28
 // fp32 blobs; a call is bound by the host's 7.1).
 //
-// Statistics: sums of x - s and (x - s)^2 with s one of the values summed, over
-// at most a few hundred terms of a thread; means and squared deviations of
-// channels and chunks are then merged in 64 bits (the sum of squares about a
-// common mean is the sum of the parts' plus count * (difference of means)^2).
-// A large mean beside a small spread therefore loses nothing, as it would in
-// E[x^2] - E[x]^2.  A thread's sums are fp32; those of fp32 values' first
-// powers are 64 bits, so that results near 0 keep their digits (an element
-// costs a conversion and an addition more, hidden behind its four bytes).
+// Statistics: sums of x - s and (x - s)^2 in 64 bits, s being one of the values
+// (16-bit types: blocks of at most kBlock values in fp32 first); means and
+// squared deviations of channels and chunks are then merged in 64 bits (the sum
+// of squares about a common mean is the sum of the parts' plus count *
+// (difference of means)^2).  A large mean beside a small spread loses nothing so,
+// as it would in E[x^2] - E[x]^2, nor does an s far from all others: what the
+// subtraction leaves is at least 1 / (count + 1) of the sum.  (Thread sums of
+// fp32 were off by up to 1e-3 there.)
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "elem.h"
@@ -79,29 +80,84 @@ __device__ __forceinline__ S team_sum(S v, int team) {
   return v;
 }
 
-// What a thread sums first powers in.
+// First and second powers that a thread adds up.  WIDE: each value, taken from
+// `shift`, in 64 bits.
+template <class T, bool WIDE>
+struct Powers {
+  double s1 = 0.0, s2 = 0.0;
+  __device__ __forceinline__ void begin(float) {}
+  __device__ __forceinline__ void add(float x, float shift) {
+    const double d = (double)x - (double)shift;
+    s1 += d;
+    s2 = fma(d, d, s2);
+  }
+  __device__ __forceinline__ void end(int) {}
+  __device__ __forceinline__ double first() const { return s1; }
+  __device__ __forceinline__ double second() const { return s2; }
+};
+// Else (16-bit types): a block of at most kBlock values in fp32, and the blocks
+// in 64 bits (a value's conversion to 64 bits takes four instructions' time).
+// Sums of so few values of 11 bits or less are nearly always exact.  So are those
+// of bf16 squares, 16 bits each, unless values differ by factors, and then the
+// mean's square takes little from them.  fp16's squares are taken from the mean
+// of a few of the block's values, which is near the others or, beside a value far
+// off, at most a fourth as far.  us with 64 bits value by value / in blocks: 32 x
+// 160 x 50176 f16 blobs 537 / 484, 64 x 3136 x 256 bf16 tokens 56.3 / 53.2.
+constexpr int kBlock = 32;
 template <class T>
-struct First {
-  typedef float type;
+struct Block {
+  static constexpr bool centred = std::is_same<T, f16>::value;
+  float from, b1, b2;
+  int n;
+  __device__ __forceinline__ void begin(float x, int values) {
+    from = x;
+    b1 = b2 = 0.f;
+    n = values;
+  }
+  __device__ __forceinline__ void add(float x, float) {
+    const float d = centred ? x - from : x;
+    b1 += x;
+    b2 = fmaf(d, d, b2);
+  }
+  // sums of x and x^2
+  __device__ __forceinline__ double first() const { return b1; }
+  __device__ __forceinline__ double second() const {
+    if (!centred) return b2;
+    const double c = from, u = b1;
+    return fma(c, fma((double)-n, c, u + u), (double)b2);
+  }
 };
-template <>
-struct First<float> {
-  typedef double type;
+template <class T>
+struct Powers<T, false> {
+  double s1 = 0.0, s2 = 0.0;
+  Block<T> block;
+  __device__ __forceinline__ void begin(float x) { block.begin(x, 0); }
+  __device__ __forceinline__ void add(float x, float) { block.add(x, 0.f); }
+  __device__ __forceinline__ void end(int n) {
+    block.n = n;
+    s1 += block.first();
+    s2 += block.second();
+  }
+  __device__ __forceinline__ double first() const { return s1; }
+  __device__ __forceinline__ double second() const { return s2; }
 };
-// The value whose first powers are summed: x itself in 64 bits, else x - s.
-__device__ __forceinline__ float first_power(float x, float d, float) { return d; }
-__device__ __forceinline__ double first_power(float x, float d, double) { return (double)x; }
-// Squared deviations without what rounding may leave below 0.  NaN, of values
-// that are not all finite, stays.
-__device__ __forceinline__ double at_least_0(double v) { return v < 0.0 ? 0.0 : v; }
-// Mean and squared deviations of `count` values from their sums.
-__device__ __forceinline__ double2 moments(float s1, float s2, float shift, double count) {
-  const double d = (double)s1 / count;
-  return make_double2((double)shift + d, at_least_0((double)s2 - (double)s1 * d));
+
+// Mean and squared deviations of `count` values from their sums (WIDE: those of
+// x - shift).  Rounding may leave the latter below 0; NaN, of values that are
+// not all finite, stays.
+template <bool WIDE>
+__device__ __forceinline__ double2 moments(double s1, double s2, double shift, double count) {
+  if (!WIDE) {
+    s2 = fma(count * shift, shift, fma(-2.0 * shift, s1, s2));
+    s1 = fma(-count, shift, s1);
+  }
+  const double d = s1 / count, v = fma(-s1, d, s2);
+  return make_double2(shift + d, v < 0.0 ? 0.0 : v);
 }
-__device__ __forceinline__ double2 moments(double s1, float s2, float shift, double count) {
-  const double mean = s1 / count, d = mean - (double)shift;
-  return make_double2(mean, at_least_0((double)s2 - count * d * d));
+// Whether fp32 may have lost squares: above its range, or below it where eps
+// does not hide that.  Then the sums are formed again, WIDE.
+__device__ __forceinline__ bool out_of_range(double2 m, double count, float eps) {
+  return !(m.y <= 1.7976931348623157e308) || (eps < 0x1p-110f && m.y < count * 0x1p-110);
 }
 
 // Merges the chunks of image `n` for groups [g0, g1): mean and 1/sqrt(var + eps)
@@ -129,94 +185,107 @@ __device__ void merge_chunks(const NormArgs& a, int n, int g0, int g1, float2* s
   }
 }
 
-// Where the threads' sums stand: first powers, second, and each channel's of
-// several threads.
-template <class T, int V, int TH>
-struct Sums {
-  typedef typename First<T>::type S;
-  S *red1, *more1;
-  float *red2, *more2;
-  __device__ __forceinline__ explicit Sums(void* red) {
-    red1 = reinterpret_cast<S*>(red);
-    more1 = red1 + TH * V;
-    red2 = reinterpret_cast<float*>(more1 + TH);
-    more2 = red2 + TH * V;
-  }
-  __device__ __forceinline__ void put(int thread, const S (&s1)[V], const float (&s2)[V]) const {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      red1[thread * V + i] = s1[i];
-      red2[thread * V + i] = s2[i];
-    }
-  }
-};
+// LDS that sum_channels takes, in values of 64 bits.
+__host__ __device__ constexpr int sums_place(int v, int threads) { return v * (threads + 64 / v) + 2 * threads + 1; }
 
-// Adds the sums of `rows` threads for each of `cols` vectors of channels, those
-// of a channel by as many threads as there are for it, then by one: means and
-// squared deviations of `count` values each to ch.  shift: what each channel's
-// values were taken from.
-template <class T, int V, int TH>
-__device__ void sum_channels(const T* shift, int cols, int rows, double count, double2* ch, const Sums<T, V, TH>& sums) {
-  typedef typename First<T>::type S;
-  const S* red1 = sums.red1;
-  S* more1 = sums.more1;
-  const float* red2 = sums.red2;
-  float* more2 = sums.more2;
-  __syncthreads();
-  const int cv = cols * V, parts = max(1, TH / cv);
-  for (int i = threadIdx.x; i < cv * parts; i += TH) {  // parts > 1: one step
-    const int c = i % cv;
-    S u1 = 0;
-    float u2 = 0.f;
-    for (int r = i / cv; r < rows; r += parts) {
-      u1 += red1[r * cv + c];
-      u2 += red2[r * cv + c];
-    }
-    if (parts == 1) {
-      ch[c] = moments(u1, u2, (float)shift[c], count);
-    } else {
-      more1[i] = u1;
-      more2[i] = u2;
-    }
-  }
-  __syncthreads();
-  if (parts > 1) {  // uniform
-    if (threadIdx.x < cv) {
-      S u1 = 0;
-      float u2 = 0.f;
-      for (int q = 0; q < parts; ++q) {
-        u1 += more1[q * cv + threadIdx.x];
-        u2 += more2[q * cv + threadIdx.x];
-      }
-      ch[threadIdx.x] = moments(u1, u2, (float)shift[threadIdx.x], count);
+// Adds the sums of `rows` threads for each of `cols` vectors of channels
+// (thread row * cols + col), those of a channel by as many threads as there are
+// for it, then by one: means and squared deviations of `count` values each to
+// ch.  shift: what each channel's values are taken from.  First and second powers
+// go through the same place (red, sums_place) one after the other, a vector's
+// channels in rows of their own, which begin in different banks.  Whether some
+// channel is out_of_range.
+template <bool WIDE, class T, int V, int TH, class P>
+__device__ bool sum_channels(const NormArgs& a, const T* shift, int cols, int rows, int col, int row, double count,
+                             double2* ch, double* red, const P (&sums)[V]) {
+  constexpr int ROW = TH + 64 / V;
+  double* more = red + V * ROW;
+  int* found = reinterpret_cast<int*>(more + 2 * TH);
+  const int mine = threadIdx.x, cv = cols * V;
+  const int parts = rows / V;  // threads of a channel; 0: a thread has several channels
+  const float from = row < V && row < rows ? (float)shift[col * V + row] : 0.f;
+  bool odd = false;
+  const auto done = [&](int c, double u1, double u2, float s) {
+    ch[c] = moments<WIDE>(u1, u2, (double)s, count);
+    odd |= out_of_range(ch[c], count, a.eps);
+  };
+  const auto put = [&](int power) {
+    __syncthreads();
+    if (power == 1 && mine == 0) *found = 0;  // (all have read what an earlier call left)
+    if (row < rows)
+#pragma unroll
+      for (int i = 0; i < V; ++i) red[i * ROW + mine] = power == 1 ? sums[i].first() : sums[i].second();
+    __syncthreads();
+  };
+  const auto add = [&](int i, int part, int step) {  // rows part, part + step, ..
+    const double* of = red + i * ROW + col;
+    double u = 0.0;
+#pragma unroll 4
+    for (int r = part; r < rows; r += step) u += of[r * cols];
+    return u;
+  };
+  if (parts) {  // uniform
+    put(1);
+    const bool in = row < parts * V;
+    const double u1 = in ? add(row % V, row / V, parts) : 0.0;
+    put(2);
+    const double u2 = in ? add(row % V, row / V, parts) : 0.0;
+    if (in) {  // vectors' i-th channels side by side, as the threads of row i
+      const int to = row / V * cv + row % V * cols + col;
+      more[to] = u1;
+      more[TH + to] = u2;
     }
     __syncthreads();
+    if (row < V) {
+      double v1 = 0.0, v2 = 0.0;
+#pragma unroll 8
+      for (int q = 0; q < parts; ++q) {
+        v1 += more[q * cv + mine];
+        v2 += more[TH + q * cv + mine];
+      }
+      done(col * V + row, v1, v2, from);
+    }
+  } else {
+    put(1);
+    if (row < rows)
+      for (int i = row; i < V; i += rows) ch[col * V + i].x = add(i, 0, 1);
+    put(2);
+    if (row < rows)
+      for (int i = row; i < V; i += rows) {
+        const int c = col * V + i;
+        done(c, ch[c].x, add(i, 0, 1), (float)shift[c]);
+      }
   }
+  if (!WIDE && odd) *found = 1;
+  __syncthreads();
+  return !WIDE && *found;
 }
 
 // Means and squared deviations of channels [c0, c0 + cn) over pixels [p0, p1)
 // of one image (x: its first pixel), channels last, to ch[0, cn).  A thread
 // keeps its V channels and walks pixels; `red` holds the threads' sums.
-template <class T, int V, int TH>
-__device__ void channel_moments(const NormArgs& a, const T* x, int c0, int cn, int64_t p0, int64_t p1, double2* ch, void* red) {
-  typedef typename First<T>::type S;
-  const Sums<T, V, TH> sums(red);
+// Whether some channel is out_of_range.
+template <bool WIDE, class T, int V, int TH>
+__device__ bool channel_powers(const NormArgs& a, const T* x, int c0, int cn, int64_t p0, int64_t p1, double2* ch, double* red) {
+  bool odd = false;
   const int vecs = cn / V;
   for (int v0 = 0; v0 < vecs; v0 += TH) {
     const int cols = min(TH, vecs - v0), rows = TH / cols;
     const int col = threadIdx.x % cols, row = threadIdx.x / cols;
-    S s1[V] = {};
-    float s2[V] = {}, shift[V];
+    Powers<T, WIDE> sums[V];
     if (row < rows) {
       const T* px = x + c0 + (int64_t)(v0 + col) * V;
-      Vec<T, V>::load(px + p0 * a.row_stride, shift);
+      float shift[V];
+      if constexpr (WIDE) Vec<T, V>::load(px + p0 * a.row_stride, shift);
+      int n = 0;  // values of the open block
       const auto add = [&](const float(&t)[V]) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = t[i] - shift[i];
-          s1[i] += first_power(t[i], d, S());
-          s2[i] = fmaf(d, d, s2[i]);
-        }
+        for (int i = 0; i < V; ++i) sums[i].add(t[i], WIDE ? shift[i] : 0.f);
+      };
+      const auto end = [&] {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sums[i].end(n);
+        n = 0;
       };
       const int64_t step = rows * a.row_stride;
       int64_t p = p0 + row;
@@ -225,18 +294,37 @@ __device__ void channel_moments(const NormArgs& a, const T* x, int c0, int cn, i
         float t[kDeep][V];
 #pragma unroll
         for (int u = 0; u < kDeep; ++u) Vec<T, V>::load(at + u * step, t[u]);
+        if (n == 0)
+#pragma unroll
+          for (int i = 0; i < V; ++i) sums[i].begin((t[0][i] + t[1][i] + t[2][i] + t[3][i]) * 0.25f);
 #pragma unroll
         for (int u = 0; u < kDeep; ++u) add(t[u]);
+        n += kDeep;
+        if (n > kBlock - kDeep) end();
       }
-      for (; p < p1; p += rows, at += step) {
+      for (; p < p1; p += rows, at += step) {  // fewer than kDeep of them, for which the block has room
         float t[V];
         Vec<T, V>::load(at, t);
+        if (n == 0)
+#pragma unroll
+          for (int i = 0; i < V; ++i) sums[i].begin(t[i]);
         add(t);
+        ++n;
       }
-      sums.put(row * cols + col, s1, s2);
+      if (n) end();
     }
-    sum_channels<T, V, TH>(x + p0 * a.row_stride + c0 + v0 * V, cols, rows, (double)(p1 - p0), ch + v0 * V, sums);
+    odd |= sum_channels<WIDE, T, V, TH>(a, x + p0 * a.row_stride + c0 + v0 * V, cols, rows, col, row, (double)(p1 - p0), ch + v0 * V, red, sums);
   }
+  return odd;
+}
+static_assert(kDeep == 4, "the mean of a block's first values");
+
+template <class T, int V, int TH>
+__device__ __forceinline__ void channel_moments(const NormArgs& a, const T* x, int c0, int cn, int64_t p0, int64_t p1, double2* ch, double* red) {
+  if constexpr (sizeof(T) == 4)
+    channel_powers<true, T, V, TH>(a, x, c0, cn, p0, p1, ch, red);
+  else if (__builtin_expect(channel_powers<false, T, V, TH>(a, x, c0, cn, p0, p1, ch, red), false))
+    channel_powers<true, T, 1, TH>(a, x, c0, cn, p0, p1, ch, red);  // (V = 1: few registers)
 }
 
 // Merges channels of `count` values each into `groups` groups: calls
@@ -312,7 +400,7 @@ __global__ __launch_bounds__(kThreads) void norm_stats_tokens_kernel(NormArgs a)
   extern __shared__ double2 lds[];  // [channels] mean, deviations; then the threads' sums
   const int n = blockIdx.x / a.chunks, k = blockIdx.x % a.chunks;
   const int64_t p0 = (int64_t)k * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
-  channel_moments<T, V, kThreads>(a, (const T*)a.x + n * a.image_stride, 0, a.channels, p0, p1, lds, lds + a.channels);
+  channel_moments<T, V, kThreads>(a, (const T*)a.x + n * a.image_stride, 0, a.channels, p0, p1, lds, (double*)(lds + a.channels));
   merge_channels<kThreads>(a, lds, a.groups, (double)(p1 - p0),
                  [&](int g, double m, double v) { a.part[(int64_t)blockIdx.x * a.groups + g] = make_double2(m, v); });
 }
@@ -338,7 +426,7 @@ __global__ __launch_bounds__(kOneThreads) void norm_one_tokens_kernel(NormArgs a
   const int parts = a.groups / groups, n = blockIdx.x / parts, g0 = blockIdx.x % parts * groups;
   const T* x = (const T*)a.x + n * a.image_stride;
   const int cn = groups * a.cpg;
-  channel_moments<T, V, kOneThreads>(a, x, g0 * a.cpg, cn, 0, a.pixels, lds, lds + cn);
+  channel_moments<T, V, kOneThreads>(a, x, g0 * a.cpg, cn, 0, a.pixels, lds, (double*)(lds + cn));
   float2* stats = reinterpret_cast<float2*>(lds + cn);
   const double all = (double)a.pixels * a.cpg, eps = a.eps;
   merge_channels<kOneThreads>(a, lds, groups, (double)a.pixels,
@@ -351,8 +439,7 @@ __global__ __launch_bounds__(kOneThreads) void norm_one_tokens_kernel(NormArgs a
 // hold, so that x is read once: all loads first, then the statistics, then the
 // results.  (At most kHeld times the workgroup's rows of pixels; whole vectors.)
 template <class T, int V, int ACT, int TH, bool STREAM>
-__global__ __launch_bounds__(TH) void norm_held_tokens_kernel(NormArgs a, int groups, int wgs) {
-  typedef typename First<T>::type S;
+__global__ __launch_bounds__(TH, 4) void norm_held_tokens_kernel(NormArgs a, int groups, int wgs) {
   extern __shared__ double2 lds[];  // as norm_one_tokens_kernel's
   // workgroups go to the eight dies in turn: an image's parts, which share
   // lines of memory, to one of them
@@ -367,24 +454,33 @@ __global__ __launch_bounds__(TH) void norm_held_tokens_kernel(NormArgs a, int gr
   for (int u = 0; u < kHeld; ++u)  // (past the last pixel: that one again)
     if (u * rows < pixels) held[u] = *reinterpret_cast<const typename Vec<T, V>::type*>(x + min(row + u * rows, pixels - 1) * a.row_stride + col * V);
   float shift[V];
-  Vec<T, V>::load(x + col * V, shift);
+  if constexpr (sizeof(T) == 4) Vec<T, V>::load(x + col * V, shift);
   const int mine = row < rows ? (pixels - row + rows - 1) / rows : 0;  // vectors that count
-  const Sums<T, V, TH> sums(lds + cn);
+  constexpr bool WIDE = sizeof(T) == 4;
+  static_assert(kHeld <= kBlock, "one block");
+  bool odd;
   {
-    S s1[V] = {};
-    float s2[V] = {};
+    typename std::conditional<WIDE, Powers<T, WIDE>, Block<T>>::type sums[V];
+    if constexpr (!WIDE) {
+      const float part = 1.f / (float)max(1, min(mine, 4));
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float from = (float)held[0][i];
+#pragma unroll
+        for (int u = 1; u < 4; ++u) from += u < mine ? (float)held[u][i] : 0.f;
+        sums[i].begin(from * part, mine);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) asm volatile("" : "+v"(held[u]));  // widened again below, not kept
+    }
 #pragma unroll
     for (int u = 0; u < kHeld; ++u)
       if (u < mine)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float t = (float)held[u][i], d = t - shift[i];
-          s1[i] += first_power(t, d, S());
-          s2[i] = fmaf(d, d, s2[i]);
-        }
-    if (row < rows) sums.put(row * cols + col, s1, s2);
+        for (int i = 0; i < V; ++i) sums[i].add((float)held[u][i], WIDE ? shift[i] : 0.f);
+    odd = sum_channels<WIDE, T, V, TH>(a, x, cols, rows, col, row, (double)a.pixels, lds, (double*)(lds + cn), sums);
   }
-  sum_channels<T, V, TH>(x, cols, rows, (double)a.pixels, lds, sums);
+  if (__builtin_expect(odd, false)) channel_powers<true, T, 1, TH>(a, x, 0, cn, 0, a.pixels, lds, (double*)(lds + cn));
   float2* stats = reinterpret_cast<float2*>(lds + cn);
   const double all = (double)a.pixels * a.cpg, eps = a.eps;
   merge_channels<TH>(a, lds, groups, (double)a.pixels,
@@ -410,45 +506,63 @@ __global__ __launch_bounds__(TH) void norm_held_tokens_kernel(NormArgs a, int gr
 }
 
 // Mean and squared deviations of pixels [p0, p1) of one group's channels,
-// channels first (x: the group's first channel); valid in thread 0.
+// channels first (x: the group's first channel), the same in every thread.
 template <class T, int V, int TH>
 __device__ double2 group_moments(const NormArgs& a, const T* x, int64_t p0, int64_t p1) {
-  typedef typename First<T>::type S;
-  __shared__ S red1[TH / 64];
-  __shared__ float red2[TH / 64];
+  __shared__ double red1[TH / 64], red2[TH / 64];
   const float shift = (float)x[p0];
   const int vecs = (int)((p1 - p0) / V);
-  S s1 = 0;
-  float s2 = 0.f;
   const int lanes = min(TH, (vecs + 63) / 64 * 64);
   const int rows = TH / lanes, row = threadIdx.x / lanes, col = threadIdx.x % lanes;
-  if (row < rows)
-    for (int c = row; c < a.cpg; c += rows)
-#pragma unroll 4
-      for (int v = col; v < vecs; v += lanes) {
-        float t[V];
-        Vec<T, V>::load(x + c * a.row_stride + p0 + (int64_t)v * V, t);
+  const double count = (double)(p1 - p0) * a.cpg;
+  const auto pass = [&](auto wide) {
+    Powers<T, wide> sums;
+    const auto add = [&](auto& t, int n) {  // n vectors, a block
+      sums.begin(n > 1 ? (t[0][0] + t[n / 4][0] + t[n / 2][0] + t[n - 1][0]) * 0.25f
+                       : (t[0][0] + t[0][V / 4] + t[0][V / 2] + t[0][V - 1]) * 0.25f);
+      for (int u = 0; u < n; ++u)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = t[i] - shift;
-          s1 += first_power(t[i], d, S());
-          s2 = fmaf(d, d, s2);
+        for (int i = 0; i < V; ++i) sums.add(t[u][i], shift);
+      sums.end(n * V);
+    };
+    static_assert(kDeep * V <= kBlock, "one block");
+    if (row < rows)
+      for (int c = row; c < a.cpg; c += rows) {
+        const T* at = x + c * a.row_stride + p0;
+        int v = col;
+        for (; v + (kDeep - 1) * lanes < vecs; v += kDeep * lanes) {
+          float t[kDeep][V];
+#pragma unroll
+          for (int u = 0; u < kDeep; ++u) Vec<T, V>::load(at + (int64_t)(v + u * lanes) * V, t[u]);
+          add(t, kDeep);
+        }
+#pragma unroll 3
+        for (; v < vecs; v += lanes) {
+          float t[1][V];
+          Vec<T, V>::load(at + (int64_t)v * V, t[0]);
+          add(t, 1);
         }
       }
-  s1 = team_sum(s1, 64);
-  s2 = team_sum(s2, 64);
-  if ((threadIdx.x & 63) == 0) {
-    red1[threadIdx.x / 64] = s1;
-    red2[threadIdx.x / 64] = s2;
+    const double s1 = team_sum(sums.s1, 64), s2 = team_sum(sums.s2, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+      red1[threadIdx.x / 64] = s1;
+      red2[threadIdx.x / 64] = s2;
+    }
+    __syncthreads();
+    double u1 = 0.0, u2 = 0.0;
+    for (int i = 0; i < TH / 64; ++i) {
+      u1 += red1[i];
+      u2 += red2[i];
+    }
+    return moments<wide>(u1, u2, (double)shift, count);
+  };
+  if constexpr (sizeof(T) == 4) {
+    return pass(std::true_type());
+  } else {
+    const double2 m = pass(std::false_type());
+    return out_of_range(m, count, a.eps) ? pass(std::true_type()) : m;  // the same in all threads
   }
-  __syncthreads();
-  S u1 = 0;
-  float u2 = 0.f;
-  for (int i = 0; i < TH / 64; ++i) {
-    u1 += red1[i];
-    u2 += red2[i];
-  }
-  return moments(u1, u2, shift, (double)(p1 - p0) * a.cpg);
 }
 
 // Statistics of one chunk of pixels of one group, channels first.
@@ -599,9 +713,9 @@ int norm_apply(const NormArgs& a, int layout, int n, bool vec, hipStream_t s) {
   return check_launch("group_norm_apply");
 }
 
-template <class T>
+// Channels' moments and the threads' sums.
 size_t stats_lds(int channels, int v, int threads) {
-  return channels * sizeof(double2) + threads * (v + 1) * (sizeof(typename First<T>::type) + sizeof(float));
+  return channels * sizeof(double2) + sums_place(v, threads) * sizeof(double);
 }
 
 template <class T, int ACT>
@@ -615,7 +729,7 @@ int norm_one(const NormArgs& a, int layout, int n, int groups, bool vec, hipStre
       NHIP_LAUNCH("group_norm_one", (norm_one_blobs_kernel<T, 1, ACT>), grid, dim3(kOneThreads), 0, s, a, fast_div(a.cpg));
   } else {
     const bool wide = vec && groups * a.cpg % V == 0;
-    const size_t lds = stats_lds<T>(groups * a.cpg, wide ? V : 1, kOneThreads);
+    const size_t lds = stats_lds(groups * a.cpg, wide ? V : 1, kOneThreads);
     const void* kernel = wide ? (const void*)norm_one_tokens_kernel<T, V, ACT> : (const void*)norm_one_tokens_kernel<T, 1, ACT>;
     if (lds > 65536) NHIP_TRY(ensure_dynamic_lds(kernel, 160 * 1024));
     if (wide)
@@ -668,7 +782,7 @@ template <class T, int ACT, int TH>
 int norm_held(const NormArgs& a, int n, int groups, hipStream_t s) {
   constexpr int V = kVec<T>;
   const int wgs = n * (a.groups / groups);
-  const size_t lds = stats_lds<T>(groups * a.cpg, V, TH);
+  const size_t lds = stats_lds(groups * a.cpg, V, TH);
   const auto launch = [&](auto kernel) {
     if (lds > 65536) {
       const int st = ensure_dynamic_lds((const void*)kernel, 160 * 1024);
@@ -715,7 +829,7 @@ int norm_run(const NormArgs& a, int layout, int n, int one, hipStream_t s) {
       NHIP_LAUNCH("group_norm_stats", (norm_stats_blobs_kernel<T, 1>), grid, dim3(kBlobThreads), 0, s, a);
   } else {
     const dim3 grid((uint32_t)(n * a.chunks));
-    const size_t lds = stats_lds<T>(a.channels, vec ? V : 1, kThreads);
+    const size_t lds = stats_lds(a.channels, vec ? V : 1, kThreads);
     const auto launch = [&](auto kernel) {
       if (lds > 65536) {
         const int st = ensure_dynamic_lds((const void*)kernel, 160 * 1024);

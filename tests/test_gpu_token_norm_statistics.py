@@ -6,6 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import nhip  # noqa: E402
+import token_reference as ref  # noqa: E402
 from test_gpu_token_norm_rotary import check_norm, randn  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +42,49 @@ def test_not_finite(pixel, value, dtype, act, blobs, one):
     assert torch.isnan(y[1, :, 8:16]).all()
     y[1, :, 8:16] = 0
     assert torch.isfinite(y).all()
+
+
+@FORMS
+@LAYOUTS
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("whole", [True, False])  # every channel of the first pixel, or each group's first value alone
+@pytest.mark.parametrize("spreads", [30, 1000])
+@pytest.mark.parametrize("n,pixels,c,groups", [(2, 900, 64, 8), (1, 6001, 40, 4), (1, 20000, 16, 1)])
+def test_first_value_far_off(n, pixels, c, groups, spreads, whole, dtype, blobs, one):
+    """A corner or a first token unlike the rest: sums taken from it have to keep the others' digits."""
+    x = randn(pixels, (n, pixels, c), dtype)
+    x[:, 0, ::1 if whole else c // groups] += spreads
+    check_norm(laid(x, blobs), groups, "none", blobs)
+
+
+@FORMS
+@LAYOUTS
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("factor", [1e25, 1e-25])
+def test_squares_out_of_range(factor, dtype, blobs, one):
+    """Values whose squares fp32 would not hold."""
+    x = (randn(2, (2, 700, 32)) * factor).to(dtype)
+    check_norm(laid(x, blobs), 4, "none", blobs, eps=0.0)
+
+
+@FORMS
+@LAYOUTS
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_one_value_of_many(dtype, blobs, one):
+    """All values alike but one, by the type's last place."""
+    x = torch.full((1, 3000, 16), 96.0, dtype=dtype)
+    x[0, 1700, 5] += 96.0 * {F32: 2.0 ** -22, F16: 2.0 ** -9, BF16: 2.0 ** -6}[dtype]
+    check_norm(laid(x, blobs), 1, "none", blobs, eps=0.0)
+
+
+@FORMS
+@LAYOUTS
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_many_images(dtype, blobs, one):
+    """More images than fill the GPU: a thread sums many values."""
+    n, pixels, c = 600, 5000, 16
+    x = torch.randn((n, pixels, c), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(dtype) + 3
+    y = nhip.GroupNorm(2, c, blobs=blobs).forward(laid(x, blobs))
+    for i in (0, 333, n - 1):
+        want, bound = ref.group_norm(x[i:i + 1], 2, None, None, 1e-5, "none")
+        ref.assert_within(y[i:i + 1], want, bound)
