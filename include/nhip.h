@@ -440,7 +440,8 @@ int nhip_cross_attention_forward(
 /* A cache of keys and values in 8 bits.  A page holds block_tokens tokens of
  * one sequence: codes k, v int8 [pages][kv_heads][block_tokens][head_dim] and
  * a scale for each page and head, k_scale, v_scale fp32 [pages][kv_heads]; a
- * code q stands for q * scale.  block_tokens: 16, 32, 64, 128 or 256;
+ * code q stands for q * scale, finite and not negative where a token is held
+ * (other pages may hold anything).  block_tokens: 16, 32, 64, 128 or 256;
  * head_dim a multiple of 8, at most 256; codes 16-byte aligned; codes of a
  * page whose scale is 0 are 0.  Which pages a sequence has stands in its row
  * of a block table: int32 [batch][table_pages], token t in page

@@ -233,7 +233,10 @@ __device__ __forceinline__ TileKeys know_tile(const AttnArgs& a, TileAsk t, int 
       k.kscale = a.cache.k_scale[at];
       k.vscale = a.cache.v_scale[at];
     }
-    if (!there) k.kscale = k.vscale = 0.f;
+    // (Products take the scale of a page's first key.  A page of which no row
+    // sees a token may hold any scale; one that is not finite, times a probability
+    // of 0, would be NaN.)
+    if (!there || key0 + (lane & (KEYS - 1)) >= end) k.kscale = k.vscale = 0.f;
   }
   k.counts = __ballot(counts);
   return k;

@@ -438,9 +438,10 @@ __global__ __launch_bounds__(kWaves * 64, (TilesShape<T, DP, SRC>::per_cu)) void
           for (int u = 0; u < 2; ++u) {
             if constexpr (S::units) {
               // probabilities times a page's scale may leave fp16's range, so
-              // the sums change to its units instead
-              const float now = fminf(fmaxf(lane_float(keys.vscale, t * 32 + u * 16), kLeastUnit), kMostUnit);
-              if (now != in) {
+              // the sums change to its units instead (values of smaller ones
+              // than kLeastUnit, and of pages that nobody sees, were read as 0)
+              const float scale = lane_float(keys.vscale, t * 32 + u * 16), now = fminf(scale, kMostUnit);
+              if (!(scale < kLeastUnit) && now != in) {
                 settle(acc[0]);
                 const float r = in * __builtin_amdgcn_rcpf(now);
 #pragma unroll
