@@ -676,6 +676,9 @@ def dequantize(x, scale, bias=None, stream=None):
 # ------------------------------------------------------------ token operators
 # Small calls are bound by the host: what torch gives for good is kept, and the
 # checks are the cheap forms of themselves.
+# stream: the caller has it wait for the inputs and keeps those until it is done;
+# new results are of its memory, and may be read by the stream that was current
+# at the call once that one waits for it.
 _ELEM = {}  # element types, filled with the first call, as are the next
 _int32 = _current_device = _current_stream = _empty_like = None
 
@@ -718,15 +721,26 @@ def _ints(t, dev, shape, what):
     return t.data_ptr()
 
 
+def _new(like, shape, dtype, stream):
+    """A new tensor that `stream` may write at once: of that stream's own
+    memory, since what the current one has freed its kernels may still use."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with _torch().cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
+
+
 def _output(out, like, shape, stream, dtype=None):
-    """`out`, checked, or a new tensor that `stream` may write."""
+    """`out`, checked, or a new tensor that `stream` may write and the current
+    one read."""
     if out is None:
-        if dtype is None and like.is_contiguous() and shape == like.shape:
+        if stream is not None:
+            out = _new(like, shape, dtype, stream)
+            out.record_stream(_torch().cuda.current_stream(like.device))
+        elif dtype is None and like.is_contiguous() and shape == like.shape:
             out = _empty_like(like)  # the cheapest of torch's allocations
         else:
-            out = like.new_empty(shape, dtype=dtype)
-        if stream is not None:
-            out.record_stream(stream)
+            out = _new(like, shape, dtype, None)
     elif out.dtype != (dtype or like.dtype) or out.device != like.device or not out.is_contiguous() or out.shape != shape:
         raise ValueError(f"out has to be a contiguous {dtype or like.dtype} tensor of shape {tuple(shape)} on {like.device}")
     return out
@@ -734,13 +748,11 @@ def _output(out, like, shape, stream, dtype=None):
 
 def _scratch(workspace, nbytes, like, stream):
     """(tensor, pointer, bytes) of the caller's workspace or a new one, which
-    stays allocated until `stream` is done with it."""
+    stays allocated until the stream is done with it."""
     if workspace is None:
         if not nbytes:
             return None, None, 0
-        workspace = like.new_empty(nbytes, dtype=_torch().uint8)
-        if stream is not None:
-            workspace.record_stream(stream)
+        workspace = _new(like, nbytes, _torch().uint8, stream)
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
