@@ -753,6 +753,8 @@ def _scratch(workspace, nbytes, like, stream):
         if not nbytes:
             return None, None, 0
         workspace = _new(like, nbytes, _torch().uint8, stream)
+    elif workspace.device != like.device or not workspace.is_contiguous():
+        raise ValueError(f"workspace has to be a contiguous tensor on {like.device}")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
