@@ -75,6 +75,8 @@ class ImageDecoder:
     def _attend_own(self, x, positions, start, causal):
         """The block's attention of new tokens x to all that the cache holds with them."""
         torch, b, n = self.torch, x.shape[0], x.shape[1]
+        if start + n > self.max_tokens:  # the cache would leave out what its table has no page for
+            raise ValueError(f"{start} + {n} tokens, the cache holds {self.max_tokens}")
         q = self.own.project(self.own.q, x, self.own.heads)
         k = self.own.project(self.own.k, x, self.own.kv_heads)
         v = self.own.project(self.own.v, x, self.own.kv_heads)
@@ -92,10 +94,11 @@ class ImageDecoder:
         grid = torch.stack([torch.zeros((h * w,), dtype=torch.int32, device=self.device),
                             torch.arange(h, dtype=torch.int32, device=self.device).repeat_interleave(w),
                             torch.arange(w, dtype=torch.int32, device=self.device).repeat(h)], -1)[None]
+        y = self._attend_own(tokens, grid.contiguous(), 0, causal=False)
         self.image_k = self.cross.project(self.cross.k, tokens, self.cross.kv_heads)
         self.image_v = self.cross.project(self.cross.v, tokens, self.cross.kv_heads)
         self.held = h * w
-        return self._attend_own(tokens, grid.contiguous(), 0, causal=False)
+        return y
 
     def step(self, x, image_lengths):
         """One new token a sequence, x [batch, 1, dim]; image_lengths int32 [batch]: features of each image that
