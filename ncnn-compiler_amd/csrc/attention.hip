@@ -101,6 +101,8 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
     const int64_t workers = std::min(places, wgs * a->units * keys / 256);
     if (workers > wgs || workers == places) a->workers = (int)std::max<int64_t>(1, workers);
   }
+  const int dealt_to = setting_int("NHIP_ATTN_WORKERS", 0);
+  if (dealt_to > 0 && wgs * a->units < 0x7fffffff) a->workers = (int)std::min<int64_t>(dealt_to, wgs * a->units);
   return ok();
 }
 
