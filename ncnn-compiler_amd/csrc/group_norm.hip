@@ -6,9 +6,9 @@
 // every (image, group) over chunks of pixels (a mean and a sum of squared
 // deviations each), and a pass that merges them and writes y: x is read twice,
 // the second time from the last-level cache where the tensor fits.
-// Measured: 32 x 3136 x 256 bf16 26.6 us a call (103 MB moved, 3.9 TB/s; two
-// launches 32), 128 x 784 x 512 bf16 39.6 us (5.2 TB/s, as a large copy; two
-// launches 54); 8 x 50175 x 320 f16, in two launches, 136-142 us (some 48 and 83-94;
+// Measured: 32 x 3136 x 256 bf16 26.2-26.8 us a call (103 MB moved, 3.9 TB/s; two
+// launches 33), 128 x 784 x 512 bf16 39.6 us (5.2 TB/s, as a large copy; two
+// launches 56); 8 x 50175 x 320 f16, in two launches, 135-142 us (some 48 and 83-94;
 // floor with one reading 99).  Images two at a time, so that the second
 // reading stays in the last-level cache, were no faster (153).  Small tensors
 // take one launch that reads twice (5.5 us on the device at 1 x 128 x 28 x 28
@@ -627,11 +627,11 @@ __global__ __launch_bounds__(kBlobThreads) void norm_apply_blobs_kernel(NormArgs
 //
 // One launch spares the second's 4 us where the call is bound by launches; but
 // a workgroup walks its groups' pixels alone.  Measured, us a call (two
-// launches / one): tokens of 50 KB to a workgroup 11.8 / 9.0 (784 x 512 bf16)
-// and 12.8 / 8.2 (fp32), of 200 KB 12.7 / 13.1 (fp32) and 11.5 / 17.4 (bf16);
-// blobs of 3136 values 12 / 8, of 12544 12.0 / 10.2, of 25088 12.4 / 16.3.  Of
-// tensors past 10 MB (tokens) or 16 MB (blobs) the launches no longer count:
-// 32 x 784 x 512 fp32 30 / 42.
+// launches / one): tokens of 50 KB to a workgroup 12.6 / 9.9 (784 x 512 bf16)
+// and 12.1 / 8.9 (fp32), of 200 KB 13.2 / 15.5 (fp32) and 15.2 / 19.4 (bf16);
+// blobs of 3136 values 10.8 / 6.7, of 6272 11.1 / 8.0 (8 images 13.1 / 12.1), of 12544
+// 10.9 / 11.5 (8 images 16.3 / 18.3).  Of tensors past 10 MB (tokens) or 16 MB
+// (blobs) the launches no longer count: 32 x 784 x 512 fp32 31 / 43.
 int groups_of_one(int channels, int groups, int layout, int es, int64_t n, int64_t pixels) {
   const int cpg = channels / groups;
   int each = 1;
@@ -642,7 +642,7 @@ int groups_of_one(int channels, int groups, int layout, int es, int64_t n, int64
   if (force == 0 || force == 2 || values > (1 << 28) || n * (groups / each) > 0x7fffffff) return 0;
   const int64_t bytes = n * pixels * channels * es;
   return force == 1 || (layout == NHIP_LAYOUT_TOKENS ? values * es <= 65536 && bytes <= 10000000
-                                                     : values <= 16384 && bytes <= 16000000) ? each : 0;
+                                                     : values <= 8192 && bytes <= 16000000) ? each : 0;
 }
 
 // Chunks of an image: enough workgroups for two to a CU (tokens) or four
@@ -650,7 +650,8 @@ int groups_of_one(int channels, int groups, int layout, int es, int64_t n, int64
 // merged by every workgroup of the second pass.  Tokens, us a call at 2 / 3 / 4
 // to a CU: 32 x 3136 x 256 bf16 32.7 / 33.7 / 34.7, 8 x 50175 x 320 f16 172 /
 // 180 / 179; one image of 12544 x 320 fp32 in 128 / 256 / 512 chunks 23.6 /
-// 19.8 / 25.4.
+// 19.8 / 25.4 (all before results past the caches and the sums in 64 bits:
+// 33.3, 142 and 17.9 as chosen now).
 void chunks_of(int channels, int64_t n, int64_t pixels, int per_image, NormArgs* a) {
   const int64_t want = ceil_div((int64_t)(per_image == 1 ? 2 : 4) * cu_count(), n * per_image);
   const int64_t fit = std::max<int64_t>(1, pixels * channels / per_image / 8192);
@@ -745,13 +746,14 @@ int norm_one(const NormArgs& a, int layout, int n, int groups, bool vec, hipStre
 // pixel, more of them where threads and workgroups are left.  0: not here.
 //
 // us a call, two launches / held.  Of 256 or 512 threads, several to a CU: 64 x
-// 784 x 512 bf16 32.6 / 23.9, 128 x 53.7 / 39.0, 32 x fp32 29.8 / 20.5, 16 x
-// 1024 x 1280 f16 29.2 / 21.4; of 512 threads and 8 / 64 workgroups 11.2 / 12.0,
+// 784 x 512 bf16 34.7 / 25.2, 128 x 55.6 / 40.3, 32 x fp32 31.2 / 21.8, 16 x
+// 1024 x 1280 f16 32.5 / 23.4; of 512 threads and 8 / 64 workgroups 11.2 / 12.0,
 // 14.9 / 12.6.  Rows that are no whole 64 bytes share lines with their
 // neighbours, which costs where results are past the caches: 1024 x 640 f16 of 42
-// / 84 MB 28.0 / 21.5, 45.7 / 55.2.  Of 1024 threads, one to a CU, with nothing
-// beside its waits: 3136 x 256 bf16 of 128 / 192 / 256 / 384 / 512 / 1024
-// workgroups 20.9 / 22.0, 29.4 / 23.4, 31.4 / 25.0, 49.0 / 45.0, 53.0 / 50.8, 112 / 118.
+// MB 30.2 / 23.4, of 84 45.7 / 55.2 or, another time, 48.0 / 43.1.  Of 1024 threads,
+// one to a CU, with nothing beside its waits: 3136 x 256 bf16 of 128 / 192 / 256 / 384
+// / 512 / 1024 workgroups 22.6 / 23.5, 34.2 / 25.1, 33.2 / 26.8, 53.5 / 47.8, 54.6 /
+// 53.4, 111 / 115.
 struct Held {
   int groups, threads;
 };
