@@ -343,15 +343,23 @@ int nhip_dequantize_i32_f32(const int32_t* input, float* output, int32_t n,
 
 /* ---------------------------------------------------------------------------
  * Token operators: what follows the trunk when a decoder reads its features.
- * No counterpart in the reference (its importer has none of these layers).
+ * The reference lowers ncnn's own attention layers for the CPU
+ * (lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:3859-4668); these are calls, not
+ * layers of a graph, with the forms that serving needs (shared heads, lengths,
+ * pages, 16-bit types).  Group norm into tokens, rotary positions and the
+ * 8-bit cache have no counterpart there.
  * All pointers are device pointers unless said otherwise; `dtype` is
  * NHIP_DTYPE_F32, F16 or BF16 and holds for every tensor of a call but the
  * integer ones.  Sums, softmax statistics and angles are held in fp32 or
- * more, results rounded once.  Strides count elements; channels and head
- * channels are always contiguous.  Tensors may have any alignment that their
- * type needs, and 16-byte aligned rows take the wide loads; but queries and
- * results of the attention over the cache, values read from it and workspaces
- * have to be 16-byte aligned.  A workspace is needed where its size is not 0;
+ * more, results rounded once; attention in F16 and BF16 rounds each
+ * probability to the type too, before it meets the values (not in F16 of few
+ * rows over the cache).  Strides count elements; channels and head channels
+ * are always contiguous.  Tensors may have any alignment that their type
+ * needs, and 16-byte aligned rows take the wide loads (attention of many rows
+ * without them reads all keys again for every 16 rows, several times slower);
+ * but queries and results of the attention over the cache, values read from
+ * it and workspaces have to be 16-byte aligned.  A workspace is needed where
+ * its size is not 0;
  * the size asked for covers any strides and alignment.  The calls allocate
  * nothing, so they may be recorded into a HIP graph.
  * ------------------------------------------------------------------------- */

@@ -37,9 +37,12 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
   // are joined in a launch of their own (5 us).  So the second where the first
   // would read longer than the second computes, unless its workgroups leave most
   // CUs idle; and where the first would have several workgroups a CU, each with
-  // its own start.  The bounds are the best over 330 shapes, and 192 over the
-  // cache, of 4 to 784 rows, 8 to 4096 keys (slower than the better kernel by 0.5
-  // and 0.8% in the mean).
+  // its own start.  The bounds are the best over 336 shapes (bf16 and fp32, heads
+  // of 64 and 128; 8, 32, 80, 197, 784, 3136 keys; batch, heads, key/value heads 4,
+  // 12, 12, 16, 16, 4, 1, 16, 16, 10, 8, 4; 4 to 784 rows), and 192 over the cache (256,
+  // 1024, 4096 keys; 4, 12, 12, 16, 16, 4, 1, 32, 8; 4 to 256 rows), each timed with
+  // both kernels (NHIP_ATTN_TILES): slower than the better one by 0.5 and 0.8% in
+  // the mean.
   // us, few / many: 64 heads of 3136 keys of 128 bf16, 32 rows 38.1 / 30.9; 16 heads
   // of 784 keys of 64 fp32, 256 rows 20.5 / 31.8, of 3136 of 128 102.6 / 64.8; 64
   // heads of 197 keys, 256 rows of 64 bf16 13.4 / 9.9, of 128 24.3 / 13.6; 40 of 32

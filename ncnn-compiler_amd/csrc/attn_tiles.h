@@ -181,7 +181,8 @@ __device__ __forceinline__ int worker_of(const AttnArgs& a, uint32_t unit) {
 // the products to a score and codes to convert, so the waves' other instructions
 // bound it.
 // fp32: 4 x 784 rows of 12 heads of 64 to 197 keys 32 us, of which 12 pass before
-// the first tile and after the last; 2 x 2048 of 16 to 4096 keys 380-390 us (180
+// the first tile and after the last, and of a wave's time some 6 are vector
+// instructions, 3 matrix ones; 2 x 2048 of 16 to 4096 keys 380-390 us (180
 // TFLOP/s; the fp32 instructions' rate is 154), some 1000 vector instructions
 // of a wave, most of them splitting, beside 96 products a tile.
 template <class T, int DP, int SRC>
@@ -388,6 +389,11 @@ __global__ __launch_bounds__(kWaves * 64, (TilesShape<T, DP, SRC>::per_cu)) void
             for (int i = 0; i < 16; ++i) acc[t][i] *= keep;
         }
         const float base = m == -INFINITY ? 0.f : m;
+        // 16-bit types: probabilities are rounded to the type for the second
+        // product, as with few rows.  As the sum of two they would take another one:
+        // us with one / two 737 / 987 (2 x 3136 rows of 16 heads of 128 to 12544 keys
+        // bf16), 23.3 / 29.7 (4 x 784 of 12 of 64 to 784), 60 / 73 (fp16 over the cache).
+        // l sums them as they were; with units as rounded (sum8).
         typename std::conditional<S::split, v8f, FM>::type pf[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t)

@@ -13,7 +13,9 @@ reference's single-image [C,H,W] blobs.
 
 Behind the layers stand the token operators, for a decoder that reads a
 network's features: GroupNorm, Rotary, cross_attention and KvCache8 (float32,
-float16 and bfloat16; no counterpart in the reference).
+float16 and bfloat16).  The reference lowers ncnn's attention layers for the CPU
+(lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:3859-4668); these are calls, not layers
+of a graph, and the other three have no counterpart there.
 """
 from __future__ import annotations
 
