@@ -58,8 +58,8 @@ extern "C" {
 #define NHIP_ACT_NONE 0
 #define NHIP_ACT_RELU 1
 #define NHIP_ACT_SIGMOID 4
-/* x * sigmoid(x), ncnn's Swish layer (group norm only; no activation_type of
- * ncnn's has this value). */
+/* x * sigmoid(x), ncnn's Swish layer (group norm and 8-bit products of tokens
+ * only; no activation_type of ncnn's has this value). */
 #define NHIP_ACT_SILU 64
 
 /* Element types.  The graph's blobs are F32, I8 or I32 (Input blobs read by
@@ -499,6 +499,38 @@ int nhip_kv8_attention_forward(
     const int32_t* block_table, int64_t table_pages, const int32_t* lengths,
     int32_t causal, void* out, void* workspace, uint64_t workspace_bytes,
     void* stream);
+
+/* Products of tokens with weights in 8-bit integers, a scale for each token and
+ * each output channel; several experts' weights make it the product grouped by
+ * expert:
+ *   out[t][j] = act((sum_k q[t][k] * w[e][j][k]) * (s[t] * weight_scale[e][j]) + bias[e][j])
+ * A token's scale s is its largest |x| times fp32(1/127), at least 2^-126 (0 for
+ * a token of zeros), its codes q x * (1 / s) in fp32 to the nearest, halves away
+ * from zero; the sum is exact, the rest fp32, rounded once to the type.  A token
+ * that holds an infinity or NaN is NaN in all its results.
+ * weight: [experts][num_output][num_input], int8 with weight_scale
+ * [experts][num_output], or fp32 with weight_scale NULL (a channel's codes and
+ * scale are then found as a token's are).  bias: fp32 [experts][num_output] or
+ * NULL.  The plan keeps a copy; the tensors are read on `stream`, which the call
+ * waits for.  num_input at most 131072; activation NONE, RELU or SILU. */
+typedef struct nhip_linear8_plan* nhip_linear8_t;
+int nhip_linear8_create(int32_t experts, int32_t num_output, int32_t num_input,
+                        const void* weight, int32_t weight_is_i8,
+                        const float* weight_scale, const float* bias,
+                        int32_t activation, void* stream, nhip_linear8_t* plan);
+int nhip_linear8_workspace_size(nhip_linear8_t plan, int32_t dtype,
+                                int64_t rows, uint64_t* bytes);
+/* x: [rows][num_input], rows row_stride elements apart; out: [rows][num_output]
+ * contiguous, not overlapping x.  expert_starts: int32 [experts + 1], not
+ * falling: rows expert_starts[e] .. expert_starts[e + 1] - 1 are expert e's,
+ * rows before the first and behind the last are left as they were (starts are
+ * clamped to 0..rows).  NULL with one expert: all rows. */
+int nhip_linear8_forward(nhip_linear8_t plan, const void* x, int32_t dtype,
+                         int64_t rows, int64_t row_stride,
+                         const int32_t* expert_starts, void* out,
+                         void* workspace, uint64_t workspace_bytes,
+                         void* stream);
+int nhip_linear8_destroy(nhip_linear8_t plan);
 
 #ifdef __cplusplus
 }

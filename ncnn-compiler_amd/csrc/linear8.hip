@@ -1,0 +1,394 @@
+// Products of tokens with weights in 8-bit integers, a scale for each token and
+// each output channel: the tokens' codes, the product for few rows, the entry
+// points.  (The product for many rows: linear8_tiles.hip.)
+//
+// Compiled with -ffp-contract=off: a code is the rounding of one separately
+// rounded product, so that it can be restated bit for bit.
+#include <algorithm>
+#include <new>
+
+#include "linear8.h"
+
+struct nhip_linear8_plan {
+  int32_t experts, n, k, act, device;
+  int32_t blocks, steps;  // of 16 channels, of 64 summed indices
+  int8_t* w = nullptr;
+  float* w_scale = nullptr;  // [experts][n], the bias behind it
+};
+
+namespace nhip {
+namespace {
+
+constexpr int kMaxK = 131072;  // 128 * 127 * 131072 < 2^31 (a weight may be -128)
+constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126: the reciprocal stays finite
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+
+// Eight channels from c of a row; those at and past k are 0.
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int c, int k, float (&x)[8]) {
+  if (VEC && c + 8 <= k) {
+    constexpr int V = kVec<T>;
+#pragma unroll
+    for (int j = 0; j < 8; j += V) {
+      float t[V];
+      Vec<T, V>::load(row + c + j, t);
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[j + i] = t[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = c + i < k ? (float)row[c + i] : 0.f;
+  }
+}
+
+// One workgroup: one row of codes, its largest magnitude first.  A thread keeps
+// its first kHeld eights and reads others again.
+template <class T, bool VEC, int TH>
+__global__ __launch_bounds__(TH) void linear8_codes_kernel(const T* x, int64_t stride, int k, int kp, int8_t* codes,
+                                                           float* scales) {
+  constexpr int kHeld = 4;
+  const int64_t r = blockIdx.x;
+  const T* row = x + r * stride;
+  float held[kHeld][8], most = 0.f;
+  bool whole = true;  // finite
+  const auto widest = [&](const float(&t)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      most = fmaxf(most, fabsf(t[i]));
+      whole = whole && fabsf(t[i]) <= 3.4028235e38f;
+    }
+  };
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h)
+    if (const int c = (threadIdx.x + h * TH) * 8; c < k) {
+      load8<T, VEC>(row, c, k, held[h]);
+      widest(held[h]);
+    }
+  for (int c = (threadIdx.x + kHeld * TH) * 8; c < k; c += TH * 8) {
+    float t[8];
+    load8<T, VEC>(row, c, k, t);
+    widest(t);
+  }
+  most = wave_max(whole ? most : INFINITY);
+  if constexpr (TH > 64) {
+    __shared__ float part[TH / 64];
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TH / 64; ++i) most = fmaxf(most, part[i]);
+  }
+  const float scale = most > 0.f ? fmaxf(most * (1.f / 127.f), kLeastScale) : 0.f;
+  const float inv = scale > 0.f && most < INFINITY ? 1.f / scale : 0.f;
+  int8_t* to = codes + r * kp;
+  const auto store = [&](const float(&t)[8], int c) {
+    int q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = quantize_q(t[i], inv);
+    *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_i8x4(q[0], q[1], q[2], q[3]), pack_i8x4(q[4], q[5], q[6], q[7]));
+  };
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h)
+    if (const int c = (threadIdx.x + h * TH) * 8; c < kp) {
+      if (c >= k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) held[h][i] = 0.f;
+      store(held[h], c);
+    }
+  for (int c = (threadIdx.x + kHeld * TH) * 8; c < kp; c += TH * 8) {
+    float t[8];
+    load8<T, VEC>(row, c, k, t);
+    store(t, c);
+  }
+  // a row that holds an infinity or NaN: codes 0, results 0 * NaN
+  if (threadIdx.x == 0) scales[r] = most < INFINITY ? scale : NAN;
+}
+
+template <class T>
+int codes_run(const void* x, int64_t stride, int64_t rows, int k, int kp, int8_t* codes, float* scales, hipStream_t s) {
+  const bool vec = aligned_to(x, 16) && stride % kVec<T> == 0;
+  const int th = kp <= 1024 ? 64 : kp <= 2048 ? 128 : 256;
+  const auto launch = [&](auto kernel) {
+    NHIP_LAUNCH("linear8_codes", kernel, dim3((uint32_t)rows), dim3(th), 0, s, (const T*)x, stride, k, kp, codes, scales);
+    return check_launch("linear8_codes");
+  };
+  if (vec)
+    return th == 64    ? launch(linear8_codes_kernel<T, true, 64>)
+           : th == 128 ? launch(linear8_codes_kernel<T, true, 128>)
+                       : launch(linear8_codes_kernel<T, true, 256>);
+  return th == 64    ? launch(linear8_codes_kernel<T, false, 64>)
+         : th == 128 ? launch(linear8_codes_kernel<T, false, 128>)
+                     : launch(linear8_codes_kernel<T, false, 256>);
+}
+
+// Codes [rows][stride] into the plan's order, 16 codes to a thread; past n and k zeros.
+__global__ __launch_bounds__(256) void linear8_order_kernel(const int8_t* from, int64_t stride, int experts, int n, int k,
+                                                            int blocks, int steps, bool vec, int8_t* to) {
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (item >= (int64_t)experts * blocks * steps * 64) return;
+  const int lane = item & 63;
+  int64_t at = item >> 6;
+  const int step = (int)(at % steps);
+  at /= steps;
+  const int row = (int)(at % blocks) * 16 + (lane & 15), c = step * kStepK + (lane >> 4) * 16;
+  int4 v = make_int4(0, 0, 0, 0);
+  if (row < n && c < k) {
+    const int8_t* src = from + (at / blocks * n + row) * stride + c;
+    if (vec && c + 16 <= k) {
+      v = *reinterpret_cast<const int4*>(src);
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c + i < k) w[i >> 2] |= (uint32_t)(uint8_t)src[i] << (8 * (i & 3));
+      v = make_int4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  *reinterpret_cast<int4*>(to + item * 16) = v;
+}
+
+__global__ __launch_bounds__(256) void linear8_params_kernel(const float* scale, const float* bias, int64_t count,
+                                                             float* to) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  if (scale) to[i] = scale[i];
+  to[count + i] = bias ? bias[i] : 0.f;
+}
+
+// ---------------------------------------------------------------- few rows
+// One workgroup: NB blocks of 16 channels of one expert, 16 TG of its rows at a
+// time; its waves take the steps of the sum in turn and are joined in LDS.
+constexpr int kAhead = 4;  // steps that a wave reads before it multiplies them
+template <class T, int TG, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a) {
+  __shared__ v4i part[WAVES][TG * NB][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = (a.blocks + NB - 1) / NB;
+  const int e = blockIdx.x / groups, b0 = blockIdx.x % groups * NB;
+  int begin, end;
+  expert_rows(a, e, begin, end);
+  const int8_t* w[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    w[b] = a.w + ((int64_t)e * a.blocks + min(b0 + b, a.blocks - 1)) * a.steps * 1024 + lane * 16;
+  for (int r0 = begin; r0 < end; r0 += 16 * TG) {
+    const int8_t* x[TG];
+#pragma unroll
+    for (int t = 0; t < TG; ++t) x[t] = a.x + (int64_t)min(r0 + t * 16 + (lane & 15), end - 1) * a.kp + (lane >> 4) * 16;
+    v4i acc[TG][NB];
+#pragma unroll
+    for (int t = 0; t < TG; ++t)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[t][b] = v4i{0, 0, 0, 0};
+    for (int s = wave; s < a.steps; s += WAVES * kAhead) {
+      v4i wf[kAhead][NB], xf[kAhead][TG];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int at = min(s + u * WAVES, a.steps - 1);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) wf[u][b] = *reinterpret_cast<const v4i*>(w[b] + at * 1024);
+#pragma unroll
+        for (int t = 0; t < TG; ++t) xf[u][t] = *reinterpret_cast<const v4i*>(x[t] + at * kStepK);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (s + u * WAVES >= a.steps)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) wf[u][b] = v4i{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < TG; ++t)
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            acc[t][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][b], xf[u][t], acc[t][b], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TG; ++t)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        settle8(acc[t][b]);
+        part[wave][t * NB + b][lane] = acc[t][b];
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < TG * NB * 64; i += WAVES * 64) {
+      v4i sum = part[0][i >> 6][i & 63];
+#pragma unroll
+      for (int v = 1; v < WAVES; ++v) sum += part[v][i >> 6][i & 63];
+      const int l = i & 63, b = (i >> 6) % NB, t = (i >> 6) / NB;
+      const int row = r0 + t * 16 + (l & 15), j = (b0 + b) * 16 + 4 * (l >> 4);
+      if (row < end) {
+        const float xs = a.x_scale[row];
+        const float* ws = a.w_scale + (int64_t)e * a.n;
+        const float* bias = a.bias + (int64_t)e * a.n;
+        T* out = (T*)a.out + (int64_t)row * a.n;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (j + c < a.n) out[j + c] = (T)finish8(sum[c], xs * ws[j + c], bias[j + c], a.act);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <class T, int TG>
+int rows_run(const Linear8Args& a, hipStream_t s) {
+  const auto launch = [&](auto kernel, int nb, int waves) {
+    NHIP_LAUNCH("linear8_rows", kernel, dim3((uint32_t)(a.experts * ceil_div(a.blocks, nb))), dim3(waves * 64), 0, s, a);
+    return check_launch("linear8_rows");
+  };
+  if ((int64_t)a.experts * a.blocks > 4 * cu_count()) return launch(linear8_rows_kernel<T, TG, 2, 4>, 2, 4);
+  return launch(linear8_rows_kernel<T, TG, 1, 8>, 1, 8);
+}
+
+template <class T>
+int product_run(const Linear8Args& a, hipStream_t s) {
+  const int64_t each = ceil_div(a.rows, a.experts);
+  if (each <= 16) return rows_run<T, 1>(a, s);
+  if (each <= 32) return rows_run<T, 2>(a, s);
+  return rows_run<T, 4>(a, s);
+}
+
+// Codes of the tokens, their scales behind them.
+uint64_t workspace_of(const nhip_linear8_plan* p, int64_t rows) {
+  return (uint64_t)rows * p->steps * kStepK + (uint64_t)round_up(rows * (int64_t)sizeof(float), 16);
+}
+
+int linear8_args(const nhip_linear8_plan* p, int32_t dtype, int64_t rows) {
+  if (!p) return fail(NHIP_STATUS_NULL_POINTER, "linear8: null plan");
+  if (!elem_size(dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "linear8: dtype has to be F32, F16 or BF16");
+  if (rows < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "linear8: negative extent");
+  if (rows > 0x7ffffeff) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many rows");
+  return ok();
+}
+
+}  // namespace
+}  // namespace nhip
+
+using namespace nhip;
+
+extern "C" {
+
+int nhip_linear8_create(int32_t experts, int32_t num_output, int32_t num_input, const void* weight, int32_t weight_is_i8,
+                        const float* weight_scale, const float* bias, int32_t activation, void* stream,
+                        nhip_linear8_t* plan) {
+  if (!plan) return fail(NHIP_STATUS_NULL_POINTER, "linear8: null plan pointer");
+  *plan = nullptr;
+  if (experts <= 0 || num_output <= 0 || num_input <= 0) return fail(NHIP_STATUS_INVALID_SHAPE, "linear8: sizes have to be positive");
+  if (num_input > kMaxK) return fail(NHIP_STATUS_INVALID_SHAPE, "linear8: at most 131072 inputs, the sums are of 32 bits");
+  if (activation != NHIP_ACT_NONE && activation != NHIP_ACT_RELU && activation != NHIP_ACT_SILU)
+    return fail(NHIP_STATUS_UNSUPPORTED, "linear8: activation has to be NONE, RELU or SILU");
+  const int64_t blocks = ceil_div(num_output, 16), steps = round_up(num_input, kPadK) / kStepK;
+  if (experts * blocks > 0x7fffffff / 4 || experts * (int64_t)num_output > 0x7fffffff)
+    return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many output channels");
+  if (!weight || (weight_is_i8 && !weight_scale)) return fail(NHIP_STATUS_NULL_POINTER, "linear8: null pointer");
+  if (!weight_is_i8 && weight_scale)
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "linear8: scales come with 8-bit weights, those of fp32 weights are found here");
+  if (!aligned_to(weight, weight_is_i8 ? 1 : 4) || !aligned_to(weight_scale, 4) || !aligned_to(bias, 4))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "linear8: a tensor is not aligned to its type");
+  const hipStream_t s = as_stream(stream);
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  NHIP_TRY(check_hip(hipStreamIsCapturing(s, &capture), "hipStreamIsCapturing"));
+  if (capture != hipStreamCaptureStatusNone)
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "linear8: a plan is not made while the stream is recorded");
+  nhip_linear8_plan* p = new (std::nothrow) nhip_linear8_plan;
+  if (!p) return fail(NHIP_STATUS_DEVICE_ERROR, "linear8: out of host memory");
+  p->experts = experts;
+  p->n = num_output;
+  p->k = num_input;
+  p->act = activation;
+  p->blocks = (int32_t)blocks;
+  p->steps = (int32_t)steps;
+  const int64_t count = experts * (int64_t)num_output, items = experts * blocks * steps * 64;
+  int8_t* codes = nullptr;
+  const auto build = [&]() -> int {
+    NHIP_TRY(check_hip(hipGetDevice(&p->device), "hipGetDevice"));
+    if (ceil_div(items, 256) > 0x7fffffff) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many weights");
+    NHIP_TRY(check_hip(hipMalloc(reinterpret_cast<void**>(&p->w), items * 16), "hipMalloc(linear8 weights)"));
+    NHIP_TRY(check_hip(hipMalloc(reinterpret_cast<void**>(&p->w_scale), 2 * count * sizeof(float)), "hipMalloc(linear8 scales)"));
+    const int8_t* from = (const int8_t*)weight;
+    int64_t stride = num_input;
+    if (!weight_is_i8) {
+      stride = steps * kStepK;
+      NHIP_TRY(check_hip(hipMalloc(reinterpret_cast<void**>(&codes), count * stride), "hipMalloc(linear8 codes)"));
+      NHIP_TRY(codes_run<float>(weight, num_input, count, num_input, (int)stride, codes, p->w_scale, s));
+      from = codes;
+    }
+    NHIP_LAUNCH("linear8_order", linear8_order_kernel, dim3((uint32_t)ceil_div(items, 256)), dim3(256), 0, s, from, stride,
+                experts, num_output, num_input, (int)blocks, (int)steps, aligned_to(from, 16) && stride % 16 == 0, p->w);
+    NHIP_TRY(check_launch("linear8_order"));
+    NHIP_LAUNCH("linear8_params", linear8_params_kernel, dim3((uint32_t)ceil_div(count, 256)), dim3(256), 0, s, weight_scale,
+                bias, count, p->w_scale);
+    NHIP_TRY(check_launch("linear8_params"));
+    return check_hip(hipStreamSynchronize(s), "hipStreamSynchronize(linear8 plan)");
+  };
+  const int st = build();
+  if (codes) (void)hipFree(codes);
+  if (st != NHIP_STATUS_SUCCESS) {
+    (void)hipFree(p->w);
+    (void)hipFree(p->w_scale);
+    delete p;
+    return st;
+  }
+  *plan = p;
+  return ok();
+}
+
+int nhip_linear8_workspace_size(nhip_linear8_t plan, int32_t dtype, int64_t rows, uint64_t* bytes) {
+  if (!bytes) return fail(NHIP_STATUS_NULL_POINTER, "linear8: null pointer");
+  NHIP_TRY(linear8_args(plan, dtype, rows));
+  *bytes = rows ? workspace_of(plan, rows) : 0;
+  return ok();
+}
+
+int nhip_linear8_forward(nhip_linear8_t plan, const void* x, int32_t dtype, int64_t rows, int64_t row_stride,
+                         const int32_t* expert_starts, void* out, void* workspace, uint64_t workspace_bytes, void* stream) {
+  NHIP_TRY(linear8_args(plan, dtype, rows));
+  if (!expert_starts && plan->experts > 1)
+    return fail(NHIP_STATUS_NULL_POINTER, "linear8: rows of several experts need their starts");
+  if (rows == 0) return ok();
+  if (!x || !out || !workspace) return fail(NHIP_STATUS_NULL_POINTER, "linear8: null pointer");
+  const int es = elem_size(dtype);
+  if (!aligned_to(x, es) || !aligned_to(out, es) || !aligned_to(expert_starts, 4))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "linear8: a tensor is not aligned to its type");
+  if (row_stride < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "linear8: negative stride");
+  int dev = -1;
+  NHIP_TRY(check_hip(hipGetDevice(&dev), "hipGetDevice"));
+  if (dev != plan->device) return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "linear8: the plan is another device's");
+  if (workspace_bytes < workspace_of(plan, rows) || !aligned_to(workspace, 16))
+    return fail(NHIP_STATUS_OUTPUT_CAPACITY_INSUFFICIENT, "linear8: workspace too small or not 16-byte aligned");
+  const int kp = plan->steps * kStepK;
+  int8_t* codes = (int8_t*)workspace;
+  float* scales = (float*)(codes + rows * kp);
+  Linear8Args a{};
+  a.x = codes;
+  a.x_scale = scales;
+  a.w = plan->w;
+  a.w_scale = plan->w_scale;
+  a.bias = plan->w_scale + plan->experts * (int64_t)plan->n;
+  a.out = out;
+  a.starts = expert_starts;
+  a.rows = (int32_t)rows;
+  a.n = plan->n;
+  a.kp = kp;
+  a.steps = plan->steps;
+  a.blocks = plan->blocks;
+  a.experts = plan->experts;
+  a.act = plan->act;
+  NHIP_TRY(NHIP_FOR_ELEM(dtype, T, codes_run<T>(x, row_stride, rows, plan->k, kp, codes, scales, as_stream(stream))));
+  if (linear8_tiles_selected(a)) return linear8_tiles(a, dtype, as_stream(stream));
+  return NHIP_FOR_ELEM(dtype, T, product_run<T>(a, as_stream(stream)));
+}
+
+int nhip_linear8_destroy(nhip_linear8_t plan) {
+  if (!plan) return ok();
+  (void)hipFree(plan->w);
+  (void)hipFree(plan->w_scale);
+  delete plan;
+  return ok();
+}
+
+}  // extern "C"

@@ -36,7 +36,7 @@ STATUS_NAMES = {
 
 ALGO_AUTO, ALGO_IMPLICIT_GEMM, ALGO_WINOGRAD = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_SIGMOID = 0, 1, 4
-ACT_SILU = 64  # group norm only
+ACT_SILU = 64  # GroupNorm and Linear8 only
 
 # Every symbol include/nhip.h declares (checked by the CPU test suite).
 EXPORTS = (
@@ -61,6 +61,7 @@ EXPORTS = (
     "nhip_rotary_create", "nhip_rotary_forward", "nhip_rotary_destroy",
     "nhip_cross_attention_workspace_size", "nhip_cross_attention_forward",
     "nhip_kv8_append", "nhip_kv8_read", "nhip_kv8_attention_workspace_size", "nhip_kv8_attention_forward",
+    "nhip_linear8_create", "nhip_linear8_workspace_size", "nhip_linear8_forward", "nhip_linear8_destroy",
 )
 
 # Every symbol include/nhip_graph.h declares.
@@ -179,6 +180,10 @@ def load():
         "nhip_kv8_read": [K8, i32, i32, i32, _P, i64, _P, _P, _P, _P],
         "nhip_kv8_attention_workspace_size": [A, K8, U],
         "nhip_kv8_attention_forward": [A, K8, _P, S, _P, i64, _P, i32, _P, _P, u64, _P],
+        "nhip_linear8_create": [i32, i32, i32, _P, i32, _P, _P, i32, _P, ctypes.POINTER(_P)],
+        "nhip_linear8_workspace_size": [_P, i32, i64, U],
+        "nhip_linear8_forward": [_P, _P, i32, i64, i64, _P, _P, _P, u64, _P],
+        "nhip_linear8_destroy": [_P],
     })
     i64p, i32p, vpp = ctypes.POINTER(i64), ctypes.POINTER(i32), ctypes.POINTER(_P)
     sig.update({
@@ -866,6 +871,71 @@ class Rotary(_Plan):
         check(load().nhip_rotary_forward(self.handle, x.data_ptr(), code, b, n, h, _strides(x.stride()), pos,
                                          n * self.axes if per > 1 else 0, 1 if inverse else 0, out.data_ptr(),
                                          _strides(out.stride()), _on(stream, dev)))
+        return out
+
+
+class Linear8(_Plan):
+    """Products of tokens with weights in 8-bit integers, a scale for each token
+    and each output channel (include/nhip.h: nhip_linear8_create).  weight:
+    [num_output, num_input] or [experts, num_output, num_input], int8 with
+    weight_scale [..., num_output], or float32 without; bias [..., num_output];
+    arrays or tensors, on the device or not.  The plan is of the device that is
+    current."""
+    _destroy = "nhip_linear8_destroy"
+
+    def __init__(self, weight, weight_scale=None, bias=None, act=ACT_NONE):
+        super().__init__()
+        torch = _torch()
+        device = torch.device("cuda", torch.cuda.current_device())
+        weight = torch.as_tensor(weight)
+        if weight.dtype not in (torch.int8, torch.float32) or weight.dim() not in (2, 3):
+            raise TypeError("weight has to be int8 or float32, [num_output, num_input] or [experts, num_output, num_input]")
+        is_i8 = weight.dtype == torch.int8
+        if is_i8 != (weight_scale is not None):
+            raise ValueError("int8 weights come with weight_scale, float32 ones without")
+        values = [None if v is None else torch.as_tensor(v) for v in (weight_scale, bias)]
+        for v in values:
+            if v is not None and (v.shape != weight.shape[:-1] or v.dtype != torch.float32):
+                raise ValueError(f"weight_scale and bias have to be float32 of shape {tuple(weight.shape[:-1])}")
+        self.grouped = weight.dim() == 3
+        self.experts = weight.shape[0] if self.grouped else 1
+        self.num_output, self.num_input = weight.shape[-2:]
+        weight, scale, bias = (None if v is None else v.to(device).contiguous() for v in (weight, *values))
+        check(load().nhip_linear8_create(self.experts, self.num_output, self.num_input, _ptr(weight), 1 if is_i8 else 0,
+                                         _ptr(scale), _ptr(bias), act, _stream(), ctypes.byref(self.handle)))
+        self._sizes = {}
+
+    def workspace_size(self, dtype_code, rows) -> int:
+        n = self._sizes.get((_settings, dtype_code, rows))
+        if n is None:
+            b = ctypes.c_uint64()
+            check(load().nhip_linear8_workspace_size(self.handle, dtype_code, rows, ctypes.byref(b)))
+            if len(self._sizes) > 4096:
+                self._sizes.clear()
+            n = self._sizes[(_settings, dtype_code, rows)] = b.value
+        return n
+
+    def forward(self, x, expert_starts=None, out=None, workspace=None, stream=None):
+        """x [..., num_input] (rows of any one stride) -> [..., num_output].  Several
+        experts: x [rows, num_input] sorted by expert, expert_starts int32
+        [experts + 1]; rows of no expert are left as `out` had them."""
+        shape = x.shape
+        code, dev = _elem(x)
+        if shape[-1] != self.num_input:
+            raise ValueError(f"x has {shape[-1]} channels, expected {self.num_input}")
+        if len(shape) != 2:
+            x = x.view(-1, self.num_input)
+        rows = x.shape[0]
+        if expert_starts is not None:
+            starts = _ints(expert_starts, dev, (self.experts + 1,), "expert_starts")
+        elif self.experts > 1:
+            raise ValueError("rows of several experts need expert_starts")
+        else:
+            starts = None
+        out = _output(out, x, shape[:-1] + (self.num_output,), stream)
+        ws, ptr, nbytes = _scratch(workspace, self.workspace_size(code, rows), x, stream)
+        check(load().nhip_linear8_forward(self.handle, x.data_ptr(), code, rows, x.stride(0), starts, out.data_ptr(), ptr,
+                                          nbytes, _on(stream, dev)))
         return out
 
 
