@@ -532,6 +532,42 @@ int nhip_linear8_forward(nhip_linear8_t plan, const void* x, int32_t dtype,
                          void* stream);
 int nhip_linear8_destroy(nhip_linear8_t plan);
 
+/* The next token of each row of logits.  Tokens stand in one order, larger
+ * logits first, of equal ones the lower index, with weights
+ * w = exp((logit - largest) / temperature) in 64 bits.  Kept are
+ *   top_k  the first top_k (0: all); of those
+ *   top_p  each whose forerunners weigh less than top_p of all (1: all; the
+ *          first in any case),
+ *   min_p  each of w >= min_p,
+ * and the token is the first, by index, with which the kept weights' sum passes
+ * uniform * all of it.  temperature 0 takes the first of the order.  NaN is
+ * -infinity; a weight below 2^-45 is 0; where +infinity stands, all others weigh
+ * 0.  A row of -infinity alone has no token: -1, logprob -infinity.
+ * A *_each array holds every row's own value in place of the single one; values
+ * out of range act as the nearest allowed one (NaN: as the filter left out,
+ * temperature NaN: 0). */
+typedef struct nhip_sample_desc {
+  int32_t dtype;
+  int32_t rows;
+  int32_t vocab;
+  int64_t row_stride;
+  float temperature; /* 0 or more */
+  int32_t top_k;     /* 0 or more */
+  float top_p;       /* 0 or more */
+  float min_p;       /* 0 to 1 */
+  const float* temperature_each;
+  const int32_t* top_k_each;
+  const float* top_p_each;
+  const float* min_p_each;
+} nhip_sample_desc;
+int nhip_sample_workspace_size(const nhip_sample_desc* desc, uint64_t* bytes);
+/* logits [rows][vocab], rows row_stride elements apart; uniform fp32 [rows], 0
+ * to below 1 (others are clamped; NaN: 0).  token int32 [rows]; logprob fp32
+ * [rows]: the logarithm of the token's share of the kept weights. */
+int nhip_sample_forward(const nhip_sample_desc* desc, const void* logits,
+                        const float* uniform, int32_t* token, float* logprob,
+                        void* workspace, uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,7 @@ EXPORTS = (
     "nhip_cross_attention_workspace_size", "nhip_cross_attention_forward",
     "nhip_kv8_append", "nhip_kv8_read", "nhip_kv8_attention_workspace_size", "nhip_kv8_attention_forward",
     "nhip_linear8_create", "nhip_linear8_workspace_size", "nhip_linear8_forward", "nhip_linear8_destroy",
+    "nhip_sample_workspace_size", "nhip_sample_forward",
 )
 
 # Every symbol include/nhip_graph.h declares.
@@ -97,6 +98,13 @@ class AttentionDesc(ctypes.Structure):
 class Kv8Desc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
         ("pages", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("kv_heads", "head_dim", "block_tokens")]
+
+
+class SampleDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "rows", "vocab")] + [
+        ("row_stride", ctypes.c_int64), ("temperature", ctypes.c_float), ("top_k", ctypes.c_int32),
+        ("top_p", ctypes.c_float), ("min_p", ctypes.c_float)] + [
+        (n, ctypes.c_void_p) for n in ("temperature_each", "top_k_each", "top_p_each", "min_p_each")]
 
 
 _lib = None
@@ -184,6 +192,8 @@ def load():
         "nhip_linear8_workspace_size": [_P, i32, i64, U],
         "nhip_linear8_forward": [_P, _P, i32, i64, i64, _P, _P, _P, u64, _P],
         "nhip_linear8_destroy": [_P],
+        "nhip_sample_workspace_size": [ctypes.POINTER(SampleDesc), U],
+        "nhip_sample_forward": [ctypes.POINTER(SampleDesc), _P, _P, _P, _P, _P, u64, _P],
     })
     i64p, i32p, vpp = ctypes.POINTER(i64), ctypes.POINTER(i32), ctypes.POINTER(_P)
     sig.update({
@@ -1064,6 +1074,40 @@ class KvCache8:
                                                 out.data_ptr(), ptr, nbytes, _on(stream, dev)))
         return out
 
+def _each(value, dev, rows, dtype, what):
+    """(single value, pointer of each row's own)"""
+    torch = _torch()
+    if not isinstance(value, torch.Tensor):
+        return value, None
+    if value.shape != (rows,) or value.dtype != dtype or value.get_device() != dev or not value.is_contiguous():
+        raise ValueError(f"{what} has to be a number or a contiguous {dtype} tensor of shape ({rows},) on device {dev}")
+    return 0, value.data_ptr()
+
+
+def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, workspace=None, stream=None):
+    """The next token of each row of logits [rows, vocab] (any row stride) by
+    uniform float32 [rows] (include/nhip.h: nhip_sample_desc): (tokens int32
+    [rows], the logarithms of their probabilities float32 [rows]).  The settings
+    are numbers or device tensors [rows] (top_k int32, the others float32)."""
+    torch = _torch()
+    rows, vocab = logits.shape
+    code, dev = _elem(logits)
+    if uniform.shape != (rows,) or uniform.dtype != torch.float32 or uniform.get_device() != dev or not uniform.is_contiguous():
+        raise ValueError(f"uniform has to be a contiguous float32 tensor of shape ({rows},) on device {dev}")
+    t, t_each = _each(temperature, dev, rows, torch.float32, "temperature")
+    k, k_each = _each(top_k, dev, rows, torch.int32, "top_k")
+    p, p_each = _each(top_p, dev, rows, torch.float32, "top_p")
+    m, m_each = _each(min_p, dev, rows, torch.float32, "min_p")
+    desc = SampleDesc(code, rows, vocab, logits.stride(0), t, min(k, 0x7fffffff), p, m, t_each, k_each, p_each, m_each)
+    n = ctypes.c_uint64()
+    check(load().nhip_sample_workspace_size(desc, n))
+    token, logprob = out or (None, None)
+    token = _output(token, uniform, (rows,), stream, _int32)
+    logprob = _output(logprob, uniform, (rows,), stream)
+    ws, ptr, nbytes = _scratch(workspace, n.value, logits, stream)
+    check(load().nhip_sample_forward(desc, logits.data_ptr(), uniform.data_ptr(), token.data_ptr(), logprob.data_ptr(), ptr,
+                                     nbytes, _on(stream, dev)))
+    return token, logprob
 
 
 class Graph:
