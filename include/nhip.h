@@ -500,6 +500,27 @@ int nhip_kv8_attention_forward(
     int32_t causal, void* out, void* workspace, uint64_t workspace_bytes,
     void* stream);
 
+/* The same for a batch in which sequences share a prefix: batch / groups
+ * sequences in a row are a group, whose prefix is the first prefix_lengths[g]
+ * tokens (int32 [groups], clamped to 0..prefix_keys) of the pages in its row of
+ * prefix_table (int32 [groups][prefix_table_pages]).  A row sees its group's
+ * prefix and of its sequence's own tokens (block_table, lengths, desc->keys:
+ * tokens behind the prefix, from 0) what it sees in nhip_kv8_attention_forward.
+ * The prefix is read once for all sequences of a group. */
+int nhip_kv8_prefix_attention_workspace_size(const nhip_attention_desc* desc,
+                                             int32_t groups,
+                                             int32_t prefix_keys,
+                                             const nhip_kv8_cache* cache,
+                                             uint64_t* bytes);
+int nhip_kv8_prefix_attention_forward(
+    const nhip_attention_desc* desc, int32_t groups, int32_t prefix_keys,
+    const nhip_kv8_cache* cache, const void* query,
+    const int64_t* query_strides, const int32_t* prefix_table,
+    int64_t prefix_table_pages, const int32_t* prefix_lengths,
+    const int32_t* block_table, int64_t table_pages, const int32_t* lengths,
+    int32_t causal, void* out, void* workspace, uint64_t workspace_bytes,
+    void* stream);
+
 /* Products of tokens with weights in 8-bit integers, a scale for each token and
  * each output channel; several experts' weights make it the product grouped by
  * expert:

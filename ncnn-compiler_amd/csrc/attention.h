@@ -33,8 +33,11 @@ struct AttnArgs {
   int32_t splits;     // few rows: parts of a sequence's keys
   int32_t workers;    // many rows: workgroups
   int32_t units;      // and the parts of a row tile's keys that are dealt to them
+  int32_t parts;      // the results stay parts, also where there is one to a row
+  int32_t per;        // queries come in runs of `per`, q_run elements apart (0: one run)
+  int64_t q_run;
   float scale_log2;   // scale / ln 2
-  float* part_o;      // few rows: [batch][kv_heads][rows][splits][d]; many: [workers][2][128][d]
+  float* part_o;      // few rows: [batch][kv_heads][rows][splits][d]; many: [workers][2][128][d] ([workers + row tiles][128][d] if all are parts)
   float2* part_ml;    // the same without [d]: maximum, sum
 };
 
@@ -44,6 +47,12 @@ enum { kSrcVec = 0, kSrcAny = 1, kSrcInt8 = 2 };  // 16-byte aligned rows; any s
 int attn_run_f32(const AttnArgs& a, int src, hipStream_t s);
 int attn_run_f16(const AttnArgs& a, int src, hipStream_t s);
 int attn_run_bf16(const AttnArgs& a, int src, hipStream_t s);
+// Over the 8-bit cache: the parts of `prefix`, whose sequences are groups of
+// those of `own` in turn (their queries one behind the other), and of `own`,
+// joined to the results of `own`.
+int attn_prefix_f32(const AttnArgs& prefix, const AttnArgs& own, hipStream_t s);
+int attn_prefix_f16(const AttnArgs& prefix, const AttnArgs& own, hipStream_t s);
+int attn_prefix_bf16(const AttnArgs& prefix, const AttnArgs& own, hipStream_t s);
 
 namespace attn {
 
@@ -103,6 +112,10 @@ __device__ __forceinline__ void settle(V& sums) {
 template <class V>
 __device__ __forceinline__ void settle(V& sums, V& more) {
   asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sums), "+v"(more));
+}
+// Query qi's place among a sequence's queries.
+__device__ __forceinline__ int64_t query_at(const AttnArgs& a, int qi) {
+  return a.per ? qi / a.per * a.q_run + qi % a.per * a.qs[1] : qi * a.qs[1];
 }
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
@@ -458,7 +471,7 @@ __global__ __launch_bounds__(kWaves * 64, rows_per_cu(sizeof(T), DP, SRC)) void 
   part_of(a, length, visible, split, STEP, begin, end);
 
   FT qf[KS];
-  const T* qrow = (const T*)a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
+  const T* qrow = (const T*)a.q + b * a.qs[0] + query_at(a, qi) + head * a.qs[2];
 #pragma unroll
   for (int s = 0; s < KS; ++s)
     qf[s] = row < a.rows ? load_q<T, SRC != kSrcAny>(qrow, Tile::q_channel(s, g), a.d) : zero_frag<T>();
@@ -589,12 +602,12 @@ __global__ __launch_bounds__(kWaves * 64, rows_per_cu(sizeof(T), DP, SRC)) void 
 #pragma unroll
       for (int i = 0; i < kWaves; ++i)
         if (w[i] != 0.f) o += w[i] * mo[(i * kRowTile + r) * OS + c];
-      if (a.splits > 1)
+      if (a.splits > 1 || a.parts)
         a.part_o[prow * a.d + c] = o;
       else
         ((T*)a.o)[(((int64_t)b * a.queries + oq) * a.heads + oh) * a.d + c] = (T)(none ? (nan ? NAN : 0.f) : o / total);
     }
-    if (a.splits > 1 && lane == 0) a.part_ml[prow] = make_float2(top, none ? (nan ? -1.f : 0.f) : total);
+    if ((a.splits > 1 || a.parts) && lane == 0) a.part_ml[prow] = make_float2(top, none ? (nan ? -1.f : 0.f) : total);
   }
 }
 
@@ -678,13 +691,63 @@ int run(const AttnArgs& a, int src, hipStream_t s) {
                  : src == kSrcAny ? launch_by_dim<T, kSrcAny>(a, s)
                                   : launch_by_dim<T, kSrcInt8>(a, s);
   NHIP_TRY(st);
-  if (a.tiles || a.splits == 1) return ok();
+  if (a.tiles || a.splits == 1 || a.parts) return ok();
   const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
   if (a.d % 4 == 0 && aligned_to(a.o, 4 * sizeof(T)))
     NHIP_LAUNCH("attention_join", (attn_join_kernel<T, 4>), dim3((uint32_t)ceil_div(rows * (a.d / 4), 256)), dim3(256), 0, s, a);
   else
     NHIP_LAUNCH("attention_join", (attn_join_kernel<T, 1>), dim3((uint32_t)ceil_div(rows * a.d, 256)), dim3(256), 0, s, a);
   return check_launch("attention_join");
+}
+
+// Where the parts of a row lie: of batch b's key/value head kvh.
+struct RowParts {
+  int count;
+  int64_t first, step;  // places of the parts
+  __device__ __forceinline__ RowParts(const AttnArgs& a, int b, int kvh, int row) {
+    const int64_t head = (int64_t)b * a.kv_heads + kvh;
+    if (a.tiles) {
+      const uint32_t tile = (uint32_t)(head * a.row_tiles + row / kTilesRows);
+      const bool dealt = a.workers != a.batch * a.kv_heads * a.row_tiles;
+      const int worker = dealt ? worker_of(a, tile * a.units) : (int)tile;
+      count = dealt ? worker_of(a, (tile + 1) * a.units - 1) - worker + 1 : 1;
+      first = ((int64_t)worker + tile) * kTilesRows + row % kTilesRows;
+      step = kTilesRows;
+    } else {
+      count = a.splits;
+      first = (head * a.rows + row) * a.splits;
+      step = 1;
+    }
+  }
+  __device__ __forceinline__ int64_t place(int i) const { return first + i * step; }
+};
+
+// Joins the parts of a row's keys in the prefix and of its own.
+template <class T>
+__global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs prefix, AttnArgs a) {
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int cols = a.d / 4, c = (int)(item % cols) * 4;
+  const int64_t prow = item / cols;
+  if (prow >= (int64_t)a.batch * a.kv_heads * a.rows) return;
+  const int row = (int)(prow % a.rows), kvh = (int)(prow / a.rows % a.kv_heads), b = (int)(prow / a.rows / a.kv_heads);
+  const int members = a.batch / prefix.batch;
+  const RowParts shared(prefix, b / members, kvh, b % members * a.rows + row), own(a, b, kvh, row);
+  join_parts<T, 4>(
+      shared.count + own.count,
+      [&](int i) { return i < shared.count ? prefix.part_ml[shared.place(i)] : a.part_ml[own.place(i - shared.count)]; },
+      [&](int i) {
+        return (i < shared.count ? prefix.part_o + shared.place(i) * a.d : a.part_o + own.place(i - shared.count) * a.d) + c;
+      },
+      (T*)a.o + (((int64_t)b * a.queries + row / a.group) * a.heads + kvh * a.group + row % a.group) * a.d + c);
+}
+
+template <class T>
+int run_prefix(const AttnArgs& prefix, const AttnArgs& a, hipStream_t s) {
+  NHIP_TRY((launch_by_dim<T, kSrcInt8>(prefix, s)));
+  NHIP_TRY((launch_by_dim<T, kSrcInt8>(a, s)));
+  const int64_t items = (int64_t)a.batch * a.kv_heads * a.rows * (a.d / 4);
+  NHIP_LAUNCH("attention_prefix_join", (attn_prefix_join_kernel<T>), dim3((uint32_t)ceil_div(items, 256)), dim3(256), 0, s, prefix, a);
+  return check_launch("attention_prefix_join");
 }
 
 }  // namespace attn

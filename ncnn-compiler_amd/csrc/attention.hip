@@ -111,8 +111,12 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
 
 // Parts' (maximum, sum) pairs, an even number; their sums follow, 16-byte aligned.
 uint64_t parts_of(const AttnArgs& a) {
-  if (a.tiles) return a.workers == a.batch * a.kv_heads * a.row_tiles ? 0 : (uint64_t)a.workers * 2 * attn::kTilesRows;
-  return a.splits == 1 ? 0 : (uint64_t)round_up((int64_t)a.batch * a.kv_heads * a.rows * a.splits, 2);
+  if (a.tiles) {
+    const int64_t tiles = (int64_t)a.batch * a.kv_heads * a.row_tiles;
+    if (a.parts) return (uint64_t)(a.workers + tiles) * attn::kTilesRows;
+    return a.workers == tiles ? 0 : (uint64_t)a.workers * 2 * attn::kTilesRows;
+  }
+  return a.splits == 1 && !a.parts ? 0 : (uint64_t)round_up((int64_t)a.batch * a.kv_heads * a.rows * a.splits, 2);
 }
 
 uint64_t workspace_of(const AttnArgs& a) { return parts_of(a) * (a.d * sizeof(float) + sizeof(float2)); }
@@ -152,6 +156,28 @@ int attn_forward(AttnArgs& a, const nhip_attention_desc* d, int src, const void*
     case NHIP_DTYPE_F16: return attn_run_f16(a, src, as_stream(stream));
     default: return attn_run_bf16(a, src, as_stream(stream));
   }
+}
+
+// A prefix that `groups` groups of sequences share, and the sequences' own keys:
+// the descriptors of both.
+int prefix_args(const nhip_attention_desc* d, int32_t groups, int32_t prefix_keys, AttnArgs* prefix, AttnArgs* own) {
+  NHIP_TRY(attn_args(d, true, true, own));
+  if (groups <= 0 || d->batch % groups) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: groups have to divide the batch");
+  if (prefix_keys < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative extent");
+  nhip_attention_desc shared = *d;
+  const int64_t members = d->batch / groups;
+  if (members * d->queries > 0x7fffffff) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: too many rows");
+  shared.batch = groups;
+  shared.queries = (int32_t)(members * d->queries);
+  shared.keys = prefix_keys;
+  NHIP_TRY(attn_args(&shared, true, true, prefix));
+  prefix->parts = own->parts = 1;
+  prefix->per = d->queries;
+  return ok();
+}
+
+uint64_t prefix_workspace_of(const AttnArgs& prefix, const AttnArgs& own) {
+  return round_up(workspace_of(prefix), 16) + workspace_of(own);
 }
 
 // 16-byte aligned rows, near enough for a tile's to be reached with 31 bits.
@@ -226,6 +252,61 @@ int nhip_kv8_attention_forward(const nhip_attention_desc* desc, const nhip_kv8_c
   if (!aligned_to(query, 16) || !aligned_to(out, 16) || query_strides[0] % v || query_strides[1] % v || query_strides[2] % v)
     return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: queries and results over the cache have to be 16-byte aligned");
   return attn_forward(a, desc, kSrcInt8, query, query_strides, out, workspace, workspace_bytes, stream);
+}
+
+int nhip_kv8_prefix_attention_workspace_size(const nhip_attention_desc* desc, int32_t groups, int32_t prefix_keys,
+                                             const nhip_kv8_cache* cache, uint64_t* bytes) {
+  if (!bytes || !cache) return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
+  AttnArgs prefix{}, a{};
+  NHIP_TRY(prefix_args(desc, groups, prefix_keys, &prefix, &a));
+  *bytes = prefix_workspace_of(prefix, a);
+  return ok();
+}
+
+int nhip_kv8_prefix_attention_forward(const nhip_attention_desc* desc, int32_t groups, int32_t prefix_keys,
+                                      const nhip_kv8_cache* cache, const void* query, const int64_t* query_strides,
+                                      const int32_t* prefix_table, int64_t prefix_table_pages,
+                                      const int32_t* prefix_lengths, const int32_t* block_table, int64_t table_pages,
+                                      const int32_t* lengths, int32_t causal, void* out, void* workspace,
+                                      uint64_t workspace_bytes, void* stream) {
+  AttnArgs prefix{}, a{};
+  NHIP_TRY(prefix_args(desc, groups, prefix_keys, &prefix, &a));
+  if (desc->batch == 0 || desc->queries == 0) return ok();
+  NHIP_TRY(kv8_args(cache, prefix_table, prefix_table_pages, &prefix.cache));
+  NHIP_TRY(kv8_args(cache, block_table, table_pages, &a.cache));
+  if (cache->kv_heads != desc->kv_heads || cache->head_dim != desc->head_dim)
+    return fail(NHIP_STATUS_INVALID_SHAPE, "attention: the cache has other heads");
+  if (!query || !query_strides || !out || !lengths || !prefix_lengths || !workspace)
+    return fail(NHIP_STATUS_NULL_POINTER, "attention: null pointer");
+  if (!aligned_to(lengths, 4) || !aligned_to(prefix_lengths, 4))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: a tensor is not aligned to its type");
+  const int v = 16 / elem_size(desc->dtype);
+  for (int i = 0; i < 3; ++i) {
+    if (query_strides[i] < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative stride");
+    if (query_strides[i] % v)
+      return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: queries and results over the cache have to be 16-byte aligned");
+    prefix.qs[i] = a.qs[i] = query_strides[i];
+  }
+  if (!aligned_to(query, 16) || !aligned_to(out, 16))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "attention: queries and results over the cache have to be 16-byte aligned");
+  if (workspace_bytes < prefix_workspace_of(prefix, a) || !aligned_to(workspace, 16))
+    return fail(NHIP_STATUS_OUTPUT_CAPACITY_INSUFFICIENT, "attention: workspace too small or not 16-byte aligned");
+  prefix.q = a.q = query;
+  prefix.o = a.o = out;
+  prefix.q_run = query_strides[0];
+  prefix.qs[0] = query_strides[0] * (desc->batch / groups);
+  prefix.lengths = prefix_lengths;
+  a.lengths = lengths;
+  a.causal = causal != 0;
+  prefix.part_ml = (float2*)workspace;
+  prefix.part_o = (float*)(prefix.part_ml + parts_of(prefix));
+  a.part_ml = (float2*)((char*)workspace + round_up(workspace_of(prefix), 16));
+  a.part_o = (float*)(a.part_ml + parts_of(a));
+  switch (desc->dtype) {
+    case NHIP_DTYPE_F32: return attn_prefix_f32(prefix, a, as_stream(stream));
+    case NHIP_DTYPE_F16: return attn_prefix_f16(prefix, a, as_stream(stream));
+    default: return attn_prefix_bf16(prefix, a, as_stream(stream));
+  }
 }
 
 }  // extern "C"

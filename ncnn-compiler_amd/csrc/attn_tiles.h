@@ -229,7 +229,7 @@ __global__ __launch_bounds__(kWaves * 64, (TilesShape<T, DP, SRC>::per_cu)) void
     constexpr bool LATE = S::split && DP == 256;
     FM qf[LATE ? 1 : KS][QP];
     v8f qx[LATE ? KS : 1];
-    const T* qrow = (const T*)a.q + b * a.qs[0] + qi * a.qs[1] + head * a.qs[2];
+    const T* qrow = (const T*)a.q + b * a.qs[0] + query_at(a, qi) + head * a.qs[2];
     const auto query = [&](int s) {
       auto q = row < a.rows ? load_q<T, true>(qrow, s * 16 + h * 8, a.d) : zero_frag<T>();
       return a.scale_log2 < 0.f ? -q : q;
@@ -490,9 +490,10 @@ __global__ __launch_bounds__(kWaves * 64, (TilesShape<T, DP, SRC>::per_cu)) void
     if (l != l) m = INFINITY;                         // NaN to whoever joins this
     else if (m == -INFINITY) l = seen ? -1.f : 0.f;  // scores of -infinity alone: 0 / 0, told from a row that sees nothing
     // a whole row tile's result, or a part: the one that begins the tile goes to
-    // the worker's second place, any other to its first
-    const bool whole_tile = u1 - u0 == a.units;
-    const int64_t prow = ((int64_t)worker * 2 + (u0 == 0)) * kTilesRows + wave * 32 + col;
+    // the worker's second place, any other to its first.  (Where all results stay
+    // parts a worker may have any number: worker and row tile rise by turns.)
+    const bool whole_tile = u1 - u0 == a.units && !a.parts;
+    const int64_t prow = (a.parts ? (int64_t)worker + tile : (int64_t)worker * 2 + (u0 == 0)) * kTilesRows + wave * 32 + col;
     float* part = a.part_o + prow * a.d;
     T* out = (T*)a.o + (((int64_t)b * a.queries + qi) * a.heads + head) * a.d;
     const float scale = m == -INFINITY ? (l < 0.f ? NAN : 0.f) : in / l;
@@ -543,7 +544,7 @@ int tiles_launch(const AttnArgs& a, hipStream_t s) {
               dim3(kWaves * 64), bytes, s, a);
   NHIP_TRY(check_launch("attention_tiles"));
   const int64_t tiles = (int64_t)a.batch * a.kv_heads * a.row_tiles;
-  if (a.workers == tiles) return ok();
+  if (a.workers == tiles || a.parts) return ok();
   NHIP_LAUNCH("attention_join", attn_tiles_join_kernel<T>, dim3((uint32_t)(tiles * ceil_div(kTilesRows * (a.d / 4), 256))),
               dim3(256), 0, s, a);
   return check_launch("attention_join");

@@ -61,6 +61,7 @@ EXPORTS = (
     "nhip_rotary_create", "nhip_rotary_forward", "nhip_rotary_destroy",
     "nhip_cross_attention_workspace_size", "nhip_cross_attention_forward",
     "nhip_kv8_append", "nhip_kv8_read", "nhip_kv8_attention_workspace_size", "nhip_kv8_attention_forward",
+    "nhip_kv8_prefix_attention_workspace_size", "nhip_kv8_prefix_attention_forward",
     "nhip_linear8_create", "nhip_linear8_workspace_size", "nhip_linear8_forward", "nhip_linear8_destroy",
     "nhip_sample_workspace_size", "nhip_sample_forward",
 )
@@ -188,6 +189,8 @@ def load():
         "nhip_kv8_read": [K8, i32, i32, i32, _P, i64, _P, _P, _P, _P],
         "nhip_kv8_attention_workspace_size": [A, K8, U],
         "nhip_kv8_attention_forward": [A, K8, _P, S, _P, i64, _P, i32, _P, _P, u64, _P],
+        "nhip_kv8_prefix_attention_workspace_size": [A, i32, i32, K8, U],
+        "nhip_kv8_prefix_attention_forward": [A, i32, i32, K8, _P, S, _P, i64, _P, _P, i64, _P, i32, _P, _P, u64, _P],
         "nhip_linear8_create": [i32, i32, i32, _P, i32, _P, _P, i32, _P, ctypes.POINTER(_P)],
         "nhip_linear8_workspace_size": [_P, i32, i64, U],
         "nhip_linear8_forward": [_P, _P, i32, i64, i64, _P, _P, _P, u64, _P],
@@ -961,6 +964,15 @@ def _attention(settings, code, b, lq, lk, h, hkv, d, scale, cached=False):
     return desc, n.value
 
 
+@functools.lru_cache(4096)
+def _prefix_attention(settings, code, b, lq, lk, h, hkv, d, scale, groups, lp):
+    """(descriptor, workspace bytes)."""
+    desc = AttentionDesc(code, b, lq, lk, h, hkv, d, float(d) ** -0.5 if scale is None else float(scale))
+    n = ctypes.c_uint64()
+    check(load().nhip_kv8_prefix_attention_workspace_size(ctypes.byref(desc), groups, lp, ctypes.byref(Kv8Desc()), ctypes.byref(n)))
+    return desc, n.value
+
+
 def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, out=None, workspace=None, stream=None):
     """softmax(scale * q k^T) v: q [batch, queries, heads, d], k and v
     [batch, keys, kv_heads, d] (any strides of the first three).  key_lengths:
@@ -1073,6 +1085,36 @@ class KvCache8:
                                                 _ints(lengths, dev, (b,), "lengths"), 1 if causal else 0,
                                                 out.data_ptr(), ptr, nbytes, _on(stream, dev)))
         return out
+
+    def prefix_attention(self, q, prefix_table, prefix_lengths, block_table, lengths, max_prefix=None, max_length=None,
+                         causal=False, scale=None, out=None, workspace=None, stream=None):
+        """Attention of q [batch, queries, heads, head_dim] where batch / groups
+        sequences in a row share a prefix: the first prefix_lengths[g] tokens of
+        the pages in prefix_table [groups, pages], and behind them the first
+        lengths[b] of the sequence's own pages in block_table.  causal: the
+        queries are the last of the sequence's own tokens."""
+        b, lq, h, d = q.shape
+        code, dev = _elem(q)
+        if d != self.head_dim or dev != self._dev:
+            raise ValueError(f"q has to have {self.head_dim} channels to a head, on {self.k.device}")
+        groups, prefix_pages = prefix_table.shape
+        pages = block_table.shape[-1]
+        if groups < 1 or b % groups:
+            raise ValueError(f"{groups} groups of {b} sequences")
+        if max_prefix is None:
+            max_prefix = prefix_pages * self.block_tokens
+        if max_length is None:
+            max_length = pages * self.block_tokens
+        desc, need = _prefix_attention(_settings, code, b, lq, max_length, h, self.kv_heads, d, scale, groups, max_prefix)
+        out = _output(out, q, q.shape, stream)
+        ws, ptr, nbytes = _scratch(workspace, need, q, stream)
+        check(load().nhip_kv8_prefix_attention_forward(
+            desc, groups, max_prefix, self._desc, q.data_ptr(), _strides(q.stride()),
+            _ints(prefix_table, dev, (groups, prefix_pages), "prefix_table"), prefix_pages,
+            _ints(prefix_lengths, dev, (groups,), "prefix_lengths"), _ints(block_table, dev, (b, pages), "block_table"), pages,
+            _ints(lengths, dev, (b,), "lengths"), 1 if causal else 0, out.data_ptr(), ptr, nbytes, _on(stream, dev)))
+        return out
+
 
 def _each(value, dev, rows, dtype, what):
     """(single value, pointer of each row's own)"""
