@@ -34,12 +34,32 @@ __device__ __forceinline__ void expert_rows(const Linear8Args& a, int e, int& be
 }
 
 // The sum of a product of codes as the result.
-__device__ __forceinline__ float finish8(int sum, float scale, float bias, int act) {
-  float y = (float)sum * scale + bias;
-  if (act == NHIP_ACT_RELU) return y < 0.f ? 0.f : y;  // NaN stays
-  if (act == NHIP_ACT_SILU) return y / (1.f + __expf(-y));
+template <int ACT>
+__device__ __forceinline__ float finish8(int sum, float scale, float bias) {
+  const float y = (float)sum * scale + bias;
+  if constexpr (ACT == NHIP_ACT_RELU) return y < 0.f ? 0.f : y;  // NaN stays
+  if constexpr (ACT == NHIP_ACT_SILU) return y * __builtin_amdgcn_rcpf(1.f + __expf(-y));
   return y;
 }
+
+// Calls `f` with the activation as a constant.
+#define NHIP_FOR_ACT(act, ACT, ...)              \
+  [&]() -> int {                                 \
+    switch (act) {                               \
+      case NHIP_ACT_RELU: {                      \
+        constexpr int ACT = NHIP_ACT_RELU;       \
+        return __VA_ARGS__;                      \
+      }                                          \
+      case NHIP_ACT_SILU: {                      \
+        constexpr int ACT = NHIP_ACT_SILU;       \
+        return __VA_ARGS__;                      \
+      }                                          \
+      default: {                                 \
+        constexpr int ACT = NHIP_ACT_NONE;       \
+        return __VA_ARGS__;                      \
+      }                                          \
+    }                                            \
+  }()
 
 // Integer sums on their way out of the matrix instructions, before any branch:
 // the compiler's count of the cycles to wait was seen to miss the path on which

@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256) void linear8_params_kernel(const float* scale,
 // One workgroup: NB blocks of 16 channels of one expert, 16 TG of its rows at a
 // time; its waves take the steps of the sum in turn and are joined in LDS.
 constexpr int kAhead = 4;  // steps that a wave reads before it multiplies them
-template <class T, int TG, int NB, int WAVES>
+template <class T, int ACT, int TG, int NB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a) {
   __shared__ v4i part[WAVES][TG * NB][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -227,29 +227,29 @@ __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a)
         T* out = (T*)a.out + (int64_t)row * a.n;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          if (j + c < a.n) out[j + c] = (T)finish8(sum[c], xs * ws[j + c], bias[j + c], a.act);
+          if (j + c < a.n) out[j + c] = (T)finish8<ACT>(sum[c], xs * ws[j + c], bias[j + c]);
       }
     }
     __syncthreads();
   }
 }
 
-template <class T, int TG>
+template <class T, int ACT, int TG>
 int rows_run(const Linear8Args& a, hipStream_t s) {
   const auto launch = [&](auto kernel, int nb, int waves) {
     NHIP_LAUNCH("linear8_rows", kernel, dim3((uint32_t)(a.experts * ceil_div(a.blocks, nb))), dim3(waves * 64), 0, s, a);
     return check_launch("linear8_rows");
   };
-  if ((int64_t)a.experts * a.blocks > 4 * cu_count()) return launch(linear8_rows_kernel<T, TG, 2, 4>, 2, 4);
-  return launch(linear8_rows_kernel<T, TG, 1, 8>, 1, 8);
+  if ((int64_t)a.experts * a.blocks > 4 * cu_count()) return launch(linear8_rows_kernel<T, ACT, TG, 2, 4>, 2, 4);
+  return launch(linear8_rows_kernel<T, ACT, TG, 1, 8>, 1, 8);
 }
 
-template <class T>
+template <class T, int ACT>
 int product_run(const Linear8Args& a, hipStream_t s) {
   const int64_t each = ceil_div(a.rows, a.experts);
-  if (each <= 16) return rows_run<T, 1>(a, s);
-  if (each <= 32) return rows_run<T, 2>(a, s);
-  return rows_run<T, 4>(a, s);
+  if (each <= 16) return rows_run<T, ACT, 1>(a, s);
+  if (each <= 32) return rows_run<T, ACT, 2>(a, s);
+  return rows_run<T, ACT, 4>(a, s);
 }
 
 // Codes of the tokens, their scales behind them.
@@ -380,7 +380,7 @@ int nhip_linear8_forward(nhip_linear8_t plan, const void* x, int32_t dtype, int6
   a.act = plan->act;
   NHIP_TRY(NHIP_FOR_ELEM(dtype, T, codes_run<T>(x, row_stride, rows, plan->k, kp, codes, scales, as_stream(stream))));
   if (linear8_tiles_selected(a)) return linear8_tiles(a, dtype, as_stream(stream));
-  return NHIP_FOR_ELEM(dtype, T, product_run<T>(a, as_stream(stream)));
+  return NHIP_FOR_ELEM(dtype, T, NHIP_FOR_ACT(a.act, ACT, product_run<T, ACT>(a, as_stream(stream))));
 }
 
 int nhip_linear8_destroy(nhip_linear8_t plan) {

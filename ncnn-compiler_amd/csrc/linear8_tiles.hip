@@ -11,6 +11,7 @@ constexpr int kTile = 256, kWaves = 8;
 constexpr int kSide = kTile * kPadK;  // bytes of one operand's stage
 constexpr int kStage = 2 * kSide;
 constexpr int kLds = 2 * kStage;
+constexpr int kGroup = 4;
 
 // The expert and its row tile that tile `at` of all row tiles is: experts
 // without rows have none.  All 64 lanes call it.
@@ -45,16 +46,21 @@ __device__ __forceinline__ bool find_tile(const Linear8Args& a, int at, int& e, 
   return false;
 }
 
-template <class T>
+template <class T, int ACT>
 __global__ __launch_bounds__(kWaves * 64) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // workgroups go to the eight dies in turn: each die gets a run of the tiles
   const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
   if (id >= work) return;
+  // ... in blocks of kGroup row tiles, so that what its CUs work on at a time are
+  // few row tiles and few column tiles, which meet in its L2
+  const int band = id / (kGroup * col_tiles), in = id - band * kGroup * col_tiles;
+  const int high = min(kGroup, work / col_tiles - band * kGroup);
+  const int col = in / high;
   int e, begin, end;
-  if (!find_tile(a, id / col_tiles, e, begin, end)) return;
-  const int b0 = id % col_tiles * (kTile / 16);  // first block of channels
+  if (!find_tile(a, band * kGroup + in - col * high, e, begin, end)) return;
+  const int b0 = col * (kTile / 16);  // first block of channels
   const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
 
   // A wave's copies of a stage: 4 KB of weights, 4 KB of codes, 1 KB (16 rows, 64 codes) each.
@@ -76,6 +82,13 @@ __global__ __launch_bounds__(kWaves * 64) void linear8_tiles_kernel(Linear8Args 
     }
   };
   const int wc = wave & 1, wr = wave >> 1;  // 128 channels, 64 rows
+  // what the results need: a thread's entry of the channels' scales and biases, its rows' scales
+  static_assert(kWaves * 64 == 2 * kTile, "a thread to each channel's scale and bias");
+  const int channel = b0 * 16 + (threadIdx.x & (kTile - 1));
+  const float param = channel < a.n ? (threadIdx.x < kTile ? a.w_scale : a.bias)[(int64_t)e * a.n + channel] : 0.f;
+  float xs[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) xs[r] = a.x_scale[min(begin + wr * 64 + r * 32 + (lane & 31), end - 1)];
   v16i acc[4][2];
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -115,44 +128,63 @@ __global__ __launch_bounds__(kWaves * 64) void linear8_tiles_kernel(Linear8Args 
 #pragma unroll
     for (int r = 0; r < 2; ++r) settle8(acc[c][r]);
 
-  // lane: row lane & 31 of the 32, channels 8 (i / 4) + 4 (lane >> 5) + i % 4
-  const float* ws = a.w_scale + (int64_t)e * a.n;
-  const float* bias = a.bias + (int64_t)e * a.n;
-  const bool vec = a.n % 4 == 0 && ((uintptr_t)a.out & (4 * sizeof(T) - 1)) == 0;
+  // The results through LDS, 32 rows of a wave's 128 channels at a time, so that
+  // whole rows are stored.  A lane has row lane & 31, channels 8 (i / 4) + 4
+  // (lane >> 5) + i % 4.
+  constexpr int V = kVec<T>, STRIDE = 128 + V;  // the rows that are written together lie in different banks
+  T* stage = reinterpret_cast<T*>(lds + 2 * kTile * sizeof(float)) + wave * 32 * STRIDE;
+  float* const params = reinterpret_cast<float*>(lds);  // [2][kTile]
+  params[threadIdx.x] = param;
+  __syncthreads();
+  const bool vec = a.n % V == 0 && ((uintptr_t)a.out & 15) == 0;
+  const int j0 = b0 * 16 + wc * 128, width = min(128, a.n - j0);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int row = begin + wr * 64 + r * 32 + (lane & 31);
-    if (row >= end) continue;
-    const float xs = a.x_scale[row];
-    T* out = (T*)a.out + (int64_t)row * a.n;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        const int j = b0 * 16 + wc * 128 + c * 32 + (i >> 2) * 8 + (lane >> 5) * 4;
+        const int j = c * 32 + (i >> 2) * 8 + (lane >> 5) * 4;
+        const v4f ws = *reinterpret_cast<const v4f*>(params + wc * 128 + j);
+        const v4f bias = *reinterpret_cast<const v4f*>(params + kTile + wc * 128 + j);
         float y[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          y[u] = finish8(acc[c][r][i + u], xs * ws[min(j + u, a.n - 1)], bias[min(j + u, a.n - 1)], a.act);
-        if (vec && j < a.n)
-          Vec<T, 4>::store(out + j, y);
-        else
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (j + u < a.n) out[j + u] = (T)y[u];
+        for (int u = 0; u < 4; ++u) y[u] = finish8<ACT>(acc[c][r][i + u], xs[r] * ws[u], bias[u]);
+        Vec<T, 4>::store(stage + (lane & 31) * STRIDE + j, y);
       }
+    // the wave's LDS operations are in order; the compiler keeps them so
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int row0 = begin + wr * 64 + r * 32, rows = min(32, end - row0);
+    T* out = (T*)a.out + (int64_t)row0 * a.n + j0;
+    if (vec) {
+      constexpr int PER = 128 / V;  // vectors of a row
+      const int c = lane % PER * V;
+#pragma unroll
+      for (int i = 0; i < 32; i += 64 / PER) {
+        const int at = i + lane / PER;
+        if (at < rows && c < width)
+          *reinterpret_cast<int4*>(out + (int64_t)at * a.n + c) = *reinterpret_cast<const int4*>(stage + at * STRIDE + c);
+      }
+    } else {
+      for (int i = 0; i < rows; ++i)
+#pragma unroll
+        for (int c = lane; c < 128; c += 64)
+          if (c < width) out[(int64_t)i * a.n + c] = stage[i * STRIDE + c];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
-template <class T>
+template <class T, int ACT>
 int tiles_run(const Linear8Args& a, hipStream_t s) {
-  NHIP_TRY(ensure_dynamic_lds((const void*)linear8_tiles_kernel<T>, kLds));
+  constexpr int out = 2 * kTile * (int)sizeof(float) + kWaves * 32 * (128 + kVec<T>) * (int)sizeof(T), bytes = std::max(kLds, out);
+  NHIP_TRY(ensure_dynamic_lds((const void*)linear8_tiles_kernel<T, ACT>, bytes));
   const int64_t cols = ceil_div(a.blocks, kTile / 16);
   // every expert's last tile may be a part of one
   const int64_t rows = ceil_div(a.rows, kTile) + (a.starts ? std::min(a.experts, a.rows) : 0);
   if (rows * cols > 0x7fffff00) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
-  NHIP_LAUNCH("linear8_tiles", linear8_tiles_kernel<T>, dim3((uint32_t)round_up(rows * cols, 8)), dim3(kWaves * 64), kLds, s, a,
-              (int)cols, (int)(rows * cols));
+  NHIP_LAUNCH("linear8_tiles", (linear8_tiles_kernel<T, ACT>), dim3((uint32_t)round_up(rows * cols, 8)), dim3(kWaves * 64),
+              bytes, s, a, (int)cols, (int)(rows * cols));
   return check_launch("linear8_tiles");
 }
 
@@ -165,7 +197,7 @@ bool linear8_tiles_selected(const Linear8Args& a) {
 }
 
 int linear8_tiles(const Linear8Args& a, int dtype, hipStream_t s) {
-  return NHIP_FOR_ELEM(dtype, T, tiles_run<T>(a, s));
+  return NHIP_FOR_ELEM(dtype, T, NHIP_FOR_ACT(a.act, ACT, tiles_run<T, ACT>(a, s)));
 }
 
 }  // namespace nhip
