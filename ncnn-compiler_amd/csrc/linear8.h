@@ -6,21 +6,23 @@
 
 namespace nhip {
 
-// Operands are walked in steps of 64 of the summed index, two at a time: rows of
-// codes are padded to a multiple of kPadK, with zeros.
-constexpr int kStepK = 64, kPadK = 128;
+// Codes, of tokens and of weights, lie as the matrix instructions take them:
+// [rows / 16][steps][4][16 rows][16 codes], a step being 64 of the summed index
+// and 1 KB of 16 rows.  What is past the rows or the sum is 0.  (Copies of rows
+// of 64 bytes from codes in the tokens' own order ran at a quarter of the rate of
+// whole kilobytes: 38 and 145 GB/s into the LDS of a CU.)
+constexpr int kStepK = 64;
+__host__ __device__ inline int64_t code_at(int64_t row, int steps) { return (row >> 4) * steps * 1024 + (row & 15) * 16; }
 
-// The weights of one expert lie as the matrix instructions take them:
-// [n / 16][k / 64][4][16 rows][16 codes], 1 KB to 16 rows and 64 codes.
 struct Linear8Args {
-  const int8_t* x;       // codes [rows][kp]
+  const int8_t* x;       // codes of [rows]
   const float* x_scale;  // [rows]
-  const int8_t* w;       // [experts][blocks][steps][1024]
+  const int8_t* w;       // codes of [experts][16 blocks]
   const float* w_scale;  // [experts][n]
   const float* bias;     // [experts][n]
   void* out;             // [rows][n]
   const int32_t* starts;  // [experts + 1], or null: one expert, all rows
-  int32_t rows, n, kp, steps, blocks, experts, act;
+  int32_t rows, n, steps, blocks, experts, act;
 };
 
 // Rows of an expert, inside 0 .. rows - 1 whatever the starts say.
@@ -35,8 +37,8 @@ __device__ __forceinline__ void expert_rows(const Linear8Args& a, int e, int& be
 
 // The sum of a product of codes as the result.
 template <int ACT>
-__device__ __forceinline__ float finish8(int sum, float scale, float bias) {
-  const float y = (float)sum * scale + bias;
+__device__ __forceinline__ float finish8(int sum, float x_scale, float w_scale, float bias) {
+  const float y = fmaf((float)sum, x_scale * w_scale, bias);
   if constexpr (ACT == NHIP_ACT_RELU) return y < 0.f ? 0.f : y;  // NaN stays
   if constexpr (ACT == NHIP_ACT_SILU) return y * __builtin_amdgcn_rcpf(1.f + __expf(-y));
   return y;

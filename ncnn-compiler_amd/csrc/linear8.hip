@@ -46,15 +46,20 @@ __device__ __forceinline__ void load8(const T* row, int c, int k, float (&x)[8])
   }
 }
 
-// One workgroup: one row of codes, its largest magnitude first.  A thread keeps
-// its first kHeld eights and reads others again.
-template <class T, bool VEC, int TH>
-__global__ __launch_bounds__(TH) void linear8_codes_kernel(const T* x, int64_t stride, int k, int kp, int8_t* codes,
-                                                           float* scales) {
-  constexpr int kHeld = 4;
-  const int64_t r = blockIdx.x;
-  const T* row = x + r * stride;
-  float held[kHeld][8], most = 0.f;
+// One workgroup: 16 rows, one to a wave, which finds its largest magnitude first;
+// the codes are put in order in LDS, kChunk of a row at a time, and stored whole.
+// The first chunk is held, others are read again.
+constexpr int kChunk = 2048;
+template <class T, bool VEC>
+__global__ __launch_bounds__(1024) void linear8_codes_kernel(const T* x, int64_t stride, int rows, int k, int steps,
+                                                             int8_t* codes, float* scales) {
+  constexpr int HELD = kChunk / 8 / 64, ROW = kChunk + 16;  // (a row's chunks of 16 codes begin in different banks)
+  __shared__ __attribute__((aligned(16))) int8_t lds[16 * ROW];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = blockIdx.x * 16 + wave;
+  const int mine = r < rows ? k : 0;  // past the rows: zeros
+  const T* row = x + (int64_t)min(r, rows - 1) * stride;
+  float held[HELD][8], most = 0.f;
   bool whole = true;  // finite
   const auto widest = [&](const float(&t)[8]) {
 #pragma unroll
@@ -64,70 +69,56 @@ __global__ __launch_bounds__(TH) void linear8_codes_kernel(const T* x, int64_t s
     }
   };
 #pragma unroll
-  for (int h = 0; h < kHeld; ++h)
-    if (const int c = (threadIdx.x + h * TH) * 8; c < k) {
-      load8<T, VEC>(row, c, k, held[h]);
-      widest(held[h]);
-    }
-  for (int c = (threadIdx.x + kHeld * TH) * 8; c < k; c += TH * 8) {
+  for (int h = 0; h < HELD; ++h) load8<T, VEC>(row, (lane + h * 64) * 8, mine, held[h]);
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) widest(held[h]);
+#pragma unroll 4
+  for (int c = kChunk + lane * 8; c < mine; c += 512) {
     float t[8];
-    load8<T, VEC>(row, c, k, t);
+    load8<T, VEC>(row, c, mine, t);
     widest(t);
   }
   most = wave_max(whole ? most : INFINITY);
-  if constexpr (TH > 64) {
-    __shared__ float part[TH / 64];
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < TH / 64; ++i) most = fmaxf(most, part[i]);
-  }
   const float scale = most > 0.f ? fmaxf(most * (1.f / 127.f), kLeastScale) : 0.f;
   const float inv = scale > 0.f && most < INFINITY ? 1.f / scale : 0.f;
-  int8_t* to = codes + r * kp;
+  // a row that holds an infinity or NaN: codes 0, results 0 * NaN
+  if (lane == 0 && r < rows) scales[r] = most < INFINITY ? scale : NAN;
   const auto store = [&](const float(&t)[8], int c) {
     int q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = quantize_q(t[i], inv);
-    *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_i8x4(q[0], q[1], q[2], q[3]), pack_i8x4(q[4], q[5], q[6], q[7]));
+    *reinterpret_cast<uint2*>(lds + wave * ROW + c) = make_uint2(pack_i8x4(q[0], q[1], q[2], q[3]), pack_i8x4(q[4], q[5], q[6], q[7]));
   };
+  int8_t* to = codes + (int64_t)blockIdx.x * steps * 1024;
+  for (int c0 = 0; c0 < steps * kStepK; c0 += kChunk) {
+    const int width = min(kChunk, steps * kStepK - c0);
+    if (c0) __syncthreads();
 #pragma unroll
-  for (int h = 0; h < kHeld; ++h)
-    if (const int c = (threadIdx.x + h * TH) * 8; c < kp) {
-      if (c >= k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) held[h][i] = 0.f;
+    for (int h = 0; h < HELD; ++h) {
+      const int c = (lane + h * 64) * 8;
+      if (c >= width) break;
+      if (c0) load8<T, VEC>(row, c0 + c, mine, held[h]);
       store(held[h], c);
     }
-  for (int c = (threadIdx.x + kHeld * TH) * 8; c < kp; c += TH * 8) {
-    float t[8];
-    load8<T, VEC>(row, c, k, t);
-    store(t, c);
+    __syncthreads();
+    for (int i = threadIdx.x; i < width; i += 1024)  // 16 codes each: [steps][4][16 rows]
+      *reinterpret_cast<int4*>(to + (c0 + (int64_t)i) * 16) = *reinterpret_cast<const int4*>(lds + (i & 15) * ROW + (i >> 4) * 16);
   }
-  // a row that holds an infinity or NaN: codes 0, results 0 * NaN
-  if (threadIdx.x == 0) scales[r] = most < INFINITY ? scale : NAN;
 }
 
 template <class T>
-int codes_run(const void* x, int64_t stride, int64_t rows, int k, int kp, int8_t* codes, float* scales, hipStream_t s) {
-  const bool vec = aligned_to(x, 16) && stride % kVec<T> == 0;
-  const int th = kp <= 1024 ? 64 : kp <= 2048 ? 128 : 256;
+int codes_run(const void* x, int64_t stride, int64_t rows, int k, int steps, int8_t* codes, float* scales, hipStream_t s) {
   const auto launch = [&](auto kernel) {
-    NHIP_LAUNCH("linear8_codes", kernel, dim3((uint32_t)rows), dim3(th), 0, s, (const T*)x, stride, k, kp, codes, scales);
+    NHIP_LAUNCH("linear8_codes", kernel, dim3((uint32_t)ceil_div(rows, 16)), dim3(1024), 0, s, (const T*)x, stride, (int)rows, k,
+                steps, codes, scales);
     return check_launch("linear8_codes");
   };
-  if (vec)
-    return th == 64    ? launch(linear8_codes_kernel<T, true, 64>)
-           : th == 128 ? launch(linear8_codes_kernel<T, true, 128>)
-                       : launch(linear8_codes_kernel<T, true, 256>);
-  return th == 64    ? launch(linear8_codes_kernel<T, false, 64>)
-         : th == 128 ? launch(linear8_codes_kernel<T, false, 128>)
-                     : launch(linear8_codes_kernel<T, false, 256>);
+  return aligned_to(x, 16) && stride % kVec<T> == 0 ? launch(linear8_codes_kernel<T, true>) : launch(linear8_codes_kernel<T, false>);
 }
 
-// Codes [rows][stride] into the plan's order, 16 codes to a thread; past n and k zeros.
-__global__ __launch_bounds__(256) void linear8_order_kernel(const int8_t* from, int64_t stride, int experts, int n, int k,
-                                                            int blocks, int steps, bool vec, int8_t* to) {
+// Codes [experts][n][k] in order, 16 codes to a thread.
+__global__ __launch_bounds__(256) void linear8_order_kernel(const int8_t* from, int experts, int n, int k, int blocks, int steps,
+                                                            bool vec, int8_t* to) {
   const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (item >= (int64_t)experts * blocks * steps * 64) return;
   const int lane = item & 63;
@@ -137,7 +128,7 @@ __global__ __launch_bounds__(256) void linear8_order_kernel(const int8_t* from, 
   const int row = (int)(at % blocks) * 16 + (lane & 15), c = step * kStepK + (lane >> 4) * 16;
   int4 v = make_int4(0, 0, 0, 0);
   if (row < n && c < k) {
-    const int8_t* src = from + (at / blocks * n + row) * stride + c;
+    const int8_t* src = from + (at / blocks * n + row) * k + c;
     if (vec && c + 16 <= k) {
       v = *reinterpret_cast<const int4*>(src);
     } else {
@@ -178,7 +169,7 @@ __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a)
   for (int r0 = begin; r0 < end; r0 += 16 * TG) {
     const int8_t* x[TG];
 #pragma unroll
-    for (int t = 0; t < TG; ++t) x[t] = a.x + (int64_t)min(r0 + t * 16 + (lane & 15), end - 1) * a.kp + (lane >> 4) * 16;
+    for (int t = 0; t < TG; ++t) x[t] = a.x + code_at(min(r0 + t * 16 + (lane & 15), end - 1), a.steps) + (lane >> 4) * 256;
     v4i acc[TG][NB];
 #pragma unroll
     for (int t = 0; t < TG; ++t)
@@ -192,7 +183,7 @@ __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a)
 #pragma unroll
         for (int b = 0; b < NB; ++b) wf[u][b] = *reinterpret_cast<const v4i*>(w[b] + at * 1024);
 #pragma unroll
-        for (int t = 0; t < TG; ++t) xf[u][t] = *reinterpret_cast<const v4i*>(x[t] + at * kStepK);
+        for (int t = 0; t < TG; ++t) xf[u][t] = *reinterpret_cast<const v4i*>(x[t] + at * 1024);
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
@@ -227,7 +218,7 @@ __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a)
         T* out = (T*)a.out + (int64_t)row * a.n;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          if (j + c < a.n) out[j + c] = (T)finish8<ACT>(sum[c], xs * ws[j + c], bias[j + c]);
+          if (j + c < a.n) out[j + c] = (T)finish8<ACT>(sum[c], xs, ws[j + c], bias[j + c]);
       }
     }
     __syncthreads();
@@ -254,7 +245,7 @@ int product_run(const Linear8Args& a, hipStream_t s) {
 
 // Codes of the tokens, their scales behind them.
 uint64_t workspace_of(const nhip_linear8_plan* p, int64_t rows) {
-  return (uint64_t)rows * p->steps * kStepK + (uint64_t)round_up(rows * (int64_t)sizeof(float), 16);
+  return (uint64_t)round_up(rows, 16) * p->steps * kStepK + (uint64_t)round_up(rows * (int64_t)sizeof(float), 16);
 }
 
 int linear8_args(const nhip_linear8_plan* p, int32_t dtype, int64_t rows) {
@@ -281,7 +272,7 @@ int nhip_linear8_create(int32_t experts, int32_t num_output, int32_t num_input, 
   if (num_input > kMaxK) return fail(NHIP_STATUS_INVALID_SHAPE, "linear8: at most 131072 inputs, the sums are of 32 bits");
   if (activation != NHIP_ACT_NONE && activation != NHIP_ACT_RELU && activation != NHIP_ACT_SILU)
     return fail(NHIP_STATUS_UNSUPPORTED, "linear8: activation has to be NONE, RELU or SILU");
-  const int64_t blocks = ceil_div(num_output, 16), steps = round_up(num_input, kPadK) / kStepK;
+  const int64_t blocks = ceil_div(num_output, 16), steps = ceil_div(num_input, kStepK);
   if (experts * blocks > 0x7fffffff / 4 || experts * (int64_t)num_output > 0x7fffffff)
     return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many output channels");
   if (!weight || (weight_is_i8 && !weight_scale)) return fail(NHIP_STATUS_NULL_POINTER, "linear8: null pointer");
@@ -303,30 +294,27 @@ int nhip_linear8_create(int32_t experts, int32_t num_output, int32_t num_input, 
   p->blocks = (int32_t)blocks;
   p->steps = (int32_t)steps;
   const int64_t count = experts * (int64_t)num_output, items = experts * blocks * steps * 64;
-  int8_t* codes = nullptr;
   const auto build = [&]() -> int {
     NHIP_TRY(check_hip(hipGetDevice(&p->device), "hipGetDevice"));
     if (ceil_div(items, 256) > 0x7fffffff) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many weights");
     NHIP_TRY(check_hip(hipMalloc(reinterpret_cast<void**>(&p->w), items * 16), "hipMalloc(linear8 weights)"));
     NHIP_TRY(check_hip(hipMalloc(reinterpret_cast<void**>(&p->w_scale), 2 * count * sizeof(float)), "hipMalloc(linear8 scales)"));
-    const int8_t* from = (const int8_t*)weight;
-    int64_t stride = num_input;
-    if (!weight_is_i8) {
-      stride = steps * kStepK;
-      NHIP_TRY(check_hip(hipMalloc(reinterpret_cast<void**>(&codes), count * stride), "hipMalloc(linear8 codes)"));
-      NHIP_TRY(codes_run<float>(weight, num_input, count, num_input, (int)stride, codes, p->w_scale, s));
-      from = codes;
+    if (weight_is_i8) {
+      NHIP_LAUNCH("linear8_order", linear8_order_kernel, dim3((uint32_t)ceil_div(items, 256)), dim3(256), 0, s,
+                  (const int8_t*)weight, experts, num_output, num_input, (int)blocks, (int)steps,
+                  aligned_to(weight, 16) && num_input % 16 == 0, p->w);
+      NHIP_TRY(check_launch("linear8_order"));
+    } else {
+      for (int64_t e = 0; e < experts; ++e)
+        NHIP_TRY(codes_run<float>((const float*)weight + e * num_output * num_input, num_input, num_output, num_input, (int)steps,
+                                  p->w + e * blocks * steps * 1024, p->w_scale + e * num_output, s));
     }
-    NHIP_LAUNCH("linear8_order", linear8_order_kernel, dim3((uint32_t)ceil_div(items, 256)), dim3(256), 0, s, from, stride,
-                experts, num_output, num_input, (int)blocks, (int)steps, aligned_to(from, 16) && stride % 16 == 0, p->w);
-    NHIP_TRY(check_launch("linear8_order"));
     NHIP_LAUNCH("linear8_params", linear8_params_kernel, dim3((uint32_t)ceil_div(count, 256)), dim3(256), 0, s, weight_scale,
                 bias, count, p->w_scale);
     NHIP_TRY(check_launch("linear8_params"));
     return check_hip(hipStreamSynchronize(s), "hipStreamSynchronize(linear8 plan)");
   };
   const int st = build();
-  if (codes) (void)hipFree(codes);
   if (st != NHIP_STATUS_SUCCESS) {
     (void)hipFree(p->w);
     (void)hipFree(p->w_scale);
@@ -360,9 +348,8 @@ int nhip_linear8_forward(nhip_linear8_t plan, const void* x, int32_t dtype, int6
   if (dev != plan->device) return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "linear8: the plan is another device's");
   if (workspace_bytes < workspace_of(plan, rows) || !aligned_to(workspace, 16))
     return fail(NHIP_STATUS_OUTPUT_CAPACITY_INSUFFICIENT, "linear8: workspace too small or not 16-byte aligned");
-  const int kp = plan->steps * kStepK;
   int8_t* codes = (int8_t*)workspace;
-  float* scales = (float*)(codes + rows * kp);
+  float* scales = (float*)(codes + round_up(rows, 16) * plan->steps * kStepK);
   Linear8Args a{};
   a.x = codes;
   a.x_scale = scales;
@@ -373,12 +360,11 @@ int nhip_linear8_forward(nhip_linear8_t plan, const void* x, int32_t dtype, int6
   a.starts = expert_starts;
   a.rows = (int32_t)rows;
   a.n = plan->n;
-  a.kp = kp;
   a.steps = plan->steps;
   a.blocks = plan->blocks;
   a.experts = plan->experts;
   a.act = plan->act;
-  NHIP_TRY(NHIP_FOR_ELEM(dtype, T, codes_run<T>(x, row_stride, rows, plan->k, kp, codes, scales, as_stream(stream))));
+  NHIP_TRY(NHIP_FOR_ELEM(dtype, T, codes_run<T>(x, row_stride, rows, plan->k, plan->steps, codes, scales, as_stream(stream))));
   if (linear8_tiles_selected(a)) return linear8_tiles(a, dtype, as_stream(stream));
   return NHIP_FOR_ELEM(dtype, T, NHIP_FOR_ACT(a.act, ACT, product_run<T, ACT>(a, as_stream(stream))));
 }

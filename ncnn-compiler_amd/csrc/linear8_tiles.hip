@@ -1,4 +1,4 @@
-// Products in 8-bit integers for many rows: tiles of 256 rows and 256 channels.
+// Products in 8-bit integers for many rows: tiles of 128 rows and 256 channels.
 #include <algorithm>
 
 #include "lds_dma.h"
@@ -7,10 +7,10 @@
 namespace nhip {
 namespace {
 
-constexpr int kTile = 256, kWaves = 8;
-constexpr int kSide = kTile * kPadK;  // bytes of one operand's stage
-constexpr int kStage = 2 * kSide;
-constexpr int kLds = 2 * kStage;
+constexpr int kRows = 128, kCols = 256, kWaves = 4;  // of a workgroup; a wave has 64 rows, 128 channels
+constexpr int kStage = (kRows + kCols) * kStepK;     // bytes: the weights' steps, then the tokens'
+constexpr int kSlots = 3;                            // stages that LDS holds
+constexpr int kLds = kSlots * kStage;
 constexpr int kGroup = 4;
 
 // The expert and its row tile that tile `at` of all row tiles is: experts
@@ -19,14 +19,14 @@ __device__ __forceinline__ bool find_tile(const Linear8Args& a, int at, int& e, 
   e = 0;
   expert_rows(a, 0, begin, end);
   if (!a.starts) {
-    begin += at * kTile;
+    begin += at * kRows;
     return begin < end;
   }
   const int lane = threadIdx.x & 63;
   for (int e0 = 0; e0 < a.experts; e0 += 64) {
     int b = 0, t = 0;
     if (e0 + lane < a.experts) expert_rows(a, e0 + lane, b, t);
-    const int tiles = (t - b + kTile - 1) / kTile;
+    const int tiles = (t - b + kRows - 1) / kRows;
     int upto = tiles;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -37,7 +37,7 @@ __device__ __forceinline__ bool find_tile(const Linear8Args& a, int at, int& e, 
     if (past) {
       const int l = __builtin_ctzll(past);
       e = e0 + l;
-      begin = __builtin_amdgcn_readlane(b, l) + (at - __builtin_amdgcn_readlane(upto - tiles, l)) * kTile;
+      begin = __builtin_amdgcn_readlane(b, l) + (at - __builtin_amdgcn_readlane(upto - tiles, l)) * kRows;
       end = __builtin_amdgcn_readlane(t, l);
       return true;
     }
@@ -47,7 +47,7 @@ __device__ __forceinline__ bool find_tile(const Linear8Args& a, int at, int& e, 
 }
 
 template <class T, int ACT>
-__global__ __launch_bounds__(kWaves * 64) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work) {
+__global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // workgroups go to the eight dies in turn: each die gets a run of the tiles
@@ -60,32 +60,36 @@ __global__ __launch_bounds__(kWaves * 64) void linear8_tiles_kernel(Linear8Args 
   const int col = in / high;
   int e, begin, end;
   if (!find_tile(a, band * kGroup + in - col * high, e, begin, end)) return;
-  const int b0 = col * (kTile / 16);  // first block of channels
+  const int b0 = col * (kCols / 16);  // first block of channels
   const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
 
-  // A wave's copies of a stage: 4 KB of weights, 4 KB of codes, 1 KB (16 rows, 64 codes) each.
+  // A wave's copies of a stage: 4 KB of weights, 2 KB of tokens.
+  constexpr int WCOPIES = kCols / 16 / kWaves, XCOPIES = kRows / 16 / kWaves, COPIES = WCOPIES + XCOPIES;
   const v4i wrsrc = dma::raw_rsrc(a.w + ((int64_t)e * a.blocks + b0) * a.steps * 1024, 0x7fffffffu);
-  const v4i xrsrc = dma::raw_rsrc(a.x + (int64_t)begin * a.kp, 0x7fffffffu);
-  uint32_t woff[4], xoff[4], to[4];
+  const v4i xrsrc = dma::raw_rsrc(a.x + (int64_t)(begin >> 4) * a.steps * 1024, 0x7fffffffu);
+  uint32_t woff[WCOPIES], xoff[XCOPIES];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = wave * 4 + i, blk = c >> 1, half = c & 1;
-    woff[i] = (uint32_t)(min(blk, a.blocks - 1 - b0) * a.steps + half) * 1024u + lane * 16;
-    xoff[i] = (uint32_t)min(blk * 16 + (lane & 15), end - 1 - begin) * (uint32_t)a.kp + half * 64 + (lane >> 4) * 16;
-    to[i] = c * 1024u;
+  for (int i = 0; i < WCOPIES; ++i)
+    woff[i] = (uint32_t)(min(wave * WCOPIES + i, a.blocks - 1 - b0) * a.steps) * 1024u + lane * 16;
+#pragma unroll
+  for (int i = 0; i < XCOPIES; ++i) {
+    const int row = min((wave * XCOPIES + i) * 16 + (lane & 15), end - 1 - begin);
+    xoff[i] = (uint32_t)code_at((begin & 15) + row, a.steps) + (lane >> 4) * 256;
   }
   const auto copy = [&](int stage, int slot) {
+    const uint32_t to = lds0 + slot * kStage;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      dma::copy16(lds0 + slot * kStage + to[i], woff[i], wrsrc, stage * 2048u);
-      dma::copy16(lds0 + slot * kStage + kSide + to[i], xoff[i], xrsrc, stage * 128u);
-    }
+    for (int i = 0; i < WCOPIES; ++i) dma::copy16(to + (wave * WCOPIES + i) * 1024, woff[i], wrsrc, stage * 1024u);
+#pragma unroll
+    for (int i = 0; i < XCOPIES; ++i)
+      dma::copy16(to + (kCols / 16 + wave * XCOPIES + i) * 1024, xoff[i], xrsrc, stage * 1024u);
   };
-  const int wc = wave & 1, wr = wave >> 1;  // 128 channels, 64 rows
-  // what the results need: a thread's entry of the channels' scales and biases, its rows' scales
-  static_assert(kWaves * 64 == 2 * kTile, "a thread to each channel's scale and bias");
-  const int channel = b0 * 16 + (threadIdx.x & (kTile - 1));
-  const float param = channel < a.n ? (threadIdx.x < kTile ? a.w_scale : a.bias)[(int64_t)e * a.n + channel] : 0.f;
+  const int wc = wave & 1, wr = wave >> 1;
+  // what the results need: a thread's channel's scale and bias, its rows' scales
+  static_assert(kWaves * 64 == kCols, "a thread to each channel");
+  const int channel = b0 * 16 + threadIdx.x;
+  const float w_scale = channel < a.n ? a.w_scale[(int64_t)e * a.n + channel] : 0.f;
+  const float w_bias = channel < a.n ? a.bias[(int64_t)e * a.n + channel] : 0.f;
   float xs[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) xs[r] = a.x_scale[min(begin + wr * 64 + r * 32 + (lane & 31), end - 1)];
@@ -96,45 +100,73 @@ __global__ __launch_bounds__(kWaves * 64) void linear8_tiles_kernel(Linear8Args 
     for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[c][r][i] = 0;
-  const int stages = a.steps / 2;
-  copy(0, 0);
-  dma::wait_vmcnt<0>();
-  __syncthreads();
   // lane's 16 codes of a 32 x 32 block: row lane & 31, codes 16 (lane >> 5) ..
-  const uint32_t lane_at = ((lane >> 4) & 1) * 2048u + (lane >> 5) * 256u + (lane & 15) * 16u;
-  for (int st = 0; st < stages; ++st) {
-    const int slot = st & 1;
-    if (st + 1 < stages) copy(st + 1, slot ^ 1);
-    const char* wl = lds + slot * kStage + wc * (128 / 16) * 2048 + lane_at;
-    const char* xl = lds + slot * kStage + kSide + wr * (64 / 16) * 2048 + lane_at;
+  const uint32_t lane_at = ((lane >> 4) & 1) * 1024u + (lane >> 5) * 256u + (lane & 15) * 16u;
+  struct Step {
+    v4i w[4], x[2];
+  } step[2];
+  const auto read = [&](int slot, int k, Step& f) {
+    const char* at = lds + slot * kStage + lane_at + k * 512;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int off = (k >> 1) * 1024 + (k & 1) * 512;
-      v4i wf[4], xf[2];
+    for (int i = 0; i < 4; ++i) f.w[i] = *reinterpret_cast<const v4i*>(at + (wc * 8 + i * 2) * 1024);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) wf[c] = *reinterpret_cast<const v4i*>(wl + c * 4096 + off);
+    for (int i = 0; i < 2; ++i) f.x[i] = *reinterpret_cast<const v4i*>(at + (kCols / 16 + wr * 4 + i * 2) * 1024);
+  };
+  const auto multiply = [&](const Step& f) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) xf[r] = *reinterpret_cast<const v4i*>(xl + r * 4096 + off);
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) acc[c][r] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[c], xf[r], acc[c][r], 0, 0, 0);
-    }
+      for (int r = 0; r < 2; ++r) acc[c][r] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[c], f.x[r], acc[c][r], 0, 0, 0);
+  };
+  // One barrier a stage, before its last products, whose operands are in
+  // registers by then: behind it the stage's place in LDS is free for the stage
+  // kSlots further on, and the next one is whole, so that its first operands and
+  // the copies are under way during those products.
+  const int stages = a.steps;
+  for (int i = 0; i < min(kSlots, stages); ++i) copy(i, i);
+  if (stages >= kSlots)
+    dma::wait_vmcnt<(kSlots - 1) * COPIES>();
+  else
     dma::wait_vmcnt<0>();
-    __syncthreads();
+  __builtin_amdgcn_s_barrier();
+  read(0, 0, step[0]);
+  int slot = 0;
+  for (int st = 0; st < stages; ++st) {
+    read(slot, 1, step[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(step[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    const int next = slot + 1 == kSlots ? 0 : slot + 1;
+    if (st + kSlots <= stages)
+      dma::wait_vmcnt<(kSlots - 2) * COPIES>();
+    else
+      dma::wait_vmcnt<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (st + kSlots < stages) copy(st + kSlots, slot);
+    if (st + 1 < stages) read(next, 0, step[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(step[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    slot = next;
   }
+  // (settle8 for all of them, where they are)
+  asm volatile("s_nop 15\n\ts_nop 15");
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) settle8(acc[c][r]);
+    for (int r = 0; r < 2; ++r) asm volatile("" : "+a"(acc[c][r]));
+  __syncthreads();
 
   // The results through LDS, 32 rows of a wave's 128 channels at a time, so that
   // whole rows are stored.  A lane has row lane & 31, channels 8 (i / 4) + 4
   // (lane >> 5) + i % 4.
   constexpr int V = kVec<T>, STRIDE = 128 + V;  // the rows that are written together lie in different banks
-  T* stage = reinterpret_cast<T*>(lds + 2 * kTile * sizeof(float)) + wave * 32 * STRIDE;
-  float* const params = reinterpret_cast<float*>(lds);  // [2][kTile]
-  params[threadIdx.x] = param;
+  T* stage = reinterpret_cast<T*>(lds + 2 * kCols * sizeof(float)) + wave * 32 * STRIDE;
+  float* const params = reinterpret_cast<float*>(lds);  // [2][kCols]
+  params[threadIdx.x] = w_scale;
+  params[kCols + threadIdx.x] = w_bias;
   __syncthreads();
   const bool vec = a.n % V == 0 && ((uintptr_t)a.out & 15) == 0;
   const int j0 = b0 * 16 + wc * 128, width = min(128, a.n - j0);
@@ -146,10 +178,10 @@ __global__ __launch_bounds__(kWaves * 64) void linear8_tiles_kernel(Linear8Args 
       for (int i = 0; i < 16; i += 4) {
         const int j = c * 32 + (i >> 2) * 8 + (lane >> 5) * 4;
         const v4f ws = *reinterpret_cast<const v4f*>(params + wc * 128 + j);
-        const v4f bias = *reinterpret_cast<const v4f*>(params + kTile + wc * 128 + j);
+        const v4f bias = *reinterpret_cast<const v4f*>(params + kCols + wc * 128 + j);
         float y[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) y[u] = finish8<ACT>(acc[c][r][i + u], xs[r] * ws[u], bias[u]);
+        for (int u = 0; u < 4; ++u) y[u] = finish8<ACT>(acc[c][r][i + u], xs[r], ws[u], bias[u]);
         Vec<T, 4>::store(stage + (lane & 31) * STRIDE + j, y);
       }
     // the wave's LDS operations are in order; the compiler keeps them so
@@ -177,11 +209,11 @@ __global__ __launch_bounds__(kWaves * 64) void linear8_tiles_kernel(Linear8Args 
 
 template <class T, int ACT>
 int tiles_run(const Linear8Args& a, hipStream_t s) {
-  constexpr int out = 2 * kTile * (int)sizeof(float) + kWaves * 32 * (128 + kVec<T>) * (int)sizeof(T), bytes = std::max(kLds, out);
+  constexpr int out = 2 * kCols * (int)sizeof(float) + kWaves * 32 * (128 + kVec<T>) * (int)sizeof(T), bytes = std::max(kLds, out);
   NHIP_TRY(ensure_dynamic_lds((const void*)linear8_tiles_kernel<T, ACT>, bytes));
-  const int64_t cols = ceil_div(a.blocks, kTile / 16);
+  const int64_t cols = ceil_div(a.blocks, kCols / 16);
   // every expert's last tile may be a part of one
-  const int64_t rows = ceil_div(a.rows, kTile) + (a.starts ? std::min(a.experts, a.rows) : 0);
+  const int64_t rows = ceil_div(a.rows, kRows) + (a.starts ? std::min(a.experts, a.rows) : 0);
   if (rows * cols > 0x7fffff00) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
   NHIP_LAUNCH("linear8_tiles", (linear8_tiles_kernel<T, ACT>), dim3((uint32_t)round_up(rows * cols, 8)), dim3(kWaves * 64),
               bytes, s, a, (int)cols, (int)(rows * cols));
