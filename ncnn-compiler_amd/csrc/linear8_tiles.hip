@@ -1,5 +1,6 @@
 // Products in 8-bit integers for many rows: tiles of 128 rows and 256 channels.
 #include <algorithm>
+#include <type_traits>
 
 #include "lds_dma.h"
 #include "linear8.h"
@@ -46,6 +47,15 @@ __device__ __forceinline__ bool find_tile(const Linear8Args& a, int at, int& e, 
   return false;
 }
 
+// f of the whole numbers below N, as constants.
+template <int N, class F, int I = 0>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    each<N, F, I + 1>(f);
+  }
+}
+
 template <class T, int ACT>
 __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -76,13 +86,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Ar
     const int row = min((wave * XCOPIES + i) * 16 + (lane & 15), end - 1 - begin);
     xoff[i] = (uint32_t)code_at((begin & 15) + row, a.steps) + (lane >> 4) * 256;
   }
-  const auto copy = [&](int stage, int slot) {
+  // (past the last stage nothing is read, and zeros are written)
+  const auto copy = [&](int stage, int slot, auto i) {
+    v4i rsrc = i < WCOPIES ? wrsrc : xrsrc;
+    rsrc[2] = stage < a.steps ? 0x7fffffff : 0;
     const uint32_t to = lds0 + slot * kStage;
-#pragma unroll
-    for (int i = 0; i < WCOPIES; ++i) dma::copy16(to + (wave * WCOPIES + i) * 1024, woff[i], wrsrc, stage * 1024u);
-#pragma unroll
-    for (int i = 0; i < XCOPIES; ++i)
-      dma::copy16(to + (kCols / 16 + wave * XCOPIES + i) * 1024, xoff[i], xrsrc, stage * 1024u);
+    if constexpr (i < WCOPIES)
+      dma::copy16(to + (wave * WCOPIES + i) * 1024, woff[i], rsrc, stage * 1024u);
+    else
+      dma::copy16(to + (kCols / 16 + wave * XCOPIES + i - WCOPIES) * 1024, xoff[i - WCOPIES], rsrc, stage * 1024u);
   };
   const int wc = wave & 1, wr = wave >> 1;
   // what the results need: a thread's channel's scale and bias, its rows' scales
@@ -112,45 +124,41 @@ __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Ar
 #pragma unroll
     for (int i = 0; i < 2; ++i) f.x[i] = *reinterpret_cast<const v4i*>(at + (kCols / 16 + wr * 4 + i * 2) * 1024);
   };
-  const auto multiply = [&](const Step& f) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) acc[c][r] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[c], f.x[r], acc[c][r], 0, 0, 0);
+  // product n of eight
+  const auto product = [&](const Step& f, auto n) {
+    acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[n >> 1], f.x[n & 1], acc[n >> 1][n & 1], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
   };
   // One barrier a stage, before its last products, whose operands are in
   // registers by then: behind it the stage's place in LDS is free for the stage
   // kSlots further on, and the next one is whole, so that its first operands and
-  // the copies are under way during those products.
+  // the copies are under way during those products.  A copy goes between two
+  // products: all at once would hold the products up.
   const int stages = a.steps;
-  for (int i = 0; i < min(kSlots, stages); ++i) copy(i, i);
-  if (stages >= kSlots)
-    dma::wait_vmcnt<(kSlots - 1) * COPIES>();
-  else
-    dma::wait_vmcnt<0>();
+  for (int st = 0; st < kSlots; ++st) each<COPIES>([&](auto i) { copy(st, st, i); });
+  dma::wait_vmcnt<(kSlots - 1) * COPIES>();
   __builtin_amdgcn_s_barrier();
   read(0, 0, step[0]);
   int slot = 0;
   for (int st = 0; st < stages; ++st) {
+    const int next = slot + 1 == kSlots ? 0 : slot + 1;
     read(slot, 1, step[1]);
     __builtin_amdgcn_sched_barrier(0);
-    multiply(step[0]);
-    __builtin_amdgcn_sched_barrier(0);
-    const int next = slot + 1 == kSlots ? 0 : slot + 1;
-    if (st + kSlots <= stages)
-      dma::wait_vmcnt<(kSlots - 2) * COPIES>();
-    else
-      dma::wait_vmcnt<0>();
+    each<8>([&](auto n) { product(step[0], n); });
+    dma::wait_vmcnt<(kSlots - 2) * COPIES>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (st + kSlots < stages) copy(st + kSlots, slot);
-    if (st + 1 < stages) read(next, 0, step[0]);
+    read(next, 0, step[0]);  // (past the last stage: not used)
     __builtin_amdgcn_sched_barrier(0);
-    multiply(step[1]);
-    __builtin_amdgcn_sched_barrier(0);
+    each<8>([&](auto n) {
+      product(step[1], n);
+      if constexpr (n < COPIES) copy(st + kSlots, slot, n);
+      __builtin_amdgcn_sched_barrier(0);
+    });
     slot = next;
   }
+  dma::wait_vmcnt<0>();
   // (settle8 for all of them, where they are)
   asm volatile("s_nop 15\n\ts_nop 15");
 #pragma unroll
