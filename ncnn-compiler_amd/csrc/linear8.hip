@@ -46,17 +46,17 @@ __device__ __forceinline__ void load8(const T* row, int c, int k, float (&x)[8])
   }
 }
 
-// One workgroup: 16 rows, one to a wave, which finds its largest magnitude first;
-// the codes are put in order in LDS, kChunk of a row at a time, and stored whole.
-// The first chunk is held, others are read again.
+// One workgroup: 8 rows, one to a wave, which finds its largest magnitude first;
+// the codes are put in order in LDS, kChunk of a row at a time, and stored as the
+// 128 bytes that 8 rows have together.  The first chunk is held, others are read again.
 constexpr int kChunk = 2048;
 template <class T, bool VEC>
-__global__ __launch_bounds__(1024) void linear8_codes_kernel(const T* x, int64_t stride, int rows, int k, int steps,
+__global__ __launch_bounds__(512) void linear8_codes_kernel(const T* x, int64_t stride, int rows, int k, int steps,
                                                              int8_t* codes, float* scales) {
   constexpr int HELD = kChunk / 8 / 64, ROW = kChunk + 16;  // (a row's chunks of 16 codes begin in different banks)
-  __shared__ __attribute__((aligned(16))) int8_t lds[16 * ROW];
+  __shared__ __attribute__((aligned(16))) int8_t lds[8 * ROW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = blockIdx.x * 16 + wave;
+  const int r = blockIdx.x * 8 + wave;
   const int mine = r < rows ? k : 0;  // past the rows: zeros
   const T* row = x + (int64_t)min(r, rows - 1) * stride;
   float held[HELD][8], most = 0.f;
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(1024) void linear8_codes_kernel(const T* x, int64_t
     for (int i = 0; i < 8; ++i) q[i] = quantize_q(t[i], inv);
     *reinterpret_cast<uint2*>(lds + wave * ROW + c) = make_uint2(pack_i8x4(q[0], q[1], q[2], q[3]), pack_i8x4(q[4], q[5], q[6], q[7]));
   };
-  int8_t* to = codes + (int64_t)blockIdx.x * steps * 1024;
+  int8_t* to = codes + code_at((int64_t)blockIdx.x * 8, steps);
   for (int c0 = 0; c0 < steps * kStepK; c0 += kChunk) {
     const int width = min(kChunk, steps * kStepK - c0);
     if (c0) __syncthreads();
@@ -101,15 +101,16 @@ __global__ __launch_bounds__(1024) void linear8_codes_kernel(const T* x, int64_t
       store(held[h], c);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < width; i += 1024)  // 16 codes each: [steps][4][16 rows]
-      *reinterpret_cast<int4*>(to + (c0 + (int64_t)i) * 16) = *reinterpret_cast<const int4*>(lds + (i & 15) * ROW + (i >> 4) * 16);
+    for (int i = threadIdx.x; i < width / 2; i += 512)  // 16 codes of a row: [steps][4][16 rows]
+      *reinterpret_cast<int4*>(to + (int64_t)c0 * 16 + (i >> 3) * 256 + (i & 7) * 16) =
+          *reinterpret_cast<const int4*>(lds + (i & 7) * ROW + (i >> 3) * 16);
   }
 }
 
 template <class T>
 int codes_run(const void* x, int64_t stride, int64_t rows, int k, int steps, int8_t* codes, float* scales, hipStream_t s) {
   const auto launch = [&](auto kernel) {
-    NHIP_LAUNCH("linear8_codes", kernel, dim3((uint32_t)ceil_div(rows, 16)), dim3(1024), 0, s, (const T*)x, stride, (int)rows, k,
+    NHIP_LAUNCH("linear8_codes", kernel, dim3((uint32_t)ceil_div(rows, 16) * 2), dim3(512), 0, s, (const T*)x, stride, (int)rows, k,
                 steps, codes, scales);
     return check_launch("linear8_codes");
   };

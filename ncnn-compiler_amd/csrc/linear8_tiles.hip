@@ -1,4 +1,5 @@
-// Products in 8-bit integers for many rows: tiles of 128 rows and 256 channels.
+// Products in 8-bit integers for many rows: tiles of 128 rows and 256 channels,
+// and quarters of them where few are left over.
 #include <algorithm>
 #include <type_traits>
 
@@ -8,10 +9,24 @@
 namespace nhip {
 namespace {
 
-constexpr int kRows = 128, kCols = 256, kWaves = 4;  // of a workgroup; a wave has 64 rows, 128 channels
-constexpr int kStage = (kRows + kCols) * kStepK;     // bytes: the weights' steps, then the tokens'
-constexpr int kSlots = 3;                            // stages that LDS holds
-constexpr int kLds = kSlots * kStage;
+constexpr int kWaves = 4, kSlots = 3;  // stages that LDS holds
+
+// A workgroup's tile: its waves are two by two, each has 32 CB channels, 32 RB rows.
+template <int CB, int RB>
+struct Tile {
+  static constexpr int kCols = 64 * CB, kRows = 64 * RB;
+  static constexpr int kStage = (kRows + kCols) * kStepK;  // bytes: the weights' steps, then the tokens'
+  template <class T>
+  static constexpr int stride = 32 * CB + kVec<T>;  // of the results' rows in LDS: those written together lie in different banks
+  template <class T>
+  static constexpr int lds() {
+    constexpr int out = 2 * kCols * (int)sizeof(float) + kWaves * 32 * stride<T> * (int)sizeof(T);
+    return std::max(kSlots * kStage, out);
+  }
+};
+typedef Tile<4, 2> Large;
+typedef Tile<2, 1> Small;  // a quarter of it
+constexpr int kRows = Large::kRows;
 constexpr int kGroup = 4;
 
 // The expert and its row tile that tile `at` of all row tiles is: experts
@@ -47,6 +62,8 @@ __device__ __forceinline__ bool find_tile(const Linear8Args& a, int at, int& e, 
   return false;
 }
 
+__device__ __forceinline__ int round_up8(int v) { return (v + 7) & ~7; }
+
 // f of the whole numbers below N, as constants.
 template <int N, class F, int I = 0>
 __device__ __forceinline__ void each(F f) {
@@ -56,24 +73,14 @@ __device__ __forceinline__ void each(F f) {
   }
 }
 
-template <class T, int ACT>
-__global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+// Rows begin .. end - 1 (at most SHAPE::kRows count) and channels from block b0 of expert e.
+template <class SHAPE, int CB, int RB, class T, int ACT>
+__device__ __forceinline__ void tile_body(const Linear8Args& a, int e, int begin, int end, int b0, char* lds) {
+  constexpr int kCols = SHAPE::kCols, kRows = SHAPE::kRows, kStage = SHAPE::kStage;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // workgroups go to the eight dies in turn: each die gets a run of the tiles
-  const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  if (id >= work) return;
-  // ... in blocks of kGroup row tiles, so that what its CUs work on at a time are
-  // few row tiles and few column tiles, which meet in its L2
-  const int band = id / (kGroup * col_tiles), in = id - band * kGroup * col_tiles;
-  const int high = min(kGroup, work / col_tiles - band * kGroup);
-  const int col = in / high;
-  int e, begin, end;
-  if (!find_tile(a, band * kGroup + in - col * high, e, begin, end)) return;
-  const int b0 = col * (kCols / 16);  // first block of channels
   const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
 
-  // A wave's copies of a stage: 4 KB of weights, 2 KB of tokens.
+  // A wave's copies of a stage, 1 KB each.
   constexpr int WCOPIES = kCols / 16 / kWaves, XCOPIES = kRows / 16 / kWaves, COPIES = WCOPIES + XCOPIES;
   const v4i wrsrc = dma::raw_rsrc(a.w + ((int64_t)e * a.blocks + b0) * a.steps * 1024, 0x7fffffffu);
   const v4i xrsrc = dma::raw_rsrc(a.x + (int64_t)(begin >> 4) * a.steps * 1024, 0x7fffffffu);
@@ -98,35 +105,35 @@ __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Ar
   };
   const int wc = wave & 1, wr = wave >> 1;
   // what the results need: a thread's channel's scale and bias, its rows' scales
-  static_assert(kWaves * 64 == kCols, "a thread to each channel");
+  static_assert(kWaves * 64 >= kCols, "a thread to each channel");
   const int channel = b0 * 16 + threadIdx.x;
   const float w_scale = channel < a.n ? a.w_scale[(int64_t)e * a.n + channel] : 0.f;
   const float w_bias = channel < a.n ? a.bias[(int64_t)e * a.n + channel] : 0.f;
-  float xs[2];
+  float xs[RB];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) xs[r] = a.x_scale[min(begin + wr * 64 + r * 32 + (lane & 31), end - 1)];
-  v16i acc[4][2];
+  for (int r = 0; r < RB; ++r) xs[r] = a.x_scale[min(begin + (wr * RB + r) * 32 + (lane & 31), end - 1)];
+  v16i acc[CB][RB];
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+  for (int c = 0; c < CB; ++c)
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < RB; ++r)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[c][r][i] = 0;
   // lane's 16 codes of a 32 x 32 block: row lane & 31, codes 16 (lane >> 5) ..
   const uint32_t lane_at = ((lane >> 4) & 1) * 1024u + (lane >> 5) * 256u + (lane & 15) * 16u;
   struct Step {
-    v4i w[4], x[2];
+    v4i w[CB], x[RB];
   } step[2];
   const auto read = [&](int slot, int k, Step& f) {
     const char* at = lds + slot * kStage + lane_at + k * 512;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f.w[i] = *reinterpret_cast<const v4i*>(at + (wc * 8 + i * 2) * 1024);
+    for (int i = 0; i < CB; ++i) f.w[i] = *reinterpret_cast<const v4i*>(at + (wc * CB + i) * 2048);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) f.x[i] = *reinterpret_cast<const v4i*>(at + (kCols / 16 + wr * 4 + i * 2) * 1024);
+    for (int i = 0; i < RB; ++i) f.x[i] = *reinterpret_cast<const v4i*>(at + kCols * kStepK + (wr * RB + i) * 2048);
   };
-  // product n of eight
   const auto product = [&](const Step& f, auto n) {
-    acc[n >> 1][n & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[n >> 1], f.x[n & 1], acc[n >> 1][n & 1], 0, 0, 0);
+    constexpr int c = n / RB, r = n % RB;
+    acc[c][r] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[c], f.x[r], acc[c][r], 0, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
   };
   // One barrier a stage, before its last products, whose operands are in
@@ -144,15 +151,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Ar
     const int next = slot + 1 == kSlots ? 0 : slot + 1;
     read(slot, 1, step[1]);
     __builtin_amdgcn_sched_barrier(0);
-    each<8>([&](auto n) { product(step[0], n); });
+    each<CB * RB>([&](auto n) { product(step[0], n); });
     dma::wait_vmcnt<(kSlots - 2) * COPIES>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     read(next, 0, step[0]);  // (past the last stage: not used)
     __builtin_amdgcn_sched_barrier(0);
-    each<8>([&](auto n) {
-      product(step[1], n);
+    each<std::max(CB * RB, COPIES)>([&](auto n) {
+      if constexpr (n < CB * RB) product(step[1], n);
       if constexpr (n < COPIES) copy(st + kSlots, slot, n);
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -162,31 +169,32 @@ __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Ar
   // (settle8 for all of them, where they are)
   asm volatile("s_nop 15\n\ts_nop 15");
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+  for (int c = 0; c < CB; ++c)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) asm volatile("" : "+a"(acc[c][r]));
+    for (int r = 0; r < RB; ++r) asm volatile("" : "+a"(acc[c][r]));
   __syncthreads();
 
-  // The results through LDS, 32 rows of a wave's 128 channels at a time, so that
-  // whole rows are stored.  A lane has row lane & 31, channels 8 (i / 4) + 4
-  // (lane >> 5) + i % 4.
-  constexpr int V = kVec<T>, STRIDE = 128 + V;  // the rows that are written together lie in different banks
+  // The results through LDS, 32 rows of a wave's channels at a time, so that whole
+  // rows are stored.  A lane has row lane & 31, channels 8 (i / 4) + 4 (lane >> 5) + i % 4.
+  constexpr int V = kVec<T>, STRIDE = SHAPE::template stride<T>, WIDE = 32 * CB;
   T* stage = reinterpret_cast<T*>(lds + 2 * kCols * sizeof(float)) + wave * 32 * STRIDE;
   float* const params = reinterpret_cast<float*>(lds);  // [2][kCols]
-  params[threadIdx.x] = w_scale;
-  params[kCols + threadIdx.x] = w_bias;
+  if (threadIdx.x < kCols) {
+    params[threadIdx.x] = w_scale;
+    params[kCols + threadIdx.x] = w_bias;
+  }
   __syncthreads();
   const bool vec = a.n % V == 0 && ((uintptr_t)a.out & 15) == 0;
-  const int j0 = b0 * 16 + wc * 128, width = min(128, a.n - j0);
+  const int j0 = b0 * 16 + wc * WIDE, width = min(WIDE, a.n - j0);
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
+  for (int r = 0; r < RB; ++r) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < CB; ++c)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const int j = c * 32 + (i >> 2) * 8 + (lane >> 5) * 4;
-        const v4f ws = *reinterpret_cast<const v4f*>(params + wc * 128 + j);
-        const v4f bias = *reinterpret_cast<const v4f*>(params + kCols + wc * 128 + j);
+        const v4f ws = *reinterpret_cast<const v4f*>(params + wc * WIDE + j);
+        const v4f bias = *reinterpret_cast<const v4f*>(params + kCols + wc * WIDE + j);
         float y[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) y[u] = finish8<ACT>(acc[c][r][i + u], xs[r], ws[u], bias[u]);
@@ -194,10 +202,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Ar
       }
     // the wave's LDS operations are in order; the compiler keeps them so
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const int row0 = begin + wr * 64 + r * 32, rows = min(32, end - row0);
+    const int row0 = begin + (wr * RB + r) * 32, rows = min(32, end - row0);
     T* out = (T*)a.out + (int64_t)row0 * a.n + j0;
     if (vec) {
-      constexpr int PER = 128 / V;  // vectors of a row
+      constexpr int PER = WIDE / V;  // vectors of a row
       const int c = lane % PER * V;
 #pragma unroll
       for (int i = 0; i < 32; i += 64 / PER) {
@@ -208,23 +216,56 @@ __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Ar
     } else {
       for (int i = 0; i < rows; ++i)
 #pragma unroll
-        for (int c = lane; c < 128; c += 64)
+        for (int c = lane; c < WIDE; c += 64)
           if (c < width) out[(int64_t)i * a.n + c] = stage[i * STRIDE + c];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
+// Tiles id < large, then quarters of the tiles from `large` on.
+template <class T, int ACT>
+__global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work, int large) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const auto place = [&](int id, int& e, int& begin, int& end, int& b0) {
+    // blocks of kGroup row tiles, so that what a die's CUs work on at a time are
+    // few row tiles and few column tiles, which meet in its L2
+    const int band = id / (kGroup * col_tiles), in = id - band * kGroup * col_tiles;
+    const int high = min(kGroup, work / col_tiles - band * kGroup);
+    const int col = in / high;
+    b0 = col * (Large::kCols / 16);
+    return find_tile(a, band * kGroup + in - col * high, e, begin, end);
+  };
+  int e, begin, end, b0;
+  if ((int)blockIdx.x < round_up8(large)) {
+    // workgroups go to the eight dies in turn: each die gets a run of the tiles
+    const int id = (blockIdx.x & 7) * (round_up8(large) >> 3) + (blockIdx.x >> 3);
+    if (id >= large || !place(id, e, begin, end, b0)) return;
+    tile_body<Large, 4, 2, T, ACT>(a, e, begin, end, b0, lds);
+  } else {
+    const int id = blockIdx.x - round_up8(large);
+    if (!place(large + (id >> 2), e, begin, end, b0)) return;
+    begin += (id & 1) * Small::kRows;
+    b0 += (id >> 1 & 1) * (Small::kCols / 16);
+    if (begin >= end || b0 >= a.blocks) return;
+    tile_body<Small, 2, 1, T, ACT>(a, e, begin, min(end, begin + Small::kRows), b0, lds);
+  }
+}
+
 template <class T, int ACT>
 int tiles_run(const Linear8Args& a, hipStream_t s) {
-  constexpr int out = 2 * kCols * (int)sizeof(float) + kWaves * 32 * (128 + kVec<T>) * (int)sizeof(T), bytes = std::max(kLds, out);
+  constexpr int bytes = Large::lds<T>();
+  static_assert(bytes <= 80 * 1024 && Small::lds<T>() <= bytes, "two workgroups a CU");
   NHIP_TRY(ensure_dynamic_lds((const void*)linear8_tiles_kernel<T, ACT>, bytes));
-  const int64_t cols = ceil_div(a.blocks, kCols / 16);
+  const int64_t cols = ceil_div(a.blocks, Large::kCols / 16);
   // every expert's last tile may be a part of one
   const int64_t rows = ceil_div(a.rows, kRows) + (a.starts ? std::min(a.experts, a.rows) : 0);
-  if (rows * cols > 0x7fffff00) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
-  NHIP_LAUNCH("linear8_tiles", (linear8_tiles_kernel<T, ACT>), dim3((uint32_t)round_up(rows * cols, 8)), dim3(kWaves * 64),
-              bytes, s, a, (int)cols, (int)(rows * cols));
+  if (rows * cols > 0x7fffff00 / 4) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
+  const int64_t work = rows * cols;
+  const int64_t places = 2 * cu_count(), over = a.starts ? 0 : work % places;
+  const int64_t small = over * 4 <= places ? over : 0, large = work - small;
+  NHIP_LAUNCH("linear8_tiles", (linear8_tiles_kernel<T, ACT>), dim3((uint32_t)(round_up(large, 8) + 4 * small)), dim3(kWaves * 64),
+              bytes, s, a, (int)cols, (int)work, (int)large);
   return check_launch("linear8_tiles");
 }
 
