@@ -73,8 +73,19 @@ __device__ __forceinline__ void each(F f) {
   }
 }
 
+// STREAM: results past kStreamBytes take no place in the caches: 6272 x 8192 of
+// 2048 bf16 111 -> 106 us, 12544 x 4096 of 1024 fp16 117 -> 109.
+template <bool STREAM>
+__device__ __forceinline__ void store16(void* to, const void* from) {
+  const v4i v = *reinterpret_cast<const v4i*>(from);
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(v, reinterpret_cast<v4i*>(to));
+  else
+    *reinterpret_cast<v4i*>(to) = v;
+}
+
 // Rows begin .. end - 1 (at most SHAPE::kRows count) and channels from block b0 of expert e.
-template <class SHAPE, int CB, int RB, class T, int ACT>
+template <class SHAPE, int CB, int RB, class T, int ACT, bool STREAM>
 __device__ __forceinline__ void tile_body(const Linear8Args& a, int e, int begin, int end, int b0, char* lds) {
   constexpr int kCols = SHAPE::kCols, kRows = SHAPE::kRows, kStage = SHAPE::kStage;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -211,7 +222,7 @@ __device__ __forceinline__ void tile_body(const Linear8Args& a, int e, int begin
       for (int i = 0; i < 32; i += 64 / PER) {
         const int at = i + lane / PER;
         if (at < rows && c < width)
-          *reinterpret_cast<int4*>(out + (int64_t)at * a.n + c) = *reinterpret_cast<const int4*>(stage + at * STRIDE + c);
+          store16<STREAM>(out + (int64_t)at * a.n + c, stage + at * STRIDE + c);
       }
     } else {
       for (int i = 0; i < rows; ++i)
@@ -224,7 +235,7 @@ __device__ __forceinline__ void tile_body(const Linear8Args& a, int e, int begin
 }
 
 // Tiles id < large, then quarters of the tiles from `large` on.
-template <class T, int ACT>
+template <class T, int ACT, bool STREAM>
 __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work, int large) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const auto place = [&](int id, int& e, int& begin, int& end, int& b0) {
@@ -241,22 +252,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Ar
     // workgroups go to the eight dies in turn: each die gets a run of the tiles
     const int id = (blockIdx.x & 7) * (round_up8(large) >> 3) + (blockIdx.x >> 3);
     if (id >= large || !place(id, e, begin, end, b0)) return;
-    tile_body<Large, 4, 2, T, ACT>(a, e, begin, end, b0, lds);
+    tile_body<Large, 4, 2, T, ACT, STREAM>(a, e, begin, end, b0, lds);
   } else {
     const int id = blockIdx.x - round_up8(large);
     if (!place(large + (id >> 2), e, begin, end, b0)) return;
     begin += (id & 1) * Small::kRows;
     b0 += (id >> 1 & 1) * (Small::kCols / 16);
     if (begin >= end || b0 >= a.blocks) return;
-    tile_body<Small, 2, 1, T, ACT>(a, e, begin, min(end, begin + Small::kRows), b0, lds);
+    tile_body<Small, 2, 1, T, ACT, STREAM>(a, e, begin, min(end, begin + Small::kRows), b0, lds);
   }
 }
 
-template <class T, int ACT>
-int tiles_run(const Linear8Args& a, hipStream_t s) {
+template <class T, int ACT, bool STREAM>
+int tiles_launch(const Linear8Args& a, hipStream_t s) {
   constexpr int bytes = Large::lds<T>();
   static_assert(bytes <= 80 * 1024 && Small::lds<T>() <= bytes, "two workgroups a CU");
-  NHIP_TRY(ensure_dynamic_lds((const void*)linear8_tiles_kernel<T, ACT>, bytes));
+  NHIP_TRY(ensure_dynamic_lds((const void*)linear8_tiles_kernel<T, ACT, STREAM>, bytes));
   const int64_t cols = ceil_div(a.blocks, Large::kCols / 16);
   // every expert's last tile may be a part of one
   const int64_t rows = ceil_div(a.rows, kRows) + (a.starts ? std::min(a.experts, a.rows) : 0);
@@ -264,9 +275,14 @@ int tiles_run(const Linear8Args& a, hipStream_t s) {
   const int64_t work = rows * cols;
   const int64_t places = 2 * cu_count(), over = a.starts ? 0 : work % places;
   const int64_t small = over * 4 <= places ? over : 0, large = work - small;
-  NHIP_LAUNCH("linear8_tiles", (linear8_tiles_kernel<T, ACT>), dim3((uint32_t)(round_up(large, 8) + 4 * small)), dim3(kWaves * 64),
+  NHIP_LAUNCH("linear8_tiles", (linear8_tiles_kernel<T, ACT, STREAM>), dim3((uint32_t)(round_up(large, 8) + 4 * small)), dim3(kWaves * 64),
               bytes, s, a, (int)cols, (int)work, (int)large);
   return check_launch("linear8_tiles");
+}
+
+template <class T, int ACT>
+int tiles_run(const Linear8Args& a, hipStream_t s) {
+  return (int64_t)a.rows * a.n * (int64_t)sizeof(T) > kStreamBytes ? tiles_launch<T, ACT, true>(a, s) : tiles_launch<T, ACT, false>(a, s);
 }
 
 }  // namespace
