@@ -16,10 +16,15 @@
 namespace nhip {
 namespace {
 
-constexpr int kBins = 1024;   // of weights' exponents, or of keys, or of indices
+constexpr int kBins = 1024;    // of weights' exponents, or of keys, or of indices
 constexpr int kSorted = 1024;  // tokens that are sorted
-constexpr int kList = 4096;   // tokens that LDS holds
 constexpr float kRange = 31.5f;  // exp(-31.5) < 2^-45, which rounds to 0
+
+// What the launches before the last one leave of a row.
+struct RowParts {
+  uint64_t total;        // of all weights
+  uint64_t bins[kBins];  // counts, weights, or the sums of sets of vectors
+};
 
 struct SampleArgs {
   const void* logits;
@@ -34,6 +39,10 @@ struct SampleArgs {
   const float* min_p_each;
   int32_t* token;
   float* logprob;
+  // rows that several workgroups begin: each one's largest key and bound
+  int32_t chunks;
+  uint2* tops;      // [rows][chunks]
+  RowParts* parts;  // [rows]
 };
 
 // Keys in the order of the values; -0 and 0 are equal.
@@ -97,21 +106,21 @@ __device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
 __device__ __forceinline__ void add_to(uint64_t& bin, uint64_t m) { atomicAdd((unsigned long long*)&bin, (unsigned long long)m); }
 __device__ __forceinline__ void count_in(uint64_t& bin) { atomicAdd((uint32_t*)&bin, 1u); }  // below 2^32 of them
 
-// A row in 16-byte vectors from the aligned place at or before its start, dealt
-// to the waves in runs; what lies outside the row is -infinity and is not read.
-// NaN is -infinity.
-template <class T, int WAVES>
+// A row in 16-byte vectors from the aligned place at or before its start; what
+// lies outside the row is -infinity and is not read.  NaN is -infinity.  A wave has
+// a run of them: share `part` of `parts`.
+template <class T>
 struct Row {
   static constexpr int V = kVec<T>;
   typedef T VT __attribute__((ext_vector_type(V)));
   const T* from;  // aligned
-  int shift, vocab, all, begin, end;  // vectors of the row, the wave's
-  __device__ __forceinline__ Row(const T* row, int vocab, int wave) : vocab(vocab) {
+  int shift, vocab, all, begin, end;  // vectors of the row, of the wave
+  __device__ __forceinline__ Row(const T* row, int vocab, int part, int parts) : vocab(vocab) {
     shift = (int)(((uintptr_t)row & 15) / sizeof(T));
     from = row - shift;
     all = (int)(((int64_t)vocab + shift + V - 1) / V);
-    begin = (int)((int64_t)wave * all / WAVES);
-    end = (int)((int64_t)(wave + 1) * all / WAVES);
+    begin = (int)((int64_t)part * all / parts);
+    end = (int)((int64_t)(part + 1) * all / parts);
   }
   __device__ __forceinline__ int first(int vec) const { return vec * V - shift; }
   __device__ __forceinline__ VT load(int vec) const {
@@ -141,16 +150,92 @@ struct Row {
           for (int j = 0; j < V; ++j) f(fmaxf((float)v[u][j], -INFINITY), first(c + u * 64) + j);
     }
   }
+  // Weights of a vector's tokens and their sum: vector `lane` of set `set` of 64.
+  template <class F>
+  __device__ __forceinline__ uint64_t set_sum(int set, int lane, uint64_t (&w)[V], VT& v, F weight) const {
+    uint64_t sum = 0;
+    const int vec = set * 64 + lane;
+    if (vec < all) {
+      v = load(vec);
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum += w[j] = weight(fmaxf((float)v[j], -INFINITY), first(vec) + j);
+    }
+    return sum;
+  }
+  __device__ __forceinline__ int sets() const { return (all + 63) / 64; }
+  // sets of a bin: a power of two
+  __device__ __forceinline__ int set_shift() const {
+    int s = 0;
+    while ((sets() - 1) >> s >= kBins) ++s;
+    return s;
+  }
 };
+
+// A row's settings.
+struct Settings {
+  float temperature, top_p, min_p;
+  int k;
+  __device__ __forceinline__ Settings(const SampleArgs& a, int64_t r) {
+    temperature = a.temperature_each ? a.temperature_each[r] : a.temperature;
+    top_p = a.top_p_each ? a.top_p_each[r] : a.top_p;
+    min_p = a.min_p_each ? a.min_p_each[r] : a.min_p;
+    min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
+    k = a.top_k_each ? a.top_k_each[r] : a.top_k;
+    if (k <= 0 || k > a.vocab) k = a.vocab;
+    if (!(temperature > 0.f)) k = 1;
+  }
+  // few: a bound on the logits finds the first k
+  __device__ __forceinline__ bool few(int vocab) const { return k <= kSorted && k < vocab; }
+  __device__ __forceinline__ bool unfiltered(int vocab) const { return k == vocab && !(top_p < 1.f) && min_p == 0.f; }
+};
+
+// Distances from the largest logit, in halves, so that none overflows: how far
+// tokens weigh anything, and how far the histogram for top-p goes at first (the
+// tokens past it seldom hold 1 - top_p of all; they are most of a row, and each
+// costs an LDS atomic).
+struct Distances {
+  float half_top, reach, scope;
+  __device__ __forceinline__ Distances(float top, const Settings& c) {
+    half_top = 0.5f * top;
+    reach = fminf(0.5f * kRange * c.temperature, 3.4e38f);
+    const float near = 6.f - 2.5f * __logf(fmaxf(1.f - c.top_p, 1e-6f));
+    scope = c.k < 0x7fffffff && c.top_p < 1.f ? fminf(reach, 0.5f * near * c.temperature) : reach;
+  }
+  __device__ __forceinline__ float below(float l) const { return fmaf(-0.5f, l, half_top); }
+  __device__ __forceinline__ int bin(float l, float rate) const { return (int)fminf(below(l) * rate, (float)(kBins - 1)); }
+};
+
+// A bound that at least as many tokens of the wave reach as is its share of the
+// first k: by its lanes' largest.
+template <class T>
+__device__ __forceinline__ uint32_t wave_bound(const Row<T>& row, float mine, int k) {
+  if (row.begin >= row.end) return 0xffffffffu;
+  const int want = (int)(((int64_t)k * (row.end - row.begin) + row.all - 1) / row.all);
+  const uint32_t key = key_of(mine);
+  uint32_t bound = 0;
+  for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+    if (__popcll(__ballot(key >= (bound | bit))) >= want) bound |= bit;
+  return bound;
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
 
 template <int WAVES>
 struct SampleLds {
+  static constexpr int kList = WAVES > 4 ? 12288 : 4096;  // tokens that LDS holds
   uint64_t list[kList];
+  uint64_t sorted[kSorted];
   uint64_t bins[kBins];
   double table[64];
   uint64_t part[WAVES];
   uint32_t keys[WAVES];
-  int32_t count, at;
+  int32_t count, at, index;
+  float logit;
+  uint64_t total;
 };
 
 // list[0 .. n) in falling order, n at most kSorted.  Steps that stay inside 128
@@ -204,61 +289,142 @@ __device__ __forceinline__ uint64_t scan_bins(SampleLds<WAVES>& s, int lane, int
   return all;
 }
 
-// One workgroup: one row.
-//
-// top-k of few: a bound that at least k tokens reach, from the lanes' largest
-// ones, leaves a few hundred, which are compared with each other.  Otherwise a
-// histogram of the tokens by their weights' exponents, of counts for top-k and of
-// weights for top-p, says in which bin the border lies; its tokens are compared
-// with each other, or if they are too many the bin is divided further by the
-// logits' bits, down to equal ones, of which the first by index are kept.
-// The draw sums the weights by index: of the kept tokens, put together in LDS, or
-// if they are too many, of all.
-template <class T, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
-  constexpr int TH = WAVES * 64;
-  __shared__ SampleLds<WAVES> s;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t r = blockIdx.x;
-  const Row<T, WAVES> row((const T*)a.logits + r * a.stride, a.vocab, wave);
-  const float temperature = a.temperature_each ? a.temperature_each[r] : a.temperature;
-  const float top_p = a.top_p_each ? a.top_p_each[r] : a.top_p;
-  float min_p = a.min_p_each ? a.min_p_each[r] : a.min_p;
-  min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
-  int k = a.top_k_each ? a.top_k_each[r] : a.top_k;
-  if (k <= 0 || k > a.vocab) k = a.vocab;
-  if (!(temperature > 0.f)) k = 1;
+constexpr int kPartWaves = 4;
 
+// The first of three launches for long rows: the largest logit of a part of a row, and
+// the bound on its share of the first k.
+template <class T>
+__global__ __launch_bounds__(kPartWaves * 64) void sample_top_kernel(SampleArgs a) {
+  __shared__ uint2 part[kPartWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t r = blockIdx.x / a.chunks;
+  const int chunk = blockIdx.x % a.chunks;
+  const Row<T> row((const T*)a.logits + r * a.stride, a.vocab, chunk * kPartWaves + wave, a.chunks * kPartWaves);
+  const Settings c(a, r);
   float mine = -INFINITY;
   row.each(lane, [&](float l, int) { mine = fmaxf(mine, l); });
-  float top = mine;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  // A bound that at least k tokens reach: of each wave, as many as its share of the
-  // row, by its lanes' largest.
-  uint32_t bound = 0xffffffffu;
-  const bool few = k <= kSorted && k < a.vocab;
-  if (few && k > 1 && row.begin < row.end) {
-    const int want = (int)(((int64_t)k * (row.end - row.begin) + row.all - 1) / row.all);
-    const uint32_t key = key_of(mine);
-    bound = 0;
-    for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-      if (__popcll(__ballot(key >= (bound | bit))) >= want) bound |= bit;
-  }
-  if (lane == 0) {
-    s.part[wave] = key_of(top);
-    s.keys[wave] = bound;
-  }
-  if (threadIdx.x == 0) s.count = 0;
-  if (threadIdx.x < 64) s.table[threadIdx.x] = exp2((double)threadIdx.x / 64);
+  const float top = wave_max(mine);
+  const uint32_t bound = c.few(a.vocab) && c.k > 1 ? wave_bound(row, mine, c.k) : 0;
+  if (lane == 0) part[wave] = make_uint2(key_of(top), bound);
+  for (int i = chunk * kPartWaves * 64 + threadIdx.x; i <= kBins; i += a.chunks * kPartWaves * 64) (&a.parts[r].total)[i] = 0;
   __syncthreads();
-  uint32_t top_key = 0;
+  if (threadIdx.x == 0) {
+    uint2 v = part[0];
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    top_key = max(top_key, (uint32_t)s.part[w]);
-    bound = min(bound, s.keys[w]);
+    for (int w = 1; w < kPartWaves; ++w) v = make_uint2(max(v.x, part[w].x), min(v.y, part[w].y));
+    a.tops[r * a.chunks + chunk] = v;
   }
-  top = of_key(top_key);
+}
+
+// Largest key and bound of a row's parts, for every lane.
+__device__ __forceinline__ uint2 row_top(const SampleArgs& a, int64_t r, int lane) {
+  uint2 v = make_uint2(0, 0xffffffffu);
+  for (int i = lane; i < a.chunks; i += 64) {
+    const uint2 t = a.tops[r * a.chunks + i];
+    v = make_uint2(max(v.x, t.x), min(v.y, t.y));
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = make_uint2(max(v.x, (uint32_t)__shfl_xor((int)v.x, o)), min(v.y, (uint32_t)__shfl_xor((int)v.y, o)));
+  return v;
+}
+
+// The second: of a part of a row the histogram that the row's border is first
+// looked for in, or without a filter the sums of its sets.
+template <class T>
+__global__ __launch_bounds__(kPartWaves * 64) void sample_bins_kernel(SampleArgs a) {
+  __shared__ uint64_t bins[kBins];
+  __shared__ double table[64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t r = blockIdx.x / a.chunks;
+  const int chunk = blockIdx.x % a.chunks;
+  const Settings c(a, r);
+  const bool unfiltered = c.unfiltered(a.vocab);
+  if (c.few(a.vocab) || (c.k == a.vocab && !(c.top_p < 1.f) && !unfiltered)) return;
+  const float top = of_key(row_top(a, r, lane).x);
+  if (!(fabsf(top) < INFINITY)) return;
+  const Row<T> row((const T*)a.logits + r * a.stride, a.vocab, chunk * kPartWaves + wave, a.chunks * kPartWaves);
+  const Distances d(top, c);
+  const Weights weight{(double)top, 64 * 1.4426950408889634074 / (double)c.temperature, table};
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64);
+  if (unfiltered) {
+    __syncthreads();
+    const int shift = row.set_shift(), sets = row.sets();
+    for (int set = chunk * kPartWaves + wave; set < sets; set += a.chunks * kPartWaves) {
+      uint64_t w[Row<T>::V];
+      typename Row<T>::VT v;
+      const uint64_t sum = wave_sum(row.set_sum(set, lane, w, v, [&](float l, int) { return weight(l); }));
+      if (lane == 0) add_to(a.parts[r].bins[set >> shift], sum);
+    }
+    return;
+  }
+  for (int i = threadIdx.x; i < kBins; i += kPartWaves * 64) bins[i] = 0;
+  __syncthreads();
+  const float scope = c.k < a.vocab ? d.reach : d.scope, rate = (float)kBins / scope;
+  uint64_t sum = 0;
+  if (c.k < a.vocab)
+    row.each(lane, [&](float l, int) {
+      if (d.below(l) <= scope) count_in(bins[d.bin(l, rate)]);
+    });
+  else
+    row.each(lane, [&](float l, int) {
+      const uint64_t w = weight(l);
+      sum += w;
+      if (d.below(l) <= scope) add_to(bins[d.bin(l, rate)], w);
+    });
+  sum = wave_sum(sum);
+  if (lane == 0 && sum) add_to(a.parts[r].total, sum);
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kPartWaves * 64)
+    if (bins[i]) add_to(a.parts[r].bins[i], bins[i]);
+}
+
+// One workgroup: one row, or what is left of it to do.
+//
+// Tokens that may be kept are put together in LDS.  For top-k of few a bound that
+// at least k tokens reach, from the lanes' largest ones, leaves a few hundred.
+// Otherwise a histogram of the tokens by their weights' exponents, of counts for
+// top-k and of weights for top-p, says in which bin the border lies.  The tokens
+// about the border are sorted, or if they are too many their bin is divided
+// further by the logits' bits, down to equal ones, of which the first by index are
+// kept.  The draw sums weights by index: of the tokens in LDS, or, if they do not
+// fit there, of all.
+template <class T, int WAVES, bool PARTS>
+__global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
+  constexpr int TH = WAVES * 64;
+  constexpr int kList = SampleLds<WAVES>::kList;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  SampleLds<WAVES>& s = *reinterpret_cast<SampleLds<WAVES>*>(lds);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t r = blockIdx.x;
+  const Row<T> row((const T*)a.logits + r * a.stride, a.vocab, wave, WAVES);
+  const Settings c(a, r);
+  const int k = c.k;
+
+  uint32_t top_key = 0, bound = 0xffffffffu;
+  if constexpr (PARTS) {
+    const uint2 v = row_top(a, r, lane);
+    top_key = v.x;
+    bound = v.y;
+    if (threadIdx.x < 64) s.table[threadIdx.x] = exp2((double)threadIdx.x / 64);
+    __syncthreads();
+  } else {
+    float mine = -INFINITY;
+    row.each(lane, [&](float l, int) { mine = fmaxf(mine, l); });
+    const float top = wave_max(mine);
+    if (c.few(a.vocab) && k > 1) bound = wave_bound(row, mine, k);
+    if (lane == 0) {
+      s.part[wave] = key_of(top);
+      s.keys[wave] = bound;
+    }
+    if (threadIdx.x < 64) s.table[threadIdx.x] = exp2((double)threadIdx.x / 64);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      top_key = max(top_key, (uint32_t)s.part[w]);
+      bound = min(bound, s.keys[w]);
+    }
+  }
+  const float top = of_key(top_key);
   if (top == -INFINITY) {  // no token
     if (threadIdx.x == 0) {
       a.token[r] = -1;
@@ -266,41 +432,79 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     }
     return;
   }
-  // (of an infinite largest one: 0 where it stands, others as far below as there is)
-  const bool infinite = top == INFINITY;
-  const Weights exact{infinite ? 0.0 : (double)top, 64 * 1.4426950408889634074 / (double)(temperature > 0.f ? temperature : 1.f), s.table};
-  const auto weight = [&](float l) { return exact(infinite ? (l == top ? 0.f : -INFINITY) : l); };
-  // half a logit's distance from the largest, and how far tokens weigh anything (halves, so that no difference overflows)
-  const float half_top = 0.5f * top, half_reach = fminf(0.5f * kRange * temperature, 3.4e38f);
-  const auto below = [&](float l) { return l == top ? 0.f : fmaf(-0.5f, l, half_top); };
+  const Distances d(top, c);
+  const Weights weight{(double)top, 64 * 1.4426950408889634074 / (double)(c.temperature > 0.f ? c.temperature : 1.f), s.table};
   const double u = fmin(fmax((double)a.uniform[r], 0.0), 1.0 - 0x1p-53);  // NaN: 0
-  const auto finish = [&](int index, float l, uint64_t total) {
-    const double x = l == top ? 0.0 : ((double)l - (double)top) / (double)temperature;
-    a.token[r] = index;
-    a.logprob[r] = (float)(x - log((double)total * 0x1p-44));
-  };
   // the first whose cumulated weight is past this
   const auto target_of = [&](uint64_t total) { return min((uint64_t)((double)total * u), total - 1); };
-  // s.bins: the sums of `measure` over the first n <= kSorted of s.list up to each, and behind them the whole
-  const auto sum_list = [&](int n, auto measure) {
-    for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = i < n ? measure(of_key((uint32_t)(s.list[i] >> 32))) : 0;
-    __syncthreads();
-    scan_bins(s, lane, wave);
+  const auto too_light = [&](uint64_t w) { return (double)w * 0x1p-44 < (double)c.min_p; };
+  // one thread has found the token; all call the second
+  const auto found = [&](int index, float l, uint64_t total) {
+    s.index = index;
+    s.logit = l;
+    s.total = total;
   };
-  // the one of the first n of s.list that is drawn, the weights before it being `begin` and all `total`
-  const auto draw_list = [&](int n, uint64_t begin, uint64_t total) {
+  const auto finish = [&]() {
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += TH) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;  // ~index falls: rising indices
-    __syncthreads();
-    sort_list<WAVES>(s.list, n);
-    for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = i < n ? weight(of_key((uint32_t)s.list[i])) : 0;
-    __syncthreads();
-    scan_bins(s, lane, wave);
-    const uint64_t target = target_of(total) - begin;
-    for (int i = threadIdx.x; i < n; i += TH)
-      if (target < s.bins[i] && target >= (i ? s.bins[i - 1] : 0)) finish((int)~(uint32_t)(s.list[i] >> 32), of_key((uint32_t)s.list[i]), total);
+    if (threadIdx.x == 0) {
+      const double x = s.logit == top ? 0.0 : ((double)s.logit - (double)top) / (double)c.temperature;
+      a.token[r] = s.index;
+      a.logprob[r] = (float)(x - log((double)s.total * 0x1p-44));
+    }
   };
-  const auto too_light = [&](uint64_t w) { return (double)w * 0x1p-44 < (double)min_p; };
+  const auto zero_bins = [&]() {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = 0;
+    if (threadIdx.x == 0) s.count = s.at = 0;
+    __syncthreads();
+  };
+  // s.at: the first bin of the sums whose sum is past this
+  const auto find_bin = [&](uint64_t target) {
+    for (int i = threadIdx.x; i < kBins; i += TH)
+      if (target < s.bins[i] && target >= (i ? s.bins[i - 1] : 0)) s.at = i;
+    __syncthreads();
+  };
+  // tokens of a value: how many, and (behind that) s.at the index of the `left`-th, from 1
+  const auto count_equal = [&](float value) {
+    int held = 0;
+    row.each(lane, [&](float l, int) { held += l == value; });
+    const int of_wave = (int)wave_sum((uint64_t)held);
+    __syncthreads();
+    if (lane == 0) s.keys[wave] = of_wave;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all += s.keys[w];
+    return all;
+  };
+  const auto find_equal = [&](float value, int left) {
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      if (w < wave) left -= (int)s.keys[w];
+    if (left > 0 && left <= (int)s.keys[wave]) {
+      // this wave has it: a vector to a lane, rising
+      for (int v0 = row.begin; v0 < row.end; v0 += 64) {
+        int n = 0;
+        typename Row<T>::VT v;
+        if (v0 + lane < row.end) {
+          v = row.load(v0 + lane);
+#pragma unroll
+          for (int j = 0; j < Row<T>::V; ++j) n += (float)v[j] == value;
+        }
+        const int upto = (int)wave_scan((uint64_t)n, lane);
+        if (upto >= left && upto - n < left) {
+          int need = left - (upto - n);
+#pragma unroll
+          for (int j = 0; j < Row<T>::V; ++j)
+            if ((float)v[j] == value && --need == 0) s.at = row.first(v0 + lane) + j;
+        }
+        const int all_here = __builtin_amdgcn_readlane(upto, 63);
+        if (all_here >= left) break;
+        left -= all_here;
+      }
+    }
+    __syncthreads();
+  };
 
   if (k == 1) {
     // the lowest index of the largest
@@ -316,68 +520,115 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     if (threadIdx.x == 0) {
 #pragma unroll
       for (int w = 1; w < WAVES; ++w) low = min(low, (int)s.keys[w]);
-      finish(low, top, uint64_t(1) << 44);
+      a.token[r] = low;
+      a.logprob[r] = 0.f;
     }
     return;
   }
-  if (few) {
-    // ------------------------------------------------ few tokens are kept
-    const float least = bound > key_of(-INFINITY) ? of_key(bound) : -INFINITY;
-    row.each(lane, [&](float l, int index) {
-      if (l >= least && below(l) <= half_reach) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < kSorted) s.list[at] = place_of(key_of(l), index);
-      }
-    });
-    __syncthreads();
-    int n = s.count;
-    if (n <= kSorted) {
-      sort_list<WAVES>(s.list, n);
-      n = min(n, k);
-      sum_list(n, weight);
-      // (the first one always)
-      const double limit = top_p < 1.f ? fmax((double)top_p * (double)s.bins[kBins - 1], 1.0) : INFINITY;
-      if (threadIdx.x == 0) s.at = 1;
-      __syncthreads();
-      for (int i = threadIdx.x; i < n; i += TH) {
-        const uint64_t before = i ? s.bins[i - 1] : 0;
-        if ((double)before < limit && !too_light(s.bins[i] - before)) atomicMax(&s.at, i + 1);
-      }
-      __syncthreads();
-      n = s.at;
-      draw_list(n, 0, s.bins[n - 1]);
-      return;
-    }
+  if (top == INFINITY) {
+    // infinite ones weigh the same, others nothing
+    const int64_t all = min(count_equal(top), (int64_t)k);
+    const int kept = (int)fmin(fmax(c.top_p < 1.f ? ceil((double)c.top_p * (double)all) : (double)all, 1.0), (double)all);
+    const uint64_t total = (uint64_t)kept << 44;
+    find_equal(top, (int)(target_of(total) >> 44) + 1);
+    if (threadIdx.x == 0) found(s.at, top, total);
+    finish();
+    return;
   }
 
-  // --------------------------------------------------- any number is kept
-  // everything up to (last, last_index) of the order, as far as it weighs anything
+  // what is kept: everything up to (last, last_index) of the order, as far as it weighs anything
   float last = -INFINITY;
   int last_index = 0x7fffffff;
-  const float rate = (float)kBins / half_reach;
-  const auto bin_of = [&](float l) { return (int)fminf(below(l) * rate, (float)(kBins - 1)); };
-  const auto inside = [&](float l, int index) { return below(l) <= half_reach && (l > last || (l == last && index <= last_index)); };
-#pragma unroll 1
-  for (int by = 0; by < 2; ++by) {  // top-k by count, then top-p by weight
-    if (by == 0 ? k == a.vocab : !(top_p < 1.f)) continue;
-    const auto measure = [&](float l) { return by ? weight(l) : (uint64_t)1; };
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = 0;
-    __syncthreads();
+  const auto inside = [&](float l, int index) { return d.below(l) <= d.reach && l >= last && (l > last || index <= last_index); };
+  const auto inside_place = [&](uint64_t p) { return inside(of_key((uint32_t)(p >> 32)), (int)~(uint32_t)p); };
+  // the tokens from `least` on together in LDS, n of them; false: they do not fit
+  int n = 0;
+  const auto collect = [&](float least) {
+    zero_bins();
     row.each(lane, [&](float l, int index) {
-      if (inside(l, index))
-        by ? add_to(s.bins[bin_of(l)], weight(l)) : count_in(s.bins[bin_of(l)]);
+      if (l >= least && inside(l, index)) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kList) s.list[at] = place_of(key_of(l), index);
+      }
     });
     __syncthreads();
-    const uint64_t all = scan_bins(s, lane, wave);
-    const double limit = by ? fmax((double)top_p * (double)all, 1.0) : (double)k;  // (the first one always)
+    n = s.count;
+    return n <= kList;
+  };
+  // s.bins: the sums of `measure` over the first m of s.sorted up to each, and behind them the whole
+  const auto sum_sorted = [&](int m, auto measure) {
+    for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = i < m ? measure(s.sorted[i]) : 0;
+    __syncthreads();
+    return scan_bins(s, lane, wave);
+  };
+  const auto weight_of = [&](uint64_t place) { return weight(of_key((uint32_t)(place >> 32))); };
+
+  bool listed = false;
+  uint64_t mass = 0;  // of all that top-k has left, if top-p's histogram was made
+  if (c.few(a.vocab)) {
+    const float least = bound > key_of(-INFINITY) ? of_key(bound) : -INFINITY;
+    listed = collect(least);
+  }
+#pragma unroll 1
+  for (int by = 0; by < 2; ++by) {  // top-k by count, then top-p by weight
+    if (by == 0 ? k == a.vocab : !(c.top_p < 1.f)) continue;
+    if (listed && n <= kSorted) break;  // all in one go, below
+    const auto measure = [&](float l) { return by ? weight(l) : (uint64_t)1; };
+    float scope = d.reach;
+    double limit;
+    for (bool again = false;; again = true) {
+      // (with both filters the second looks at what the first has left)
+      scope = by && k == a.vocab && !again ? d.scope : d.reach;
+      const float rate = (float)kBins / scope;
+      uint64_t all;
+      zero_bins();
+      if (listed) {
+        for (int i = threadIdx.x; i < n; i += TH)
+          if (const float l = of_key((uint32_t)(s.list[i] >> 32)); inside_place(s.list[i])) add_to(s.bins[d.bin(l, rate)], measure(l));
+        __syncthreads();
+        all = scan_bins(s, lane, wave);
+      } else if (PARTS && !again && (by == 0 ? !c.few(a.vocab) : k == a.vocab)) {
+        for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = a.parts[r].bins[i];
+        __syncthreads();
+        all = scan_bins(s, lane, wave);
+        if (by) all = a.parts[r].total;
+      } else if (by == 0) {
+        row.each(lane, [&](float l, int) {
+          if (d.below(l) <= scope) count_in(s.bins[d.bin(l, rate)]);
+        });
+        __syncthreads();
+        all = scan_bins(s, lane, wave);
+      } else {
+        uint64_t sum = 0;
+        row.each(lane, [&](float l, int index) {
+          const uint64_t w = weight(l);
+          if (inside(l, index)) {
+            sum += w;
+            if (d.below(l) <= scope) add_to(s.bins[d.bin(l, rate)], w);
+          }
+        });
+        sum = wave_sum(sum);
+        __syncthreads();
+        scan_bins(s, lane, wave);
+        if (lane == 0) s.part[wave] = sum;
+        __syncthreads();
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) all += s.part[w];
+      }
+      limit = by ? fmax((double)c.top_p * (double)all, 1.0) : (double)k;  // (the first one always)
+      if (by) mass = all;
+      if (scope == d.reach || (double)s.bins[kBins - 1] >= limit) break;
+    }
     // kept: those with less than `limit` before them; the last of them lies in the bin that reaches it
-    if ((double)all < limit || (by == 0 && all <= (uint64_t)k)) continue;
+    if ((double)s.bins[kBins - 1] < limit || (by == 0 && s.bins[kBins - 1] <= (uint64_t)k)) continue;
+    const float rate = (float)kBins / scope;
     uint64_t before = 0;                   // the measure of what comes before the present bin
     uint32_t low = 0, high = 0xffffffffu;  // its keys
     int bin = -1, shift = 0;               // its bin of weights
     for (;;) {
       // the first bin with which the sum reaches the limit
+      __syncthreads();
       if (threadIdx.x == 0) {
         s.at = kBins - 1;
         s.count = 0;
@@ -387,46 +638,60 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
         if ((double)(before + s.bins[i]) >= limit && s.bins[i]) atomicMin(&s.at, i);
       __syncthreads();
       const int at = s.at;
+      before += at ? s.bins[at - 1] : 0;
       if (bin < 0) {
         bin = at;
+        // all up to the bin's last value into LDS
+        // (the margin: a bin's rounding)
+        if (!listed) {
+          const float under = d.half_top - (float)(bin + 1) / rate;
+          listed = collect(bin == kBins - 1 ? -INFINITY : 2.f * (under - 1e-6f * (fabsf(d.half_top) + scope)));
+          if (listed && n <= kSorted) break;
+        }
       } else {  // bins of keys: the largest first
         const uint32_t width = 1u << shift;
         high -= (uint32_t)at * width;
         low = high - low >= width ? high - (width - 1) : low;
       }
-      before += at ? s.bins[at - 1] : 0;
+      __syncthreads();
+      if (threadIdx.x == 0) s.count = 0;
+      __syncthreads();
       const auto here = [&](float l, int index) {
-        if (!inside(l, index) || bin_of(l) != bin) return false;
+        if (!inside(l, index) || d.below(l) > scope || d.bin(l, rate) != bin) return false;
         const uint32_t key = key_of(l);
         return key >= low && key <= high;
       };
       uint32_t most = 0, least = 0xffffffffu;
-      row.each(lane, [&](float l, int index) {
+      const auto take = [&](float l, int index) {
         if (here(l, index)) {
           const uint32_t key = key_of(l);
           most = max(most, key);
           least = min(least, key);
           const int i = atomicAdd(&s.count, 1);
-          if (i < kSorted) s.list[i] = place_of(key, index);
+          if (i < kSorted) s.sorted[i] = place_of(key, index);
         }
-      });
+      };
+      if (listed)
+        for (int i = threadIdx.x; i < n; i += TH) take(of_key((uint32_t)(s.list[i] >> 32)), (int)~(uint32_t)s.list[i]);
+      else
+        row.each(lane, take);
 #pragma unroll
       for (int o = 32; o; o >>= 1) {
-        most = max(most, (uint32_t)__shfl_xor(most, o));
-        least = min(least, (uint32_t)__shfl_xor(least, o));
+        most = max(most, (uint32_t)__shfl_xor((int)most, o));
+        least = min(least, (uint32_t)__shfl_xor((int)least, o));
       }
       if (lane == 0) s.part[wave] = (uint64_t)most << 32 | least;
       __syncthreads();
       const int count = s.count;
       if (count <= kSorted) {
-        sort_list<WAVES>(s.list, count);
-        sum_list(count, measure);
+        sort_list<WAVES>(s.sorted, count);
+        sum_sorted(count, [&](uint64_t place) { return measure(of_key((uint32_t)(place >> 32))); });
         if (threadIdx.x == 0) s.at = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < count; i += TH)
           if ((double)(before + (i ? s.bins[i - 1] : 0)) < limit) atomicMax(&s.at, i);
         __syncthreads();
-        const uint64_t place = s.list[s.at];
+        const uint64_t place = s.sorted[s.at];
         last = of_key((uint32_t)(place >> 32));
         last_index = (int)~(uint32_t)place;
         __syncthreads();
@@ -441,42 +706,11 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
       }
       __syncthreads();
       if (low == high) {
-        // one value: the first so many by index
+        // one value: the first so many by index (of those that top-k has left)
         const float value = of_key(low);
         const int keep = (int)fmax(1.0, fmin(ceil((limit - (double)before) / (double)measure(value)), (double)count));
-        int held = 0;
-        row.each(lane, [&](float l, int index) { held += l == value && inside(l, index); });
-        const uint64_t wave_held = wave_sum((uint64_t)held);
-        if (lane == 0) s.part[wave] = wave_held;
-        __syncthreads();
-        int left = keep;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w)
-          if (w < wave) left -= (int)s.part[w];
-        if (left > 0 && left <= (int)wave_held) {
-          // this wave has the last of them: a vector to a lane, rising
-          for (int c = row.begin; c < row.end; c += 64) {
-            int n = 0;
-            typename Row<T, WAVES>::VT v;
-            if (c + lane < row.end) {
-              v = row.load(c + lane);
-#pragma unroll
-              for (int j = 0; j < Row<T, WAVES>::V; ++j)
-                n += (float)v[j] == value && inside((float)v[j], row.first(c + lane) + j);
-            }
-            const int upto = (int)wave_scan((uint64_t)n, lane);
-            if (upto >= left && upto - n < left) {
-              int need = left - (upto - n);
-#pragma unroll
-              for (int j = 0; j < Row<T, WAVES>::V; ++j)
-                if ((float)v[j] == value && inside((float)v[j], row.first(c + lane) + j) && --need == 0) s.at = row.first(c + lane) + j;
-            }
-            const int all_here = __builtin_amdgcn_readlane(upto, 63);
-            if (all_here >= left) break;
-            left -= all_here;
-          }
-        }
-        __syncthreads();
+        count_equal(value);
+        find_equal(value, keep);
         last = value;
         last_index = s.at;
         break;
@@ -484,63 +718,81 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
       // the bin's keys, largest first, into kBins parts
       shift = 0;
       while (((high - low) >> shift) >= (uint32_t)kBins) ++shift;
-      for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = 0;
-      __syncthreads();
-      row.each(lane, [&](float l, int index) {
-        if (here(l, index))
-          by ? add_to(s.bins[(high - key_of(l)) >> shift], weight(l)) : count_in(s.bins[(high - key_of(l)) >> shift]);
-      });
+      zero_bins();
+      const auto divide = [&](float l, int index) {
+        if (here(l, index)) add_to(s.bins[(high - key_of(l)) >> shift], measure(l));
+      };
+      if (listed)
+        for (int i = threadIdx.x; i < n; i += TH) divide(of_key((uint32_t)(s.list[i] >> 32)), (int)~(uint32_t)s.list[i]);
+      else
+        row.each(lane, divide);
       __syncthreads();
       scan_bins(s, lane, wave);
     }
+    if (listed && n <= kSorted) break;
+  }
+
+  if (listed && n <= kSorted) {
+    // ------------------------- all that may be kept, sorted: every filter at once
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += TH) s.sorted[i] = inside_place(s.list[i]) ? s.list[i] : 0;
+    __syncthreads();
+    sort_list<WAVES>(s.sorted, n);
+    const int first = min(n, k);
+    const uint64_t sum = sum_sorted(first, weight_of);
+    if (!mass) mass = sum;  // (the list holds the first k)
+    const double limit = c.top_p < 1.f ? fmax((double)c.top_p * (double)mass, 1.0) : INFINITY;  // (the first one always)
+    if (threadIdx.x == 0) s.at = 1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < first; i += TH) {
+      const uint64_t before = i ? s.bins[i - 1] : 0;
+      if ((double)before < limit && !too_light(s.bins[i] - before)) atomicMax(&s.at, i + 1);
+    }
+    __syncthreads();
+    const uint64_t place = s.sorted[s.at - 1];
+    last = of_key((uint32_t)(place >> 32));
+    last_index = (int)~(uint32_t)place;
+  } else if (!listed && c.min_p > 0.f) {
+    // a logit below this is too light (to a margin: its weight decides)
+    const float cut = (float)((double)top + (double)c.temperature * (log((double)c.min_p) - 1e-6) - 1e-6 * fabs((double)top));
+    listed = collect(fmaxf(last, cut));
+  } else if (!listed && last > -INFINITY) {
+    listed = collect(last);
   }
 
   // the draw: weights by index
-  if (last > -INFINITY || min_p > 0.f) {
-    // a logit below this is too light (to a margin: its weight decides)
-    const float cut = fmaxf(last, min_p > 0.f ? (float)((double)top + (double)temperature * (log((double)min_p) - 1e-6) -
-                                                        1e-6 * fabs((double)top)) : -INFINITY);
+  if (listed) {
+    int shift = 0;
+    while ((a.vocab - 1) >> shift >= kBins) ++shift;
+    const auto drawn = [&](uint64_t place) -> uint64_t {
+      if (!inside_place(place)) return 0;
+      const uint64_t w = weight_of(place);
+      return too_light(w) ? 0 : w;
+    };
+    zero_bins();
+    for (int i = threadIdx.x; i < n; i += TH)
+      if (const uint64_t w = drawn(s.list[i])) add_to(s.bins[~(uint32_t)s.list[i] >> shift], w);
     __syncthreads();
-    if (threadIdx.x == 0) s.count = 0;
-    for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = 0;
-    __syncthreads();
-    row.each(lane, [&](float l, int index) {
-      if (l >= cut && inside(l, index)) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < kList) s.list[at] = place_of(key_of(l), index);
+    const uint64_t total = scan_bins(s, lane, wave), target = target_of(total);
+    find_bin(target);
+    const int at = s.at;
+    const uint64_t begin = at ? s.bins[at - 1] : 0;
+    for (int i = threadIdx.x; i < n; i += TH)
+      if ((int)(~(uint32_t)s.list[i] >> shift) == at && drawn(s.list[i])) {
+        const int m = atomicAdd(&s.count, 1);
+        // (the index turned round: falling order is rising index)
+        if (m < kSorted) s.sorted[m] = s.list[i] << 32 | s.list[i] >> 32;
       }
-    });
     __syncthreads();
-    const int n = s.count;
-    if (n <= kList) {
-      int shift = 0;
-      while ((a.vocab - 1) >> shift >= kBins) ++shift;
-      const auto light = [&](uint64_t place) {
-        const uint64_t w = weight(of_key((uint32_t)(place >> 32)));
-        return too_light(w) ? 0 : w;
-      };
-      for (int i = threadIdx.x; i < n; i += TH) add_to(s.bins[~(uint32_t)s.list[i] >> shift], light(s.list[i]));
-      __syncthreads();
-      const uint64_t total = scan_bins(s, lane, wave), target = target_of(total);
-      for (int i = threadIdx.x; i < kBins; i += TH)
-        if (target < s.bins[i] && target >= (i ? s.bins[i - 1] : 0)) s.at = i;
-      uint64_t held[kList / TH];
-#pragma unroll
-      for (int e = 0; e < kList / TH; ++e) held[e] = (int)threadIdx.x + e * TH < n ? s.list[threadIdx.x + e * TH] : 0;
-      if (threadIdx.x == 0) s.count = 0;
-      __syncthreads();
-      const int at = s.at;
-      const uint64_t begin = at ? s.bins[at - 1] : 0;
-#pragma unroll
-      for (int e = 0; e < kList / TH; ++e)
-        if ((int)threadIdx.x + e * TH < n && (int)(~(uint32_t)held[e] >> shift) == at && light(held[e]))
-          s.list[atomicAdd(&s.count, 1)] = held[e];
-      __syncthreads();
-      const int m = s.count;
-      if (m <= kSorted) {
-        draw_list(m, begin, total);
-        return;
-      }
+    const int m = s.count;
+    if (m <= kSorted) {
+      sort_list<WAVES>(s.sorted, m);
+      sum_sorted(m, [&](uint64_t place) { return weight(of_key((uint32_t)place)); });
+      const uint64_t rest = target - begin;
+      for (int i = threadIdx.x; i < m; i += TH)
+        if (rest < s.bins[i] && rest >= (i ? s.bins[i - 1] : 0)) found((int)~(uint32_t)(s.sorted[i] >> 32), of_key((uint32_t)s.sorted[i]), total);
+      finish();
+      return;
     }
   }
   const auto drawn = [&](float l, int index) -> uint64_t {
@@ -548,71 +800,84 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     const uint64_t w = weight(l);
     return too_light(w) ? 0 : w;
   };
-  // sums of the weights of 64 vectors each, or of a power of two of them
-  __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = 0;
-  __syncthreads();
-  const int sets = (row.all + 63) / 64;
-  int shift = 0;
-  while ((sets - 1) >> shift >= kBins) ++shift;
-  const auto set_sum = [&](int set, uint64_t(&w)[Row<T, WAVES>::V], typename Row<T, WAVES>::VT& v) {
-    uint64_t sum = 0;
-    const int vec = set * 64 + lane;
-    if (vec < row.all) {
-      v = row.load(vec);
-#pragma unroll
-      for (int j = 0; j < Row<T, WAVES>::V; ++j) sum += w[j] = drawn(fmaxf((float)v[j], -INFINITY), row.first(vec) + j);
+  const int set_shift = row.set_shift(), sets = row.sets();
+  zero_bins();
+  if (PARTS && c.unfiltered(a.vocab)) {
+    for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = a.parts[r].bins[i];
+  } else {
+#pragma unroll 1
+    for (int set = wave; set < sets; set += WAVES) {
+      uint64_t w[Row<T>::V];
+      typename Row<T>::VT v;
+      const uint64_t sum = wave_sum(row.set_sum(set, lane, w, v, drawn));
+      if (lane == 0) add_to(s.bins[set >> set_shift], sum);
     }
-    return sum;
-  };
-#pragma unroll 2
-  for (int set = wave; set < sets; set += WAVES) {
-    uint64_t w[Row<T, WAVES>::V];
-    typename Row<T, WAVES>::VT v;
-    const uint64_t sum = wave_sum(set_sum(set, w, v));
-    if (lane == 0) add_to(s.bins[set >> shift], sum);
   }
   __syncthreads();
   const uint64_t total = scan_bins(s, lane, wave), target = target_of(total);
-  for (int i = threadIdx.x; i < kBins; i += TH)
-    if (target < s.bins[i] && target >= (i ? s.bins[i - 1] : 0)) s.at = i;
-  __syncthreads();
-  if (wave) return;
-  const int at = s.at;
-  uint64_t begin = at ? s.bins[at - 1] : 0;
-  for (int set = at << shift; set < min(sets, (at + 1) << shift); ++set) {
-    uint64_t w[Row<T, WAVES>::V];
-    typename Row<T, WAVES>::VT v;
-    const uint64_t sum = set_sum(set, w, v), upto = wave_scan(sum, lane), all = lane64(upto, 63);
-    if (target < begin + all) {
-      uint64_t from = begin + upto - sum;
-      if (target >= from && target < from + sum) {
+  find_bin(target);
+  if (wave == 0) {
+    const int at = s.at;
+    uint64_t begin = at ? s.bins[at - 1] : 0;
+    for (int set = at << set_shift; set < min(sets, (at + 1) << set_shift); ++set) {
+      uint64_t w[Row<T>::V];
+      typename Row<T>::VT v;
+      const uint64_t sum = row.set_sum(set, lane, w, v, drawn), upto = wave_scan(sum, lane), all = lane64(upto, 63);
+      if (target < begin + all) {
+        uint64_t from = begin + upto - sum;
+        if (target >= from && target < from + sum) {
 #pragma unroll
-        for (int j = 0; j < Row<T, WAVES>::V; ++j) {
-          if (target >= from && target < from + w[j]) finish(row.first(set * 64 + lane) + j, fmaxf((float)v[j], -INFINITY), total);
-          from += w[j];
+          for (int j = 0; j < Row<T>::V; ++j) {
+            if (target >= from && target < from + w[j]) found(row.first(set * 64 + lane) + j, fmaxf((float)v[j], -INFINITY), total);
+            from += w[j];
+          }
         }
+        break;
       }
-      return;
+      begin += all;
     }
-    begin += all;
   }
+  finish();
+}
+
+// Workgroups that begin a row, 0: one does all of it.
+int chunks_of(const nhip_sample_desc* d) {
+  const int force = setting_int("NHIP_SAMPLE_CHUNKS", -1);
+  if (force >= 0) return std::min(force, 64);
+  if (d->vocab <= 16384) return 0;
+  const int64_t want = ceil_div(4 * cu_count(), std::max(d->rows, 1));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, d->vocab / 2048, 64}));
+}
+
+uint64_t workspace_of(const nhip_sample_desc* d) {
+  const int chunks = chunks_of(d);
+  return chunks ? d->rows * (sizeof(RowParts) + (uint64_t)chunks * sizeof(uint2)) : 0;
+}
+
+template <class T, int WAVES, bool PARTS>
+int sample_last(const SampleArgs& a, int rows, hipStream_t s) {
+  constexpr int bytes = (int)sizeof(SampleLds<WAVES>);
+  if (bytes > 65536) NHIP_TRY(ensure_dynamic_lds((const void*)sample_kernel<T, WAVES, PARTS>, bytes));
+  NHIP_LAUNCH("sample", (sample_kernel<T, WAVES, PARTS>), dim3((uint32_t)rows), dim3(WAVES * 64), bytes, s, a);
+  return check_launch("sample");
 }
 
 template <class T>
 int sample_run(const SampleArgs& a, int rows, hipStream_t s) {
-  if (a.vocab <= 8192)
-    NHIP_LAUNCH("sample", (sample_kernel<T, 4>), dim3((uint32_t)rows), dim3(256), 0, s, a);
-  else
-    NHIP_LAUNCH("sample", (sample_kernel<T, 16>), dim3((uint32_t)rows), dim3(1024), 0, s, a);
-  return check_launch("sample");
+  if (!a.chunks) return a.vocab <= 8192 ? sample_last<T, 4, false>(a, rows, s) : sample_last<T, 16, false>(a, rows, s);
+  const dim3 grid((uint32_t)((int64_t)rows * a.chunks)), block(kPartWaves * 64);
+  NHIP_LAUNCH("sample_top", (sample_top_kernel<T>), grid, block, 0, s, a);
+  NHIP_TRY(check_launch("sample_top"));
+  NHIP_LAUNCH("sample_bins", (sample_bins_kernel<T>), grid, block, 0, s, a);
+  NHIP_TRY(check_launch("sample_bins"));
+  return sample_last<T, 16, true>(a, rows, s);
 }
 
 int sample_args(const nhip_sample_desc* d) {
   if (!d) return fail(NHIP_STATUS_NULL_POINTER, "sample: null descriptor");
   if (!elem_size(d->dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "sample: dtype has to be F32, F16 or BF16");
   if (d->rows < 0 || d->vocab <= 0) return fail(NHIP_STATUS_INVALID_SHAPE, "sample: a row holds at least one logit");
-  if (d->vocab > 1 << 30) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "sample: at most 2^30 logits to a row");
+  if (d->vocab > 1 << 30 || d->rows > 1 << 24) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "sample: at most 2^24 rows of 2^30 logits");
   if (d->row_stride < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "sample: negative stride");
   // (values that a tensor holds for each row are read on the device, where these mean the same as the nearest that is allowed)
   if (!(d->temperature >= 0.f) || d->top_k < 0 || !(d->top_p >= 0.f) || !(d->min_p >= 0.f) || d->min_p > 1.f)
@@ -633,22 +898,26 @@ extern "C" {
 int nhip_sample_workspace_size(const nhip_sample_desc* desc, uint64_t* bytes) {
   if (!bytes) return fail(NHIP_STATUS_NULL_POINTER, "sample: null pointer");
   NHIP_TRY(sample_args(desc));
-  *bytes = 0;
+  *bytes = workspace_of(desc);
   return ok();
 }
 
 int nhip_sample_forward(const nhip_sample_desc* desc, const void* logits, const float* uniform, int32_t* token,
                         float* logprob, void* workspace, uint64_t workspace_bytes, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   NHIP_TRY(sample_args(desc));
   if (desc->rows == 0) return ok();
   if (!logits || !uniform || !token || !logprob) return fail(NHIP_STATUS_NULL_POINTER, "sample: null pointer");
   if (!aligned_to(logits, elem_size(desc->dtype)) || !aligned_to(uniform, 4) || !aligned_to(token, 4) || !aligned_to(logprob, 4))
     return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "sample: a tensor is not aligned to its type");
+  const uint64_t need = workspace_of(desc);
+  if (need && !workspace) return fail(NHIP_STATUS_NULL_POINTER, "sample: null workspace");
+  if (need && (workspace_bytes < need || !aligned_to(workspace, 16)))
+    return fail(NHIP_STATUS_OUTPUT_CAPACITY_INSUFFICIENT, "sample: workspace too small or not 16-byte aligned");
+  RowParts* parts = (RowParts*)workspace;
   const SampleArgs a{logits,           desc->row_stride,       desc->vocab,      uniform,          desc->temperature,
                      desc->top_p,      desc->min_p,            desc->top_k,      desc->temperature_each,
-                     desc->top_k_each, desc->top_p_each,       desc->min_p_each, token,            logprob};
+                     desc->top_k_each, desc->top_p_each,       desc->min_p_each, token,            logprob,
+                     chunks_of(desc),  (uint2*)(parts + desc->rows), parts};
   return NHIP_FOR_ELEM(desc->dtype, T, sample_run<T>(a, desc->rows, as_stream(stream)));
 }
 
