@@ -17,7 +17,8 @@ namespace nhip {
 namespace {
 
 constexpr int kBins = 1024;    // of weights' exponents, or of keys, or of indices
-constexpr int kSorted = 1024;  // tokens that are sorted
+constexpr int kSorted = 1024;  // tokens that are sorted at most
+constexpr int kOnce = 128;     // and for all filters at once, rather than about each one's border
 constexpr float kRange = 31.5f;  // exp(-31.5) < 2^-45, which rounds to 0
 
 // What the launches before the last one leave of a row.
@@ -81,27 +82,31 @@ struct Weights {
   }
 };
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-  return (uint64_t)__shfl_xor((uint32_t)(v >> 32), o) << 32 | __shfl_xor((uint32_t)v, o);
+// Sums of the lanes up to each, by moves inside the vector unit: within rows of 16
+// lanes, then the rows' last lanes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += shfl_xor64(v, o);
-  return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+  return (uint64_t)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | moved<CTRL, ROWS>((uint32_t)v);
 }
-// Sum of the lanes up to this one.
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t u = (uint64_t)__shfl_up((uint32_t)(v >> 32), o) << 32 | __shfl_up((uint32_t)v, o);
-    if (lane >= o) v += u;
-  }
+template <class N>
+__device__ __forceinline__ N wave_scan(N v) {
+  v += moved<0x111, 0xf>(v);  // from 1, 2, 4, 8 lanes before
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);  // the last lane of the row before, to rows 1 and 3
+  v += moved<0x143, 0xc>(v);  // lane 31, to rows 2 and 3
   return v;
 }
 __device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
          (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return lane64(wave_scan(v), 63); }
 
 __device__ __forceinline__ void add_to(uint64_t& bin, uint64_t m) { atomicAdd((unsigned long long*)&bin, (unsigned long long)m); }
 __device__ __forceinline__ void count_in(uint64_t& bin) { atomicAdd((uint32_t*)&bin, 1u); }  // below 2^32 of them
@@ -148,6 +153,41 @@ struct Row {
         if (c + u * 64 < end)
 #pragma unroll
           for (int j = 0; j < V; ++j) f(fmaxf((float)v[u][j], -INFINITY), first(c + u * 64) + j);
+    }
+  }
+  // The wave's tokens that reach `least` (of value `last` up to index `last_index`)
+  // behind each other: `reserve` gives the wave room for so many, put(place, value,
+  // index) takes them.  One reservation for U vectors of every lane.
+  template <class R, class F>
+  __device__ __forceinline__ void each_from(int lane, float least, float last, int last_index, R reserve, F put) const {
+    constexpr int U = 8;
+    for (int c = begin + lane; c - lane < end; c += 64 * U) {
+      VT v[U];
+      uint32_t on[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c + u * 64 < end) v[u] = load(c + u * 64);
+      int mine = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        on[u] = 0;
+        if (c + u * 64 < end) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float l = (float)v[u][j];
+            on[u] |= l >= least && (l != last || first(c + u * 64) + j <= last_index) ? 1u << j : 0;  // (no NaN)
+          }
+        }
+        mine += __popc(on[u]);
+      }
+      if (!__any(mine)) continue;
+      const int upto = (int)wave_scan((uint32_t)mine);
+      int at = reserve(__builtin_amdgcn_readlane(upto, 63)) + upto - mine;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (on[u] >> j & 1) put(at++, (float)v[u][j], first(c + u * 64) + j);
     }
   }
   // Weights of a vector's tokens and their sum: vector `lane` of set `set` of 64.
@@ -274,7 +314,7 @@ __device__ __forceinline__ uint64_t scan_bins(SampleLds<WAVES>& s, int lane, int
   uint64_t v[EACH], sum = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) v[i] = sum += s.bins[threadIdx.x * EACH + i];
-  const uint64_t upto = wave_scan(sum, lane);
+  const uint64_t upto = wave_scan(sum);
   if (lane == 63) s.part[wave] = upto;
   __syncthreads();
   uint64_t before = upto - sum, all = 0;
@@ -491,7 +531,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
 #pragma unroll
           for (int j = 0; j < Row<T>::V; ++j) n += (float)v[j] == value;
         }
-        const int upto = (int)wave_scan((uint64_t)n, lane);
+        const int upto = (int)wave_scan((uint32_t)n);
         if (upto >= left && upto - n < left) {
           int need = left - (upto - n);
 #pragma unroll
@@ -545,12 +585,18 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
   int n = 0;
   const auto collect = [&](float least) {
     zero_bins();
-    row.each(lane, [&](float l, int index) {
-      if (l >= least && inside(l, index)) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < kList) s.list[at] = place_of(key_of(l), index);
-      }
-    });
+    // (tokens that weigh nothing are left out, to a margin)
+    const float far = 2.f * (d.half_top - d.reach - 1e-6f * (fabsf(d.half_top) + d.reach));
+    row.each_from(
+        lane, fmaxf(fmaxf(least, last), fmaxf(far, -3.4028235e38f)), last, last_index,
+        [&](int m) {
+          int at = 0;
+          if (lane == 0) at = atomicAdd(&s.count, m);
+          return __builtin_amdgcn_readfirstlane(at);
+        },
+        [&](int at, float l, int index) {
+          if (at < kList) s.list[at] = place_of(key_of(l), index);
+        });
     __syncthreads();
     n = s.count;
     return n <= kList;
@@ -572,7 +618,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
 #pragma unroll 1
   for (int by = 0; by < 2; ++by) {  // top-k by count, then top-p by weight
     if (by == 0 ? k == a.vocab : !(c.top_p < 1.f)) continue;
-    if (listed && n <= kSorted) break;  // all in one go, below
+    if (listed && n <= kOnce) break;  // all in one go, below
     const auto measure = [&](float l) { return by ? weight(l) : (uint64_t)1; };
     float scope = d.reach;
     double limit;
@@ -635,7 +681,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
       }
       __syncthreads();
       for (int i = threadIdx.x; i < kBins; i += TH)
-        if ((double)(before + s.bins[i]) >= limit && s.bins[i]) atomicMin(&s.at, i);
+        if ((double)(before + s.bins[i]) >= limit && !(i && (double)(before + s.bins[i - 1]) >= limit)) s.at = i;
       __syncthreads();
       const int at = s.at;
       before += at ? s.bins[at - 1] : 0;
@@ -646,7 +692,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
         if (!listed) {
           const float under = d.half_top - (float)(bin + 1) / rate;
           listed = collect(bin == kBins - 1 ? -INFINITY : 2.f * (under - 1e-6f * (fabsf(d.half_top) + scope)));
-          if (listed && n <= kSorted) break;
+          if (listed && n <= kOnce) break;
         }
       } else {  // bins of keys: the largest first
         const uint32_t width = 1u << shift;
@@ -729,10 +775,10 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
       __syncthreads();
       scan_bins(s, lane, wave);
     }
-    if (listed && n <= kSorted) break;
+    if (listed && n <= kOnce) break;
   }
 
-  if (listed && n <= kSorted) {
+  if (listed && n <= kOnce) {
     // ------------------------- all that may be kept, sorted: every filter at once
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += TH) s.sorted[i] = inside_place(s.list[i]) ? s.list[i] : 0;
@@ -822,7 +868,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     for (int set = at << set_shift; set < min(sets, (at + 1) << set_shift); ++set) {
       uint64_t w[Row<T>::V];
       typename Row<T>::VT v;
-      const uint64_t sum = row.set_sum(set, lane, w, v, drawn), upto = wave_scan(sum, lane), all = lane64(upto, 63);
+      const uint64_t sum = row.set_sum(set, lane, w, v, drawn), upto = wave_scan(sum), all = lane64(upto, 63);
       if (target < begin + all) {
         uint64_t from = begin + upto - sum;
         if (target >= from && target < from + sum) {
