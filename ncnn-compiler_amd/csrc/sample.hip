@@ -155,39 +155,41 @@ struct Row {
           for (int j = 0; j < V; ++j) f(fmaxf((float)v[u][j], -INFINITY), first(c + u * 64) + j);
     }
   }
-  // The wave's tokens that reach `least` (of value `last` up to index `last_index`)
-  // behind each other: `reserve` gives the wave room for so many, put(place, value,
-  // index) takes them.  One reservation for U vectors of every lane.
+  // The indices of the wave's tokens that reach `least` (of value `last` up to index
+  // `last_index`): `reserve` gives the wave room for so many, put(place, index)
+  // takes them.  One reservation for U vectors of every lane; a lane goes through
+  // the bits that it has set, so that the few cost little (with the values at hand
+  // every place was a branch of its own: 64 x 131072 bf16 70 us, so XX).
   template <class R, class F>
   __device__ __forceinline__ void each_from(int lane, float least, float last, int last_index, R reserve, F put) const {
     constexpr int U = 8;
     for (int c = begin + lane; c - lane < end; c += 64 * U) {
       VT v[U];
-      uint32_t on[U];
+      uint64_t on = 0;  // bit u V + j
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (c + u * 64 < end) v[u] = load(c + u * 64);
-      int mine = 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        on[u] = 0;
+      for (int u = 0; u < U; ++u)
         if (c + u * 64 < end) {
+          uint32_t bits = 0;
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float l = (float)v[u][j];
-            on[u] |= l >= least && (l != last || first(c + u * 64) + j <= last_index) ? 1u << j : 0;  // (no NaN)
+          for (int j = 0; j < V; ++j) bits |= (float)v[u][j] >= least ? 1u << j : 0;  // (no NaN)
+          if (least == last && bits) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+              if ((float)v[u][j] == last && first(c + u * 64) + j > last_index) bits &= ~(1u << j);
           }
+          on |= (uint64_t)bits << (u * V);
         }
-        mine += __popc(on[u]);
-      }
+      const int mine = __popcll(on);
       if (!__any(mine)) continue;
       const int upto = (int)wave_scan((uint32_t)mine);
       int at = reserve(__builtin_amdgcn_readlane(upto, 63)) + upto - mine;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (on[u] >> j & 1) put(at++, (float)v[u][j], first(c + u * 64) + j);
+      for (; on; on &= on - 1) {
+        const int bit = __builtin_ctzll(on);
+        put(at++, first(c + bit / V * 64) + bit % V);
+      }
     }
   }
   // Weights of a vector's tokens and their sum: vector `lane` of set `set` of 64.
@@ -304,6 +306,17 @@ __device__ __forceinline__ void sort_list(uint64_t* list, int n) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   __syncthreads();
+}
+
+// A place to a lane: the sum of the weights of those of `n` lanes that lie before
+// it in the order.
+__device__ __forceinline__ uint64_t before_me(uint64_t place, uint64_t w, int n) {
+  uint64_t sum = 0;
+  for (int j = 0; j < n; ++j) {
+    const uint64_t q = lane64(place, j), add = lane64(w, j);
+    sum += q > place ? add : 0;
+  }
+  return sum;
 }
 
 // The sum over the bins (or any kBins numbers) up to each, in place; returns the
@@ -594,9 +607,12 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
           if (lane == 0) at = atomicAdd(&s.count, m);
           return __builtin_amdgcn_readfirstlane(at);
         },
-        [&](int at, float l, int index) {
-          if (at < kList) s.list[at] = place_of(key_of(l), index);
+        [&](int at, int index) {
+          if (at < kList) s.list[at] = (uint32_t)index;
         });
+    __syncthreads();
+    if (s.count <= kList)
+      for (int i = threadIdx.x; i < s.count; i += TH) s.list[i] = place_of(key_of((float)row.from[(int64_t)s.list[i] + row.shift]), (int)s.list[i]);
     __syncthreads();
     n = s.count;
     return n <= kList;
@@ -729,6 +745,22 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
       if (lane == 0) s.part[wave] = (uint64_t)most << 32 | least;
       __syncthreads();
       const int count = s.count;
+      if (count <= 64) {
+        if (wave == 0) {
+          const uint64_t place = lane < count ? s.sorted[lane] : 0;
+          const uint64_t m = lane < count ? measure(of_key((uint32_t)(place >> 32))) : 0;
+          const uint64_t ahead = before_me(place, m, count);
+          // the last of those that stay: nobody that stays is behind it
+          const bool stays = lane < count && ((double)(before + ahead) < limit || ahead == 0);
+          const uint64_t behind = before_me(stays ? ~place : ~uint64_t(0), stays ? 1 : 0, count);
+          if (stays && behind == 0) s.part[0] = place;
+        }
+        __syncthreads();
+        last = of_key((uint32_t)(s.part[0] >> 32));
+        last_index = (int)~(uint32_t)s.part[0];
+        __syncthreads();
+        break;
+      }
       if (count <= kSorted) {
         sort_list<WAVES>(s.sorted, count);
         sum_sorted(count, [&](uint64_t place) { return measure(of_key((uint32_t)(place >> 32))); });
@@ -831,6 +863,15 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
       }
     __syncthreads();
     const int m = s.count;
+    if (m <= 64) {
+      if (wave == 0) {
+        const uint64_t place = lane < m ? s.sorted[lane] : 0, w = lane < m ? weight(of_key((uint32_t)place)) : 0;
+        const uint64_t from = before_me(place, w, m), rest = target - begin;
+        if (lane < m && rest >= from && rest < from + w) found((int)~(uint32_t)(place >> 32), of_key((uint32_t)place), total);
+      }
+      finish();
+      return;
+    }
     if (m <= kSorted) {
       sort_list<WAVES>(s.sorted, m);
       sum_sorted(m, [&](uint64_t place) { return weight(of_key((uint32_t)place)); });
