@@ -268,7 +268,7 @@ __device__ __forceinline__ float wave_max(float v) {
 
 template <int WAVES>
 struct SampleLds {
-  static constexpr int kList = WAVES > 4 ? 12288 : 4096;  // tokens that LDS holds
+  static constexpr int kList = WAVES > 4 ? 16384 : 4096;  // tokens that LDS holds
   uint64_t list[kList];
   uint64_t sorted[kSorted];
   uint64_t bins[kBins];
@@ -611,8 +611,19 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
           if (at < kList) s.list[at] = (uint32_t)index;
         });
     __syncthreads();
-    if (s.count <= kList)
-      for (int i = threadIdx.x; i < s.count; i += TH) s.list[i] = place_of(key_of((float)row.from[(int64_t)s.list[i] + row.shift]), (int)s.list[i]);
+    if (s.count <= kList)  // the values, four of a thread on their way at a time
+      for (int i0 = threadIdx.x; i0 < s.count; i0 += 4 * TH) {
+        int index[4];
+        float l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          index[e] = i0 + e * TH < s.count ? (int)s.list[i0 + e * TH] : 0;  // (others' entries may be places already)
+          l[e] = (float)row.from[(int64_t)index[e] + row.shift];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i0 + e * TH < s.count) s.list[i0 + e * TH] = place_of(key_of(l[e]), index[e]);
+      }
     __syncthreads();
     n = s.count;
     return n <= kList;
@@ -750,10 +761,13 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
           const uint64_t place = lane < count ? s.sorted[lane] : 0;
           const uint64_t m = lane < count ? measure(of_key((uint32_t)(place >> 32))) : 0;
           const uint64_t ahead = before_me(place, m, count);
-          // the last of those that stay: nobody that stays is behind it
-          const bool stays = lane < count && ((double)(before + ahead) < limit || ahead == 0);
-          const uint64_t behind = before_me(stays ? ~place : ~uint64_t(0), stays ? 1 : 0, count);
-          if (stays && behind == 0) s.part[0] = place;
+          // the last of those that stay has the most before it
+          const bool stays = m && (double)(before + ahead) < limit;
+          if (lane == 0) s.total = 0;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          if (stays) atomicMax((unsigned long long*)&s.total, (unsigned long long)ahead + 1);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          if (stays && ahead + 1 == *(volatile uint64_t*)&s.total) s.part[0] = place;
         }
         __syncthreads();
         last = of_key((uint32_t)(s.part[0] >> 32));
