@@ -442,15 +442,13 @@ struct RowsTile {
 // 5.2); over the cache 16 of 12544 keys 71 us (316 MB, 4.4 TB/s, 5 us of it the
 // launch that joins the parts).
 template <class T, int DP, int SRC>
-__global__ __launch_bounds__(kWaves * 64, rows_per_cu(sizeof(T), DP, SRC)) void attn_rows_kernel(AttnArgs a) {
+__device__ __forceinline__ void rows_body(const AttnArgs& a, uint32_t at, char* lds) {
   typedef typename Second<T, SRC>::type P;
   typedef typename Frag<T>::type FT;
   typedef typename Frag<P>::type FP;
   typedef RowsTile<T, DP, SRC> Tile;
   constexpr int KS = DP / 32, DT = DP / 16, STRIDE = DP + kPad16<P>, STEP = kWaves * kKeyTile;
-  extern __shared__ char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id(), g = lane >> 4, col = lane & 15;
-  uint32_t at = blockIdx.x;
   const int rt = at % a.row_tiles;
   at /= a.row_tiles;
   const int split = at % a.splits;
@@ -611,6 +609,12 @@ __global__ __launch_bounds__(kWaves * 64, rows_per_cu(sizeof(T), DP, SRC)) void 
   }
 }
 
+template <class T, int DP, int SRC>
+__global__ __launch_bounds__(kWaves * 64, rows_per_cu(sizeof(T), DP, SRC)) void attn_rows_kernel(AttnArgs a) {
+  extern __shared__ char lds[];
+  rows_body<T, DP, SRC>(a, blockIdx.x, lds);
+}
+
 // Joins parts of one row's result for V of its channels: part i's maximum and
 // sum at ml(i), its sums at o(i).
 template <class T, int V, class ML, class O>
@@ -741,10 +745,42 @@ __global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs prefix, 
       (T*)a.o + (((int64_t)b * a.queries + row / a.group) * a.heads + kvh * a.group + row % a.group) * a.d + c);
 }
 
+// Both parts in one launch: the sequences' own keys, few rows each, and then the
+// prefix.
+template <class T, int DP, bool TILES>
+__global__ __launch_bounds__(kWaves * 64, (TILES ? TilesShape<T, DP, kSrcInt8>::per_cu : rows_per_cu(sizeof(T), DP, kSrcInt8))) void
+attn_prefix_kernel(AttnArgs prefix, AttnArgs own, uint32_t own_wgs) {
+  extern __shared__ char lds[];
+  if (blockIdx.x < own_wgs)
+    rows_body<T, DP, kSrcInt8>(own, blockIdx.x, lds);
+  else if constexpr (TILES)
+    tiles_body<T, DP, kSrcInt8>(prefix, blockIdx.x - own_wgs, gridDim.x - own_wgs, lds);
+  else
+    rows_body<T, DP, kSrcInt8>(prefix, blockIdx.x - own_wgs, lds);
+}
+
+template <class T, int DP, bool TILES>
+int prefix_launch(const AttnArgs& prefix, const AttnArgs& own, hipStream_t s) {
+  constexpr int rows = rows_lds<T, DP, kSrcInt8>(), tiles = TilesShape<T, DP, kSrcInt8>::bytes;
+  constexpr int bytes = TILES && tiles > rows ? tiles : rows;
+  if (bytes > 65536) NHIP_TRY(ensure_dynamic_lds((const void*)attn_prefix_kernel<T, DP, TILES>, bytes));
+  const int64_t own_wgs = (int64_t)own.batch * own.kv_heads * own.splits * own.row_tiles;
+  const int64_t wgs = TILES ? ceil_div(prefix.workers, 8) * 8 : (int64_t)prefix.batch * prefix.kv_heads * prefix.splits * prefix.row_tiles;
+  NHIP_LAUNCH("attention_prefix", (attn_prefix_kernel<T, DP, TILES>), dim3((uint32_t)(own_wgs + wgs)), dim3(kWaves * 64), bytes, s,
+              prefix, own, (uint32_t)own_wgs);
+  return check_launch("attention_prefix");
+}
+
+template <class T, int DP>
+int prefix_parts(const AttnArgs& prefix, const AttnArgs& own, hipStream_t s) {
+  if (!own.tiles) return prefix.tiles ? prefix_launch<T, DP, true>(prefix, own, s) : prefix_launch<T, DP, false>(prefix, own, s);
+  NHIP_TRY((launch<T, DP, kSrcInt8>(prefix, s)));
+  return launch<T, DP, kSrcInt8>(own, s);
+}
+
 template <class T>
 int run_prefix(const AttnArgs& prefix, const AttnArgs& a, hipStream_t s) {
-  NHIP_TRY((launch_by_dim<T, kSrcInt8>(prefix, s)));
-  NHIP_TRY((launch_by_dim<T, kSrcInt8>(a, s)));
+  NHIP_TRY(a.d <= 64 ? (prefix_parts<T, 64>(prefix, a, s)) : a.d <= 128 ? (prefix_parts<T, 128>(prefix, a, s)) : (prefix_parts<T, 256>(prefix, a, s)));
   const int64_t items = (int64_t)a.batch * a.kv_heads * a.rows * (a.d / 4);
   NHIP_LAUNCH("attention_prefix_join", (attn_prefix_join_kernel<T>), dim3((uint32_t)ceil_div(items, 256)), dim3(256), 0, s, prefix, a);
   return check_launch("attention_prefix_join");

@@ -10,8 +10,8 @@ namespace {
 
 // Checks the sizes and fills them in, chooses the kernel (vec: rows that the
 // one for many rows takes; cache: over the 8-bit cache) and the number of parts
-// of the keys.
-int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
+// of the keys.  choice: 0 few rows, 1 many, -1 by the rule here.
+int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a, int choice = -1) {
   if (!d) return fail(NHIP_STATUS_NULL_POINTER, "attention: null descriptor");
   if (!elem_size(d->dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "attention: dtype has to be F32, F16 or BF16");
   if (d->batch < 0 || d->queries < 0 || d->keys < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative extent");
@@ -55,7 +55,7 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a) {
   const double few = (double)kv_heads * tiles16 / cu_count();  // workgroups of the first to a CU
   const bool full = cache ? few >= (f32 ? 3 : 4) : d->head_dim > 64 ? few >= 1.5 : f32 ? few > 2 : few >= 3;
   const double again = cache ? (f32 ? 28e6 : 90e6) : f32 ? 215e6 : 64e6;  // bytes
-  a->tiles = vec && force != 0 && (force == 1 || full || (few >= 0.25 && (tiles16 - 1) * bytes > again));
+  a->tiles = choice >= 0 ? choice : vec && force != 0 && (force == 1 || full || (few >= 0.25 && (tiles16 - 1) * bytes > again));
   const int tile = a->tiles ? attn::kTilesRows : attn::kRowTile;
   a->row_tiles = (int)ceil_div(std::max(a->rows, 1), tile);
   const int64_t heads = (int64_t)d->batch * d->kv_heads;
@@ -158,10 +158,24 @@ int attn_forward(AttnArgs& a, const nhip_attention_desc* d, int src, const void*
   }
 }
 
+// Which kernel the parts of a prefix or of the own keys take, both being joined by
+// a launch in any case: few rows read the keys again for every 16 rows (6.5 TB/s
+// from the L2s), many rows compute 128 rows whatever there are (560 TFLOP/s; fp32
+// is some 3 times as slow with either).  us, few / many: 48 sequences of 28 rows to
+// 1568 keys, 8 heads of 128 fp16 48.6 / 72.5; 4 of 64 rows to 3136 bf16 27.7 / 24.4;
+// 1 of 1344 rows to 12544 fp16 322 / 117.
+int prefix_choice(const nhip_attention_desc& d) {
+  const int force = setting_int("NHIP_ATTN_TILES", -1);
+  if (force >= 0) return force != 0;
+  const double keys = (double)d.batch * d.kv_heads * d.keys * d.head_dim, rows = (double)d.queries * (d.heads / d.kv_heads);
+  return std::ceil(rows / 16) * keys * 2 / 6.5e6 > std::ceil(rows / attn::kTilesRows) * keys * 4 * attn::kTilesRows / 560e6;
+}
+
 // A prefix that `groups` groups of sequences share, and the sequences' own keys:
 // the descriptors of both.
 int prefix_args(const nhip_attention_desc* d, int32_t groups, int32_t prefix_keys, AttnArgs* prefix, AttnArgs* own) {
   NHIP_TRY(attn_args(d, true, true, own));
+  NHIP_TRY(attn_args(d, true, true, own, prefix_choice(*d)));
   if (groups <= 0 || d->batch % groups) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: groups have to divide the batch");
   if (prefix_keys < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative extent");
   nhip_attention_desc shared = *d;
@@ -170,7 +184,7 @@ int prefix_args(const nhip_attention_desc* d, int32_t groups, int32_t prefix_key
   shared.batch = groups;
   shared.queries = (int32_t)(members * d->queries);
   shared.keys = prefix_keys;
-  NHIP_TRY(attn_args(&shared, true, true, prefix));
+  NHIP_TRY(attn_args(&shared, true, true, prefix, prefix_choice(shared)));
   prefix->parts = own->parts = 1;
   prefix->per = d->queries;
   return ok();

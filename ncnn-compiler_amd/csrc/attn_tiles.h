@@ -186,17 +186,16 @@ __device__ __forceinline__ int worker_of(const AttnArgs& a, uint32_t unit) {
 // TFLOP/s; the fp32 instructions' rate is 154), some 1000 vector instructions
 // of a wave, most of them splitting, beside 96 products a tile.
 template <class T, int DP, int SRC>
-__global__ __launch_bounds__(kWaves * 64, (TilesShape<T, DP, SRC>::per_cu)) void attn_tiles_kernel(AttnArgs a) {
+__device__ __forceinline__ void tiles_body(const AttnArgs& a, uint32_t block, uint32_t blocks, char* lds) {
   typedef TilesShape<T, DP, SRC> S;
   typedef typename S::M M;
   typedef typename Frag<M>::type FM;
   constexpr int KT = S::KT, NT = KT / 32, KS = DP / 16, DT = DP / 32, KP = S::KP, QP = S::QP;
   constexpr int AHEAD = S::split ? 1 : KS < 8 ? KS : 8;  // operands read ahead of their products
-  extern __shared__ char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id(), h = lane >> 5, col = lane & 31;
   // workgroups go to the eight dies in turn: each die gets a run of workers, so
   // that those of one head meet in its L2
-  const uint32_t worker = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const uint32_t worker = (block & 7) * (blocks >> 3) + (block >> 3);
   if (worker >= (uint32_t)a.workers) return;
   const bool dealt = a.workers != a.batch * a.kv_heads * a.row_tiles;
   uint32_t unit = dealt ? first_unit(a, worker) : 0, unit_end = dealt ? first_unit(a, worker + 1) : (uint32_t)a.units;
@@ -516,6 +515,12 @@ __global__ __launch_bounds__(kWaves * 64, (TilesShape<T, DP, SRC>::per_cu)) void
         }
     }
   }
+}
+
+template <class T, int DP, int SRC>
+__global__ __launch_bounds__(kWaves * 64, (TilesShape<T, DP, SRC>::per_cu)) void attn_tiles_kernel(AttnArgs a) {
+  extern __shared__ char lds[];
+  tiles_body<T, DP, SRC>(a, blockIdx.x, gridDim.x, lds);
 }
 
 // Joins the parts of the row tiles that several workers share.
