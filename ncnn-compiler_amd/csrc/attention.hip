@@ -168,7 +168,7 @@ int prefix_choice(const nhip_attention_desc& d) {
   const int force = setting_int("NHIP_ATTN_TILES", -1);
   if (force >= 0) return force != 0;
   const double keys = (double)d.batch * d.kv_heads * d.keys * d.head_dim, rows = (double)d.queries * (d.heads / d.kv_heads);
-  return std::ceil(rows / 16) * keys * 2 / 6.5e6 > std::ceil(rows / attn::kTilesRows) * keys * 4 * attn::kTilesRows / 560e6;
+  return std::ceil(rows / 16) * keys * 2 / 6.5e6 > 1.5 * std::ceil(rows / attn::kTilesRows) * keys * 4 * attn::kTilesRows / 560e6;
 }
 
 // A prefix that `groups` groups of sequences share, and the sequences' own keys:
