@@ -30,6 +30,7 @@ struct AttnArgs {
   int32_t rows;       // queries * group
   int32_t tiles;      // the kernel of many rows
   int32_t row_tiles;  // row tiles of a key/value head
+  int32_t reps;       // few rows: times 16 rows of a workgroup (2 only of own keys behind a prefix)
   int32_t splits;     // few rows: parts of a sequence's keys
   int32_t workers;    // many rows: workgroups
   int32_t units;      // and the parts of a row tile's keys that are dealt to them
@@ -433,6 +434,38 @@ struct RowsTile {
   }
 };
 
+// Row `in` of the waves' 16, row orow of the key/value head's.
+template <class T, int OS>
+__device__ __forceinline__ void join_waves(const AttnArgs& a, const float* mo, const float2* ml, int in, int orow, int b, int kvh,
+                                           int split, int lane) {
+      if (orow >= a.rows) return;
+      float top = -INFINITY, total = 0.f, w[kWaves];
+      bool nan = false;
+  #pragma unroll
+      for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ml[i * kRowTile + in].x);
+  #pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        const float2 t = ml[i * kRowTile + in];
+        nan |= t.y < 0.f;
+        w[i] = t.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t.x - top);
+        total += t.x == -INFINITY ? 0.f : w[i] * t.y;
+      }
+      const bool none = top == -INFINITY;
+      const int oq = orow / a.group, oh = kvh * a.group + orow % a.group;
+      const int64_t prow = (((int64_t)b * a.kv_heads + kvh) * a.rows + orow) * a.splits + split;
+      for (int c = lane; c < a.d; c += 64) {
+        float o = 0.f;
+  #pragma unroll
+        for (int i = 0; i < kWaves; ++i)
+          if (w[i] != 0.f) o += w[i] * mo[(i * kRowTile + in) * OS + c];
+        if (a.splits > 1 || a.parts)
+          a.part_o[prow * a.d + c] = o;
+        else
+          ((T*)a.o)[(((int64_t)b * a.queries + oq) * a.heads + oh) * a.d + c] = (T)(none ? (nan ? NAN : 0.f) : o / total);
+      }
+      if ((a.splits > 1 || a.parts) && lane == 0) a.part_ml[prow] = make_float2(top, none ? (nan ? -1.f : 0.f) : total);
+}
+
 // One workgroup: 16 query rows of one key/value head over one part of the
 // keys, its four waves every fourth tile of 32 keys, joined at the end.  Keys
 // go from memory to the registers that the products read, values through the
@@ -441,13 +474,14 @@ struct RowsTile {
 // keys, 8 heads of 128 bf16 67 us a call (326 MB, 4.9 TB/s, a large copy's rate
 // 5.2); over the cache 16 of 12544 keys 71 us (316 MB, 4.4 TB/s, 5 us of it the
 // launch that joins the parts).
-template <class T, int DP, int SRC>
+// R: times 16 rows, which share what is read and converted of the keys.
+template <class T, int DP, int SRC, int R = 1>
 __device__ __forceinline__ void rows_body(const AttnArgs& a, uint32_t at, char* lds) {
   typedef typename Second<T, SRC>::type P;
   typedef typename Frag<T>::type FT;
   typedef typename Frag<P>::type FP;
   typedef RowsTile<T, DP, SRC> Tile;
-  constexpr int KS = DP / 32, DT = DP / 16, STRIDE = DP + kPad16<P>, STEP = kWaves * kKeyTile;
+  constexpr int KS = DP / 32, DT = DP / 16, STRIDE = DP + kPad16<P>, STEP = kWaves * kKeyTile, ROWS = kRowTile * R;
   const int lane = threadIdx.x & 63, wave = wave_id(), g = lane >> 4, col = lane & 15;
   const int rt = at % a.row_tiles;
   at /= a.row_tiles;
@@ -456,30 +490,38 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint32_t at, char* 
   const int kvh = at % a.kv_heads, b = at / a.kv_heads;
 
   const int length = a.lengths ? max(0, min(a.lengths[b], a.keys)) : a.keys;
-  const int row = rt * kRowTile + col;  // the lane's row
-  const int qi = row / a.group, head = kvh * a.group + row % a.group;
-  // keys that the lane's row sees, and that any row of the tile does
-  int sees = length, all_see = length, visible = length, begin, end;
+  // keys that the lane's rows see, and that any row of the tile does
+  int sees[R], all_see = length, visible = length, begin, end;
+  FT qf[R][KS];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = rt * ROWS + r * kRowTile + col;  // the lane's row
+    const int qi = row / a.group, head = kvh * a.group + row % a.group;
+    sees[r] = a.causal ? max(0, length - a.queries + 1 + qi) : length;
+    const T* qrow = (const T*)a.q + b * a.qs[0] + query_at(a, qi) + head * a.qs[2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      qf[r][s] = row < a.rows ? load_q<T, SRC != kSrcAny>(qrow, Tile::q_channel(s, g), a.d) : zero_frag<T>();
+  }
   if (a.causal) {
-    const int last = min(rt * kRowTile + kRowTile - 1, a.rows - 1) / a.group;
-    sees = max(0, length - a.queries + 1 + qi);
-    all_see = max(0, length - a.queries + 1 + rt * kRowTile / a.group);
+    const int last = min(rt * ROWS + ROWS - 1, a.rows - 1) / a.group;
+    all_see = max(0, length - a.queries + 1 + rt * ROWS / a.group);
     visible = max(0, min(length, length - a.queries + 1 + last));
   }
   part_of(a, length, visible, split, STEP, begin, end);
 
-  FT qf[KS];
-  const T* qrow = (const T*)a.q + b * a.qs[0] + query_at(a, qi) + head * a.qs[2];
-#pragma unroll
-  for (int s = 0; s < KS; ++s)
-    qf[s] = row < a.rows ? load_q<T, SRC != kSrcAny>(qrow, Tile::q_channel(s, g), a.d) : zero_frag<T>();
-
   P* vt = reinterpret_cast<P*>(lds) + wave * kKeyTile * STRIDE;
-  v4f acc[DT];
+  v4f acc[R][DT];
+  float m[R], l[R];
+  bool seen[R];
 #pragma unroll
-  for (int t = 0; t < DT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-  bool seen = false;
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    seen[r] = false;
+  }
   const T* kbase = (const T*)a.k + b * a.ks[0] + kvh * a.ks[2];
   const T* vbase = (const T*)a.v + b * a.vs[0] + kvh * a.vs[2];
 
@@ -491,62 +533,71 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint32_t at, char* 
     TileAsk ask = ask_tile<SRC, kKeyTile>(a, b, key0 + STEP, lane);
     for (; key0 < end; key0 += STEP) {
       const TileKeys keys = tile.keys;
-      v4f s[2];
+      v4f s[R][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        s[t] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < KS; ++i) s[t] = mma16(tile.k_frag(t, i), qf[i], s[t]);
+        for (int r = 0; r < R; ++r) s[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          const FT kf = tile.k_frag(t, i);
+#pragma unroll
+          for (int r = 0; r < R; ++r) s[r][t] = mma16(kf, qf[r][i], s[r][t]);
+        }
       }
       tile.template store_v<STRIDE>(vt, lane);  // rows that do not count are 0
-      settle(s[0], s[1]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) settle(s[r][0], s[r][1]);
       // the next tile (past the end: nothing counts, nothing is read)
       tile.keys = know_tile<SRC, kKeyTile>(a, ask, kvh, key0 + STEP, end, lane);
       tile.load(a, kbase, vbase, kvh, min(key0 + STEP, a.keys), begin, lane);
       ask = ask_tile<SRC, kKeyTile>(a, b, min(key0 + 2 * STEP, a.keys), lane);
 
-      // scores in units of ln 2 (over the cache with the page's scale)
-      float x[8], top = -INFINITY;
-      float vscale[2];
+      FP pf[R][Second<T, SRC>::parts];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const float c = SRC == kSrcInt8 ? a.scale_log2 * lane_float(keys.kscale, t * 16) : a.scale_log2;
-        vscale[t] = SRC == kSrcInt8 ? lane_float(keys.vscale, t * 16) : 1.f;
+      for (int r = 0; r < R; ++r) {
+        // scores in units of ln 2 (over the cache with the page's scale)
+        float x[8], top = -INFINITY;
+        float vscale[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[t * 4 + j] = s[t][j] * c;
-      }
-      if ((uint32_t)keys.counts == 0xffffffffu && key0 + kKeyTile <= all_see) {  // uniform
-        seen = true;
-      } else {
-        const int n = min(max(sees - key0, 0), kKeyTile);
-        const uint32_t on = (uint32_t)keys.counts & (uint32_t)((1ull << n) - 1), mine = on >> (4 * g);
-        seen |= on != 0;
+        for (int t = 0; t < 2; ++t) {
+          const float c = SRC == kSrcInt8 ? a.scale_log2 * lane_float(keys.kscale, t * 16) : a.scale_log2;
+          vscale[t] = SRC == kSrcInt8 ? lane_float(keys.vscale, t * 16) : 1.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (!(mine >> ((i >> 2) * 16 + (i & 3)) & 1)) x[i] = -INFINITY;
-      }
+          for (int j = 0; j < 4; ++j) x[t * 4 + j] = s[r][t][j] * c;
+        }
+        if ((uint32_t)keys.counts == 0xffffffffu && key0 + kKeyTile <= all_see) {  // uniform
+          seen[r] = true;
+        } else {
+          const int n = min(max(sees[r] - key0, 0), kKeyTile);
+          const uint32_t on = (uint32_t)keys.counts & (uint32_t)((1ull << n) - 1), mine = on >> (4 * g);
+          seen[r] |= on != 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
-      top = max32(max16(top));
-      if (__any(top > m + kRoom<P>)) {
-        const float to = fmaxf(m, top - kBelow<P>);
-        const float keep = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
-        m = to;
-        l *= keep;
+          for (int i = 0; i < 8; ++i)
+            if (!(mine >> ((i >> 2) * 16 + (i & 3)) & 1)) x[i] = -INFINITY;
+        }
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
+        top = max32(max16(top));
+        if (__any(top > m[r] + kRoom<P>)) {
+          const float to = fmaxf(m[r], top - kBelow<P>);
+          const float keep = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - to);
+          m[r] = to;
+          l[r] *= keep;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][i] *= keep;
-      }
-      const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet, or only scores of -infinity
-      FP pf[Second<T, SRC>::parts];
+          for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float p = __builtin_amdgcn_exp2f(x[i] - base);
-        l += p;
-        if constexpr (SRC == kSrcInt8) p *= vscale[i >> 2];
-        pf[0][i] = (P)p;
-        if constexpr (Second<T, SRC>::parts == 2) pf[1][i] = (P)(p - (float)pf[0][i]);
+            for (int i = 0; i < 4; ++i) acc[r][t][i] *= keep;
+        }
+        const float base = m[r] == -INFINITY ? 0.f : m[r];  // nothing seen yet, or only scores of -infinity
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float p = __builtin_amdgcn_exp2f(x[i] - base);
+          l[r] += p;
+          if constexpr (SRC == kSrcInt8) p *= vscale[i >> 2];
+          pf[r][0][i] = (P)p;
+          if constexpr (Second<T, SRC>::parts == 2) pf[r][1][i] = (P)(p - (float)pf[r][0][i]);
+        }
       }
       // the wave's LDS operations are in order; the compiler keeps them so
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -554,58 +605,39 @@ __device__ __forceinline__ void rows_body(const AttnArgs& a, uint32_t at, char* 
       for (int t = 0; t < DT; ++t) {
         const FP vf = load_v16<P, STRIDE>(vt, t * 16, lane);
 #pragma unroll
-        for (int i = 0; i < Second<T, SRC>::parts; ++i) acc[t] = mma16(vf, pf[i], acc[t]);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < Second<T, SRC>::parts; ++i) acc[r][t] = mma16(vf, pf[r][i], acc[r][t]);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 #pragma unroll
-    for (int t = 0; t < DT; ++t) settle(acc[t]);
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int t = 0; t < DT; ++t) settle(acc[r][t]);
   }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  int any = seen;
-  any |= __shfl_xor(any, 16);
-  any |= __shfl_xor(any, 32);
-  if (l != l) m = INFINITY;                        // NaN to whoever joins this
-  else if (m == -INFINITY) l = any ? -1.f : 0.f;  // scores of -infinity alone: 0 / 0, told from a row that sees nothing
 
-  // join the waves
-  __syncthreads();
-  constexpr int OS = DP + 4;
-  float* mo = reinterpret_cast<float*>(lds);                            // [waves][16][OS]
-  float2* ml = reinterpret_cast<float2*>(mo + kWaves * kRowTile * OS);  // [waves][16]
 #pragma unroll
-  for (int t = 0; t < DT; ++t) *reinterpret_cast<v4f*>(mo + (wave * kRowTile + col) * OS + t * 16 + 4 * g) = acc[t];
-  if (g == 0) ml[wave * kRowTile + col] = make_float2(m, l);
-  __syncthreads();
-  for (int r = wave * (kRowTile / kWaves); r < (wave + 1) * (kRowTile / kWaves); ++r) {
-    const int orow = rt * kRowTile + r;
-    if (orow >= a.rows) break;
-    float top = -INFINITY, total = 0.f, w[kWaves];
-    bool nan = false;
+  for (int r = 0; r < R; ++r) {
+    l[r] += __shfl_xor(l[r], 16);
+    l[r] += __shfl_xor(l[r], 32);
+    int any = seen[r];
+    any |= __shfl_xor(any, 16);
+    any |= __shfl_xor(any, 32);
+    if (l[r] != l[r]) m[r] = INFINITY;                     // NaN to whoever joins this
+    else if (m[r] == -INFINITY) l[r] = any ? -1.f : 0.f;  // scores of -infinity alone: 0 / 0, told from a row that sees nothing
+
+    // join the waves
+    __syncthreads();
+    constexpr int OS = DP + 4;
+    float* mo = reinterpret_cast<float*>(lds);                            // [waves][16][OS]
+    float2* ml = reinterpret_cast<float2*>(mo + kWaves * kRowTile * OS);  // [waves][16]
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ml[i * kRowTile + r].x);
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const float2 t = ml[i * kRowTile + r];
-      nan |= t.y < 0.f;
-      w[i] = t.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t.x - top);
-      total += t.x == -INFINITY ? 0.f : w[i] * t.y;
-    }
-    const bool none = top == -INFINITY;
-    const int oq = orow / a.group, oh = kvh * a.group + orow % a.group;
-    const int64_t prow = (((int64_t)b * a.kv_heads + kvh) * a.rows + orow) * a.splits + split;
-    for (int c = lane; c < a.d; c += 64) {
-      float o = 0.f;
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i)
-        if (w[i] != 0.f) o += w[i] * mo[(i * kRowTile + r) * OS + c];
-      if (a.splits > 1 || a.parts)
-        a.part_o[prow * a.d + c] = o;
-      else
-        ((T*)a.o)[(((int64_t)b * a.queries + oq) * a.heads + oh) * a.d + c] = (T)(none ? (nan ? NAN : 0.f) : o / total);
-    }
-    if ((a.splits > 1 || a.parts) && lane == 0) a.part_ml[prow] = make_float2(top, none ? (nan ? -1.f : 0.f) : total);
+    for (int t = 0; t < DT; ++t) *reinterpret_cast<v4f*>(mo + (wave * kRowTile + col) * OS + t * 16 + 4 * g) = acc[r][t];
+    if (g == 0) ml[wave * kRowTile + col] = make_float2(m[r], l[r]);
+    __syncthreads();
+    for (int i = wave * (kRowTile / kWaves); i < (wave + 1) * (kRowTile / kWaves); ++i)
+      join_waves<T, OS>(a, mo, ml, i, rt * ROWS + r * kRowTile + i, b, kvh, split, lane);
   }
 }
 
@@ -747,33 +779,37 @@ __global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs prefix, 
 
 // Both parts in one launch: the sequences' own keys, few rows each, and then the
 // prefix.
-template <class T, int DP, bool TILES>
-__global__ __launch_bounds__(kWaves * 64, (TILES ? TilesShape<T, DP, kSrcInt8>::per_cu : rows_per_cu(sizeof(T), DP, kSrcInt8))) void
+template <class T, int DP, bool TILES, int OWN>
+__global__ __launch_bounds__(kWaves * 64, (TILES ? TilesShape<T, DP, kSrcInt8>::per_cu : rows_per_cu(sizeof(T), DP, kSrcInt8) - (OWN == 2 && DP == 128 && sizeof(T) == 2))) void
 attn_prefix_kernel(AttnArgs prefix, AttnArgs own, uint32_t own_wgs) {
   extern __shared__ char lds[];
   if (blockIdx.x < own_wgs)
-    rows_body<T, DP, kSrcInt8>(own, blockIdx.x, lds);
+    rows_body<T, DP, kSrcInt8, OWN>(own, blockIdx.x, lds);
   else if constexpr (TILES)
     tiles_body<T, DP, kSrcInt8>(prefix, blockIdx.x - own_wgs, gridDim.x - own_wgs, lds);
   else
     rows_body<T, DP, kSrcInt8>(prefix, blockIdx.x - own_wgs, lds);
 }
 
-template <class T, int DP, bool TILES>
+template <class T, int DP, bool TILES, int OWN>
 int prefix_launch(const AttnArgs& prefix, const AttnArgs& own, hipStream_t s) {
   constexpr int rows = rows_lds<T, DP, kSrcInt8>(), tiles = TilesShape<T, DP, kSrcInt8>::bytes;
   constexpr int bytes = TILES && tiles > rows ? tiles : rows;
-  if (bytes > 65536) NHIP_TRY(ensure_dynamic_lds((const void*)attn_prefix_kernel<T, DP, TILES>, bytes));
+  if (bytes > 65536) NHIP_TRY(ensure_dynamic_lds((const void*)attn_prefix_kernel<T, DP, TILES, OWN>, bytes));
   const int64_t own_wgs = (int64_t)own.batch * own.kv_heads * own.splits * own.row_tiles;
   const int64_t wgs = TILES ? ceil_div(prefix.workers, 8) * 8 : (int64_t)prefix.batch * prefix.kv_heads * prefix.splits * prefix.row_tiles;
-  NHIP_LAUNCH("attention_prefix", (attn_prefix_kernel<T, DP, TILES>), dim3((uint32_t)(own_wgs + wgs)), dim3(kWaves * 64), bytes, s,
+  NHIP_LAUNCH("attention_prefix", (attn_prefix_kernel<T, DP, TILES, OWN>), dim3((uint32_t)(own_wgs + wgs)), dim3(kWaves * 64), bytes, s,
               prefix, own, (uint32_t)own_wgs);
   return check_launch("attention_prefix");
 }
 
 template <class T, int DP>
 int prefix_parts(const AttnArgs& prefix, const AttnArgs& own, hipStream_t s) {
-  if (!own.tiles) return prefix.tiles ? prefix_launch<T, DP, true>(prefix, own, s) : prefix_launch<T, DP, false>(prefix, own, s);
+  if (!own.tiles) {
+    if constexpr (DP <= 128)
+      if (own.reps == 2) return prefix.tiles ? prefix_launch<T, DP, true, 2>(prefix, own, s) : prefix_launch<T, DP, false, 2>(prefix, own, s);
+    return prefix.tiles ? prefix_launch<T, DP, true, 1>(prefix, own, s) : prefix_launch<T, DP, false, 1>(prefix, own, s);
+  }
   NHIP_TRY((launch<T, DP, kSrcInt8>(prefix, s)));
   return launch<T, DP, kSrcInt8>(own, s);
 }

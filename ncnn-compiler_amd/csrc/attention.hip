@@ -10,8 +10,9 @@ namespace {
 
 // Checks the sizes and fills them in, chooses the kernel (vec: rows that the
 // one for many rows takes; cache: over the 8-bit cache) and the number of parts
-// of the keys.  choice: 0 few rows, 1 many, -1 by the rule here.
-int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a, int choice = -1) {
+// of the keys.  choice: 0 few rows, 1 many, -1 by
+// the rule here; reps: times 16 few rows of a workgroup.
+int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a, int choice = -1, int reps = 1) {
   if (!d) return fail(NHIP_STATUS_NULL_POINTER, "attention: null descriptor");
   if (!elem_size(d->dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "attention: dtype has to be F32, F16 or BF16");
   if (d->batch < 0 || d->queries < 0 || d->keys < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative extent");
@@ -56,7 +57,8 @@ int attn_args(const nhip_attention_desc* d, bool vec, bool cache, AttnArgs* a, i
   const bool full = cache ? few >= (f32 ? 3 : 4) : d->head_dim > 64 ? few >= 1.5 : f32 ? few > 2 : few >= 3;
   const double again = cache ? (f32 ? 28e6 : 90e6) : f32 ? 215e6 : 64e6;  // bytes
   a->tiles = choice >= 0 ? choice : vec && force != 0 && (force == 1 || full || (few >= 0.25 && (tiles16 - 1) * bytes > again));
-  const int tile = a->tiles ? attn::kTilesRows : attn::kRowTile;
+  a->reps = reps;
+  const int tile = a->tiles ? attn::kTilesRows : attn::kRowTile * reps;
   a->row_tiles = (int)ceil_div(std::max(a->rows, 1), tile);
   const int64_t heads = (int64_t)d->batch * d->kv_heads;
   if (heads > 0x7fffff00 / attn::kTilesRows / a->row_tiles)
@@ -175,7 +177,11 @@ int prefix_choice(const nhip_attention_desc& d) {
 // the descriptors of both.
 int prefix_args(const nhip_attention_desc* d, int32_t groups, int32_t prefix_keys, AttnArgs* prefix, AttnArgs* own) {
   NHIP_TRY(attn_args(d, true, true, own));
-  NHIP_TRY(attn_args(d, true, true, own, prefix_choice(*d)));
+  // Own keys: twice 16 rows of a workgroup share what is read and converted of the
+  // keys, where there are as many (48 sequences of 28 rows: 184 -> 175 us a call).  Not
+  // the prefix, whose workgroups are few (4 of 64 rows: 37 -> 42).
+  const int reps = own->rows > attn::kRowTile && d->head_dim <= 128 ? 2 : 1;
+  NHIP_TRY(attn_args(d, true, true, own, prefix_choice(*d), reps));
   if (groups <= 0 || d->batch % groups) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: groups have to divide the batch");
   if (prefix_keys < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "attention: negative extent");
   nhip_attention_desc shared = *d;
