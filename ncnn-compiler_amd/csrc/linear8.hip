@@ -46,6 +46,35 @@ __device__ __forceinline__ void load8(const T* row, int c, int k, float (&x)[8])
   }
 }
 
+// A row's scale from its largest magnitude (infinite: the row holds an infinity or NaN,
+// its codes are 0 and its results 0 * NaN), and what x is multiplied by.
+struct RowScale {
+  float scale, inv;
+  __device__ __forceinline__ explicit RowScale(float most) {
+    scale = most > 0.f ? fmaxf(most * (1.f / 127.f), kLeastScale) : 0.f;
+    inv = scale > 0.f && most < INFINITY ? 1.f / scale : 0.f;
+    if (!(most < INFINITY)) scale = NAN;
+  }
+};
+struct Widest {
+  float most = 0.f;
+  bool whole = true;  // finite
+  __device__ __forceinline__ void show(const float (&t)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      most = fmaxf(most, fabsf(t[i]));
+      whole = whole && fabsf(t[i]) <= 3.4028235e38f;
+    }
+  }
+  __device__ __forceinline__ RowScale of_wave() const { return RowScale(wave_max(whole ? most : INFINITY)); }
+};
+__device__ __forceinline__ uint2 codes8(const float (&t)[8], float inv) {
+  int q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i] = quantize_q(t[i], inv);
+  return make_uint2(pack_i8x4(q[0], q[1], q[2], q[3]), pack_i8x4(q[4], q[5], q[6], q[7]));
+}
+
 // One workgroup: 8 rows, one to a wave, which finds its largest magnitude first;
 // the codes are put in order in LDS, kChunk of a row at a time, and stored as the
 // 128 bytes that 8 rows have together.  The first chunk is held, others are read again.
@@ -59,36 +88,20 @@ __global__ __launch_bounds__(512) void linear8_codes_kernel(const T* x, int64_t 
   const int r = blockIdx.x * 8 + wave;
   const int mine = r < rows ? k : 0;  // past the rows: zeros
   const T* row = x + (int64_t)min(r, rows - 1) * stride;
-  float held[HELD][8], most = 0.f;
-  bool whole = true;  // finite
-  const auto widest = [&](const float(&t)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      most = fmaxf(most, fabsf(t[i]));
-      whole = whole && fabsf(t[i]) <= 3.4028235e38f;
-    }
-  };
+  float held[HELD][8];
+  Widest widest;
 #pragma unroll
   for (int h = 0; h < HELD; ++h) load8<T, VEC>(row, (lane + h * 64) * 8, mine, held[h]);
 #pragma unroll
-  for (int h = 0; h < HELD; ++h) widest(held[h]);
+  for (int h = 0; h < HELD; ++h) widest.show(held[h]);
 #pragma unroll 4
   for (int c = kChunk + lane * 8; c < mine; c += 512) {
     float t[8];
     load8<T, VEC>(row, c, mine, t);
-    widest(t);
+    widest.show(t);
   }
-  most = wave_max(whole ? most : INFINITY);
-  const float scale = most > 0.f ? fmaxf(most * (1.f / 127.f), kLeastScale) : 0.f;
-  const float inv = scale > 0.f && most < INFINITY ? 1.f / scale : 0.f;
-  // a row that holds an infinity or NaN: codes 0, results 0 * NaN
-  if (lane == 0 && r < rows) scales[r] = most < INFINITY ? scale : NAN;
-  const auto store = [&](const float(&t)[8], int c) {
-    int q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = quantize_q(t[i], inv);
-    *reinterpret_cast<uint2*>(lds + wave * ROW + c) = make_uint2(pack_i8x4(q[0], q[1], q[2], q[3]), pack_i8x4(q[4], q[5], q[6], q[7]));
-  };
+  const RowScale scale = widest.of_wave();
+  if (lane == 0 && r < rows) scales[r] = scale.scale;
   int8_t* to = codes + code_at((int64_t)blockIdx.x * 8, steps);
   for (int c0 = 0; c0 < steps * kStepK; c0 += kChunk) {
     const int width = min(kChunk, steps * kStepK - c0);
@@ -98,7 +111,7 @@ __global__ __launch_bounds__(512) void linear8_codes_kernel(const T* x, int64_t 
       const int c = (lane + h * 64) * 8;
       if (c >= width) break;
       if (c0) load8<T, VEC>(row, c0 + c, mine, held[h]);
-      store(held[h], c);
+      *reinterpret_cast<uint2*>(lds + wave * ROW + c) = codes8(held[h], scale.inv);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < width / 2; i += 512)  // 16 codes of a row: [steps][4][16 rows]
@@ -152,22 +165,23 @@ __global__ __launch_bounds__(256) void linear8_params_kernel(const float* scale,
 }
 
 // ---------------------------------------------------------------- few rows
-// One workgroup: NB blocks of 16 channels of one expert, 16 TG of its rows at a
-// time; its waves take the steps of the sum in turn and are joined in LDS.
+// One workgroup: NB blocks of 16 channels of one expert, 16 TG of its rows, and if
+// it has more than its share the rows `chunks` times as far on; its waves take the steps of the sum in turn and are joined in LDS.
 constexpr int kAhead = 4;  // steps that a wave reads before it multiplies them
 template <class T, int ACT, int TG, int NB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a) {
+__global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a, int chunks) {
   __shared__ v4i part[WAVES][TG * NB][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int groups = (a.blocks + NB - 1) / NB;
-  const int e = blockIdx.x / groups, b0 = blockIdx.x % groups * NB;
+  const uint32_t of = blockIdx.x / groups;
+  const int e = of / chunks, b0 = blockIdx.x % groups * NB;
   int begin, end;
   expert_rows(a, e, begin, end);
   const int8_t* w[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
     w[b] = a.w + ((int64_t)e * a.blocks + min(b0 + b, a.blocks - 1)) * a.steps * 1024 + lane * 16;
-  for (int r0 = begin; r0 < end; r0 += 16 * TG) {
+  for (int r0 = begin + of % chunks * (16 * TG); r0 < end; r0 += chunks * (16 * TG)) {
     const int8_t* x[TG];
 #pragma unroll
     for (int t = 0; t < TG; ++t) x[t] = a.x + code_at(min(r0 + t * 16 + (lane & 15), end - 1), a.steps) + (lane >> 4) * 256;
@@ -182,7 +196,7 @@ __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a)
       for (int u = 0; u < kAhead; ++u) {
         const int at = min(s + u * WAVES, a.steps - 1);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) wf[u][b] = *reinterpret_cast<const v4i*>(w[b] + at * 1024);
+        for (int b = 0; b < NB; ++b) wf[u][b] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(w[b] + at * 1024));
 #pragma unroll
         for (int t = 0; t < TG; ++t) xf[u][t] = *reinterpret_cast<const v4i*>(x[t] + at * 1024);
       }
@@ -226,13 +240,112 @@ __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a)
   }
 }
 
+// At most 16 rows in all, and few workgroups: each makes the codes itself, while the
+// first weights are on their way, which spares a launch.  One block of 16 channels
+// of one expert; the waves take the steps in turn.  Latency bounds it: 16 rows of
+// 2048 to 2048 bf16 XX us a call, in two launches 10.0.
+template <class T, int ACT, bool VEC>
+__global__ __launch_bounds__(512) void linear8_few_kernel(Linear8Args a, const T* x, int64_t stride, int k) {
+  constexpr int WAVES = 8, HELD = 4;
+  extern __shared__ __attribute__((aligned(16))) int8_t codes[];  // [steps][4][16 rows][16]
+  __shared__ v4i part[WAVES][64];
+  __shared__ float scales[16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int e = blockIdx.x / a.blocks, b = blockIdx.x % a.blocks;
+  int begin, end;
+  expert_rows(a, e, begin, end);
+  if (begin >= end) return;
+  const int8_t* w = a.w + ((int64_t)e * a.blocks + b) * a.steps * 1024 + lane * 16;
+  v4i wf[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) wf[u] = *reinterpret_cast<const v4i*>(w + min(wave + u * WAVES, a.steps - 1) * 1024);
+#pragma unroll
+  for (int r = wave; r < 16; r += WAVES) {
+    const int mine = begin + r < end ? k : 0;  // past the rows: zeros
+    const T* row = x + (int64_t)min(begin + r, end - 1) * stride;
+    const int wide = a.steps * kStepK;
+    float held[HELD][8];
+    Widest widest;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) load8<T, VEC>(row, (lane + h * 64) * 8, mine, held[h]);
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) widest.show(held[h]);
+    for (int c = HELD * 512 + lane * 8; c < mine; c += 512) {
+      float t[8];
+      load8<T, VEC>(row, c, mine, t);
+      widest.show(t);
+    }
+    const RowScale scale = widest.of_wave();
+    if (lane == 0) scales[r] = scale.scale;
+    const auto put = [&](const float(&t)[8], int c) {
+      *reinterpret_cast<uint2*>(codes + (c >> 4) * 256 + r * 16 + (c & 8)) = codes8(t, scale.inv);
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+      if (const int c = (lane + h * 64) * 8; c < wide) put(held[h], c);
+    for (int c = HELD * 512 + lane * 8; c < wide; c += 512) {
+      float t[8];
+      load8<T, VEC>(row, c, mine, t);
+      put(t, c);
+    }
+  }
+  __syncthreads();
+  v4i acc = {0, 0, 0, 0};
+  for (int s = wave; s < a.steps; s += WAVES * kAhead) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = s + u * WAVES;
+      if (at < a.steps)
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], *reinterpret_cast<const v4i*>(codes + at * 1024 + lane * 16), acc, 0, 0, 0);
+      wf[u] = *reinterpret_cast<const v4i*>(w + min(at + WAVES * kAhead, a.steps - 1) * 1024);
+    }
+  }
+  settle8(acc);
+  part[wave][lane] = acc;
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int v = 1; v < WAVES; ++v) acc += part[v][lane];
+  const int row = begin + (lane & 15), j = b * 16 + 4 * (lane >> 4);
+  if (row >= end) return;
+  const float xs = scales[lane & 15];
+  T* out = (T*)a.out + (int64_t)row * a.n;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (j + c < a.n) out[j + c] = (T)finish8<ACT>(acc[c], xs, a.w_scale[(int64_t)e * a.n + j + c], a.bias[(int64_t)e * a.n + j + c]);
+}
+
+// (LDS for the codes of 16 rows)
+bool few_selected(const Linear8Args& a) {
+  // (the switch that pins the other kernels pins them here too)
+  if (a.rows > 16 || a.steps > 128 || setting_int("NHIP_LINEAR8_TILES", -1) >= 0) return false;
+  return (int64_t)a.experts * a.blocks <= 2 * cu_count();
+}
+
+template <class T, int ACT>
+int few_run(const Linear8Args& a, const void* x, int64_t stride, int k, hipStream_t s) {
+  const auto launch = [&](auto kernel) {
+    const int bytes = a.steps * 1024;
+    if (bytes > 48 * 1024) NHIP_TRY(ensure_dynamic_lds((const void*)kernel, 128 * 1024));
+    NHIP_LAUNCH("linear8_few", kernel, dim3((uint32_t)(a.experts * (int64_t)a.blocks)), dim3(512), bytes, s, a, (const T*)x, stride, k);
+    return check_launch("linear8_few");
+  };
+  return aligned_to(x, 16) && stride % kVec<T> == 0 ? launch(linear8_few_kernel<T, ACT, true>) : launch(linear8_few_kernel<T, ACT, false>);
+}
+
 template <class T, int ACT, int TG>
 int rows_run(const Linear8Args& a, hipStream_t s) {
+  const int64_t chunks = ceil_div(ceil_div(a.rows, a.experts), 16 * TG), wgs = a.experts * (int64_t)a.blocks * chunks;
+  if (wgs > 0x7fffffff) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
   const auto launch = [&](auto kernel, int nb, int waves) {
-    NHIP_LAUNCH("linear8_rows", kernel, dim3((uint32_t)(a.experts * ceil_div(a.blocks, nb))), dim3(waves * 64), 0, s, a);
+    NHIP_LAUNCH("linear8_rows", kernel, dim3((uint32_t)(a.experts * chunks * ceil_div(a.blocks, nb))), dim3(waves * 64), 0, s, a, (int)chunks);
     return check_launch("linear8_rows");
   };
-  if ((int64_t)a.experts * a.blocks > 4 * cu_count()) return launch(linear8_rows_kernel<T, ACT, TG, 2, 4>, 2, 4);
+  // us (NB, waves): 48 rows of 2048 to 50021 (3127 blocks) fp16 2, 2 31.8; 2, 4 33.4; 4, 4
+  // 34.1; 1, 4 42.7; 128 rows of 16 experts, 2048 to 1024 (1024 blocks) bf16 2, 4 12.1; 1, 8
+  // 13.2; 2, 2 13.4; 4, 4 15.0.
+  if (wgs > 8 * cu_count()) return launch(linear8_rows_kernel<T, ACT, TG, 2, 2>, 2, 2);
+  if (wgs > 2 * cu_count()) return launch(linear8_rows_kernel<T, ACT, TG, 2, 4>, 2, 4);
   return launch(linear8_rows_kernel<T, ACT, TG, 1, 8>, 1, 8);
 }
 
@@ -241,6 +354,7 @@ int product_run(const Linear8Args& a, hipStream_t s) {
   const int64_t each = ceil_div(a.rows, a.experts);
   if (each <= 16) return rows_run<T, ACT, 1>(a, s);
   if (each <= 32) return rows_run<T, ACT, 2>(a, s);
+  if (each <= 48) return rows_run<T, ACT, 3>(a, s);
   return rows_run<T, ACT, 4>(a, s);
 }
 
@@ -365,6 +479,8 @@ int nhip_linear8_forward(nhip_linear8_t plan, const void* x, int32_t dtype, int6
   a.blocks = plan->blocks;
   a.experts = plan->experts;
   a.act = plan->act;
+  if (few_selected(a))
+    return NHIP_FOR_ELEM(dtype, T, NHIP_FOR_ACT(a.act, ACT, few_run<T, ACT>(a, x, row_stride, plan->k, as_stream(stream))));
   NHIP_TRY(NHIP_FOR_ELEM(dtype, T, codes_run<T>(x, row_stride, rows, plan->k, plan->steps, codes, scales, as_stream(stream))));
   if (linear8_tiles_selected(a)) return linear8_tiles(a, dtype, as_stream(stream));
   return NHIP_FOR_ELEM(dtype, T, NHIP_FOR_ACT(a.act, ACT, product_run<T, ACT>(a, as_stream(stream))));

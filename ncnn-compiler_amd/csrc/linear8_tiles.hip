@@ -290,7 +290,12 @@ int tiles_run(const Linear8Args& a, hipStream_t s) {
 bool linear8_tiles_selected(const Linear8Args& a) {
   const int force = setting_int("NHIP_LINEAR8_TILES", -1);
   if (force >= 0) return force != 0;
-  return a.rows > 64 * (int64_t)a.experts;
+  // Few tiles leave CUs idle and each walks the whole sum alone; the other kernel has
+  // a workgroup for 64 rows and 16 channels, whose waves share the sum, and reads
+  // the operands more often.  us a call, it / this: 200 x 1000 of 8192 (32 quarter
+  // tiles) bf16 27 / 41, 400 x 1000 (56) 43 / 41, 100 x 4096 (64) 33 / 45, 200 x 4096
+  // (128) 41 / 44, 400 x 4096 (224) 67 / 46, 1600 x 1000 of 2048 (200) 25 / 16.
+  return a.rows > 64 * (int64_t)a.experts && ceil_div(a.rows, Small::kRows) * ceil_div(a.blocks, Small::kCols / 16) > cu_count() / 2;
 }
 
 int linear8_tiles(const Linear8Args& a, int dtype, hipStream_t s) {
