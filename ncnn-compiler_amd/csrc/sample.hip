@@ -24,8 +24,13 @@ constexpr float kRange = 31.5f;  // exp(-31.5) < 2^-45, which rounds to 0
 // What the launches before the last one leave of a row.
 struct RowParts {
   uint64_t total;        // of all weights
+  uint64_t count;        // of tokens listed (an int32 is counted in)
   uint64_t bins[kBins];  // counts, weights, or the sums of sets of vectors
+  // where the border was found: its bin, and what comes before that (bin + 1, 0: not found)
+  uint64_t before;
+  uint64_t found;
 };
+constexpr int kRowZeros = kBins + 4;  // of 64 bits, to begin with
 
 struct SampleArgs {
   const void* logits;
@@ -44,7 +49,10 @@ struct SampleArgs {
   int32_t chunks;
   uint2* tops;      // [rows][chunks]
   RowParts* parts;  // [rows]
+  uint32_t* lists;  // [rows][kLongList]: indices of tokens that may be kept
 };
+
+constexpr int kLongList = 16384;
 
 // Keys in the order of the values; -0 and 0 are equal.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -159,7 +167,7 @@ struct Row {
   // `last_index`): `reserve` gives the wave room for so many, put(place, index)
   // takes them.  One reservation for U vectors of every lane; a lane goes through
   // the bits that it has set, so that the few cost little (with the values at hand
-  // every place was a branch of its own: 64 x 131072 bf16 70 us, so XX).
+  // every place was a branch of its own: 64 x 131072 bf16 59 us a call, so 48).
   template <class R, class F>
   __device__ __forceinline__ void each_from(int lane, float least, float last, int last_index, R reserve, F put) const {
     constexpr int U = 8;
@@ -244,6 +252,12 @@ struct Distances {
     scope = c.k < 0x7fffffff && c.top_p < 1.f ? fminf(reach, 0.5f * near * c.temperature) : reach;
   }
   __device__ __forceinline__ float below(float l) const { return fmaf(-0.5f, l, half_top); }
+  // a logit that no token of weight is below
+  __device__ __forceinline__ float least() const { return fmaxf(2.f * (half_top - reach - 1e-6f * (fabsf(half_top) + reach)), -3.4028235e38f); }
+  // ... or of bins 0 .. bin of the histogram up to `scope` (the margin: a bin's rounding)
+  __device__ __forceinline__ float least_of(int bin, float rate, float scope) const {
+    return bin == kBins - 1 ? least() : fmaxf(least(), 2.f * (half_top - (float)(bin + 1) / rate - 1e-6f * (fabsf(half_top) + scope)));
+  }
   __device__ __forceinline__ int bin(float l, float rate) const { return (int)fminf(below(l) * rate, (float)(kBins - 1)); }
 };
 
@@ -359,7 +373,7 @@ __global__ __launch_bounds__(kPartWaves * 64) void sample_top_kernel(SampleArgs 
   const float top = wave_max(mine);
   const uint32_t bound = c.few(a.vocab) && c.k > 1 ? wave_bound(row, mine, c.k) : 0;
   if (lane == 0) part[wave] = make_uint2(key_of(top), bound);
-  for (int i = chunk * kPartWaves * 64 + threadIdx.x; i <= kBins; i += a.chunks * kPartWaves * 64) (&a.parts[r].total)[i] = 0;
+  for (int i = chunk * kPartWaves * 64 + threadIdx.x; i < kRowZeros; i += a.chunks * kPartWaves * 64) (&a.parts[r].total)[i] = 0;
   __syncthreads();
   if (threadIdx.x == 0) {
     uint2 v = part[0];
@@ -381,8 +395,25 @@ __device__ __forceinline__ uint2 row_top(const SampleArgs& a, int64_t r, int lan
   return v;
 }
 
+// A wave's tokens from `least` on into the row's list.
+template <class T>
+__device__ __forceinline__ void list_tokens(const SampleArgs& a, int64_t r, const Row<T>& row, int lane, float least) {
+  uint32_t* list = a.lists + r * kLongList;
+  row.each_from(
+      lane, least, INFINITY, 0,
+      [&](int m) {
+        int at = 0;
+        if (lane == 0) at = atomicAdd((int*)&a.parts[r].count, m);
+        return __builtin_amdgcn_readfirstlane(at);
+      },
+      [&](int at, int index) {
+        if (at < kLongList) list[at] = (uint32_t)index;
+      });
+}
+
 // The second: of a part of a row the histogram that the row's border is first
-// looked for in, or without a filter the sums of its sets.
+// looked for in, or without a filter the sums of its sets; of rows with top-k of few
+// the tokens that reach the bound.
 template <class T>
 __global__ __launch_bounds__(kPartWaves * 64) void sample_bins_kernel(SampleArgs a) {
   __shared__ uint64_t bins[kBins];
@@ -392,12 +423,17 @@ __global__ __launch_bounds__(kPartWaves * 64) void sample_bins_kernel(SampleArgs
   const int chunk = blockIdx.x % a.chunks;
   const Settings c(a, r);
   const bool unfiltered = c.unfiltered(a.vocab);
-  if (c.few(a.vocab) || (c.k == a.vocab && !(c.top_p < 1.f) && !unfiltered)) return;
-  const float top = of_key(row_top(a, r, lane).x);
+  if (c.k == 1 || (c.k == a.vocab && !(c.top_p < 1.f) && !unfiltered)) return;
+  const uint2 keys = row_top(a, r, lane);
+  const float top = of_key(keys.x);
   if (!(fabsf(top) < INFINITY)) return;
   const Row<T> row((const T*)a.logits + r * a.stride, a.vocab, chunk * kPartWaves + wave, a.chunks * kPartWaves);
   const Distances d(top, c);
   const Weights weight{(double)top, 64 * 1.4426950408889634074 / (double)c.temperature, table};
+  if (c.few(a.vocab)) {
+    list_tokens(a, r, row, lane, fmaxf(d.least(), keys.y > key_of(-INFINITY) ? of_key(keys.y) : -INFINITY));
+    return;
+  }
   if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64);
   if (unfiltered) {
     __syncthreads();
@@ -429,6 +465,53 @@ __global__ __launch_bounds__(kPartWaves * 64) void sample_bins_kernel(SampleArgs
   __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += kPartWaves * 64)
     if (bins[i]) add_to(a.parts[r].bins[i], bins[i]);
+}
+
+// The third, of rows with a histogram: the bin of the border, and the tokens up to it.
+template <class T>
+__global__ __launch_bounds__(kPartWaves * 64) void sample_list_kernel(SampleArgs a) {
+  __shared__ uint64_t part[kPartWaves];
+  __shared__ int found;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t r = blockIdx.x / a.chunks;
+  const int chunk = blockIdx.x % a.chunks;
+  const Settings c(a, r);
+  if (c.few(a.vocab) || (c.k == a.vocab && !(c.top_p < 1.f))) return;
+  const float top = of_key(row_top(a, r, lane).x);
+  if (!(fabsf(top) < INFINITY)) return;
+  constexpr int EACH = kBins / (kPartWaves * 64);
+  uint64_t v[EACH], sum = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) v[i] = sum += a.parts[r].bins[threadIdx.x * EACH + i];
+  const double limit = c.k < a.vocab ? (double)c.k : fmax((double)c.top_p * (double)a.parts[r].total, 1.0);
+  const uint64_t upto = wave_scan(sum);
+  if (lane == 63) part[wave] = upto;
+  if (threadIdx.x == 0) found = -1;
+  __syncthreads();
+  uint64_t before = upto - sum, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPartWaves; ++w) {
+    if (w < wave) before += part[w];
+    all += part[w];
+  }
+  // (no border: all are kept, or it lies past the histogram)
+  if ((double)all < limit || (c.k < a.vocab && all <= (uint64_t)c.k)) return;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const uint64_t ahead = before + (i ? v[i - 1] : 0);
+    if ((double)(before + v[i]) >= limit && (double)ahead < limit) {
+      found = threadIdx.x * EACH + i;
+      if (chunk == 0) {
+        a.parts[r].before = ahead;
+        a.parts[r].found = found + 1;
+      }
+    }
+  }
+  __syncthreads();
+  const Distances d(top, c);
+  const float scope = c.k < a.vocab ? d.reach : d.scope;
+  const Row<T> row((const T*)a.logits + r * a.stride, a.vocab, chunk * kPartWaves + wave, a.chunks * kPartWaves);
+  list_tokens(a, r, row, lane, d.least_of(found, (float)kBins / scope, scope));
 }
 
 // One workgroup: one row, or what is left of it to do.
@@ -594,14 +677,29 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
   int last_index = 0x7fffffff;
   const auto inside = [&](float l, int index) { return d.below(l) <= d.reach && l >= last && (l > last || index <= last_index); };
   const auto inside_place = [&](uint64_t p) { return inside(of_key((uint32_t)(p >> 32)), (int)~(uint32_t)p); };
-  // the tokens from `least` on together in LDS, n of them; false: they do not fit
+  // n tokens by their indices into s.list, the values of four of a thread on their way at a time
   int n = 0;
+  const auto gather = [&](auto index_of) {
+    if (n <= kList)
+      for (int i0 = threadIdx.x; i0 < n; i0 += 4 * TH) {
+        int index[4];
+        float l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          index[e] = i0 + e * TH < n ? (int)index_of(i0 + e * TH) : 0;  // (others' entries may be places already)
+          l[e] = (float)row.from[(int64_t)index[e] + row.shift];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i0 + e * TH < n) s.list[i0 + e * TH] = place_of(key_of(l[e]), index[e]);
+      }
+    __syncthreads();
+  };
+  // the tokens from `least` on together in LDS; false: they do not fit
   const auto collect = [&](float least) {
     zero_bins();
-    // (tokens that weigh nothing are left out, to a margin)
-    const float far = 2.f * (d.half_top - d.reach - 1e-6f * (fabsf(d.half_top) + d.reach));
     row.each_from(
-        lane, fmaxf(fmaxf(least, last), fmaxf(far, -3.4028235e38f)), last, last_index,
+        lane, fmaxf(fmaxf(least, last), d.least()), last, last_index,
         [&](int m) {
           int at = 0;
           if (lane == 0) at = atomicAdd(&s.count, m);
@@ -611,21 +709,15 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
           if (at < kList) s.list[at] = (uint32_t)index;
         });
     __syncthreads();
-    if (s.count <= kList)  // the values, four of a thread on their way at a time
-      for (int i0 = threadIdx.x; i0 < s.count; i0 += 4 * TH) {
-        int index[4];
-        float l[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          index[e] = i0 + e * TH < s.count ? (int)s.list[i0 + e * TH] : 0;  // (others' entries may be places already)
-          l[e] = (float)row.from[(int64_t)index[e] + row.shift];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i0 + e * TH < s.count) s.list[i0 + e * TH] = place_of(key_of(l[e]), index[e]);
-      }
-    __syncthreads();
     n = s.count;
+    gather([&](int i) { return (uint32_t)s.list[i]; });
+    return n <= kList;
+  };
+  // ... from the row's list, where it was begun by others
+  const auto collect_listed = [&]() {
+    n = (int)a.parts[r].count;
+    const uint32_t* list = a.lists + r * kLongList;
+    gather([&](int i) { return list[i]; });
     return n <= kList;
   };
   // s.bins: the sums of `measure` over the first m of s.sorted up to each, and behind them the whole
@@ -640,7 +732,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
   uint64_t mass = 0;  // of all that top-k has left, if top-p's histogram was made
   if (c.few(a.vocab)) {
     const float least = bound > key_of(-INFINITY) ? of_key(bound) : -INFINITY;
-    listed = collect(least);
+    listed = PARTS ? collect_listed() : collect(least);
   }
 #pragma unroll 1
   for (int by = 0; by < 2; ++by) {  // top-k by count, then top-p by weight
@@ -649,82 +741,90 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     const auto measure = [&](float l) { return by ? weight(l) : (uint64_t)1; };
     float scope = d.reach;
     double limit;
-    for (bool again = false;; again = true) {
-      // (with both filters the second looks at what the first has left)
-      scope = by && k == a.vocab && !again ? d.scope : d.reach;
-      const float rate = (float)kBins / scope;
-      uint64_t all;
-      zero_bins();
-      if (listed) {
-        for (int i = threadIdx.x; i < n; i += TH)
-          if (const float l = of_key((uint32_t)(s.list[i] >> 32)); inside_place(s.list[i])) add_to(s.bins[d.bin(l, rate)], measure(l));
-        __syncthreads();
-        all = scan_bins(s, lane, wave);
-      } else if (PARTS && !again && (by == 0 ? !c.few(a.vocab) : k == a.vocab)) {
-        for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = a.parts[r].bins[i];
-        __syncthreads();
-        all = scan_bins(s, lane, wave);
-        if (by) all = a.parts[r].total;
-      } else if (by == 0) {
-        row.each(lane, [&](float l, int) {
-          if (d.below(l) <= scope) count_in(s.bins[d.bin(l, rate)]);
-        });
-        __syncthreads();
-        all = scan_bins(s, lane, wave);
-      } else {
-        uint64_t sum = 0;
-        row.each(lane, [&](float l, int index) {
-          const uint64_t w = weight(l);
-          if (inside(l, index)) {
-            sum += w;
-            if (d.below(l) <= scope) add_to(s.bins[d.bin(l, rate)], w);
-          }
-        });
-        sum = wave_sum(sum);
-        __syncthreads();
-        scan_bins(s, lane, wave);
-        if (lane == 0) s.part[wave] = sum;
-        __syncthreads();
-        all = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) all += s.part[w];
-      }
-      limit = by ? fmax((double)c.top_p * (double)all, 1.0) : (double)k;  // (the first one always)
-      if (by) mass = all;
-      if (scope == d.reach || (double)s.bins[kBins - 1] >= limit) break;
-    }
-    // kept: those with less than `limit` before them; the last of them lies in the bin that reaches it
-    if ((double)s.bins[kBins - 1] < limit || (by == 0 && s.bins[kBins - 1] <= (uint64_t)k)) continue;
-    const float rate = (float)kBins / scope;
     uint64_t before = 0;                   // the measure of what comes before the present bin
     uint32_t low = 0, high = 0xffffffffu;  // its keys
     int bin = -1, shift = 0;               // its bin of weights
-    for (;;) {
-      // the first bin with which the sum reaches the limit
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        s.at = kBins - 1;
-        s.count = 0;
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < kBins; i += TH)
-        if ((double)(before + s.bins[i]) >= limit && !(i && (double)(before + s.bins[i - 1]) >= limit)) s.at = i;
-      __syncthreads();
-      const int at = s.at;
-      before += at ? s.bins[at - 1] : 0;
-      if (bin < 0) {
-        bin = at;
-        // all up to the bin's last value into LDS
-        // (the margin: a bin's rounding)
-        if (!listed) {
-          const float under = d.half_top - (float)(bin + 1) / rate;
-          listed = collect(bin == kBins - 1 ? -INFINITY : 2.f * (under - 1e-6f * (fabsf(d.half_top) + scope)));
-          if (listed && n <= kOnce) break;
+    const bool begun = PARTS && (by == 0 ? !c.few(a.vocab) : k == a.vocab);
+    if (begun && a.parts[r].found) {
+      scope = by ? d.scope : d.reach;
+      if (by) mass = a.parts[r].total;
+      limit = by ? fmax((double)c.top_p * (double)mass, 1.0) : (double)k;
+      before = a.parts[r].before;
+      bin = (int)a.parts[r].found - 1;
+      listed = collect_listed();
+      if (listed && n <= kOnce) break;
+    } else {
+      for (bool again = false;; again = true) {
+        // (with both filters the second looks at what the first has left)
+        scope = by && k == a.vocab && !again ? d.scope : d.reach;
+        const float rate = (float)kBins / scope;
+        uint64_t all;
+        zero_bins();
+        if (listed) {
+          for (int i = threadIdx.x; i < n; i += TH)
+            if (const float l = of_key((uint32_t)(s.list[i] >> 32)); inside_place(s.list[i])) add_to(s.bins[d.bin(l, rate)], measure(l));
+          __syncthreads();
+          all = scan_bins(s, lane, wave);
+        } else if (begun && !again) {
+          for (int i = threadIdx.x; i < kBins; i += TH) s.bins[i] = a.parts[r].bins[i];
+          __syncthreads();
+          all = scan_bins(s, lane, wave);
+          if (by) all = a.parts[r].total;
+        } else if (by == 0) {
+          row.each(lane, [&](float l, int) {
+            if (d.below(l) <= scope) count_in(s.bins[d.bin(l, rate)]);
+          });
+          __syncthreads();
+          all = scan_bins(s, lane, wave);
+        } else {
+          uint64_t sum = 0;
+          row.each(lane, [&](float l, int index) {
+            const uint64_t w = weight(l);
+            if (inside(l, index)) {
+              sum += w;
+              if (d.below(l) <= scope) add_to(s.bins[d.bin(l, rate)], w);
+            }
+          });
+          sum = wave_sum(sum);
+          __syncthreads();
+          scan_bins(s, lane, wave);
+          if (lane == 0) s.part[wave] = sum;
+          __syncthreads();
+          all = 0;
+#pragma unroll
+          for (int w = 0; w < WAVES; ++w) all += s.part[w];
         }
-      } else {  // bins of keys: the largest first
-        const uint32_t width = 1u << shift;
-        high -= (uint32_t)at * width;
-        low = high - low >= width ? high - (width - 1) : low;
+        limit = by ? fmax((double)c.top_p * (double)all, 1.0) : (double)k;  // (the first one always)
+        if (by) mass = all;
+        if (scope == d.reach || (double)s.bins[kBins - 1] >= limit) break;
+      }
+      // kept: those with less than `limit` before them; the last of them lies in the bin that reaches it
+      if ((double)s.bins[kBins - 1] < limit || (by == 0 && s.bins[kBins - 1] <= (uint64_t)k)) continue;
+    }
+    const float rate = (float)kBins / scope;
+    for (bool first = bin < 0, again = false;; again = true) {
+      if (first || again) {
+        // the first bin with which the sum reaches the limit
+        __syncthreads();
+        if (threadIdx.x == 0) s.at = kBins - 1;
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins; i += TH)
+          if ((double)(before + s.bins[i]) >= limit && !(i && (double)(before + s.bins[i - 1]) >= limit)) s.at = i;
+        __syncthreads();
+        const int at = s.at;
+        before += at ? s.bins[at - 1] : 0;
+        if (!again) {
+          bin = at;
+          // all up to the bin's last value into LDS
+          if (!listed) {
+            listed = collect(d.least_of(bin, rate, scope));
+            if (listed && n <= kOnce) break;
+          }
+        } else {  // bins of keys: the largest first
+          const uint32_t width = 1u << shift;
+          high -= (uint32_t)at * width;
+          low = high - low >= width ? high - (width - 1) : low;
+        }
       }
       __syncthreads();
       if (threadIdx.x == 0) s.count = 0;
@@ -941,18 +1041,20 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
   finish();
 }
 
-// Workgroups that begin a row, 0: one does all of it.
+// Workgroups that begin a row, 0: one does all of it.  us a call, one / several:
+// 16 rows of 30000 bf16 by top-p 0.9 42 / 31, of 64 x 131072 145 / 56, without a filter 61 /
+// 25, top-k of 50 33 / 25, the largest 16 / 19; four to a CU of all rows.
 int chunks_of(const nhip_sample_desc* d) {
   const int force = setting_int("NHIP_SAMPLE_CHUNKS", -1);
   if (force >= 0) return std::min(force, 64);
-  if (d->vocab <= 16384) return 0;
+  if (d->vocab <= 16384 || (!d->temperature_each && d->temperature == 0.f)) return 0;
   const int64_t want = ceil_div(4 * cu_count(), std::max(d->rows, 1));
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, d->vocab / 2048, 64}));
 }
 
 uint64_t workspace_of(const nhip_sample_desc* d) {
   const int chunks = chunks_of(d);
-  return chunks ? d->rows * (sizeof(RowParts) + (uint64_t)chunks * sizeof(uint2)) : 0;
+  return chunks ? d->rows * (sizeof(RowParts) + (uint64_t)chunks * sizeof(uint2) + kLongList * sizeof(uint32_t)) : 0;
 }
 
 template <class T, int WAVES, bool PARTS>
@@ -971,6 +1073,15 @@ int sample_run(const SampleArgs& a, int rows, hipStream_t s) {
   NHIP_TRY(check_launch("sample_top"));
   NHIP_LAUNCH("sample_bins", (sample_bins_kernel<T>), grid, block, 0, s, a);
   NHIP_TRY(check_launch("sample_bins"));
+  // (no launch where the settings of all rows leave it nothing to do, nor where the
+  // last launch has a workgroup for every CU to do it with: 64 rows of 131072 bf16, each
+  // its own settings 50 us without, 45 with; 256 of 50021 fp32 74 and 79)
+  const bool some_k = a.top_k_each || a.top_k == 0 || a.top_k > kSorted, some_p = a.top_p_each || a.top_p < 1.f;
+  const bool many_k = a.top_k_each || (a.top_k > kSorted && a.top_k < a.vocab);
+  if (rows <= cu_count() / 2 && (a.temperature_each || a.temperature > 0.f) && some_k && (some_p || many_k)) {
+    NHIP_LAUNCH("sample_list", (sample_list_kernel<T>), grid, block, 0, s, a);
+    NHIP_TRY(check_launch("sample_list"));
+  }
   return sample_last<T, 16, true>(a, rows, s);
 }
 
@@ -978,7 +1089,8 @@ int sample_args(const nhip_sample_desc* d) {
   if (!d) return fail(NHIP_STATUS_NULL_POINTER, "sample: null descriptor");
   if (!elem_size(d->dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "sample: dtype has to be F32, F16 or BF16");
   if (d->rows < 0 || d->vocab <= 0) return fail(NHIP_STATUS_INVALID_SHAPE, "sample: a row holds at least one logit");
-  if (d->vocab > 1 << 30 || d->rows > 1 << 24) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "sample: at most 2^24 rows of 2^30 logits");
+  // (2^19 weights of 2^44 each are the most that 64 bits sum)
+  if (d->vocab > 1 << 19 || d->rows > 1 << 24) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "sample: at most 2^24 rows of 2^19 logits");
   if (d->row_stride < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "sample: negative stride");
   // (values that a tensor holds for each row are read on the device, where these mean the same as the nearest that is allowed)
   if (!(d->temperature >= 0.f) || d->top_k < 0 || !(d->top_p >= 0.f) || !(d->min_p >= 0.f) || d->min_p > 1.f)
@@ -1015,10 +1127,11 @@ int nhip_sample_forward(const nhip_sample_desc* desc, const void* logits, const 
   if (need && (workspace_bytes < need || !aligned_to(workspace, 16)))
     return fail(NHIP_STATUS_OUTPUT_CAPACITY_INSUFFICIENT, "sample: workspace too small or not 16-byte aligned");
   RowParts* parts = (RowParts*)workspace;
+  uint2* tops = (uint2*)(parts + desc->rows);
   const SampleArgs a{logits,           desc->row_stride,       desc->vocab,      uniform,          desc->temperature,
                      desc->top_p,      desc->min_p,            desc->top_k,      desc->temperature_each,
                      desc->top_k_each, desc->top_p_each,       desc->min_p_each, token,            logprob,
-                     chunks_of(desc),  (uint2*)(parts + desc->rows), parts};
+                     chunks_of(desc),  tops, parts, (uint32_t*)(tops + (int64_t)desc->rows * chunks_of(desc))};
   return NHIP_FOR_ELEM(desc->dtype, T, sample_run<T>(a, desc->rows, as_stream(stream)));
 }
 

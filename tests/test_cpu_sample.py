@@ -14,12 +14,12 @@ def desc(**kw):
     return nhip.SampleDesc(**v)
 
 
-def forward(d, logits=ONE, uniform=ONE, token=ONE, logprob=ONE):
-    return nhip.load().nhip_sample_forward(d, logits, uniform, token, logprob, None, 0, None)
+def forward(d, logits=ONE, uniform=ONE, token=ONE, logprob=ONE, ws=None, nbytes=0):
+    return nhip.load().nhip_sample_forward(d, logits, uniform, token, logprob, ws, nbytes, None)
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(dtype=nhip.DTYPE_I8), 7), (dict(rows=-1), 2), (dict(vocab=0), 2), (dict(vocab=2 ** 30 + 1), 4), (dict(row_stride=-1), 2),
+    (dict(dtype=nhip.DTYPE_I8), 7), (dict(rows=-1), 2), (dict(vocab=0), 2), (dict(vocab=2 ** 19 + 1), 4), (dict(rows=2 ** 24 + 1), 4), (dict(row_stride=-1), 2),
     (dict(temperature=-0.5), 3), (dict(temperature=float("nan")), 3), (dict(top_k=-1), 3), (dict(top_p=-1.0), 3),
     (dict(top_p=float("nan")), 3), (dict(min_p=-0.1), 3), (dict(min_p=1.1), 3), (dict(min_p=float("nan")), 3),
     (dict(temperature_each=ONE + 2), 3), (dict(top_k_each=ONE + 1), 3), (dict(top_p_each=ONE + 3), 3), (dict(min_p_each=ONE + 2), 3)])
@@ -38,3 +38,10 @@ def test_arguments():
         assert forward(desc(), **{name: None}) == 1, name
         assert forward(desc(), **{name: ONE + 1}) == 3, name
     assert forward(desc(rows=0)) == 0
+
+
+def test_workspace():
+    d, n = desc(vocab=100000), ctypes.c_uint64()
+    assert nhip.load().nhip_sample_workspace_size(d, ctypes.byref(n)) == 0 and n.value > 0
+    assert forward(d) == 1 and forward(d, ws=ONE, nbytes=n.value - 1) == 5 and forward(d, ws=ONE + 8, nbytes=n.value) == 5
+    assert nhip.load().nhip_sample_workspace_size(desc(), ctypes.byref(n)) == 0 and n.value == 0

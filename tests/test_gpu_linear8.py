@@ -54,6 +54,35 @@ def test_product(nhip_env, rows, k, n, dtype, tiles):
     check(plan.forward(x.cuda()), ref.product(x, w, ws, b, act))
 
 
+@pytest.mark.parametrize("rows,k,n", [(16, 8192, 40), (9, 8200, 17), (1, 4100, 33), (16, 2049, 9000), (7, 33, 20000), (3000, 64, 3000),
+                                      (49, 300, 40000), (40, 300, 70000), (700, 8192, 100)])
+def test_kernels_of_few_and_many(rows, k, n):
+    """Sizes on either side of the rules that choose a kernel."""
+    gen = torch.Generator().manual_seed(rows)
+    x, (w, ws, b) = tokens(gen, rows, k, torch.bfloat16), weights(gen, (n, k), True)
+    plan = nhip.Linear8(w.cuda(), ws.cuda(), b.cuda(), nhip.ACT_RELU)
+    check(plan.forward(x.cuda()), ref.product(x, w, ws, b, "relu"))
+
+
+def test_offsets_past_32_bits():
+    """Results of more than 2^32 elements' bytes, weights of as many: their ends."""
+    gen = torch.Generator().manual_seed(11)
+    w, ws, _ = weights(gen, (4096, 64), False)
+    plan = nhip.Linear8(w.cuda(), ws.cuda())
+    x = torch.randn((600000, 64), device="cuda").half()  # 4.9 GB of results
+    got = plan.forward(x)
+    for at in (slice(0, 200), slice(599700, 600000)):
+        check(got[at], ref.product(x[at], w, ws, None, "none"))
+    del got
+    many = torch.randint(-127, 128, (300, 4096, 4096), dtype=torch.int8, device="cuda")  # 5 GB of codes
+    plan = nhip.Linear8(many, torch.ones((300, 4096), device="cuda"))
+    starts = torch.tensor([0] * 150 + [3] * 150 + [8], dtype=torch.int32, device="cuda")
+    x = torch.randn((8, 4096), device="cuda")
+    got = plan.forward(x, expert_starts=starts)
+    for e, at in ((149, slice(0, 3)), (299, slice(3, 8))):
+        check(got[at], ref.product(x[at], many[e], torch.ones(4096), None, "none"))
+
+
 @pytest.mark.parametrize("rows", [5, 300])
 def test_shapes_strides_alignment(rows):
     """Rows further apart than their length, not 16-byte aligned, in three dimensions; plans of host arrays."""
@@ -76,9 +105,9 @@ def test_shapes_strides_alignment(rows):
     assert plan.forward(torch.empty((0, 96), device="cuda")).shape == (0, 70)
 
 
-@pytest.mark.parametrize("tiles", ["0", "1"])
+@pytest.mark.parametrize("tiles", ["-1", "0", "1"])
 @pytest.mark.parametrize("counts", [
-    [1], [0, 0, 5], [17, 0, 1, 64, 3], [300, 0, 0, 1, 257], [1] * 70, [0] * 66 + [40, 0, 2], [130, 2, 256, 0, 512, 1]])
+    [1], [3, 0, 13], [0, 16], [0, 0, 5], [17, 0, 1, 64, 3], [300, 0, 0, 1, 257], [1] * 70, [0] * 66 + [40, 0, 2], [130, 2, 256, 0, 512, 1]])
 def test_experts(nhip_env, counts, tiles):
     """Ragged, some without rows, more experts than a wave has lanes; rows before the first and behind the last stay."""
     nhip_env.setenv("NHIP_LINEAR8_TILES", tiles)
@@ -99,7 +128,7 @@ def test_experts(nhip_env, counts, tiles):
                 check(out[at], ref.product(x[at], w[i], ws[i], b[i], "silu"), f"expert {i}")
 
 
-@pytest.mark.parametrize("tiles", ["0", "1"])
+@pytest.mark.parametrize("tiles", ["-1", "0", "1"])
 def test_starts_out_of_range(nhip_env, tiles):
     """Starts are clamped to the rows there are; one that falls leaves an expert without rows."""
     nhip_env.setenv("NHIP_LINEAR8_TILES", tiles)
@@ -127,14 +156,15 @@ def test_longest_sum(nhip_env, tiles):
     check(got, ref.product(x, w, torch.ones(17), None, "none"))
 
 
-@pytest.mark.parametrize("tiles", ["0", "1"])
-def test_values(nhip_env, tiles):
+@pytest.mark.parametrize("rows", [12, 20])
+@pytest.mark.parametrize("tiles", ["-1", "0", "1"])
+def test_values(nhip_env, tiles, rows):
     """Subnormal and huge tokens; one with an infinity or NaN is NaN, the others are not touched by it."""
     nhip_env.setenv("NHIP_LINEAR8_TILES", tiles)
     gen = torch.Generator().manual_seed(1)
     w, ws, b = weights(gen, (33, 300), True)
     plan = nhip.Linear8(w.cuda(), ws.cuda(), b.cuda(), nhip.ACT_RELU)
-    x = torch.randn((20, 300), generator=gen)
+    x = torch.randn((rows, 300), generator=gen)
     x[3] *= 2.0 ** -140
     x[4] = torch.tensor([2.0 ** -149] * 300)
     x[5] *= 2.0 ** 124 / x[5].abs().max()
@@ -142,7 +172,7 @@ def test_values(nhip_env, tiles):
     bad = x.clone()
     bad[7, 299], bad[8, 0], bad[9, 17] = float("inf"), -float("inf"), float("nan")
     got = plan.forward(bad.cuda()).cpu()
-    hurt = torch.zeros(20, dtype=torch.bool)
+    hurt = torch.zeros(rows, dtype=torch.bool)
     hurt[7:10] = True
     assert got[hurt].isnan().all()
     check(got[~hurt], (want[~hurt], bound[~hurt]))

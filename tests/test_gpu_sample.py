@@ -89,8 +89,32 @@ def test_settings(dtype, settings):
         check(nhip.sample(logits.cuda(), u.cuda(), *settings), logits, u, settings)
 
 
+@pytest.mark.parametrize("chunks", ["0", "1", "5", "64"])
+@pytest.mark.parametrize("settings", SETTINGS + [(1.0, 0, 0.999, 0.0), (1.2, 0, 0.3, 0.0)])
+def test_rows_begun_by_several(nhip_env, settings, chunks):
+    """Long rows are begun by so many workgroups each, here rows of any length."""
+    nhip_env.setenv("NHIP_SAMPLE_CHUNKS", chunks)
+    gen = torch.Generator().manual_seed(8)
+    for (vocab, rows), dtype in zip(((1, 2), (70, 5), (3001, 6), (20011, 5), (60000, 3)), ("f32", "bf16", "f16", "f32", "bf16")):
+        logits = (torch.randn((rows, vocab), generator=gen) * 3).to(TYPES[dtype])
+        u = torch.rand((rows,), generator=gen)
+        check(nhip.sample(logits.cuda(), u.cuda(), *settings), logits, u, settings)
+
+
+def test_many_rows_and_many_kept():
+    """More rows than CUs; more kept tokens than LDS holds, by one filter and by both; the largest vocabulary."""
+    gen = torch.Generator().manual_seed(12)
+    for rows, vocab, scale, settings in ((300, 17001, 3.0, (1.0, 0, 0.9, 0.0)), (3, 120011, 1.0, (1.5, 0, 0.95, 0.0)),
+                                         (3, 120011, 1.0, (1.5, 60000, 0.9, 0.001)), (2, 120011, 0.5, (2.0, 0, 1.0, 0.05)),
+                                         (2, 2 ** 19, 2.0, (1.0, 0, 0.99, 0.0)), (2, 2 ** 19, 0.0, (1.0, 0, 1.0, 0.0))):
+        logits, u = torch.randn((rows, vocab), generator=gen) * scale, torch.rand((rows,), generator=gen)
+        check(nhip.sample(logits.cuda(), u.cuda(), *settings), logits, u, settings)
+
+
+@pytest.mark.parametrize("chunks", ["0", "3"])
 @pytest.mark.parametrize("dtype", TYPES)
-def test_each_row_its_own(dtype):
+def test_each_row_its_own(nhip_env, dtype, chunks):
+    nhip_env.setenv("NHIP_SAMPLE_CHUNKS", chunks)
     gen = torch.Generator().manual_seed(6)
     rows, vocab = 40, 20011
     wide = (torch.randn((rows, vocab + 30), generator=gen) * 4).to(TYPES[dtype])
@@ -102,9 +126,11 @@ def test_each_row_its_own(dtype):
     check(got, logits, u, settings)
 
 
+@pytest.mark.parametrize("chunks", ["0", "-1"])
 @pytest.mark.parametrize("spread", [0.0, 1e-3, 30.0, 3000.0])
-def test_spreads(spread):
+def test_spreads(nhip_env, spread, chunks):
     """Logits that are all alike, hardly apart (borders lie among thousands of neighbours), or very far apart."""
+    nhip_env.setenv("NHIP_SAMPLE_CHUNKS", chunks)
     gen = torch.Generator().manual_seed(7)
     for dtype in TYPES.values():
         logits = (torch.randn((4, 30011), generator=gen) * spread + 5).to(dtype)
@@ -116,7 +142,7 @@ def test_spreads(spread):
 
 def test_equal_logits():
     """Of equal ones the lower index comes first, and borders that the sums meet exactly are not passed."""
-    for vocab in (8, 1000, 9000, 40000):
+    for vocab in (8, 1000, 9000, 40000, 262144):
         logits = torch.zeros((64, vocab), device="cuda")
         u = (torch.arange(64, device="cuda") + 0.5) / 64
         for settings, kept in (((1.0, 0, 0.5, 0.0), vocab // 2), ((1.0, vocab // 4, 1.0, 0.0), vocab // 4),
@@ -144,9 +170,11 @@ def test_shares():
     assert (logprob.double() - share[token.long()].log()).abs().max() < 1e-6
 
 
+@pytest.mark.parametrize("chunks", ["0", "2"])
 @pytest.mark.parametrize("vocab", [7, 3000, 20000])
 @pytest.mark.parametrize("dtype", TYPES)
-def test_infinities_and_nan(dtype, vocab):
+def test_infinities_and_nan(nhip_env, dtype, vocab, chunks):
+    nhip_env.setenv("NHIP_SAMPLE_CHUNKS", chunks)
     gen = torch.Generator().manual_seed(9)
     logits = (torch.randn((10, vocab), generator=gen) * 2).to(TYPES[dtype])
     lowest = torch.finfo(TYPES[dtype]).min
