@@ -569,7 +569,7 @@ int nhip_linear8_destroy(nhip_linear8_t plan);
  * temperature NaN: 0). */
 typedef struct nhip_sample_desc {
   int32_t dtype;
-  int32_t rows;
+  int32_t rows;  /* below 2^22 */
   int32_t vocab; /* 1 to 2^19 */
   int64_t row_stride;
   float temperature; /* 0 or more */

@@ -438,32 +438,32 @@ struct RowsTile {
 template <class T, int OS>
 __device__ __forceinline__ void join_waves(const AttnArgs& a, const float* mo, const float2* ml, int in, int orow, int b, int kvh,
                                            int split, int lane) {
-      if (orow >= a.rows) return;
-      float top = -INFINITY, total = 0.f, w[kWaves];
-      bool nan = false;
-  #pragma unroll
-      for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ml[i * kRowTile + in].x);
-  #pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
-        const float2 t = ml[i * kRowTile + in];
-        nan |= t.y < 0.f;
-        w[i] = t.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t.x - top);
-        total += t.x == -INFINITY ? 0.f : w[i] * t.y;
-      }
-      const bool none = top == -INFINITY;
-      const int oq = orow / a.group, oh = kvh * a.group + orow % a.group;
-      const int64_t prow = (((int64_t)b * a.kv_heads + kvh) * a.rows + orow) * a.splits + split;
-      for (int c = lane; c < a.d; c += 64) {
-        float o = 0.f;
-  #pragma unroll
-        for (int i = 0; i < kWaves; ++i)
-          if (w[i] != 0.f) o += w[i] * mo[(i * kRowTile + in) * OS + c];
-        if (a.splits > 1 || a.parts)
-          a.part_o[prow * a.d + c] = o;
-        else
-          ((T*)a.o)[(((int64_t)b * a.queries + oq) * a.heads + oh) * a.d + c] = (T)(none ? (nan ? NAN : 0.f) : o / total);
-      }
-      if ((a.splits > 1 || a.parts) && lane == 0) a.part_ml[prow] = make_float2(top, none ? (nan ? -1.f : 0.f) : total);
+  if (orow >= a.rows) return;
+  float top = -INFINITY, total = 0.f, w[kWaves];
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ml[i * kRowTile + in].x);
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const float2 t = ml[i * kRowTile + in];
+    nan |= t.y < 0.f;
+    w[i] = t.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t.x - top);
+    total += t.x == -INFINITY ? 0.f : w[i] * t.y;
+  }
+  const bool none = top == -INFINITY;
+  const int oq = orow / a.group, oh = kvh * a.group + orow % a.group;
+  const int64_t prow = (((int64_t)b * a.kv_heads + kvh) * a.rows + orow) * a.splits + split;
+  for (int c = lane; c < a.d; c += 64) {
+    float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i)
+      if (w[i] != 0.f) o += w[i] * mo[(i * kRowTile + in) * OS + c];
+    if (a.splits > 1 || a.parts)
+      a.part_o[prow * a.d + c] = o;
+    else
+      ((T*)a.o)[(((int64_t)b * a.queries + oq) * a.heads + oh) * a.d + c] = (T)(none ? (nan ? NAN : 0.f) : o / total);
+  }
+  if ((a.splits > 1 || a.parts) && lane == 0) a.part_ml[prow] = make_float2(top, none ? (nan ? -1.f : 0.f) : total);
 }
 
 // One workgroup: 16 query rows of one key/value head over one part of the
@@ -474,7 +474,7 @@ __device__ __forceinline__ void join_waves(const AttnArgs& a, const float* mo, c
 // keys, 8 heads of 128 bf16 67 us a call (326 MB, 4.9 TB/s, a large copy's rate
 // 5.2); over the cache 16 of 12544 keys 71 us (316 MB, 4.4 TB/s, 5 us of it the
 // launch that joins the parts).
-// R: times 16 rows, which share what is read and converted of the keys.
+// R: times 16 rows of a workgroup, which share what is read and converted of the keys.
 template <class T, int DP, int SRC, int R = 1>
 __device__ __forceinline__ void rows_body(const AttnArgs& a, uint32_t at, char* lds) {
   typedef typename Second<T, SRC>::type P;
@@ -758,7 +758,9 @@ struct RowParts {
   __device__ __forceinline__ int64_t place(int i) const { return first + i * step; }
 };
 
-// Joins the parts of a row's keys in the prefix and of its own.
+// Joins the parts of a row's keys in the prefix and of its own, four channels to a
+// thread: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  Bytes bound it, most of them
+// still in the last-level cache: 48 sequences of 28 rows, 8 heads of 128 10.4 us.
 template <class T>
 __global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs prefix, AttnArgs a) {
   const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -778,7 +780,14 @@ __global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs prefix, 
 }
 
 // Both parts in one launch: the sequences' own keys, few rows each, and then the
-// prefix.
+// prefix, whose rows are those of a whole group of sequences, so that its keys are
+// read and converted once for all of them.  Each workgroup is one of the kernels above, and its
+// result a part; one launch because either alone leaves CUs idle (one group of 5
+// sequences, 12 heads of 64, 197 and 37 keys fp32 20.4 us a call in two, 14.1 in one; 48
+// of 28 rows, 12544 and 1568 keys 211 and 185).  The products and the codes' conversion
+// bound it where a group has many rows (the latter 165 us without the join, fp16, 8 heads
+// of 128), waits for loads where it has few (4 groups of 64 rows, 3136 and 256 keys,
+// bf16 34 us; 51 MB).  OWN == 2 has too many registers for as many workgroups to a CU.
 template <class T, int DP, bool TILES, int OWN>
 __global__ __launch_bounds__(kWaves * 64, (TILES ? TilesShape<T, DP, kSrcInt8>::per_cu : rows_per_cu(sizeof(T), DP, kSrcInt8) - (OWN == 2 && DP == 128 && sizeof(T) == 2))) void
 attn_prefix_kernel(AttnArgs prefix, AttnArgs own, uint32_t own_wgs) {

@@ -193,6 +193,10 @@ int prefix_args(const nhip_attention_desc* d, int32_t groups, int32_t prefix_key
   NHIP_TRY(attn_args(&shared, true, true, prefix, prefix_choice(shared)));
   prefix->parts = own->parts = 1;
   prefix->per = d->queries;
+  // launches of below 2^32 threads
+  const int64_t wgs = ((int64_t)own->batch * own->row_tiles * own->splits + (int64_t)prefix->batch * prefix->row_tiles * prefix->splits) * d->kv_heads;
+  if (wgs > 0xffff00 || (int64_t)d->batch * d->kv_heads * own->rows * (d->head_dim / 4) > 0xffffff00)
+    return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "attention: too many rows");
   return ok();
 }
 

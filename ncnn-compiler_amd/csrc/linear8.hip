@@ -20,6 +20,7 @@ namespace nhip {
 namespace {
 
 constexpr int kMaxK = 131072;  // 128 * 127 * 131072 < 2^31 (a weight may be -128)
+constexpr int kMaxRows = 0x3fffff0;  // a wave to each in a launch of below 2^32 threads
 constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126: the reciprocal stays finite
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -78,6 +79,8 @@ __device__ __forceinline__ uint2 codes8(const float (&t)[8], float inv) {
 // One workgroup: 8 rows, one to a wave, which finds its largest magnitude first;
 // the codes are put in order in LDS, kChunk of a row at a time, and stored as the
 // 128 bytes that 8 rows have together.  The first chunk is held, others are read again.
+// Bytes bound it, at sizes like these with a launch's start and end beside them: 6272
+// rows of 2048 bf16 11 us (39 MB, 3.5 TB/s), 12544 of 1024 fp16 12.5.
 constexpr int kChunk = 2048;
 template <class T, bool VEC>
 __global__ __launch_bounds__(512) void linear8_codes_kernel(const T* x, int64_t stride, int rows, int k, int steps,
@@ -166,7 +169,12 @@ __global__ __launch_bounds__(256) void linear8_params_kernel(const float* scale,
 
 // ---------------------------------------------------------------- few rows
 // One workgroup: NB blocks of 16 channels of one expert, 16 TG of its rows, and if
-// it has more than its share the rows `chunks` times as far on; its waves take the steps of the sum in turn and are joined in LDS.
+// the expert has more than its share the rows `chunks` times as far on; its waves take
+// the steps of the sum in turn and are joined in LDS.  Weights go from memory to the
+// registers that the products read, past the caches, every wave's next kAhead steps
+// under way at a time.  Reading them bounds it: 48 rows of 2048 to 50021 fp16 27 us for
+// 102 MB (3.8 TB/s; a large copy 5.1) and 5 for the codes; where an expert has few rows,
+// latency (128 rows of 16 experts, 2048 to 1024 12.1 us, 34 MB).
 constexpr int kAhead = 4;  // steps that a wave reads before it multiplies them
 template <class T, int ACT, int TG, int NB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a, int chunks) {
@@ -240,14 +248,16 @@ __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a,
   }
 }
 
-// At most 16 rows in all, and few workgroups: each makes the codes itself, while the
-// first weights are on their way, which spares a launch.  One block of 16 channels
-// of one expert; the waves take the steps in turn.  Latency bounds it: 16 rows of
-// 2048 to 2048 bf16 XX us a call, in two launches 10.0.
+// At most 16 rows in all, of at most kFewK, and few workgroups: each makes the codes
+// itself, while the first weights are on their way, which spares a launch.  One block
+// of 16 channels of one expert; the waves take the steps in turn.  Latency bounds it:
+// 16 rows of 2048 to 2048 bf16 7.5 us a call (4 MB of weights: 0.8 at a large copy's
+// rate), in two launches 10.0.
+constexpr int kFewK = 2048;  // a row in the registers of a wave
 template <class T, int ACT, bool VEC>
 __global__ __launch_bounds__(512) void linear8_few_kernel(Linear8Args a, const T* x, int64_t stride, int k) {
-  constexpr int WAVES = 8, HELD = 4;
-  extern __shared__ __attribute__((aligned(16))) int8_t codes[];  // [steps][4][16 rows][16]
+  constexpr int WAVES = 8, HELD = kFewK / 8 / 64;
+  __shared__ __attribute__((aligned(16))) int8_t codes[16 * kFewK];  // [steps][4][16 rows][16]
   __shared__ v4i part[WAVES][64];
   __shared__ float scales[16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -263,31 +273,18 @@ __global__ __launch_bounds__(512) void linear8_few_kernel(Linear8Args a, const T
   for (int r = wave; r < 16; r += WAVES) {
     const int mine = begin + r < end ? k : 0;  // past the rows: zeros
     const T* row = x + (int64_t)min(begin + r, end - 1) * stride;
-    const int wide = a.steps * kStepK;
     float held[HELD][8];
     Widest widest;
 #pragma unroll
     for (int h = 0; h < HELD; ++h) load8<T, VEC>(row, (lane + h * 64) * 8, mine, held[h]);
 #pragma unroll
     for (int h = 0; h < HELD; ++h) widest.show(held[h]);
-    for (int c = HELD * 512 + lane * 8; c < mine; c += 512) {
-      float t[8];
-      load8<T, VEC>(row, c, mine, t);
-      widest.show(t);
-    }
     const RowScale scale = widest.of_wave();
     if (lane == 0) scales[r] = scale.scale;
-    const auto put = [&](const float(&t)[8], int c) {
-      *reinterpret_cast<uint2*>(codes + (c >> 4) * 256 + r * 16 + (c & 8)) = codes8(t, scale.inv);
-    };
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
-      if (const int c = (lane + h * 64) * 8; c < wide) put(held[h], c);
-    for (int c = HELD * 512 + lane * 8; c < wide; c += 512) {
-      float t[8];
-      load8<T, VEC>(row, c, mine, t);
-      put(t, c);
-    }
+      if (const int c = (lane + h * 64) * 8; c < a.steps * kStepK)
+        *reinterpret_cast<uint2*>(codes + (c >> 4) * 256 + r * 16 + (c & 8)) = codes8(held[h], scale.inv);
   }
   __syncthreads();
   v4i acc = {0, 0, 0, 0};
@@ -315,19 +312,22 @@ __global__ __launch_bounds__(512) void linear8_few_kernel(Linear8Args a, const T
     if (j + c < a.n) out[j + c] = (T)finish8<ACT>(acc[c], xs, a.w_scale[(int64_t)e * a.n + j + c], a.bias[(int64_t)e * a.n + j + c]);
 }
 
-// (LDS for the codes of 16 rows)
+// Every workgroup makes the codes of its rows again, which must not take longer than
+// the launch that it spares.  us a call (one after the other, four layers in turn),
+// this / in two launches, 16 rows bf16: 2048 to 2048 (128 workgroups) 9.0 / 12.0, to 8192
+// (512) 10.7 / 12.6, to 12288 (768) 13.5 / 12.4, to 16384 17.4 / 12.6; 16 experts, 1024 to
+// 512 (512) 9.6 / 12.5, 2048 to 1024 (1024) 17.4 / 12.5; with rows read twice, 4096 to 4096
+// (256) 14.6 / 11.8, 8192 to 2048 (128) 24.0 / 18.5.
 bool few_selected(const Linear8Args& a) {
   // (the switch that pins the other kernels pins them here too)
-  if (a.rows > 16 || a.steps > 128 || setting_int("NHIP_LINEAR8_TILES", -1) >= 0) return false;
+  if (a.rows > 16 || a.steps * kStepK > kFewK || setting_int("NHIP_LINEAR8_TILES", -1) >= 0) return false;
   return (int64_t)a.experts * a.blocks <= 2 * cu_count();
 }
 
 template <class T, int ACT>
 int few_run(const Linear8Args& a, const void* x, int64_t stride, int k, hipStream_t s) {
   const auto launch = [&](auto kernel) {
-    const int bytes = a.steps * 1024;
-    if (bytes > 48 * 1024) NHIP_TRY(ensure_dynamic_lds((const void*)kernel, 128 * 1024));
-    NHIP_LAUNCH("linear8_few", kernel, dim3((uint32_t)(a.experts * (int64_t)a.blocks)), dim3(512), bytes, s, a, (const T*)x, stride, k);
+    NHIP_LAUNCH("linear8_few", kernel, dim3((uint32_t)(a.experts * (int64_t)a.blocks)), dim3(512), 0, s, a, (const T*)x, stride, k);
     return check_launch("linear8_few");
   };
   return aligned_to(x, 16) && stride % kVec<T> == 0 ? launch(linear8_few_kernel<T, ACT, true>) : launch(linear8_few_kernel<T, ACT, false>);
@@ -336,7 +336,7 @@ int few_run(const Linear8Args& a, const void* x, int64_t stride, int k, hipStrea
 template <class T, int ACT, int TG>
 int rows_run(const Linear8Args& a, hipStream_t s) {
   const int64_t chunks = ceil_div(ceil_div(a.rows, a.experts), 16 * TG), wgs = a.experts * (int64_t)a.blocks * chunks;
-  if (wgs > 0x7fffffff) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
+  if (wgs > 0x1ffffff) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
   const auto launch = [&](auto kernel, int nb, int waves) {
     NHIP_LAUNCH("linear8_rows", kernel, dim3((uint32_t)(a.experts * chunks * ceil_div(a.blocks, nb))), dim3(waves * 64), 0, s, a, (int)chunks);
     return check_launch("linear8_rows");
@@ -367,7 +367,7 @@ int linear8_args(const nhip_linear8_plan* p, int32_t dtype, int64_t rows) {
   if (!p) return fail(NHIP_STATUS_NULL_POINTER, "linear8: null plan");
   if (!elem_size(dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "linear8: dtype has to be F32, F16 or BF16");
   if (rows < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "linear8: negative extent");
-  if (rows > 0x7ffffeff) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many rows");
+  if (rows > kMaxRows) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many rows");
   return ok();
 }
 
@@ -388,7 +388,7 @@ int nhip_linear8_create(int32_t experts, int32_t num_output, int32_t num_input, 
   if (activation != NHIP_ACT_NONE && activation != NHIP_ACT_RELU && activation != NHIP_ACT_SILU)
     return fail(NHIP_STATUS_UNSUPPORTED, "linear8: activation has to be NONE, RELU or SILU");
   const int64_t blocks = ceil_div(num_output, 16), steps = ceil_div(num_input, kStepK);
-  if (experts * blocks > 0x7fffffff / 4 || experts * (int64_t)num_output > 0x7fffffff)
+  if (num_output > kMaxRows || experts * blocks > 0x7fffffff / 4 || experts * (int64_t)num_output > 0x7fffffff)
     return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many output channels");
   if (!weight || (weight_is_i8 && !weight_scale)) return fail(NHIP_STATUS_NULL_POINTER, "linear8: null pointer");
   if (!weight_is_i8 && weight_scale)
@@ -411,7 +411,7 @@ int nhip_linear8_create(int32_t experts, int32_t num_output, int32_t num_input, 
   const int64_t count = experts * (int64_t)num_output, items = experts * blocks * steps * 64;
   const auto build = [&]() -> int {
     NHIP_TRY(check_hip(hipGetDevice(&p->device), "hipGetDevice"));
-    if (ceil_div(items, 256) > 0x7fffffff) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many weights");
+    if (items > 0xffffff00) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many weights");
     NHIP_TRY(check_hip(hipMalloc(reinterpret_cast<void**>(&p->w), items * 16), "hipMalloc(linear8 weights)"));
     NHIP_TRY(check_hip(hipMalloc(reinterpret_cast<void**>(&p->w_scale), 2 * count * sizeof(float)), "hipMalloc(linear8 scales)"));
     if (weight_is_i8) {

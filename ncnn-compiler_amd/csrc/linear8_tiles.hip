@@ -27,7 +27,10 @@ struct Tile {
 typedef Tile<4, 2> Large;
 typedef Tile<2, 1> Small;  // a quarter of it
 constexpr int kRows = Large::kRows;
-constexpr int kGroup = 4;
+// Row tiles that are taken together (below).  us a call at 1 / 2 / 8: 6272 x 8192 of 2048
+// bf16 148 / 121 / 117, 8192 x 8192 of 8192 657 / 509 / 504, 2048 x 8192 of 4096 91 / 74 / 74;
+// 4 and 16 as 8.
+constexpr int kGroup = 8;
 
 // The expert and its row tile that tile `at` of all row tiles is: experts
 // without rows have none.  All 64 lanes call it.
@@ -234,7 +237,15 @@ __device__ __forceinline__ void tile_body(const Linear8Args& a, int e, int begin
   }
 }
 
-// Tiles id < large, then quarters of the tiles from `large` on.
+// Tiles id < large, then quarters of the tiles from `large` on: a last round of the
+// CUs' places that large tiles would fill to a quarter or less takes a quarter of its
+// time so (6272 x 8192 of 2048: 1568 tiles on 512 places).
+// Matrix instructions bound it, and the power they draw: 8192 x 8192 of 8192 504 us with
+// the codes (2180 TOPS; the library's product 2068), 6272 x 8192 of 2048 107 us without
+// (1970; 1647).  32 x 32 x 32 instructions ran at 4775 TOPS from registers on zeros and
+// 3400 on random codes, at a clock of some 1.7 GHz, 16 x 16 x 64 ones at 2590, so
+// large instructions; two workgroups of 4 waves a CU, so that one's results and starts
+// are beside the other's products.
 template <class T, int ACT, bool STREAM>
 __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work, int large) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -271,7 +282,7 @@ int tiles_launch(const Linear8Args& a, hipStream_t s) {
   const int64_t cols = ceil_div(a.blocks, Large::kCols / 16);
   // every expert's last tile may be a part of one
   const int64_t rows = ceil_div(a.rows, kRows) + (a.starts ? std::min(a.experts, a.rows) : 0);
-  if (rows * cols > 0x7fffff00 / 4) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
+  if (rows * cols > 0xff0000) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
   const int64_t work = rows * cols;
   const int64_t places = 2 * cu_count(), over = a.starts ? 0 : work % places;
   const int64_t small = over * 4 <= places ? over : 0, large = work - small;

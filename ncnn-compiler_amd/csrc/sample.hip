@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kBins = 1024;    // of weights' exponents, or of keys, or of indices
 constexpr int kSorted = 1024;  // tokens that are sorted at most
-constexpr int kOnce = 128;     // and for all filters at once, rather than about each one's border
+constexpr int kOnce = 128;     // and for all filters at once, rather than about each one's border (a sort of more takes barriers)
 constexpr float kRange = 31.5f;  // exp(-31.5) < 2^-45, which rounds to 0
 
 // What the launches before the last one leave of a row.
@@ -51,8 +51,8 @@ struct SampleArgs {
   RowParts* parts;  // [rows]
   uint32_t* lists;  // [rows][kLongList]: indices of tokens that may be kept
 };
-
 constexpr int kLongList = 16384;
+
 
 // Keys in the order of the values; -0 and 0 are equal.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -358,8 +358,9 @@ __device__ __forceinline__ uint64_t scan_bins(SampleLds<WAVES>& s, int lane, int
 
 constexpr int kPartWaves = 4;
 
-// The first of three launches for long rows: the largest logit of a part of a row, and
-// the bound on its share of the first k.
+// The first launch for long rows: the largest logit of a part of a row, and the bound
+// on its share of the first k.  Bytes bound it: 256 rows of 50021 fp32 10.4 us (51 MB, 4.9
+// TB/s), 64 of 131072 bf16 5.8 (16.8 MB, most of it a launch's start and end).
 template <class T>
 __global__ __launch_bounds__(kPartWaves * 64) void sample_top_kernel(SampleArgs a) {
   __shared__ uint2 part[kPartWaves];
@@ -413,7 +414,9 @@ __device__ __forceinline__ void list_tokens(const SampleArgs& a, int64_t r, cons
 
 // The second: of a part of a row the histogram that the row's border is first
 // looked for in, or without a filter the sums of its sets; of rows with top-k of few
-// the tokens that reach the bound.
+// the tokens that reach the bound.  The weights' arithmetic in 64 bits and the 64-bit
+// LDS atomics bound it (0.85 lanes of a CU a cycle, of 32 bits 1.7: counts have those):
+// 256 rows of 50021 fp32 by top-p 0.95 23.6 us, 64 of 131072 bf16, each its own filters, 10.9.
 template <class T>
 __global__ __launch_bounds__(kPartWaves * 64) void sample_bins_kernel(SampleArgs a) {
   __shared__ uint64_t bins[kBins];
@@ -468,6 +471,7 @@ __global__ __launch_bounds__(kPartWaves * 64) void sample_bins_kernel(SampleArgs
 }
 
 // The third, of rows with a histogram: the bin of the border, and the tokens up to it.
+// 64 rows of 131072 bf16 6.2 us: every workgroup sums the histogram before it reads.
 template <class T>
 __global__ __launch_bounds__(kPartWaves * 64) void sample_list_kernel(SampleArgs a) {
   __shared__ uint64_t part[kPartWaves];
@@ -524,6 +528,12 @@ __global__ __launch_bounds__(kPartWaves * 64) void sample_list_kernel(SampleArgs
 // further by the logits' bits, down to equal ones, of which the first by index are
 // kept.  The draw sums weights by index: of the tokens in LDS, or, if they do not
 // fit there, of all.
+//
+// A chain of steps between barriers bounds it, of which each has little to do: 64 rows
+// of 131072 bf16, each its own filters, 23 us behind the launches above; 16 of 1000 fp32 by
+// top-k 11.8 a call.  256 of 50021 fp32 by top-p 0.95, all in this launch, 67: the largest,
+// the histogram and the tokens that it leaves (some 9000) are a pass over the row each,
+// of one CU, and the tokens are summed twice.
 template <class T, int WAVES, bool PARTS>
 __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
   constexpr int TH = WAVES * 64;
@@ -1041,13 +1051,37 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
   finish();
 }
 
-// Workgroups that begin a row, 0: one does all of it.  us a call, one / several:
-// 16 rows of 30000 bf16 by top-p 0.9 42 / 31, of 64 x 131072 145 / 56, without a filter 61 /
-// 25, top-k of 50 33 / 25, the largest 16 / 19; four to a CU of all rows.
+// What of a filter all rows surely leave out.
+bool no_top_k(const nhip_sample_desc* d) { return !d->top_k_each && (d->top_k == 0 || d->top_k >= d->vocab); }
+bool no_top_p(const nhip_sample_desc* d) { return !d->top_p_each && d->top_p >= 1.f; }
+bool no_filter(const nhip_sample_desc* d) { return no_top_k(d) && no_top_p(d) && !d->min_p_each && d->min_p == 0.f; }
+
+// Workgroups that begin a row, 0: one does all of it.  They save of its passes over
+// the row what the other CUs can take, and cost two or three launches.  us a call, one /
+// several, rows x logits fp32 (bf16 alike but for 128 rows and more, which it reads faster):
+//            top-p 0.9           no filter           top-k of 3000       top-k of 50
+//           32768 65536 131072   32768 65536 131072  65536    131072     65536     131072
+//     1     28/23 46/27 80/34    22/17 38/17 68/17   32/29    53/37      24/25     31/28
+//    64     32/35 49/41 88/56    23/18 38/21 69/28   39/44    55/53      25/28     34/32
+//   128     32/39 51/51 107/86   23/21 39/29 79/45   40/54    73/77      26/31     45/48
+//   256     32/44 72/77 133/128  23/28 50/45 87/70   67/78   100/108     42/48     64/62
+// The largest alone (16 x 131072) 16 / 19.
 int chunks_of(const nhip_sample_desc* d) {
   const int force = setting_int("NHIP_SAMPLE_CHUNKS", -1);
   if (force >= 0) return std::min(force, 64);
-  if (d->vocab <= 16384 || (!d->temperature_each && d->temperature == 0.f)) return 0;
+  if (!d->temperature_each && d->temperature == 0.f) return 0;
+  const double cus = cu_count(), rows = std::max(d->rows, 1);
+  double per, cost, share = 1 - rows / cus;  // ns of a logit, us, of the passes
+  if (no_filter(d)) {
+    per = 0.38, cost = 8, share = std::max(0.5, 1 - rows / (2 * cus));  // (the last launch reads few)
+  } else if (!d->top_k_each && d->top_k > 0 && d->top_k < d->vocab) {
+    per = d->top_k <= kSorted ? 0.05 : 0.13, cost = d->top_k <= kSorted ? 6 : 9;
+  } else if (no_top_p(d) && no_top_k(d)) {  // min-p alone: as of few
+    per = 0.05, cost = 6;
+  } else {
+    per = 0.35, cost = 9;
+  }
+  if (per * 1e-3 * d->vocab * share < cost) return 0;
   const int64_t want = ceil_div(4 * cu_count(), std::max(d->rows, 1));
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, d->vocab / 2048, 64}));
 }
@@ -1066,17 +1100,25 @@ int sample_last(const SampleArgs& a, int rows, hipStream_t s) {
 }
 
 template <class T>
-int sample_run(const SampleArgs& a, int rows, hipStream_t s) {
-  if (!a.chunks) return a.vocab <= 8192 ? sample_last<T, 4, false>(a, rows, s) : sample_last<T, 16, false>(a, rows, s);
+int sample_run(const SampleArgs& a, const nhip_sample_desc* d, hipStream_t s) {
+  const int rows = d->rows;
+  // 16 waves a row, one row a CU, or 4, three a CU, where barriers cost more than the
+  // passes or the rows are more than the CUs.  us, 4 / 16: 16 rows of 4096 fp32 by top-k of
+  // 50 16.7 / 19.5, of 3000 21.5 / 17.7, top-p 0.9 20.5 / 22.4; of 16384 20.8 / 20.0, 36.6 / 27,
+  // 32.4 / 26.1; 1024 of 16384 51 / 83, 81 / 98, 73 / 97, of 32768 bf16 53 / 86, 95 / 124, 101 /
+  // 131; past that what top-p keeps seldom fits their part of LDS (512 of 131072 419 / 200).
+  if (!a.chunks)
+    return a.vocab <= (rows > cu_count() ? 32768 : 8192) ? sample_last<T, 4, false>(a, rows, s) : sample_last<T, 16, false>(a, rows, s);
   const dim3 grid((uint32_t)((int64_t)rows * a.chunks)), block(kPartWaves * 64);
   NHIP_LAUNCH("sample_top", (sample_top_kernel<T>), grid, block, 0, s, a);
   NHIP_TRY(check_launch("sample_top"));
   NHIP_LAUNCH("sample_bins", (sample_bins_kernel<T>), grid, block, 0, s, a);
   NHIP_TRY(check_launch("sample_bins"));
+  if (no_filter(d)) return sample_last<T, 4, true>(a, rows, s);  // (reads a 1024th of a row)
   // (no launch where the settings of all rows leave it nothing to do, nor where the
   // last launch has a workgroup for every CU to do it with: 64 rows of 131072 bf16, each
   // its own settings 50 us without, 45 with; 256 of 50021 fp32 74 and 79)
-  const bool some_k = a.top_k_each || a.top_k == 0 || a.top_k > kSorted, some_p = a.top_p_each || a.top_p < 1.f;
+  const bool some_k = a.top_k_each || a.top_k == 0 || a.top_k > kSorted, some_p = !no_top_p(d);
   const bool many_k = a.top_k_each || (a.top_k > kSorted && a.top_k < a.vocab);
   if (rows <= cu_count() / 2 && (a.temperature_each || a.temperature > 0.f) && some_k && (some_p || many_k)) {
     NHIP_LAUNCH("sample_list", (sample_list_kernel<T>), grid, block, 0, s, a);
@@ -1089,8 +1131,8 @@ int sample_args(const nhip_sample_desc* d) {
   if (!d) return fail(NHIP_STATUS_NULL_POINTER, "sample: null descriptor");
   if (!elem_size(d->dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "sample: dtype has to be F32, F16 or BF16");
   if (d->rows < 0 || d->vocab <= 0) return fail(NHIP_STATUS_INVALID_SHAPE, "sample: a row holds at least one logit");
-  // (2^19 weights of 2^44 each are the most that 64 bits sum)
-  if (d->vocab > 1 << 19 || d->rows > 1 << 24) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "sample: at most 2^24 rows of 2^19 logits");
+  // (2^19 weights of 2^44 each are the most that 64 bits sum; a launch has below 2^32 threads)
+  if (d->vocab > 1 << 19 || d->rows >= 1 << 22) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "sample: below 2^22 rows of at most 2^19 logits");
   if (d->row_stride < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "sample: negative stride");
   // (values that a tensor holds for each row are read on the device, where these mean the same as the nearest that is allowed)
   if (!(d->temperature >= 0.f) || d->top_k < 0 || !(d->top_p >= 0.f) || !(d->min_p >= 0.f) || d->min_p > 1.f)
@@ -1132,7 +1174,7 @@ int nhip_sample_forward(const nhip_sample_desc* desc, const void* logits, const 
                      desc->top_p,      desc->min_p,            desc->top_k,      desc->temperature_each,
                      desc->top_k_each, desc->top_p_each,       desc->min_p_each, token,            logprob,
                      chunks_of(desc),  tops, parts, (uint32_t*)(tops + (int64_t)desc->rows * chunks_of(desc))};
-  return NHIP_FOR_ELEM(desc->dtype, T, sample_run<T>(a, desc->rows, as_stream(stream)));
+  return NHIP_FOR_ELEM(desc->dtype, T, sample_run<T>(a, desc, as_stream(stream)));
 }
 
 }  // extern "C"

@@ -19,7 +19,7 @@ def forward(d, logits=ONE, uniform=ONE, token=ONE, logprob=ONE, ws=None, nbytes=
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(dtype=nhip.DTYPE_I8), 7), (dict(rows=-1), 2), (dict(vocab=0), 2), (dict(vocab=2 ** 19 + 1), 4), (dict(rows=2 ** 24 + 1), 4), (dict(row_stride=-1), 2),
+    (dict(dtype=nhip.DTYPE_I8), 7), (dict(rows=-1), 2), (dict(vocab=0), 2), (dict(vocab=2 ** 19 + 1), 4), (dict(rows=2 ** 22), 4), (dict(row_stride=-1), 2),
     (dict(temperature=-0.5), 3), (dict(temperature=float("nan")), 3), (dict(top_k=-1), 3), (dict(top_p=-1.0), 3),
     (dict(top_p=float("nan")), 3), (dict(min_p=-0.1), 3), (dict(min_p=1.1), 3), (dict(min_p=float("nan")), 3),
     (dict(temperature_each=ONE + 2), 3), (dict(top_k_each=ONE + 1), 3), (dict(top_p_each=ONE + 3), 3), (dict(min_p_each=ONE + 2), 3)])
