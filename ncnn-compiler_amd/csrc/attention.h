@@ -787,7 +787,8 @@ __global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs prefix, 
 // of 28 rows, 12544 and 1568 keys 211 and 185).  The products and the codes' conversion
 // bound it where a group has many rows (the latter 165 us without the join, fp16, 8 heads
 // of 128), waits for loads where it has few (4 groups of 64 rows, 3136 and 256 keys,
-// bf16 34 us; 51 MB).  OWN == 2 has too many registers for as many workgroups to a CU.
+// bf16 34 us; 51 MB read, 124 past the L2s: the dies' own or one's, the time is the same;
+// with the prefix first 2 us more).  OWN == 2 has too many registers for as many workgroups to a CU.
 template <class T, int DP, bool TILES, int OWN>
 __global__ __launch_bounds__(kWaves * 64, (TILES ? TilesShape<T, DP, kSrcInt8>::per_cu : rows_per_cu(sizeof(T), DP, kSrcInt8) - (OWN == 2 && DP == 128 && sizeof(T) == 2))) void
 attn_prefix_kernel(AttnArgs prefix, AttnArgs own, uint32_t own_wgs) {

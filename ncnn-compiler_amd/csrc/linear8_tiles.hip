@@ -237,9 +237,7 @@ __device__ __forceinline__ void tile_body(const Linear8Args& a, int e, int begin
   }
 }
 
-// Tiles id < large, then quarters of the tiles from `large` on: a last round of the
-// CUs' places that large tiles would fill to a quarter or less takes a quarter of its
-// time so (6272 x 8192 of 2048: 1568 tiles on 512 places).
+// Quarters of the first `small` tiles, then the other tiles whole.
 // Matrix instructions bound it, and the power they draw: 8192 x 8192 of 8192 504 us with
 // the codes (2180 TOPS; the library's product 2068), 6272 x 8192 of 2048 107 us without
 // (1970; 1647).  32 x 32 x 32 instructions ran at 4775 TOPS from registers on zeros and
@@ -247,7 +245,7 @@ __device__ __forceinline__ void tile_body(const Linear8Args& a, int e, int begin
 // large instructions; two workgroups of 4 waves a CU, so that one's results and starts
 // are beside the other's products.
 template <class T, int ACT, bool STREAM>
-__global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work, int large) {
+__global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Args a, int col_tiles, int work, int small) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const auto place = [&](int id, int& e, int& begin, int& end, int& b0) {
     // blocks of kGroup row tiles, so that what a die's CUs work on at a time are
@@ -258,15 +256,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void linear8_tiles_kernel(Linear8Ar
     b0 = col * (Large::kCols / 16);
     return find_tile(a, band * kGroup + in - col * high, e, begin, end);
   };
+  // workgroups go to the eight dies in turn: each die gets a run of the tiles
+  const auto run = [](int block, int blocks) { return (block & 7) * (blocks >> 3) + (block >> 3); };
+  const int smalls = round_up8(4 * small);
   int e, begin, end, b0;
-  if ((int)blockIdx.x < round_up8(large)) {
-    // workgroups go to the eight dies in turn: each die gets a run of the tiles
-    const int id = (blockIdx.x & 7) * (round_up8(large) >> 3) + (blockIdx.x >> 3);
-    if (id >= large || !place(id, e, begin, end, b0)) return;
+  if ((int)blockIdx.x >= smalls) {
+    const int id = small + run(blockIdx.x - smalls, gridDim.x - smalls);
+    if (id >= work || !place(id, e, begin, end, b0)) return;
     tile_body<Large, 4, 2, T, ACT, STREAM>(a, e, begin, end, b0, lds);
   } else {
-    const int id = blockIdx.x - round_up8(large);
-    if (!place(large + (id >> 2), e, begin, end, b0)) return;
+    const int id = run(blockIdx.x, smalls);
+    if (id >= 4 * small || !place(id >> 2, e, begin, end, b0)) return;
     begin += (id & 1) * Small::kRows;
     b0 += (id >> 1 & 1) * (Small::kCols / 16);
     if (begin >= end || b0 >= a.blocks) return;
@@ -285,9 +285,18 @@ int tiles_launch(const Linear8Args& a, hipStream_t s) {
   if (rows * cols > 0xff0000) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "linear8: too many tiles");
   const int64_t work = rows * cols;
   const int64_t places = 2 * cu_count(), over = a.starts ? 0 : work % places;
-  const int64_t small = over * 4 <= places ? over : 0, large = work - small;
-  NHIP_LAUNCH("linear8_tiles", (linear8_tiles_kernel<T, ACT, STREAM>), dim3((uint32_t)(round_up(large, 8) + 4 * small)), dim3(kWaves * 64),
-              bytes, s, a, (int)cols, (int)work, (int)large);
+  // A round of the CUs' places that whole tiles would fill to a quarter or less takes
+  // about a quarter of its time so: 6272 x 8192 of 2048 bf16 (1568 tiles on 512 places) 125.6 us
+  // without, 120.7 with.  Where sums are short, storing takes a good part of a tile's time, and
+  // the places all store at once unless some begin with a part: without / with an eighth of
+  // the places' number 6272 x 4096 of 1024 52.8 / 46.7, 12544 x 4096 of 1024, 32 experts 108.2 /
+  // 103.5, 6000 x 4096 of 512 34.8 / 33.8; not in longer ones, 25088 x 2048 of 2048 133 / 133,
+  // 6272 x 8192 of 2048 120.9 / 122.7, nor in one round, 12544 x 1024 of 2048 52.9 / 59.2.
+  int64_t small = over * 4 <= places ? over : 0;
+  if (work > places && a.steps <= 16) small = std::max(small, places / 8);
+  const int64_t large = work - small;
+  NHIP_LAUNCH("linear8_tiles", (linear8_tiles_kernel<T, ACT, STREAM>), dim3((uint32_t)(round_up(4 * small, 8) + round_up(large, 8))), dim3(kWaves * 64),
+              bytes, s, a, (int)cols, (int)work, (int)small);
   return check_launch("linear8_tiles");
 }
 

@@ -55,7 +55,7 @@ def test_product(nhip_env, rows, k, n, dtype, tiles):
 
 
 @pytest.mark.parametrize("rows,k,n", [(16, 8192, 40), (9, 8200, 17), (1, 4100, 33), (16, 2049, 9000), (7, 33, 20000), (3000, 64, 3000),
-                                      (49, 300, 40000), (40, 300, 70000), (700, 8192, 100)])
+                                      (49, 300, 40000), (40, 300, 70000), (700, 8192, 100), (16, 2048, 40), (5, 2000, 8192)])
 def test_kernels_of_few_and_many(rows, k, n):
     """Sizes on either side of the rules that choose a kernel."""
     gen = torch.Generator().manual_seed(rows)

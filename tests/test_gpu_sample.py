@@ -126,7 +126,7 @@ def test_each_row_its_own(nhip_env, dtype, chunks):
     check(got, logits, u, settings)
 
 
-@pytest.mark.parametrize("chunks", ["0", "-1"])
+@pytest.mark.parametrize("chunks", ["0", "-1", "4"])
 @pytest.mark.parametrize("spread", [0.0, 1e-3, 30.0, 3000.0])
 def test_spreads(nhip_env, spread, chunks):
     """Logits that are all alike, hardly apart (borders lie among thousands of neighbours), or very far apart."""
