@@ -346,8 +346,9 @@ int nhip_dequantize_i32_f32(const int32_t* input, float* output, int32_t n,
  * The reference lowers ncnn's own attention layers for the CPU
  * (lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:3859-4668); these are calls, not
  * layers of a graph, with the forms that serving needs (shared heads, lengths,
- * pages, 16-bit types).  Group norm into tokens, rotary positions and the
- * 8-bit cache have no counterpart there.
+ * pages, 16-bit types).  Group norm into tokens, rotary positions, the 8-bit
+ * cache, products of tokens in 8-bit integers and the draw of a token have no
+ * counterpart there.
  * All pointers are device pointers unless said otherwise; `dtype` is
  * NHIP_DTYPE_F32, F16 or BF16 and holds for every tensor of a call but the
  * integer ones.  Sums, softmax statistics and angles are held in fp32 or

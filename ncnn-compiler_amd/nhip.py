@@ -12,10 +12,10 @@ Layer objects mirror the reference's ncnn layer parameters
 reference's single-image [C,H,W] blobs.
 
 Behind the layers stand the token operators, for a decoder that reads a
-network's features: GroupNorm, Rotary, cross_attention and KvCache8 (float32,
-float16 and bfloat16).  The reference lowers ncnn's attention layers for the CPU
-(lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:3859-4668); these are calls, not layers
-of a graph, and the other three have no counterpart there.
+network's features: GroupNorm, Rotary, cross_attention, KvCache8, Linear8 and
+sample (float32, float16 and bfloat16).  The reference lowers ncnn's attention
+layers for the CPU (lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:3859-4668); these are
+calls, not layers of a graph, and the others have no counterpart there.
 """
 from __future__ import annotations
 
