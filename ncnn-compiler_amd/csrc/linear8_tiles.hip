@@ -292,7 +292,10 @@ int tiles_launch(const Linear8Args& a, hipStream_t s) {
   // the places' number 6272 x 4096 of 1024 52.8 / 46.7, 12544 x 4096 of 1024, 32 experts 108.2 /
   // 103.5, 6000 x 4096 of 512 34.8 / 33.8; not in longer ones, 25088 x 2048 of 2048 133 / 133,
   // 6272 x 8192 of 2048 120.9 / 122.7, nor in one round, 12544 x 1024 of 2048 52.9 / 59.2.
-  int64_t small = over * 4 <= places ? over : 0;
+  // Few tiles in all, each expert's counted with a part of one: quarters for every one, 3356
+  // rows of 5792 over 20 experts to 320 fp32 (94 tiles) 38.3 / 27.2, 2000 of 1024 over 8 to 1024
+  // bf16 14.1 / 11.0; not for more than a quarter of the places, 3000 x 1500 of 8192 54 / 67.
+  int64_t small = work * 4 <= places ? work : over * 4 <= places ? over : 0;
   if (work > places && a.steps <= 16) small = std::max(small, places / 8);
   const int64_t large = work - small;
   NHIP_LAUNCH("linear8_tiles", (linear8_tiles_kernel<T, ACT, STREAM>), dim3((uint32_t)(round_up(4 * small, 8) + round_up(large, 8))), dim3(kWaves * 64),
