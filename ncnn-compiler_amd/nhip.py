@@ -1091,8 +1091,9 @@ class KvCache8:
         """Attention of q [batch, queries, heads, head_dim] where batch / groups
         sequences in a row share a prefix: the first prefix_lengths[g] tokens of
         the pages in prefix_table [groups, pages], and behind them the first
-        lengths[b] of the sequence's own pages in block_table.  causal: the
-        queries are the last of the sequence's own tokens."""
+        lengths[b] of the sequence's own pages in block_table (at most max_prefix
+        and max_length; default what the tables hold).  causal: the queries are the
+        last of the sequence's own tokens."""
         b, lq, h, d = q.shape
         code, dev = _elem(q)
         if d != self.head_dim or dev != self._dev:
