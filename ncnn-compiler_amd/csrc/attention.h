@@ -783,7 +783,7 @@ __global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs prefix, 
 // prefix, whose rows are those of a whole group of sequences, so that its keys are
 // read and converted once for all of them.  Each workgroup is one of the kernels above, and its
 // result a part; one launch because either alone leaves CUs idle (one group of 5
-// sequences, 12 heads of 64, 197 and 37 keys fp32 20.4 us a call in two, 14.1 in one; 48
+// sequences, 12 heads of 64, 197 and 37 keys fp32 20.4 us a call in two, 14.1 in one, the prefix whole; 48
 // of 28 rows, 12544 and 1568 keys 211 and 185).  The products and the codes' conversion
 // bound it where a group has many rows (the latter 165 us without the join, fp16, 8 heads
 // of 128), waits for loads where it has few (4 groups of 64 rows, 3136 and 256 keys,

@@ -191,6 +191,15 @@ int prefix_args(const nhip_attention_desc* d, int32_t groups, int32_t prefix_key
   shared.queries = (int32_t)(members * d->queries);
   shared.keys = prefix_keys;
   NHIP_TRY(attn_args(&shared, true, true, prefix, prefix_choice(shared)));
+  if (!prefix->tiles) {
+    // Few rows: parts are joined in any case, so up to 16 of at least 128 keys, until there
+    // is a workgroup for every CU.  us a call, parts of 512 keys / so: one row of 16 heads on 4
+    // to 400 keys bf16 17.3 / 13.5, 16 to 800 18.3 / 14.6, 4 groups of 4 rows of 4 heads on 1 to
+    // 300 16.1 / 13.8; with three workgroups a CU 8 heads of 8 groups to 1311 18.3 / 21.1.  Own keys
+    // are left in longer parts: the 64 sequences of 256 behind 3136 38.3 / 42.1.
+    const int64_t wgs = std::max<int64_t>(1, (int64_t)prefix->batch * prefix->kv_heads * prefix->row_tiles);
+    prefix->splits = (int)std::max<int64_t>(prefix->splits, std::min<int64_t>({(cu_count() + wgs / 2) / wgs, ceil_div(prefix_keys, 128), 16}));
+  }
   prefix->parts = own->parts = 1;
   prefix->per = d->queries;
   // launches of below 2^32 threads

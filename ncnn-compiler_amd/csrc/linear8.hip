@@ -170,11 +170,20 @@ __global__ __launch_bounds__(256) void linear8_params_kernel(const float* scale,
 // One workgroup: NB blocks of 16 channels of one expert, 16 TG of its rows, and if
 // the expert has more than its share the rows `chunks` times as far on; its waves take
 // the steps of the sum in turn and are joined in LDS.  Weights go from memory to the
-// registers that the products read, past the caches, every wave's next kAhead steps
-// under way at a time.  Reading them bounds it: 48 rows of 2048 to 50021 fp16 27 us for
-// 102 MB (3.8 TB/s; a large copy 5.1) and 5 for the codes; where an expert has few rows,
-// latency (128 rows of 16 experts, 2048 to 1024 12.1 us, 34 MB).
+// registers that the products read, every wave's next kAhead steps under way at a time.
+// Reading them bounds it: 48 rows of 2048 to 50021 fp16 27 us for 102 MB (3.8 TB/s; a
+// large copy 5.1) and 5 for the codes; where an expert has few rows, latency (128 rows of
+// 16 experts, 2048 to 1024 12.1 us, 34 MB).
 constexpr int kAhead = 4;  // steps that a wave reads before it multiplies them
+// Weights take no place in the caches where each is read once.  With more than 48 rows
+// to an expert others read them too, or the next to it: us past the caches / through
+// them, three layers in turn, 64 rows of 4096 to 16384 25.9 / 24.4, 319 of 1920 over 6
+// experts to 7488 36.7 / 31.4, 1200 of 8192 to 528 34.8 / 25.7; 48 of 2048 to 50021 31.2 / 32.9.
+template <bool ONCE>
+__device__ __forceinline__ v4i load_w(const int8_t* w) {
+  const v4i* const at = reinterpret_cast<const v4i*>(w);
+  return ONCE ? __builtin_nontemporal_load(at) : *at;
+}
 template <class T, int ACT, int TG, int NB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a, int chunks) {
   __shared__ v4i part[WAVES][TG * NB][64];
@@ -203,7 +212,7 @@ __global__ __launch_bounds__(WAVES * 64) void linear8_rows_kernel(Linear8Args a,
       for (int u = 0; u < kAhead; ++u) {
         const int at = min(s + u * WAVES, a.steps - 1);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) wf[u][b] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(w[b] + at * 1024));
+        for (int b = 0; b < NB; ++b) wf[u][b] = load_w<TG < 4>(w[b] + at * 1024);
 #pragma unroll
         for (int t = 0; t < TG; ++t) xf[u][t] = *reinterpret_cast<const v4i*>(x[t] + at * 1024);
       }

@@ -315,9 +315,10 @@ bool linear8_tiles_selected(const Linear8Args& a) {
   if (force >= 0) return force != 0;
   // Few tiles leave CUs idle and each walks the whole sum alone; the other kernel has
   // a workgroup for 64 rows and 16 channels, whose waves share the sum, and reads
-  // the operands more often.  us a call, it / this: 200 x 1000 of 8192 (32 quarter
-  // tiles) bf16 27 / 41, 400 x 1000 (56) 43 / 41, 100 x 4096 (64) 33 / 45, 200 x 4096
-  // (128) 41 / 44, 400 x 4096 (224) 67 / 46, 1600 x 1000 of 2048 (200) 25 / 16.
+  // the operands more often.  us, it / this, bf16: 300 x 1000 of 8192 (40 quarter tiles) 18.6 /
+  // 27.6, 600 x 1000 (80) 23.1 / 30.6, 1200 x 1000 (152) 28.6 / 31.5, 2400 x 528 (190) 35.8 /
+  // 30.1; of 3600 15.0 / 17.1 (80), 18.8 / 17.7 (152), 21.6 / 17.5 (190); of 1024 7.7 / 8.8 (40),
+  // 9.4 / 9.1 (80), 11.3 / 9.1 (152), 12.4 / 9.5 (190).
   return a.rows > 64 * (int64_t)a.experts && ceil_div(a.rows, Small::kRows) * ceil_div(a.blocks, Small::kCols / 16) > cu_count() / 2;
 }
 
