@@ -935,7 +935,8 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
   }
 
   if (listed && n <= kOnce) {
-    // ------------------------- all that may be kept, sorted: every filter at once
+    // ------------------------- all that may be kept, sorted: every filter at once (a listed
+    // token may lie outside, by the margin of `least`, and takes no place in the order)
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += TH) s.sorted[i] = inside_place(s.list[i]) ? s.list[i] : 0;
     __syncthreads();
@@ -948,7 +949,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     __syncthreads();
     for (int i = threadIdx.x; i < first; i += TH) {
       const uint64_t before = i ? s.bins[i - 1] : 0;
-      if ((double)before < limit && !too_light(s.bins[i] - before)) atomicMax(&s.at, i + 1);
+      if (s.bins[i] != before && (double)before < limit && !too_light(s.bins[i] - before)) atomicMax(&s.at, i + 1);
     }
     __syncthreads();
     const uint64_t place = s.sorted[s.at - 1];

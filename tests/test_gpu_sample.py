@@ -207,6 +207,22 @@ def test_settings_out_of_range():
     check(nhip.sample(logits.cuda(), u.cuda(), *(v.cuda() for v in given)), logits, clamped, means)
 
 
+@pytest.mark.parametrize("chunks", ["0", "5"])
+@pytest.mark.parametrize("vocab", [60, 3000, 20011])
+def test_next_to_weightless(nhip_env, vocab, chunks):
+    """Tokens as far from the largest as weights are not 0, to a rounding of fp32: fewer than top_k weigh anything."""
+    nhip_env.setenv("NHIP_SAMPLE_CHUNKS", chunks)
+    for top, near, low, temperature in ((20.0, 16.84999, -50.0, 0.1), (100000.0, 99999.65, 0.0, 0.01), (-7000.0, -7031.5005, -8000.0, 1.0)):
+        logits = torch.full((8, vocab), low)
+        logits[:, 41] = top
+        logits[:4, 7] = near
+        logits[4:, 20:40] = near
+        u = torch.tensor([0.0, 0.3, 0.9, 0.999] * 2)
+        for top_k, top_p, min_p in ((2, 1.0, 0.0), (20, 1.0, 0.0), (50, 1.0, 0.0), (50, 0.9, 0.0), (50, 1.0, 1e-3), (0, 0.9, 0.0), (0, 1.0, 0.0)):
+            token, logprob = nhip.sample(logits.cuda(), u.cuda(), temperature, top_k, top_p, min_p)
+            assert (token == 41).all() and (logprob.abs() < 1e-9).all(), (top, top_k, top_p, token, logprob)
+
+
 def test_refusals():
     x, u = torch.zeros((4, 50), device="cuda"), torch.zeros(4, device="cuda")
     for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=-0.1), dict(min_p=1.5),
