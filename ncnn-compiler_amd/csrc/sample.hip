@@ -247,7 +247,7 @@ struct Distances {
   float half_top, reach, scope;
   __device__ __forceinline__ Distances(float top, const Settings& c) {
     half_top = 0.5f * top;
-    reach = fminf(0.5f * kRange * c.temperature, 3.4e38f);
+    reach = fminf(0.5f * kRange * c.temperature, 3.4028235e38f);  // (finite: -infinity stays outside)
     const float near = 6.f - 2.5f * __logf(fmaxf(1.f - c.top_p, 1e-6f));
     scope = c.k < 0x7fffffff && c.top_p < 1.f ? fminf(reach, 0.5f * near * c.temperature) : reach;
   }

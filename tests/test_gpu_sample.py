@@ -223,6 +223,20 @@ def test_next_to_weightless(nhip_env, vocab, chunks):
             assert (token == 41).all() and (logprob.abs() < 1e-9).all(), (top, top_k, top_p, token, logprob)
 
 
+@pytest.mark.parametrize("chunks", ["0", "5"])
+def test_farthest_logits(nhip_env, chunks):
+    """Logits at either end of fp32, at temperatures that leave both some weight."""
+    nhip_env.setenv("NHIP_SAMPLE_CHUNKS", chunks)
+    most = torch.finfo(torch.float32).max
+    for vocab in (50, 9001):
+        logits = torch.full((6, vocab), -most)
+        logits[:, 3] = most
+        logits[2:4, 5::2] = 0
+        u = torch.tensor([0.2, 0.999, 0.5, 0.99, 0.7, 0.05])
+        for settings in ((1e38, 0, 1.0, 0.0), (3e38, 0, 0.999, 0.0), (3e38, 40, 1.0, 0.0), (2e38, 0, 1.0, 0.01), (3e38, 2000, 0.99, 0.0)):
+            check(nhip.sample(logits.cuda(), u.cuda(), *settings), logits, u, settings)
+
+
 def test_refusals():
     x, u = torch.zeros((4, 50), device="cuda"), torch.zeros(4, device="cuda")
     for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=-0.1), dict(min_p=1.5),
