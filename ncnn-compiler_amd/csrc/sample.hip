@@ -6,9 +6,10 @@
 // kept is all up to one (logit, index) pair, and is found without sorting the
 // row.  Weights exp((l - largest) / T) are formed in 64 bits and held as whole
 // multiples of 2^-44: their sums are exact and the same in any order, so results
-// do not depend on which atomic came first, and a token next to a border is on
-// the side where the exact sums put it (but for those 2^-45).  A weight that
-// rounds to 0 is never drawn.
+// do not depend on which atomic came first.  What they are compared with, top-p's
+// and the uniform number's share of a sum, is rounded to the whole number that
+// decides the same, so a token next to a border is on the side where the exact sums
+// of these weights put it.  A weight that rounds to 0 is never drawn.
 #include <algorithm>
 
 #include "elem.h"
@@ -89,6 +90,22 @@ struct Weights {
     return __builtin_bit_cast(uint64_t, fma(p, __builtin_bit_cast(double, t), 4503599627370496.0)) & ((uint64_t(1) << 52) - 1);
   }
 };
+
+// f n, 0 < f < 1, rounded down or up to a whole number: f is 24 bits times a power of 2.
+__device__ __forceinline__ uint64_t share_of(uint64_t n, float f, bool up) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, f), exponent = max(bits >> 23, 1u);
+  const uint64_t m = (bits & 0x7fffffu) | (bits >> 23 ? 0x800000u : 0u);
+  const uint64_t low = n * m, high = __umul64hi(n, m);  // of n m, below 2^88
+  const uint32_t shift = 150 - exponent;                // 24 to 149
+  if (shift < 64) return (high << (64 - shift) | low >> shift) + (up && low << (64 - shift));
+  if (shift == 64) return high + (up && low);
+  const uint64_t q = shift < 128 ? high >> (shift - 64) : 0;
+  return q + (up && (low || (shift < 128 ? high << (128 - shift) : high)));
+}
+// The least sum that reaches top-p's share: a token stays if less comes before it (and the first always).
+__device__ __forceinline__ uint64_t limit_of(uint64_t total, float top_p) {
+  return top_p > 0.f ? max(share_of(total, top_p, true), uint64_t(1)) : 1;
+}
 
 // Sums of the lanes up to each, by moves inside the vector unit: within rows of 16
 // lanes, then the rows' last lanes.
@@ -487,7 +504,7 @@ __global__ __launch_bounds__(kPartWaves * 64) void sample_list_kernel(SampleArgs
   uint64_t v[EACH], sum = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) v[i] = sum += a.parts[r].bins[threadIdx.x * EACH + i];
-  const double limit = c.k < a.vocab ? (double)c.k : fmax((double)c.top_p * (double)a.parts[r].total, 1.0);
+  const uint64_t limit = c.k < a.vocab ? (uint64_t)c.k : limit_of(a.parts[r].total, c.top_p);
   const uint64_t upto = wave_scan(sum);
   if (lane == 63) part[wave] = upto;
   if (threadIdx.x == 0) found = -1;
@@ -499,11 +516,11 @@ __global__ __launch_bounds__(kPartWaves * 64) void sample_list_kernel(SampleArgs
     all += part[w];
   }
   // (no border: all are kept, or it lies past the histogram)
-  if ((double)all < limit || (c.k < a.vocab && all <= (uint64_t)c.k)) return;
+  if (all < limit || (c.k < a.vocab && all == limit)) return;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const uint64_t ahead = before + (i ? v[i - 1] : 0);
-    if ((double)(before + v[i]) >= limit && (double)ahead < limit) {
+    if (before + v[i] >= limit && ahead < limit) {
       found = threadIdx.x * EACH + i;
       if (chunk == 0) {
         a.parts[r].before = ahead;
@@ -580,9 +597,9 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
   }
   const Distances d(top, c);
   const Weights weight{(double)top, 64 * 1.4426950408889634074 / (double)(c.temperature > 0.f ? c.temperature : 1.f), s.table};
-  const double u = fmin(fmax((double)a.uniform[r], 0.0), 1.0 - 0x1p-53);  // NaN: 0
-  // the first whose cumulated weight is past this
-  const auto target_of = [&](uint64_t total) { return min((uint64_t)((double)total * u), total - 1); };
+  const float u = a.uniform[r];
+  // the first whose cumulated weight is past this (NaN: 0)
+  const auto target_of = [&](uint64_t total) { return u >= 1.f ? total - 1 : u > 0.f ? share_of(total, u, false) : 0; };
   const auto too_light = [&](uint64_t w) { return (double)w * 0x1p-44 < (double)c.min_p; };
   // one thread has found the token; all call the second
   const auto found = [&](int index, float l, uint64_t total) {
@@ -674,7 +691,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
   if (top == INFINITY) {
     // infinite ones weigh the same, others nothing
     const int64_t all = min(count_equal(top), (int64_t)k);
-    const int kept = (int)fmin(fmax(c.top_p < 1.f ? ceil((double)c.top_p * (double)all) : (double)all, 1.0), (double)all);
+    const int kept = (int)(c.top_p < 1.f ? limit_of(all, c.top_p) : all);
     const uint64_t total = (uint64_t)kept << 44;
     find_equal(top, (int)(target_of(total) >> 44) + 1);
     if (threadIdx.x == 0) found(s.at, top, total);
@@ -750,7 +767,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     if (listed && n <= kOnce) break;  // all in one go, below
     const auto measure = [&](float l) { return by ? weight(l) : (uint64_t)1; };
     float scope = d.reach;
-    double limit;
+    uint64_t limit;
     uint64_t before = 0;                   // the measure of what comes before the present bin
     uint32_t low = 0, high = 0xffffffffu;  // its keys
     int bin = -1, shift = 0;               // its bin of weights
@@ -758,7 +775,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     if (begun && a.parts[r].found) {
       scope = by ? d.scope : d.reach;
       if (by) mass = a.parts[r].total;
-      limit = by ? fmax((double)c.top_p * (double)mass, 1.0) : (double)k;
+      limit = by ? limit_of(mass, c.top_p) : (uint64_t)k;
       before = a.parts[r].before;
       bin = (int)a.parts[r].found - 1;
       listed = collect_listed();
@@ -804,12 +821,12 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
 #pragma unroll
           for (int w = 0; w < WAVES; ++w) all += s.part[w];
         }
-        limit = by ? fmax((double)c.top_p * (double)all, 1.0) : (double)k;  // (the first one always)
+        limit = by ? limit_of(all, c.top_p) : (uint64_t)k;
         if (by) mass = all;
-        if (scope == d.reach || (double)s.bins[kBins - 1] >= limit) break;
+        if (scope == d.reach || s.bins[kBins - 1] >= limit) break;
       }
       // kept: those with less than `limit` before them; the last of them lies in the bin that reaches it
-      if ((double)s.bins[kBins - 1] < limit || (by == 0 && s.bins[kBins - 1] <= (uint64_t)k)) continue;
+      if (s.bins[kBins - 1] < limit || (by == 0 && s.bins[kBins - 1] == limit)) continue;
     }
     const float rate = (float)kBins / scope;
     for (bool first = bin < 0, again = false;; again = true) {
@@ -819,7 +836,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
         if (threadIdx.x == 0) s.at = kBins - 1;
         __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += TH)
-          if ((double)(before + s.bins[i]) >= limit && !(i && (double)(before + s.bins[i - 1]) >= limit)) s.at = i;
+          if (before + s.bins[i] >= limit && !(i && before + s.bins[i - 1] >= limit)) s.at = i;
         __syncthreads();
         const int at = s.at;
         before += at ? s.bins[at - 1] : 0;
@@ -872,7 +889,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
           const uint64_t m = lane < count ? measure(of_key((uint32_t)(place >> 32))) : 0;
           const uint64_t ahead = before_me(place, m, count);
           // the last of those that stay has the most before it
-          const bool stays = m && (double)(before + ahead) < limit;
+          const bool stays = m && before + ahead < limit;
           if (lane == 0) s.total = 0;
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           if (stays) atomicMax((unsigned long long*)&s.total, (unsigned long long)ahead + 1);
@@ -891,7 +908,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
         if (threadIdx.x == 0) s.at = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < count; i += TH)
-          if ((double)(before + (i ? s.bins[i - 1] : 0)) < limit) atomicMax(&s.at, i);
+          if (before + (i ? s.bins[i - 1] : 0) < limit) atomicMax(&s.at, i);
         __syncthreads();
         const uint64_t place = s.sorted[s.at];
         last = of_key((uint32_t)(place >> 32));
@@ -910,7 +927,8 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
       if (low == high) {
         // one value: the first so many by index (of those that top-k has left)
         const float value = of_key(low);
-        const int keep = (int)fmax(1.0, fmin(ceil((limit - (double)before) / (double)measure(value)), (double)count));
+        const uint64_t each = max(measure(value), uint64_t(1));
+        const int keep = (int)min((limit - before + each - 1) / each, (uint64_t)count);
         count_equal(value);
         find_equal(value, keep);
         last = value;
@@ -944,12 +962,12 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     const int first = min(n, k);
     const uint64_t sum = sum_sorted(first, weight_of);
     if (!mass) mass = sum;  // (the list holds the first k)
-    const double limit = c.top_p < 1.f ? fmax((double)c.top_p * (double)mass, 1.0) : INFINITY;  // (the first one always)
+    const uint64_t limit = c.top_p < 1.f ? limit_of(mass, c.top_p) : ~uint64_t(0);
     if (threadIdx.x == 0) s.at = 1;
     __syncthreads();
     for (int i = threadIdx.x; i < first; i += TH) {
       const uint64_t before = i ? s.bins[i - 1] : 0;
-      if (s.bins[i] != before && (double)before < limit && !too_light(s.bins[i] - before)) atomicMax(&s.at, i + 1);
+      if (s.bins[i] != before && before < limit && !too_light(s.bins[i] - before)) atomicMax(&s.at, i + 1);
     }
     __syncthreads();
     const uint64_t place = s.sorted[s.at - 1];

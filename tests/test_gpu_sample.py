@@ -1,4 +1,6 @@
 """Drawing the next token (sample) against its definition in 64 bits."""
+from fractions import Fraction
+
 import numpy as np
 import pytest
 
@@ -235,6 +237,55 @@ def test_farthest_logits(nhip_env, chunks):
         u = torch.tensor([0.2, 0.999, 0.5, 0.99, 0.7, 0.05])
         for settings in ((1e38, 0, 1.0, 0.0), (3e38, 0, 0.999, 0.0), (3e38, 40, 1.0, 0.0), (2e38, 0, 1.0, 0.01), (3e38, 2000, 0.99, 0.0)):
             check(nhip.sample(logits.cuda(), u.cuda(), *settings), logits, u, settings)
+
+
+def whole(logit):
+    """The weight of a logit as a whole multiple of 2^-44, None next to a half: 64 bits leave 2^-7 of it uncertain."""
+    w = np.exp(float(logit)) * 2.0 ** 44
+    return None if abs(w - np.floor(w) - 0.5) < 0.05 else int(np.rint(w))
+
+
+def draw_exactly(weights, order, top_p, u):
+    """(token, kept) by whole numbers and fractions alone."""
+    total, before, kept = sum(weights), 0, []
+    for i in order:
+        if top_p >= 1 or before < Fraction(top_p) * total or not kept:
+            kept.append(i)
+        before += weights[i]
+    target, upto = Fraction(u) * sum(weights[i] for i in kept), 0
+    for i in sorted(kept):
+        upto += weights[i]
+        if upto > target:
+            return i, kept
+    raise AssertionError
+
+
+@pytest.mark.parametrize("chunks", ["0", "3"])
+@pytest.mark.parametrize("off", [2, -2, 6])
+@pytest.mark.parametrize("spread", [(0.01, 0.01), (0.001, 0.001), (0.02, 0.6)])
+def test_borders_of_large_sums(nhip_env, spread, off, chunks):
+    """Sums past 2^53 units, off from a border by less than a 64-bit float holds: 1024 logits of 0, the others weigh
+    2^54 + off together (chosen one by one to that), so that half of all lies off / 2 beyond the first 1024."""
+    nhip_env.setenv("NHIP_SAMPLE_CHUNKS", chunks)
+    left, rest = 2 ** 54 + off, []
+    low = np.linspace(*spread, 2048).astype(np.float32)
+    while left:
+        at = min(-low[len(rest)], np.float32(np.log(left * 2.0 ** -44)))
+        while whole(at) is None or whole(at) > left:
+            at = np.nextafter(at, np.float32(-100))
+        rest.append(at)
+        left -= whole(at)
+    logits = torch.cat([torch.zeros(1024), torch.from_numpy(np.array(rest, dtype=np.float32))])
+    weights = [whole(v) for v in logits]
+    assert sum(weights) == 2 ** 55 + off
+    order = sorted(range(len(weights)), key=lambda i: (-float(logits[i]), i))
+    for settings, us in (((1.0, 0, 0.5, 0.0), (0.5, 1 - 2.0 ** -24)), ((1.0, 0, 1.0, 0.0), (0.5, 0.25))):
+        u = torch.tensor(us)
+        token, logprob = nhip.sample(logits.repeat(2, 1).cuda(), u.cuda(), *settings)
+        for r in range(2):
+            want, kept = draw_exactly(weights, order, settings[2], us[r])
+            assert int(token[r]) == want, (settings, us[r])
+            assert abs(float(logprob[r]) - (float(logits[want]) - np.log(sum(weights[i] for i in kept) * 2.0 ** -44))) < 2e-6
 
 
 def test_refusals():
