@@ -1074,6 +1074,12 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
 bool no_top_k(const nhip_sample_desc* d) { return !d->top_k_each && (d->top_k == 0 || d->top_k >= d->vocab); }
 bool no_top_p(const nhip_sample_desc* d) { return !d->top_p_each && d->top_p >= 1.f; }
 bool no_filter(const nhip_sample_desc* d) { return no_top_k(d) && no_top_p(d) && !d->min_p_each && d->min_p == 0.f; }
+// Rows of which the largest alone counts, or all that min-p leaves, have neither a histogram nor a list.
+bool greedy(const nhip_sample_desc* d) {
+  return (!d->temperature_each && d->temperature == 0.f) || (!d->top_k_each && d->top_k == 1);
+}
+bool has_lists(const nhip_sample_desc* d) { return !greedy(d) && !(no_top_k(d) && no_top_p(d)); }
+bool has_bins(const nhip_sample_desc* d) { return !greedy(d) && (has_lists(d) || no_filter(d)); }
 
 // Workgroups that begin a row, 0: one does all of it.  They save of its passes over
 // the row what the other CUs can take, and cost two or three launches.  us a call, one /
@@ -1084,7 +1090,7 @@ bool no_filter(const nhip_sample_desc* d) { return no_top_k(d) && no_top_p(d) &&
 //    64     32/35 49/41 88/56    23/18 38/21 69/28   39/44    55/53      25/28     34/32
 //   128     32/39 51/51 107/86   23/21 39/29 79/45   40/54    73/77      26/31     45/48
 //   256     32/44 72/77 133/128  23/28 50/45 87/70   67/78   100/108     42/48     64/62
-// The largest alone (16 x 131072) 16 / 19.
+// The largest alone (16 x 131072, three tensors in turn) 20.6 / 20.1.
 int chunks_of(const nhip_sample_desc* d) {
   const int force = setting_int("NHIP_SAMPLE_CHUNKS", -1);
   if (force >= 0) return std::min(force, 64);
@@ -1131,8 +1137,10 @@ int sample_run(const SampleArgs& a, const nhip_sample_desc* d, hipStream_t s) {
   const dim3 grid((uint32_t)((int64_t)rows * a.chunks)), block(kPartWaves * 64);
   NHIP_LAUNCH("sample_top", (sample_top_kernel<T>), grid, block, 0, s, a);
   NHIP_TRY(check_launch("sample_top"));
-  NHIP_LAUNCH("sample_bins", (sample_bins_kernel<T>), grid, block, 0, s, a);
-  NHIP_TRY(check_launch("sample_bins"));
+  if (has_bins(d)) {
+    NHIP_LAUNCH("sample_bins", (sample_bins_kernel<T>), grid, block, 0, s, a);
+    NHIP_TRY(check_launch("sample_bins"));
+  }
   if (no_filter(d)) return sample_last<T, 4, true>(a, rows, s);  // (reads a 1024th of a row)
   // (no launch where the settings of all rows leave it nothing to do, nor where the
   // last launch has a workgroup for every CU to do it with: 64 rows of 131072 bf16, each

@@ -288,6 +288,20 @@ def test_borders_of_large_sums(nhip_env, spread, off, chunks):
             assert abs(float(logprob[r]) - (float(logits[want]) - np.log(sum(weights[i] for i in kept) * 2.0 ** -44))) < 2e-6
 
 
+@pytest.mark.parametrize("settings,most", [((0.0, 0, 1.0, 0.0), 2), ((0.0, 40, 0.9, 0.0), 2), ((1.0, 1, 0.9, 0.0), 2), ((1.0, 0, 1.0, 0.1), 2),
+                                           ((1.0, 0, 1.0, 0.0), 3), ((1.0, 40, 0.9, 0.0), 3), ((1.0, 0, 0.9, 0.0), 4)])
+def test_launches(nhip_env, settings, most):
+    """No launch where the settings leave all rows nothing for it to do."""
+    nhip_env.setenv("NHIP_SAMPLE_CHUNKS", "4")
+    gen = torch.Generator().manual_seed(13)
+    logits, u = torch.randn((6, 30011), generator=gen) * 3, torch.rand((6,), generator=gen)
+    nhip.timer_start()
+    got = nhip.sample(logits.cuda(), u.cuda(), *settings)
+    torch.cuda.synchronize()
+    assert nhip.timer_stop()[0] <= most
+    check(got, logits, u, settings)
+
+
 def test_refusals():
     x, u = torch.zeros((4, 50), device="cuda"), torch.zeros(4, device="cuda")
     for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=-0.1), dict(min_p=1.5),
