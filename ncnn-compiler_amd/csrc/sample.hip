@@ -50,7 +50,7 @@ struct SampleArgs {
   int32_t chunks;
   uint2* tops;      // [rows][chunks]
   RowParts* parts;  // [rows]
-  uint32_t* lists;  // [rows][kLongList]: indices of tokens that may be kept
+  uint32_t* lists;  // [rows][kLongList]: indices of tokens that may be kept (only if a row can have a list)
 };
 constexpr int kLongList = 16384;
 
@@ -1113,7 +1113,8 @@ int chunks_of(const nhip_sample_desc* d) {
 
 uint64_t workspace_of(const nhip_sample_desc* d) {
   const int chunks = chunks_of(d);
-  return chunks ? d->rows * (sizeof(RowParts) + (uint64_t)chunks * sizeof(uint2) + kLongList * sizeof(uint32_t)) : 0;
+  const uint64_t list = has_lists(d) ? kLongList * sizeof(uint32_t) : 0;
+  return chunks ? d->rows * (sizeof(RowParts) + (uint64_t)chunks * sizeof(uint2) + list) : 0;
 }
 
 template <class T, int WAVES, bool PARTS>
@@ -1200,7 +1201,7 @@ int nhip_sample_forward(const nhip_sample_desc* desc, const void* logits, const 
   const SampleArgs a{logits,           desc->row_stride,       desc->vocab,      uniform,          desc->temperature,
                      desc->top_p,      desc->min_p,            desc->top_k,      desc->temperature_each,
                      desc->top_k_each, desc->top_p_each,       desc->min_p_each, token,            logprob,
-                     chunks_of(desc),  tops, parts, (uint32_t*)(tops + (int64_t)desc->rows * chunks_of(desc))};
+                     chunks_of(desc),  tops, parts, has_lists(desc) ? (uint32_t*)(tops + (int64_t)desc->rows * chunks_of(desc)) : nullptr};
   return NHIP_FOR_ELEM(desc->dtype, T, sample_run<T>(a, desc, as_stream(stream)));
 }
 

@@ -45,3 +45,15 @@ def test_workspace():
     assert nhip.load().nhip_sample_workspace_size(d, ctypes.byref(n)) == 0 and n.value > 0
     assert forward(d) == 1 and forward(d, ws=ONE, nbytes=n.value - 1) == 5 and forward(d, ws=ONE + 8, nbytes=n.value) == 5
     assert nhip.load().nhip_sample_workspace_size(desc(), ctypes.byref(n)) == 0 and n.value == 0
+
+
+@pytest.mark.parametrize("change,listed", [
+    (dict(), False), (dict(min_p=0.1), False), (dict(top_k=1), False), (dict(temperature=0.0, top_k=40, top_p=0.9), False),
+    (dict(top_k=40), True), (dict(top_k=3000), True), (dict(top_p=0.9), True), (dict(top_k_each=ONE), True), (dict(top_p_each=ONE), True),
+    (dict(temperature=0.0, temperature_each=ONE, top_p=0.9), True), (dict(top_k=1, top_k_each=ONE), True), (dict(top_k=2 ** 18), False)])
+def test_workspace_of_lists(nhip_env, change, listed):
+    """Rows begun by several workgroups: 64 KB each for a list of tokens, only where a row can have one."""
+    nhip_env.setenv("NHIP_SAMPLE_CHUNKS", "4")
+    n = ctypes.c_uint64()
+    assert nhip.load().nhip_sample_workspace_size(desc(vocab=100000, rows=1000, **change), ctypes.byref(n)) == 0
+    assert (n.value >= 1000 * 65536) == listed and n.value >= 1000 * (1024 * 8 + 4 * 8)
