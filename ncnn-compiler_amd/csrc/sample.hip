@@ -18,6 +18,7 @@ namespace nhip {
 namespace {
 
 constexpr int kBins = 1024;    // of weights' exponents, or of keys, or of indices
+constexpr int kMostLogits = 1 << 19;  // of a row: as many weights of 2^44 are the most that 64 bits sum
 constexpr int kSorted = 1024;  // tokens that are sorted at most
 constexpr int kOnce = 128;     // and for all filters at once, rather than about each one's border (a sort of more takes barriers)
 constexpr float kRange = 31.5f;  // exp(-31.5) < 2^-45, which rounds to 0
@@ -266,7 +267,7 @@ struct Distances {
     half_top = 0.5f * top;
     reach = fminf(0.5f * kRange * c.temperature, 3.4028235e38f);  // (finite: -infinity stays outside)
     const float near = 6.f - 2.5f * __logf(fmaxf(1.f - c.top_p, 1e-6f));
-    scope = c.k < 0x7fffffff && c.top_p < 1.f ? fminf(reach, 0.5f * near * c.temperature) : reach;
+    scope = c.top_p < 1.f ? fminf(reach, 0.5f * near * c.temperature) : reach;
   }
   __device__ __forceinline__ float below(float l) const { return fmaf(-0.5f, l, half_top); }
   // a logit that no token of weight is below
@@ -983,6 +984,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
 
   // the draw: weights by index
   if (listed) {
+    static_assert(kMostLogits / kBins <= kSorted, "a bin of indices fits s.sorted");
     int shift = 0;
     while ((a.vocab - 1) >> shift >= kBins) ++shift;
     const auto drawn = [&](uint64_t place) -> uint64_t {
@@ -1000,9 +1002,8 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
     const uint64_t begin = at ? s.bins[at - 1] : 0;
     for (int i = threadIdx.x; i < n; i += TH)
       if ((int)(~(uint32_t)s.list[i] >> shift) == at && drawn(s.list[i])) {
-        const int m = atomicAdd(&s.count, 1);
         // (the index turned round: falling order is rising index)
-        if (m < kSorted) s.sorted[m] = s.list[i] << 32 | s.list[i] >> 32;
+        s.sorted[atomicAdd(&s.count, 1)] = s.list[i] << 32 | s.list[i] >> 32;
       }
     __syncthreads();
     const int m = s.count;
@@ -1015,15 +1016,13 @@ __global__ __launch_bounds__(WAVES * 64) void sample_kernel(SampleArgs a) {
       finish();
       return;
     }
-    if (m <= kSorted) {
-      sort_list<WAVES>(s.sorted, m);
-      sum_sorted(m, [&](uint64_t place) { return weight(of_key((uint32_t)place)); });
-      const uint64_t rest = target - begin;
-      for (int i = threadIdx.x; i < m; i += TH)
-        if (rest < s.bins[i] && rest >= (i ? s.bins[i - 1] : 0)) found((int)~(uint32_t)(s.sorted[i] >> 32), of_key((uint32_t)s.sorted[i]), total);
-      finish();
-      return;
-    }
+    sort_list<WAVES>(s.sorted, m);
+    sum_sorted(m, [&](uint64_t place) { return weight(of_key((uint32_t)place)); });
+    const uint64_t rest = target - begin;
+    for (int i = threadIdx.x; i < m; i += TH)
+      if (rest < s.bins[i] && rest >= (i ? s.bins[i - 1] : 0)) found((int)~(uint32_t)(s.sorted[i] >> 32), of_key((uint32_t)s.sorted[i]), total);
+    finish();
+    return;
   }
   const auto drawn = [&](float l, int index) -> uint64_t {
     if (!inside(l, index)) return 0;
@@ -1159,8 +1158,8 @@ int sample_args(const nhip_sample_desc* d) {
   if (!d) return fail(NHIP_STATUS_NULL_POINTER, "sample: null descriptor");
   if (!elem_size(d->dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "sample: dtype has to be F32, F16 or BF16");
   if (d->rows < 0 || d->vocab <= 0) return fail(NHIP_STATUS_INVALID_SHAPE, "sample: a row holds at least one logit");
-  // (2^19 weights of 2^44 each are the most that 64 bits sum; a launch has below 2^32 threads)
-  if (d->vocab > 1 << 19 || d->rows >= 1 << 22) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "sample: below 2^22 rows of at most 2^19 logits");
+  // (a launch has below 2^32 threads)
+  if (d->vocab > kMostLogits || d->rows >= 1 << 22) return fail(NHIP_STATUS_SHAPE_ARITHMETIC_OVERFLOW, "sample: below 2^22 rows of at most 2^19 logits");
   if (d->row_stride < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "sample: negative stride");
   // (values that a tensor holds for each row are read on the device, where these mean the same as the nearest that is allowed)
   if (!(d->temperature >= 0.f) || d->top_k < 0 || !(d->top_p >= 0.f) || !(d->min_p >= 0.f) || d->min_p > 1.f)
