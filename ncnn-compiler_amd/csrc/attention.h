@@ -727,7 +727,7 @@ int run(const AttnArgs& a, int src, hipStream_t s) {
                  : src == kSrcAny ? launch_by_dim<T, kSrcAny>(a, s)
                                   : launch_by_dim<T, kSrcInt8>(a, s);
   NHIP_TRY(st);
-  if (a.tiles || a.splits == 1 || a.parts) return ok();
+  if (a.tiles || a.splits == 1) return ok();
   const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
   if (a.d % 4 == 0 && aligned_to(a.o, 4 * sizeof(T)))
     NHIP_LAUNCH("attention_join", (attn_join_kernel<T, 4>), dim3((uint32_t)ceil_div(rows * (a.d / 4), 256)), dim3(256), 0, s, a);
