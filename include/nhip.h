@@ -543,7 +543,7 @@ int nhip_linear8_create(int32_t experts, int32_t num_output, int32_t num_input,
 int nhip_linear8_workspace_size(nhip_linear8_t plan, int32_t dtype,
                                 int64_t rows, uint64_t* bytes);
 /* x: [rows][num_input], rows row_stride elements apart; out: [rows][num_output]
- * contiguous, not overlapping x.  expert_starts: int32 [experts + 1], not
+ * contiguous; one that overlaps a row of x is refused.  expert_starts: int32 [experts + 1], not
  * falling: rows expert_starts[e] .. expert_starts[e + 1] - 1 are expert e's,
  * rows before the first and behind the last are left as they were (starts are
  * clamped to 0..rows).  NULL with one expert: all rows. */

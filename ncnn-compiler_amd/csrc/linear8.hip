@@ -369,6 +369,14 @@ uint64_t workspace_of(const nhip_linear8_plan* p, int64_t rows) {
   return (uint64_t)round_up(rows, 16) * p->steps * kStepK + (uint64_t)round_up(rows * (int64_t)sizeof(float), 16);
 }
 
+// Whether any of the rows, `stride` bytes apart, holds a byte of `out`.
+bool rows_meet(const void* x, int64_t rows, int64_t stride, int64_t row_bytes, const void* out, int64_t out_bytes) {
+  const int64_t off = (int64_t)((uintptr_t)out - (uintptr_t)x);
+  // the first row that ends behind the beginning of `out`
+  const int64_t r = off < row_bytes ? 0 : stride ? (off - row_bytes) / stride + 1 : rows;
+  return r < rows && r * stride < off + out_bytes;
+}
+
 int linear8_args(const nhip_linear8_plan* p, int32_t dtype, int64_t rows) {
   if (!p) return fail(NHIP_STATUS_NULL_POINTER, "linear8: null plan");
   if (!elem_size(dtype)) return fail(NHIP_STATUS_UNSUPPORTED, "linear8: dtype has to be F32, F16 or BF16");
@@ -464,6 +472,9 @@ int nhip_linear8_forward(nhip_linear8_t plan, const void* x, int32_t dtype, int6
   if (!aligned_to(x, es) || !aligned_to(out, es) || !aligned_to(expert_starts, 4))
     return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "linear8: a tensor is not aligned to its type");
   if (row_stride < 0) return fail(NHIP_STATUS_INVALID_SHAPE, "linear8: negative stride");
+  // (workgroups read tokens while others store results)
+  if (rows_meet(x, rows, row_stride * es, (int64_t)plan->k * es, out, rows * plan->n * es))
+    return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "linear8: the results overlap the tokens");
   int dev = -1;
   NHIP_TRY(check_hip(hipGetDevice(&dev), "hipGetDevice"));
   if (dev != plan->device) return fail(NHIP_STATUS_CONSTRAINT_VIOLATION, "linear8: the plan is another device's");

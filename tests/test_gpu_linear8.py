@@ -222,6 +222,38 @@ def test_refusals():
         plan.forward(x, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
 
 
+@pytest.mark.parametrize("rows", [3, 40])
+def test_results_over_tokens(rows):
+    """Results that overlap a token's row are refused, whatever the number of rows; those beside or between them are not."""
+    gen = torch.Generator().manual_seed(4)
+    w, ws, b = weights(gen, (64, 64), True)
+    plan = nhip.Linear8(w.cuda(), ws.cuda(), b.cuda())
+    x = tokens(gen, rows, 64, torch.float16)
+    want = ref.product(x, w, ws, b, "none")
+    size = rows * 64
+    flat = torch.zeros(3 * size, dtype=torch.float16, device="cuda")
+
+    def at(start):
+        return flat[start:start + size].view(rows, 64)
+
+    at(size).copy_(x)
+    for start in (size, size - 64, size + 64, 1, 2 * size - 1):
+        with pytest.raises(nhip.NhipError):
+            plan.forward(at(size), out=at(start))
+    assert torch.equal(at(size).cpu(), x)  # refused before anything is launched
+    for start in (0, 2 * size):
+        check(plan.forward(at(size), out=at(start)), want)
+    # the results between two rows that lie apart, and over one of them
+    wide = torch.zeros((2, 4 * 64), dtype=torch.float16, device="cuda")
+    wide[:, :64] = x[:2].cuda()
+    between, over = wide.flatten()[64:192].view(2, 64), wide.flatten()[192:320].view(2, 64)
+    check(plan.forward(wide[:, :64], out=between), ref.product(x[:2], w, ws, b, "none"))
+    with pytest.raises(nhip.NhipError):
+        plan.forward(wide[:, :64], out=over)
+    one = x[:1].cuda().expand(rows, 64)
+    check(plan.forward(one, out=torch.zeros((rows, 64), dtype=torch.float16, device="cuda")), ref.product(one, w, ws, b, "none"))
+
+
 def test_plan_not_made_in_a_capture():
     w, ws = torch.zeros((8, 16), dtype=torch.int8, device="cuda"), torch.ones(8, device="cuda")
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
