@@ -1141,7 +1141,8 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=
     k, k_each = _each(top_k, dev, rows, torch.int32, "top_k")
     p, p_each = _each(top_p, dev, rows, torch.float32, "top_p")
     m, m_each = _each(min_p, dev, rows, torch.float32, "min_p")
-    desc = SampleDesc(code, rows, vocab, logits.stride(0), t, min(k, 0x7fffffff), p, m, t_each, k_each, p_each, m_each)
+    # (more than 32 bits hold is all of them, or refused below 0)
+    desc = SampleDesc(code, rows, vocab, logits.stride(0), t, max(-1, min(k, 0x7fffffff)), p, m, t_each, k_each, p_each, m_each)
     n = ctypes.c_uint64()
     check(load().nhip_sample_workspace_size(desc, n))
     token, logprob = out or (None, None)

@@ -302,6 +302,15 @@ def test_launches(nhip_env, settings, most):
     check(got, logits, u, settings)
 
 
+def test_settings_past_32_bits():
+    x, u = torch.zeros((4, 50), device="cuda"), torch.zeros(4, device="cuda")
+    for top_k in (-1, -2 ** 31 - 1, -2 ** 32 + 5, -2 ** 40):
+        with pytest.raises(nhip.NhipError):
+            nhip.sample(x, u, top_k=top_k)
+    for top_k in (2 ** 31, 2 ** 32 + 5):  # all of them
+        assert torch.allclose(nhip.sample(x, u, top_k=top_k)[1].cpu(), -torch.log(torch.tensor(50.0)))
+
+
 def test_refusals():
     x, u = torch.zeros((4, 50), device="cuda"), torch.zeros(4, device="cuda")
     for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=-0.1), dict(min_p=1.5),
