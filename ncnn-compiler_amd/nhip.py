@@ -952,10 +952,17 @@ class Linear8(_Plan):
         return out
 
 
+def _limit(v):
+    """A number of keys that 32 bits hold (ctypes would take what is left of it)."""
+    if not -2 ** 31 <= v < 2 ** 31:
+        raise ValueError(f"{v} keys do not fit 32 bits")
+    return v
+
+
 @functools.lru_cache(4096)
 def _attention(settings, code, b, lq, lk, h, hkv, d, scale, cached=False):
     """(descriptor, workspace bytes)."""
-    desc = AttentionDesc(code, b, lq, lk, h, hkv, d, float(d) ** -0.5 if scale is None else float(scale))
+    desc = AttentionDesc(code, b, lq, _limit(lk), h, hkv, d, float(d) ** -0.5 if scale is None else float(scale))
     n = ctypes.c_uint64()
     if cached:  # the size goes by the descriptor alone
         check(load().nhip_kv8_attention_workspace_size(ctypes.byref(desc), ctypes.byref(Kv8Desc()), ctypes.byref(n)))
@@ -967,9 +974,9 @@ def _attention(settings, code, b, lq, lk, h, hkv, d, scale, cached=False):
 @functools.lru_cache(4096)
 def _prefix_attention(settings, code, b, lq, lk, h, hkv, d, scale, groups, lp):
     """(descriptor, workspace bytes)."""
-    desc = AttentionDesc(code, b, lq, lk, h, hkv, d, float(d) ** -0.5 if scale is None else float(scale))
+    desc = AttentionDesc(code, b, lq, _limit(lk), h, hkv, d, float(d) ** -0.5 if scale is None else float(scale))
     n = ctypes.c_uint64()
-    check(load().nhip_kv8_prefix_attention_workspace_size(ctypes.byref(desc), groups, lp, ctypes.byref(Kv8Desc()), ctypes.byref(n)))
+    check(load().nhip_kv8_prefix_attention_workspace_size(ctypes.byref(desc), groups, _limit(lp), ctypes.byref(Kv8Desc()), ctypes.byref(n)))
     return desc, n.value
 
 

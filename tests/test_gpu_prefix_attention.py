@@ -215,6 +215,19 @@ def test_streams_graphs_and_bits():
             assert torch.equal(held[i][1], want[(r + i) % 4])
 
 
+def test_limits_past_32_bits():
+    """Limits that 32 bits do not hold are refused, not taken for what is left of them."""
+    cache = filled(8, 2, 64, 16)
+    q, shared, table = randn(1, (4, 1, 4, 64)).cuda(), ints([[0, 1], [2, 3]]), ints([[4], [5], [6], [7]])
+    for name in ("max_prefix", "max_length"):
+        for v in (2 ** 31, 2 ** 32 + 1, -2 ** 32 + 5):
+            with pytest.raises(ValueError):
+                cache.prefix_attention(q, shared, ints([30, 30]), table, ints([1, 2, 3, 4]), **{name: v})
+    for v in (2 ** 31, 2 ** 32 + 1, -2 ** 32 + 5):
+        with pytest.raises(ValueError):
+            cache.attention(q, table, ints([1, 2, 3, 4]), max_length=v)
+
+
 def test_refusals():
     cache = filled(8, 2, 64, 16)
     q, shared, table = torch.zeros((4, 1, 4, 64), device="cuda"), ints([[0, 1], [2, 3]]), ints([[4], [5], [6], [7]])
