@@ -788,7 +788,14 @@ __global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs prefix, 
 // bound it where a group has many rows (the latter 165 us without the join, fp16, 8 heads
 // of 128), waits for loads where it has few (4 groups of 64 rows, 3136 and 256 keys,
 // bf16 34 us; 51 MB read, 124 past the L2s: the dies' own or one's, the time is the same;
-// with the prefix first 2 us more).  OWN == 2 has too many registers for as many workgroups to a CU.
+// with the prefix first 2 us more).  All results pass through memory as fp32 parts and a
+// join, which pays where many sequences of few queries share a long prefix.  us, so / the
+// attention over one table of both, 32 heads on 8 of 128 bf16, one group, causal, as many
+// own keys as queries: 64 sequences of 1 query behind 197 / 3136 / 12544 keys 28 / 14, 40 / 62,
+// 49 / 195, of 4 32 / 15, 51 / 66, 96 / 199, of 16 58 / 23, 147 / 140, 312 / 524, of 32 63 / 27, 179
+// / 145, 568 / 535; 16 of 1 16 / 12, 21 / 27, 39 / 58, of 16 26 / 15, 51 / 51, 97 / 146; 4 of 1 17 /
+// 12, 18 / 18, 24 / 29; prompts of 4 x 512 behind 197 and 3136 81 / 44 and 197 / 163, of 16 x 1024
+// 596 / 355 and 1513 / 1289.  OWN == 2 has too many registers for as many workgroups to a CU.
 template <class T, int DP, bool TILES, int OWN>
 __global__ __launch_bounds__(kWaves * 64, (TILES ? TilesShape<T, DP, kSrcInt8>::per_cu : rows_per_cu(sizeof(T), DP, kSrcInt8) - (OWN == 2 && DP == 128 && sizeof(T) == 2))) void
 attn_prefix_kernel(AttnArgs prefix, AttnArgs own, uint32_t own_wgs) {

@@ -238,9 +238,11 @@ __device__ __forceinline__ void tile_body(const Linear8Args& a, int e, int begin
 }
 
 // Quarters of the first `small` tiles, then the other tiles whole.
-// Matrix instructions bound it, and the power they draw: 8192 x 8192 of 8192 504 us with
-// the codes (2180 TOPS; the library's product 2068), 6272 x 8192 of 2048 107 us without
-// (1970; 1647).  32 x 32 x 32 instructions ran at 4775 TOPS from registers on zeros and
+// 8192 x 8192 of 8192 504 us with the codes (2180 TOPS; the library's product 2068), 6272 x
+// 8192 of 2048 bf16 107 us without (1970; 1647). Of the latter the matrix units are busy 46%;
+// waits for stages and barriers stand beside them (93 us with no results stored, 115 with, each
+// launch timed by itself), then the results' way through LDS; 12544 x 4096 of 1024, 32 experts,
+// 66 and 95 so.  32 x 32 x 32 instructions ran at 4775 TOPS from registers on zeros and
 // 3400 on random codes, at a clock of some 1.7 GHz, 16 x 16 x 64 ones at 2590, so
 // large instructions; two workgroups of 4 waves a CU, so that one's results and starts
 // are beside the other's products.

@@ -437,7 +437,7 @@ __device__ __forceinline__ void list_tokens(const SampleArgs& a, int64_t r, cons
 // looked for in, or without a filter the sums of its sets; of rows with top-k of few
 // the tokens that reach the bound.  The weights' arithmetic in 64 bits and the 64-bit
 // LDS atomics bound it (0.85 lanes of a CU a cycle, of 32 bits 1.7: counts have those):
-// 256 rows of 50021 fp32 by top-p 0.95 23.6 us, 64 of 131072 bf16, each its own filters, 10.9.
+// 256 rows of 50021 fp32 by top-p 0.95 23.6 us, 64 of 131072 bf16, each its own filters, 10.4.
 template <class T>
 __global__ __launch_bounds__(kPartWaves * 64) void sample_bins_kernel(SampleArgs a) {
   __shared__ uint64_t bins[kBins];
@@ -551,8 +551,8 @@ __global__ __launch_bounds__(kPartWaves * 64) void sample_list_kernel(SampleArgs
 // fit there, of all.
 //
 // A chain of steps between barriers bounds it, of which each has little to do: 64 rows
-// of 131072 bf16, each its own filters, 23 us behind the launches above; 16 of 1000 fp32 by
-// top-k 11.8 a call.  256 of 50021 fp32 by top-p 0.95, all in this launch, 67: the largest,
+// of 131072 bf16, each its own filters, 22.4 us behind the launches above; 16 of 1000 fp32 by
+// top-k 12.1 a call.  256 of 50021 fp32 by top-p 0.95, all in this launch, 68: the largest,
 // the histogram and the tokens that it leaves (some 9000) are a pass over the row each,
 // of one CU, and the tokens are summed twice.
 template <class T, int WAVES, bool PARTS>

@@ -1100,7 +1100,10 @@ class KvCache8:
         the pages in prefix_table [groups, pages], and behind them the first
         lengths[b] of the sequence's own pages in block_table (at most max_prefix
         and max_length; default what the tables hold).  causal: the queries are the
-        last of the sequence's own tokens."""
+        last of the sequence's own tokens.  Made for many sequences of few queries
+        behind a long prefix: with a few hundred tokens in it, or 32 queries to a
+        sequence, attention() over one table of both is the faster (where the
+        prefix ends with a page)."""
         b, lq, h, d = q.shape
         code, dev = _elem(q)
         if d != self.head_dim or dev != self._dev:
