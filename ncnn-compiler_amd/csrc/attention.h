@@ -164,7 +164,8 @@ __device__ __forceinline__ typename Frag<T>::type codes8(uint32_t lo, uint32_t h
 // parts that a probability is the sum of.  16-bit types take one, a rounding
 // (the error against 64 bits is 2.3e-3 of the result's norm in bf16, where rounding
 // the result alone leaves 1.7e-3; 2.9e-4 and 2.1e-4 in fp16).  A second part takes up to
-// 3% more time, over the cache 1 to 6%, but it may be 0 or negative, and an
+// 3% more time, over the cache 1 to 6% (64 samples behind four prefixes of 3136 keys 37.7 ->
+// 38.5 us), but it may be 0 or negative, and an
 // infinite value that it meets NaN.  The sum l is of the probabilities as they
 // were.  Codes times probabilities times a page's scale may leave fp16's range,
 // so fp16 queries over the cache take bf16, which needs both parts for fp16's

@@ -391,7 +391,8 @@ __device__ __forceinline__ void tiles_body(const AttnArgs& a, uint32_t block, ui
         // 16-bit types: probabilities are rounded to the type for the second
         // product, as with few rows.  As the sum of two they would take another one:
         // us with one / two 737 / 987 (2 x 3136 rows of 16 heads of 128 to 12544 keys
-        // bf16), 23.3 / 29.7 (4 x 784 of 12 of 64 to 784), 60 / 73 (fp16 over the cache).
+        // bf16), 23.3 / 29.7 (4 x 784 of 12 of 64 to 784), 60 / 73 (fp16 over the cache),
+        // 176 / 198 (48 sequences of 28 rows behind a prefix of 12544 fp16).
         // l sums them as they were; with units as rounded (sum8).
         typename std::conditional<S::split, v8f, FM>::type pf[NT][2];
 #pragma unroll
